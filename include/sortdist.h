@@ -324,6 +324,61 @@ int sd_mask_count(uint32_t seed, int C, float q);
  * of the C channels, ascending (the reference's sort(topk(rand(S, G, C), count).indices)). */
 int sd_sample_index_lists(uint32_t seed, int S, int G, int C, int count, int* out, sd_stream_t stream);
 
+/* ---- training a head's logits (no reference launcher: the losses of main.py:329-379 are torch ops on one label per sample) ----
+ * Logits may be fp32, bf16 or fp16; everything per row is fp32.  Unlike the entry points above these use no scratch of the
+ * library: the caller passes `scratch` (16-byte aligned, sd_label_scratch() floats, any contents), so calls that overlap on several streams
+ * or in several graphs share nothing. */
+#define SD_FLOAT32 0
+#define SD_BFLOAT16 1
+#define SD_FLOAT16 2
+
+/* Rows of logits with a label each.  Row r starts (r / inner) * outer_stride + (r % inner) * inner_stride elements behind `logits`, its
+ * classes are neighbours.  A row whose label is ignore_index is not read and counts nowhere; one whose label names no class has the log
+ * probability NaN and a gradient of NaN. */
+typedef struct {
+    const void* logits;
+    const int64_t* labels;      /* (rows) */
+    int64_t rows, inner, classes, outer_stride, inner_stride, ignore_index;
+    int dtype;
+} sd_label_rows;
+
+/* Floats of scratch that the calls below want for these rows (host only), or -1 where they would refuse them. */
+int64_t sd_label_scratch(const sd_label_rows* rows);
+
+/* log_probs[r] = log softmax(row r)[label], 0 where ignored.  stats (rows, 2; may be NULL) receives what sd_label_gradient needs. */
+int sd_label_log_probs(const sd_label_rows* rows, float* log_probs, float* stats, float* scratch, sd_stream_t stream);
+
+/* Paired answers: answer a holds the rows offsets[a] .. offsets[a + 1] (2 pairs + 1 entries of offset_bytes = 4 or 8 bytes, not
+ * decreasing, on the device), or `tokens` rows each where offsets is NULL; answer i is chosen over answer pairs + i.  ref (rows): log
+ * probabilities of the labels under the reference model.  With s_a the sum of (log_prob - ref) over the rows of a that are not ignored,
+ *   rewards[a] = beta s_a,  x_i = rewards[i] - rewards[pairs + i],
+ *   loss = mean_i -(1 - smoothing) log sigma(x_i) - smoothing log sigma(-x_i).
+ * stats (rows, 2) and weight (rows), both or neither NULL: d loss / d log_prob per row and what sd_label_gradient needs. */
+int sd_preference_loss(const sd_label_rows* rows, const float* ref, const void* offsets, int offset_bytes, int64_t tokens, int pairs,
+                       double beta, double smoothing, float* stats, float* weight, float* rewards, float* loss, float* scratch, sd_stream_t stream);
+
+/* Clipped policy loss: with ratio = exp(log_prob - old) and apart = ref - log_prob, the mean over the rows that are not ignored (0 where
+ * all are) of  -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl (exp(apart) - apart - 1).
+ * Row r's advantage A stands at (r / inner) * advantage_outer + (r % inner) * advantage_inner; ref may be NULL where kl = 0.
+ * means (3): the first term, the second without its factor, the share of clipped rows.  stats, weight as above; the gradient is
+ * sd_label_gradient with these and `scale` (1), which receives the reciprocal of the number of rows that count. */
+int sd_policy_loss(const sd_label_rows* rows, const float* old_log_probs, const float* advantages, int64_t advantage_outer,
+                   int64_t advantage_inner, const float* ref, double clip_low, double clip_high, double kl, float* stats, float* weight,
+                   float* scale, float* loss, float* means, float* scratch, sd_stream_t stream);
+
+/* grad[r, v] = weight[r] scale scale2 ([v = label] - softmax(row r)[v]), rows of `classes` values one behind the other, in the logits' type;
+ * scale and scale2 (one float each on the device) may be NULL.  Zeros where ignored or where the product is 0. */
+int sd_label_gradient(const sd_label_rows* rows, const float* stats, const float* weight, const float* scale, const float* scale2,
+                      void* grad, sd_stream_t stream);
+
+/* Dropout of up to three tensors of n values under one mask (inputs that are not wanted are NULL with their outputs): value i is kept
+ * where field i of the generator is below L = floor(65536 q + 0.5), and multiplied by 65536 / L.  The fields of values 2j and 2j + 1 are
+ * the low and high halves of mix(sd_rng_word(seed, 5, j >> 15, j & 32767) ^ key), mix being the generator's finaliser and key =
+ * mix((seed ^ (6 * 0x9e3779b9)) + (j >> 15)).  seed_on_device, if not NULL, holds the seed in its low 32 bits (graphs that draw
+ * a new mask in each replay).  The backward is the same call on the gradients. */
+int sd_dropout(const void* x0, const void* x1, const void* x2, int dtype, int64_t n, double q, uint32_t seed, const int64_t* seed_on_device,
+               void* y0, void* y1, void* y2, sd_stream_t stream);
+
 /* The counter RNG and the thresholds it is compared with, exposed for verification. */
 uint32_t sd_rng_word(uint32_t seed, uint32_t stream_id, uint32_t row, uint32_t col);
 uint32_t sd_mask_threshold8(float q);

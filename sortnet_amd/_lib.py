@@ -15,6 +15,17 @@ _S = ctypes.c_void_p          # hipStream_t
 _i = ctypes.c_int
 _f = ctypes.c_float
 _u = ctypes.c_uint32
+_l = ctypes.c_int64
+_d = ctypes.c_double
+
+
+class LabelRows(ctypes.Structure):
+    """sd_label_rows of include/sortdist.h."""
+    _fields_ = [("logits", _F), ("labels", _I), ("rows", _l), ("inner", _l), ("classes", _l), ("outer_stride", _l),
+                ("inner_stride", _l), ("ignore_index", _l), ("dtype", _i)]
+
+
+_R = ctypes.POINTER(LabelRows)
 
 # name -> argument types, in the order of include/sortdist.h
 SIGNATURES = {
@@ -48,6 +59,11 @@ SIGNATURES = {
     "sd_unfold": [_F, _i, _i, _i, _i, _i, _i, _i, _i, _i, _F, _S],
     "sd_fold": [_F, _i, _i, _i, _i, _i, _i, _i, _i, _i, _F, _S],
     "sd_sample_index_lists": [_u, _i, _i, _i, _i, _I, _S],
+    "sd_label_log_probs": [_R, _F, _F, _F, _S],
+    "sd_preference_loss": [_R, _F, _I, _i, _l, _i, _d, _d, _F, _F, _F, _F, _F, _S],
+    "sd_policy_loss": [_R, _F, _F, _l, _l, _F, _d, _d, _d, _F, _F, _F, _F, _F, _F, _S],
+    "sd_label_gradient": [_R, _F, _F, _F, _F, _F, _S],
+    "sd_dropout": [_F, _F, _F, _i, _l, _d, _u, _I, _F, _F, _F, _S],
 }
 _OTHER = {
     "sd_version": ([], _i),
@@ -66,6 +82,7 @@ _OTHER = {
     "sd_mask_threshold8": ([_f], _u),
     "sd_mask_threshold16": ([_f], _u),
     "sd_mask_count": ([_u, _i, _f], _i),
+    "sd_label_scratch": ([_R], _l),
 }
 
 _lib = None

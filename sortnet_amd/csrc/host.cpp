@@ -7,6 +7,7 @@
 // is a few tensor headers, one graph node and the launches; the backward runs on autograd's own thread without the
 // interpreter.  Tensors stay torch's: outputs come from its caching allocator and work is queued on its current
 // stream.
+#include <array>
 #include <cmath>
 #include <mutex>
 #include <stdexcept>
@@ -546,6 +547,300 @@ Tensor unfold(const Tensor& x_in, int kh, int kw, int dil, int pad, int stride) 
     return y;
 }
 
+// ---- losses on the log probability of a label, from logits in fp32, bf16 or fp16 --------------------------------------
+int element_type(const Tensor& t, const char* name) {
+    if (!t.is_cuda()) throw std::runtime_error(std::string(name) + " must be a CUDA tensor");
+    switch (t.scalar_type()) {
+        case at::kFloat: return SD_FLOAT32;
+        case at::kBFloat16: return SD_BFLOAT16;
+        case at::kHalf: return SD_FLOAT16;
+        default: throw std::runtime_error(std::string(name) + " must have dtype torch.float32, torch.bfloat16 or torch.float16");
+    }
+}
+
+void same_device(const Tensor& t, const char* name, const Tensor& like) {
+    if (!t.is_cuda()) throw std::runtime_error(std::string(name) + " must be a CUDA tensor");
+    if (t.device() != like.device()) throw std::runtime_error(std::string(name) + " is on another device than the outputs");
+}
+
+// The logits as the kernels read them: classes next to each other, at most two further dimensions with strides of their own
+// (padded vocabularies, rows of a larger batch); anything else is copied.
+Tensor readable_logits(const Tensor& z) {
+    const bool rows = z.dim() <= 3 && (z.size(-1) == 1 || z.stride(-1) == 1);
+    return rows ? z : z.contiguous();
+}
+
+sd_label_rows label_rows(const Tensor& z, const Tensor& labels, int64_t ignore) {
+    sd_label_rows a{};
+    a.dtype = element_type(z, "outputs");
+    a.logits = z.data_ptr();
+    a.labels = labels.data_ptr<int64_t>();
+    a.classes = z.size(-1);
+    a.rows = labels.numel();
+    if (z.dim() == 3) {
+        a.inner = z.size(1);
+        a.outer_stride = z.stride(0); a.inner_stride = z.stride(1);
+    } else {
+        a.inner = a.rows;
+        a.inner_stride = z.dim() == 2 ? z.stride(0) : z.size(-1);
+    }
+    a.ignore_index = ignore;
+    return a;
+}
+
+Tensor label_indices(const Tensor& targets, const Tensor& outputs) {
+    same_device(targets, "targets", outputs);
+    if (targets.scalar_type() != at::kLong && targets.scalar_type() != at::kInt) throw std::runtime_error("targets must have dtype torch.int64 or torch.int32");
+    if (outputs.dim() < 2 || targets.sizes() != outputs.sizes().slice(0, outputs.dim() - 1))
+        throw std::runtime_error("targets must have the sizes of outputs without their last dimension, the classes");
+    return targets.to(at::kLong).contiguous();
+}
+
+// a constant per row: no gradient flows into it
+Tensor row_constants(const Tensor& t, const char* name, const Tensor& targets) {
+    same_device(t, name, targets);
+    if (t.scalar_type() != at::kFloat) throw std::runtime_error(std::string(name) + " must have dtype torch.float32");
+    if (t.sizes() != targets.sizes()) throw std::runtime_error(std::string(name) + " must have the sizes of targets");
+    if (at::GradMode::is_enabled() && t.requires_grad())
+        throw std::runtime_error(std::string(name) + " must not require a gradient: the loss is differentiated with respect to outputs alone");
+    return t;
+}
+
+Tensor label_scratch(const sd_label_rows& a, const Tensor& like) {
+    const int64_t n = sd_label_scratch(&a);
+    if (n < 0) require(SD_ERR_ARG, "sd_label_scratch");
+    return new_floats(like, {n});
+}
+
+struct LabelNode : Node {
+    SavedVariable logits, labels, stats, weight, scale;   // weight, scale: none for plain log probabilities
+    int64_t ignore = 0;
+
+    variable_list apply(variable_list&& grads) override {
+        const Locked lock(mutex_);
+        variable_list out(1);
+        if (!task_should_compute_output(0)) return out;
+        const Tensor z = logits.unpack(), l = labels.unpack(), st = stats.unpack(), w = weight.unpack(), sc = scale.unpack();
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor g = incoming(*this, grads, 0);
+        const c10::DeviceGuard guard(z.device());
+        out[0] = at::empty(z.sizes(), z.options());
+        if (out[0].numel() == 0) return out;
+        const sd_label_rows a = label_rows(z, l, ignore);
+        const float* gp = floats(g, "grad_output");
+        if (w.defined())
+            require(sd_label_gradient(&a, floats(st, "stats"), floats(w, "weight"), sc.defined() ? floats(sc, "scale") : nullptr, gp, out[0].data_ptr(), stream_of(z)),
+                    "sd_label_gradient");
+        else
+            require(sd_label_gradient(&a, floats(st, "stats"), gp, nullptr, nullptr, out[0].data_ptr(), stream_of(z)), "sd_label_gradient");
+        return out;
+    }
+    void release_variables() override {
+        const Locked lock(mutex_);
+        logits.reset_data(); labels.reset_data(); stats.reset_data(); weight.reset_data(); scale.reset_data();
+    }
+    std::string name() const override { return "LabelNode"; }
+};
+
+// makes y the output of a node over the logits
+void attach_labels(const Tensor& y, const Tensor& outputs, const Tensor& z, const Tensor& labels, int64_t ignore, const Tensor& stats, const Tensor& weight,
+                   const Tensor& scale) {
+    auto node = new_node<LabelNode>();
+    node->set_next_edges(collect_next_edges(outputs));
+    node->ignore = ignore;
+    node->logits = SavedVariable(z, false);
+    node->labels = SavedVariable(labels, false);
+    node->stats = SavedVariable(stats, false);
+    if (weight.defined()) node->weight = SavedVariable(weight, false);
+    if (scale.defined()) node->scale = SavedVariable(scale, false);
+    set_history(y, node);
+}
+
+Tensor label_log_probs(const Tensor& outputs, const Tensor& targets, int64_t ignore) {
+    reverse_mode_only("label_log_probs", outputs);
+    const bool grad = want_grad(outputs);
+    Tensor y, z, labels, stats;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        element_type(outputs, "outputs");
+        const c10::DeviceGuard guard(outputs.device());
+        labels = label_indices(targets, outputs);
+        z = readable_logits(outputs);
+        y = new_floats(z, targets.sizes());
+        if (grad) stats = new_floats(z, {labels.numel(), 2});
+        if (y.numel() > 0) {
+            const sd_label_rows a = label_rows(z, labels, ignore);
+            const Tensor scratch = label_scratch(a, z);
+            require(sd_label_log_probs(&a, floats(y, "log_probs"), grad ? floats(stats, "stats") : nullptr, floats(scratch, "scratch"), stream_of(z)), "sd_label_log_probs");
+        }
+    }
+    if (grad) attach_labels(y, outputs, z, labels, ignore, stats, {}, {});
+    return y;
+}
+
+std::pair<Tensor, Tensor> preference_loss(const Tensor& outputs, const Tensor& targets, const Tensor& ref_in, const OptTensor& offsets_in, double beta,
+                                          double smoothing, int64_t ignore) {
+    reverse_mode_only("preference_loss", outputs);
+    const bool grad = want_grad(outputs);
+    Tensor loss, rewards, z, labels, stats, weight;
+    {
+        const bool packed = offsets_in && offsets_in->defined();
+        element_type(outputs, "outputs");
+        const Tensor ref = row_constants(ref_in, "ref_log_probs", targets).detach().contiguous();
+        at::AutoDispatchBelowADInplaceOrView below;
+        const c10::DeviceGuard guard(outputs.device());
+        labels = label_indices(targets, outputs);
+        z = readable_logits(outputs);
+        Tensor offsets;
+        int64_t answers = 0, tokens = 0;
+        if (packed) {
+            same_device(*offsets_in, "offsets", outputs);
+            if (offsets_in->scalar_type() != at::kLong && offsets_in->scalar_type() != at::kInt) throw std::runtime_error("offsets must have dtype torch.int64 or torch.int32");
+            if (offsets_in->dim() != 1 || outputs.dim() != 2) throw std::runtime_error("packed answers need outputs (rows, classes) and offsets (answers + 1)");
+            offsets = offsets_in->contiguous();
+            answers = offsets.size(0) - 1;
+        } else {
+            answers = outputs.size(0);
+            tokens = answers > 0 ? labels.numel() / answers : 0;
+        }
+        if (answers < 2 || answers % 2 != 0)
+            throw std::runtime_error("preference_loss needs an even number of answers, the chosen ones before the rejected: got " + std::to_string(answers));
+        const sd_label_rows a = label_rows(z, labels, ignore);
+        const Tensor scratch = label_scratch(a, z);
+        loss = new_floats(z, {});
+        rewards = new_floats(z, {answers});
+        if (grad) {
+            stats = new_floats(z, {labels.numel(), 2});
+            weight = new_floats(z, {labels.numel()});
+        }
+        require(sd_preference_loss(&a, floats(ref, "ref_log_probs"), packed ? offsets.data_ptr() : nullptr, packed ? (int)offsets.element_size() : 0, tokens,
+                                   (int)(answers / 2), beta, smoothing, grad ? floats(stats, "stats") : nullptr, grad ? floats(weight, "weight") : nullptr,
+                                   floats(rewards, "rewards"), floats(loss, "loss"), floats(scratch, "scratch"), stream_of(z)), "sd_preference_loss");
+    }
+    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, {});
+    return {loss, rewards};
+}
+
+std::pair<Tensor, Tensor> policy_loss(const Tensor& outputs, const Tensor& targets, const Tensor& old_in, const Tensor& advantages, const OptTensor& ref_in,
+                                      double clip_low, double clip_high, double kl, int64_t ignore) {
+    reverse_mode_only("policy_loss", outputs);
+    const bool grad = want_grad(outputs);
+    Tensor loss, means, z, labels, stats, weight, scale;
+    {
+        element_type(outputs, "outputs");
+        const Tensor old = row_constants(old_in, "old_log_probs", targets).detach().contiguous();
+        const Tensor ref = ref_in && ref_in->defined() ? row_constants(*ref_in, "ref_log_probs", targets).detach().contiguous() : Tensor();
+        Tensor adv = row_constants(advantages, "advantages", targets).detach();
+        at::AutoDispatchBelowADInplaceOrView below;
+        const c10::DeviceGuard guard(outputs.device());
+        labels = label_indices(targets, outputs);
+        z = readable_logits(outputs);
+        const sd_label_rows a = label_rows(z, labels, ignore);
+        if (adv.dim() > 2) adv = adv.contiguous();
+        // one advantage for all rows of an answer comes as an expanded tensor, which is read where it is
+        const bool two = z.dim() == 3;
+        const int64_t outer = two ? adv.stride(0) : 0, inner = two ? adv.stride(1) : adv.dim() == 1 ? adv.stride(0) : 1;
+        const Tensor scratch = label_scratch(a, z);
+        loss = new_floats(z, {});
+        means = new_floats(z, {3});
+        scale = new_floats(z, {1});
+        if (grad) {
+            stats = new_floats(z, {labels.numel(), 2});
+            weight = new_floats(z, {labels.numel()});
+        }
+        require(sd_policy_loss(&a, floats(old, "old_log_probs"), static_cast<const float*>(adv.data_ptr()), outer, inner, ref.defined() ? floats(ref, "ref_log_probs") : nullptr,
+                               clip_low, clip_high, kl, grad ? floats(stats, "stats") : nullptr, grad ? floats(weight, "weight") : nullptr, floats(scale, "scale"),
+                               floats(loss, "loss"), floats(means, "means"), floats(scratch, "scratch"), stream_of(z)), "sd_policy_loss");
+    }
+    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, scale);
+    return {loss, means};
+}
+
+// ---- dropout under a mask that is made again in the backward; up to three tensors share one --------------------------------
+void drop(const std::array<Tensor, 3>& x, const std::array<Tensor, 3>& y, double q, uint32_t seed, const Tensor& seeds) {
+    const Tensor* first = nullptr;
+    const void* in[3] = {nullptr, nullptr, nullptr};
+    void* out[3] = {nullptr, nullptr, nullptr};
+    for (int k = 0; k < 3; k++)
+        if (x[k].defined()) {
+            if (!first) first = &x[k];
+            in[k] = x[k].data_ptr(); out[k] = y[k].data_ptr();
+        }
+    if (!first || first->numel() == 0) return;
+    require(sd_dropout(in[0], in[1], in[2], element_type(*first, "input"), first->numel(), q, seed, seeds.defined() ? seeds.data_ptr<int64_t>() : nullptr,
+                       out[0], out[1], out[2], stream_of(*first)), "sd_dropout");
+}
+
+struct DropNode : Node {
+    SavedVariable seeds;
+    double q = 1.0;
+    uint32_t seed = 0;
+
+    variable_list apply(variable_list&& grads) override {
+        const Locked lock(mutex_);
+        const int count = (int)grads.size();
+        variable_list out(count);
+        const Tensor sd = seeds.unpack();
+        at::AutoDispatchBelowADInplaceOrView below;
+        std::array<Tensor, 3> g, gx;
+        c10::OptionalDeviceGuard guard;
+        for (int k = 0; k < count; k++) {
+            if (!task_should_compute_output(k)) continue;
+            g[k] = incoming(*this, grads, k);
+            guard.reset_device(g[k].device());
+            out[k] = gx[k] = at::empty(g[k].sizes(), g[k].options());
+        }
+        drop(g, gx, q, seed, sd);
+        return out;
+    }
+    void release_variables() override {
+        const Locked lock(mutex_);
+        seeds.reset_data();
+    }
+    std::string name() const override { return "DropNode"; }
+};
+
+// One output per tensor that is there, in order.
+std::vector<Tensor> dropout(const std::vector<Tensor>& inputs, double q, int64_t seed, const OptTensor& seeds) {
+    if (inputs.empty() || inputs.size() > 3) throw std::runtime_error("dropout takes one to three tensors");
+    bool grad = false;
+    for (const Tensor& t : inputs) {
+        reverse_mode_only("dropout", t);
+        element_type(t, "input");
+        if (t.sizes() != inputs[0].sizes() || t.scalar_type() != inputs[0].scalar_type() || t.device() != inputs[0].device())
+            throw std::runtime_error("tensors under one mask must have one size, dtype and device");
+        grad = grad || want_grad(t);
+    }
+    if (!(q >= 0.0 && q <= 1.0)) throw std::runtime_error("dropout: keep probability q=" + std::to_string(q) + " outside 0..1");
+    Tensor sd;
+    if (seeds && seeds->defined()) {
+        same_device(*seeds, "seed", inputs[0]);
+        if (seeds->scalar_type() != at::kLong || seeds->numel() != 1) throw std::runtime_error("a seed on the device must be one torch.int64");
+        sd = *seeds;
+    }
+    std::array<Tensor, 3> x, y;
+    std::vector<Tensor> out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const c10::DeviceGuard guard(inputs[0].device());
+        for (size_t k = 0; k < inputs.size(); k++) {
+            x[k] = inputs[k].contiguous();
+            y[k] = at::empty(x[k].sizes(), x[k].options());
+            out.push_back(y[k]);
+        }
+        drop(x, y, q, (uint32_t)seed, sd);
+    }
+    if (grad) {
+        auto node = new_node<DropNode>();
+        node->set_next_edges(collect_next_edges(inputs));
+        node->q = q;
+        node->seed = (uint32_t)seed;
+        if (sd.defined()) node->seeds = SavedVariable(sd, false);
+        set_history(out, node);
+    }
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -567,4 +862,8 @@ PYBIND11_MODULE(_host, m) {
     m.def("bound_sort_neuron_shifted", &bound_sort_neuron_shifted, released());
     m.def("sort_neuron_box_shifted", &sort_neuron_box_shifted, released());
     m.def("unfold", &unfold, released());
+    m.def("label_log_probs", &label_log_probs, released());
+    m.def("preference_loss", &preference_loss, released());
+    m.def("policy_loss", &policy_loss, released());
+    m.def("dropout", &dropout, released());
 }

@@ -1,7 +1,8 @@
 """The reference's SortNet model zoo on top of sortnet_amd.layers / sortnet_amd.heads
 (ell_inf_models.py:18-240): same constructor arguments, same `forward(x, targets, eps, up, down)` contract,
 same sub-module names (`fc_dist`, `fc_linear`, `fc_final`, `scalar`) so that reference checkpoints load.
-Extra keyword `registry`: the DropoutRegistry the distance layers share (default: the process-wide one).
+Extra keywords: `registry`, the DropoutRegistry the distance layers share (default: the process-wide one), and for the models with a
+dense head `head_dropout`, the probability with which a hidden feature is kept in training (default: all are).
 
 forward(x)                              -> logits (training / plain evaluation)
 forward(x, targets, eps)                -> (logits, worst-case margins): radius-eps ball around the distance
@@ -14,7 +15,7 @@ import math
 import torch
 import torch.nn as nn
 
-from .heads import BoundFinalLinear, BoundLinear, BoundTanh
+from .heads import BoundDropout, BoundFinalLinear, BoundLinear, BoundTanh
 from .layers import BoundSequential, NormDist, NormDistBase, NormDistConv, apply_if_not_none
 
 
@@ -79,8 +80,9 @@ class _HybridNet(_SortNet):
     def _pool(z):      # hook between the distance stack and the head
         return z
 
-    def _build_head(self, features, hidden, num_classes, scalar):
+    def _build_head(self, features, hidden, num_classes, scalar, head_dropout, registry):
         self.fc_linear = BoundSequential(BoundLinear(features, hidden, bias=True), BoundTanh())
+        self.head_drop = BoundDropout(head_dropout, registry)
         self.fc_final = BoundFinalLinear(hidden, num_classes, bias=True)
         self.scalar = _make_scalar(scalar)
 
@@ -88,7 +90,7 @@ class _HybridNet(_SortNet):
         paras = apply_if_not_none(self._distance_features(x, eps, up, down), self._pool)
         if targets is not None and (paras[1] is None or paras[2] is None):
             paras = paras[0], paras[0] - eps, paras[0] + eps
-        paras = self.fc_linear(paras)
+        paras = self.head_drop(*self.fc_linear(paras))
         out = self.fc_final(*paras, targets=targets)
         if targets is None:
             return out * self.scalar
@@ -97,14 +99,14 @@ class _HybridNet(_SortNet):
 
 class SortHybridModel(_HybridNet):
     def __init__(self, depth, width, input_dim, hidden=512, num_classes=10, dropout=0.7, std=1.0,
-                 identity_val=None, scalar=True, registry=None):
+                 identity_val=None, scalar=True, registry=None, head_dropout=None):
         super().__init__()
         kw = {"std": std, "identity_val": identity_val, "registry": registry}
         pixels = input_dim[0] * input_dim[1] * input_dim[2]
         stack = [NormDist(pixels, width, bias=False, mean_shift=True, **kw)]
         stack += [NormDist(width, width, bias=False, mean_shift=True, dropout=dropout, **kw) for _ in range(depth - 3)]
         self.fc_dist = BoundSequential(*stack)
-        self._build_head(width, hidden, num_classes, scalar)
+        self._build_head(width, hidden, num_classes, scalar, head_dropout, registry)
 
 
 class SortHybridModel2(_HybridNet):
@@ -115,7 +117,7 @@ class SortHybridModel2(_HybridNet):
     head_inputs_per_channel = 4
 
     def __init__(self, depth, width, input_dim, hidden=512, num_classes=10, dropout=0.7, stride=2, std=1.0,
-                 identity_val=None, scalar=True, registry=None):
+                 identity_val=None, scalar=True, registry=None, head_dropout=None):
         super().__init__()
         kw = {"std": std, "identity_val": identity_val, "registry": registry}
         window = (input_dim[1] - stride, input_dim[2] - stride)
@@ -123,7 +125,7 @@ class SortHybridModel2(_HybridNet):
         stack += [NormDistConv(width, width, 1, bias=False, mean_shift=True, dropout=dropout, **kw)
                   for _ in range(depth - 3)]
         self.fc_dist = BoundSequential(*stack)
-        self._build_head(width * self.head_inputs_per_channel, hidden, num_classes, scalar)
+        self._build_head(width * self.head_inputs_per_channel, hidden, num_classes, scalar, head_dropout, registry)
 
 
 class SortHybridModelAvg(SortHybridModel2):

@@ -19,7 +19,7 @@ from . import ext as _C
 __all__ = [
     "NormDistF", "NormDistDropoutF", "SortNeuronF", "BoundInfDistF", "MaskedInfDistF",
     "norm_dist", "norm_dist_dropout", "sort_neuron", "bound_sort_neuron", "bound_inf_dist", "masked_inf_dist",
-    "MeanShiftF", "mean_shift", "MeanShiftIndexF", "mean_shift_index",
+    "MeanShiftF", "mean_shift", "MeanShiftIndexF", "mean_shift_index", "dropout", "bound_dropout",
 ]
 
 
@@ -282,3 +282,29 @@ def masked_inf_dist(input, weight, q, seed, groups=1, mode=_C.MASK_TERM, tag=Non
     if q is None or q == 1.0:
         return norm_dist(input, weight, float("inf"), groups, tag=tag)
     return MaskedInfDistF.apply(input, weight, groups, q, seed, mode)
+
+
+def _dropped(tensors, q, seed):
+    on_device = isinstance(seed, torch.Tensor)
+    return _C.host().dropout(tensors, q, 0 if on_device else seed & 0xFFFFFFFF, seed if on_device else None)
+
+
+def dropout(input, q, seed):
+    """Keeps every value of `input` (fp32, bf16 or fp16, any shape) with probability q, rounded to 1/65536, and divides what
+    stays by that probability; the mask is a function of (seed, row-major index) and is never stored: the backward makes it
+    again, and so does a call with the same seed.  `seed` is a whole number or one int64 on the input's device; a captured
+    graph replays the mask of a number, and reads a device seed in each replay (change it between replays, not between a
+    forward and its backward).  Dropped values are 0 whatever they were.  q = 1 or None returns the input."""
+    if q is None or q == 1.0:
+        return input
+    return _dropped([input], q, seed)[0]
+
+
+def bound_dropout(x, lower, upper, q, seed):
+    """`dropout` of values and their bounds under one mask, in one launch (None stays None): what stays is scaled by a positive
+    number, so bounds of the input are bounds of the result."""
+    if q is None or q == 1.0:
+        return x, lower, upper
+    there = [t for t in (x, lower, upper) if t is not None]
+    done = iter(_dropped(there, q, seed) if there else ())
+    return tuple(None if t is None else next(done) for t in (x, lower, upper))

@@ -15,7 +15,8 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as TF
 
-from .layers import apply_if_not_none
+from . import functional as F
+from .layers import DEFAULT_REGISTRY, apply_if_not_none
 
 
 class BoundReLU(nn.ReLU):
@@ -26,6 +27,30 @@ class BoundReLU(nn.ReLU):
 class BoundTanh(nn.Tanh):
     def forward(self, x=None, lower=None, upper=None):
         return apply_if_not_none((x, lower, upper), torch.tanh)
+
+
+class BoundDropout(nn.Module):
+    """Dropout of a dense head's features (no counterpart in the reference): in training, values and bounds keep the same entries,
+    each with probability `q`, divided by it; in evaluation, or with q = 1 or None, nothing changes.  The mask is a function of a
+    seed and is never stored.  Seeds come from the registry that the distance layers' lists come from
+    (`layers.set_mask_seed` makes a run reproducible); `last_seed` is that of the latest pass, with which `functional.bound_dropout` makes the
+    same mask again.  A captured graph would replay one mask: `seed`, one int64 on the GPU, is then read in each replay, and is the caller's
+    to change between them."""
+
+    def __init__(self, q, registry=None, seed=None):
+        super().__init__()
+        if q is not None and not 0.0 < q <= 1.0:
+            raise ValueError("BoundDropout: keep probability q=%s outside 0..1" % (q,))
+        self.q, self.registry, self.seed, self.last_seed = q, DEFAULT_REGISTRY if registry is None else registry, seed, None
+
+    def forward(self, x=None, lower=None, upper=None):
+        if not self.training or self.q is None or self.q == 1.0:
+            return x, lower, upper
+        self.last_seed = self.registry.next_seed() if self.seed is None else self.seed
+        return F.bound_dropout(x, lower, upper, self.q, self.last_seed)
+
+    def extra_repr(self):
+        return "q=%s" % (self.q,)
 
 
 def _affine(inp, weight, bias, w_scale, b_scale):

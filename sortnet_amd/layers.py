@@ -62,14 +62,17 @@ class DropoutRegistry:
         self.next_tag += 1
         return self.next_tag
 
+    def next_seed(self):
+        self.draws += 1
+        return (self.seed * 1000003 + self.draws) & 0xFFFFFFFF
+
     def sample(self, sub_batches, groups, channels, q, device, host_paced=False):
         """Ascending kept-channel lists (sub_batches, groups, count), count ~ Binomial(channels, q).
         The lists depend on nothing but the seed, and the sampler keeps only a few compute units busy, so it
         is queued on a second stream (default priority) and overlaps the kernels already queued on the
         caller's stream; the caller's stream waits for it before going on.  With host_paced (the device would be idle
         meanwhile) the lists are drawn on the caller's stream, which spares the host the second one's events."""
-        self.draws += 1
-        seed = (self.seed * 1000003 + self.draws) & 0xFFFFFFFF
+        seed = self.next_seed()
         count = ext.mask_count(seed, channels, q)
         device = torch.device(device)
         if device.type == "cuda" and host_paced:
