@@ -361,15 +361,18 @@ int sd_preference_loss(const sd_label_rows* rows, const float* ref, const void* 
  * all are) of  -min(ratio A, clip(ratio, 1 - clip_low, 1 + clip_high) A) + kl (exp(apart) - apart - 1).
  * Row r's advantage A stands at (r / inner) * advantage_outer + (r % inner) * advantage_inner; ref may be NULL where kl = 0.
  * means (3): the first term, the second without its factor, the share of clipped rows.  stats, weight as above; the gradient is
- * sd_label_gradient with these and `scale` (1), which receives the reciprocal of the number of rows that count. */
+ * sd_label_gradient with these and `scale` (1), which receives the reciprocal of the number of rows that count.  Where sd_policy_fuses(rows)
+ * is 1, `grad` may be given (else NULL): it receives the gradient for an upstream gradient of 1, and the logits are read once less. */
+int sd_policy_fuses(const sd_label_rows* rows);
 int sd_policy_loss(const sd_label_rows* rows, const float* old_log_probs, const float* advantages, int64_t advantage_outer,
                    int64_t advantage_inner, const float* ref, double clip_low, double clip_high, double kl, float* stats, float* weight,
-                   float* scale, float* loss, float* means, float* scratch, sd_stream_t stream);
+                   float* scale, void* grad, float* loss, float* means, float* scratch, sd_stream_t stream);
 
 /* grad[r, v] = weight[r] scale scale2 ([v = label] - softmax(row r)[v]), rows of `classes` values one behind the other, in the logits' type;
- * scale and scale2 (one float each on the device) may be NULL.  Zeros where ignored or where the product is 0. */
+ * scale and scale2 (one float each on the device) may be NULL.  Zeros where ignored or where the product is 0.  With unless_one nothing is
+ * written where *scale2 is 1 (grad holds that gradient already). */
 int sd_label_gradient(const sd_label_rows* rows, const float* stats, const float* weight, const float* scale, const float* scale2,
-                      void* grad, sd_stream_t stream);
+                      int unless_one, void* grad, sd_stream_t stream);
 
 /* Dropout of up to three tensors of n values under one mask (inputs that are not wanted are NULL with their outputs): value i is kept
  * where field i of the generator is below L = floor(65536 q + 0.5), and multiplied by 65536 / L.  The fields of values 2j and 2j + 1 are

@@ -61,8 +61,8 @@ SIGNATURES = {
     "sd_sample_index_lists": [_u, _i, _i, _i, _i, _I, _S],
     "sd_label_log_probs": [_R, _F, _F, _F, _S],
     "sd_preference_loss": [_R, _F, _I, _i, _l, _i, _d, _d, _F, _F, _F, _F, _F, _S],
-    "sd_policy_loss": [_R, _F, _F, _l, _l, _F, _d, _d, _d, _F, _F, _F, _F, _F, _F, _S],
-    "sd_label_gradient": [_R, _F, _F, _F, _F, _F, _S],
+    "sd_policy_loss": [_R, _F, _F, _l, _l, _F, _d, _d, _d, _F, _F, _F, _F, _F, _F, _F, _S],
+    "sd_label_gradient": [_R, _F, _F, _F, _F, _i, _F, _S],
     "sd_dropout": [_F, _F, _F, _i, _l, _d, _u, _I, _F, _F, _F, _S],
 }
 _OTHER = {
@@ -83,6 +83,7 @@ _OTHER = {
     "sd_mask_threshold16": ([_f], _u),
     "sd_mask_count": ([_u, _i, _f], _i),
     "sd_label_scratch": ([_R], _l),
+    "sd_policy_fuses": ([_R], _i),
 }
 
 _lib = None

@@ -614,7 +614,9 @@ Tensor label_scratch(const sd_label_rows& a, const Tensor& like) {
 
 struct LabelNode : Node {
     SavedVariable logits, labels, stats, weight, scale;   // weight, scale: none for plain log probabilities
+    Tensor made;            // the gradient for an upstream gradient of 1, where the forward made it
     int64_t ignore = 0;
+    bool last = false;      // this backward is the graph's last: `made` may be given away
 
     variable_list apply(variable_list&& grads) override {
         const Locked lock(mutex_);
@@ -624,27 +626,32 @@ struct LabelNode : Node {
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor g = incoming(*this, grads, 0);
         const c10::DeviceGuard guard(z.device());
-        out[0] = at::empty(z.sizes(), z.options());
+        // A gradient that is there already is only written again for another upstream gradient than 1, which the device knows; one that a
+        // later backward may want, too, stays as it is.
+        const bool there = made.defined() && last;
+        out[0] = there ? std::move(made) : at::empty(z.sizes(), z.options());
         if (out[0].numel() == 0) return out;
         const sd_label_rows a = label_rows(z, l, ignore);
-        const float* gp = floats(g, "grad_output");
-        if (w.defined())
-            require(sd_label_gradient(&a, floats(st, "stats"), floats(w, "weight"), sc.defined() ? floats(sc, "scale") : nullptr, gp, out[0].data_ptr(), stream_of(z)),
-                    "sd_label_gradient");
-        else
-            require(sd_label_gradient(&a, floats(st, "stats"), gp, nullptr, nullptr, out[0].data_ptr(), stream_of(z)), "sd_label_gradient");
+        const float *gp = floats(g, "grad_output"), *sp = sc.defined() ? floats(sc, "scale") : nullptr;
+        const bool loss = w.defined();      // else the upstream gradient is the rows' weights
+        require(sd_label_gradient(&a, floats(st, "stats"), loss ? floats(w, "weight") : gp, sp, loss ? gp : nullptr, there, out[0].data_ptr(), stream_of(z)), "sd_label_gradient");
         return out;
+    }
+    void will_release_variables() override {
+        const Locked lock(mutex_);
+        last = true;
     }
     void release_variables() override {
         const Locked lock(mutex_);
         logits.reset_data(); labels.reset_data(); stats.reset_data(); weight.reset_data(); scale.reset_data();
+        made.reset();
     }
     std::string name() const override { return "LabelNode"; }
 };
 
 // makes y the output of a node over the logits
 void attach_labels(const Tensor& y, const Tensor& outputs, const Tensor& z, const Tensor& labels, int64_t ignore, const Tensor& stats, const Tensor& weight,
-                   const Tensor& scale) {
+                   const Tensor& scale, const Tensor& made) {
     auto node = new_node<LabelNode>();
     node->set_next_edges(collect_next_edges(outputs));
     node->ignore = ignore;
@@ -653,6 +660,7 @@ void attach_labels(const Tensor& y, const Tensor& outputs, const Tensor& z, cons
     node->stats = SavedVariable(stats, false);
     if (weight.defined()) node->weight = SavedVariable(weight, false);
     if (scale.defined()) node->scale = SavedVariable(scale, false);
+    node->made = made;
     set_history(y, node);
 }
 
@@ -674,7 +682,7 @@ Tensor label_log_probs(const Tensor& outputs, const Tensor& targets, int64_t ign
             require(sd_label_log_probs(&a, floats(y, "log_probs"), grad ? floats(stats, "stats") : nullptr, floats(scratch, "scratch"), stream_of(z)), "sd_label_log_probs");
         }
     }
-    if (grad) attach_labels(y, outputs, z, labels, ignore, stats, {}, {});
+    if (grad) attach_labels(y, outputs, z, labels, ignore, stats, {}, {}, {});
     return y;
 }
 
@@ -717,7 +725,7 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& outputs, const Tensor& t
                                    (int)(answers / 2), beta, smoothing, grad ? floats(stats, "stats") : nullptr, grad ? floats(weight, "weight") : nullptr,
                                    floats(rewards, "rewards"), floats(loss, "loss"), floats(scratch, "scratch"), stream_of(z)), "sd_preference_loss");
     }
-    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, {});
+    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, {}, {});
     return {loss, rewards};
 }
 
@@ -725,7 +733,7 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& outputs, const Tensor& targe
                                       double clip_low, double clip_high, double kl, int64_t ignore) {
     reverse_mode_only("policy_loss", outputs);
     const bool grad = want_grad(outputs);
-    Tensor loss, means, z, labels, stats, weight, scale;
+    Tensor loss, means, z, labels, stats, weight, scale, made;
     {
         element_type(outputs, "outputs");
         const Tensor old = row_constants(old_in, "old_log_probs", targets).detach().contiguous();
@@ -747,12 +755,13 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& outputs, const Tensor& targe
         if (grad) {
             stats = new_floats(z, {labels.numel(), 2});
             weight = new_floats(z, {labels.numel()});
+            if (sd_policy_fuses(&a)) made = at::empty(z.sizes(), z.options());
         }
         require(sd_policy_loss(&a, floats(old, "old_log_probs"), static_cast<const float*>(adv.data_ptr()), outer, inner, ref.defined() ? floats(ref, "ref_log_probs") : nullptr,
                                clip_low, clip_high, kl, grad ? floats(stats, "stats") : nullptr, grad ? floats(weight, "weight") : nullptr, floats(scale, "scale"),
-                               floats(loss, "loss"), floats(means, "means"), floats(scratch, "scratch"), stream_of(z)), "sd_policy_loss");
+                               made.defined() ? made.data_ptr() : nullptr, floats(loss, "loss"), floats(means, "means"), floats(scratch, "scratch"), stream_of(z)), "sd_policy_loss");
     }
-    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, scale);
+    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, scale, made);
     return {loss, means};
 }
 

@@ -7,12 +7,14 @@
 // make a NaN nor count; a row of nothing else has the log probability NaN, as have rows with +inf or NaN.
 // All sums have a fixed order: results are the same in every call.
 #include <cfloat>
+#include <type_traits>
 #include "label_rows.h"
 
 namespace sd {
 
-constexpr int kUnroll = 4;          // 16-byte loads of a work-item that are on their way together
-constexpr int kGroupVecs = 8;       // vectors per lane up to which a row is read by (a part of) one wavefront
+constexpr int kUnroll = 4;          // 16-byte loads of a work-item of a long row that are on their way together
+constexpr int kHeld = 8;            // 16-byte vectors of a short row that a lane holds, at most
+constexpr int kHeldLong = 16 * 1024;    // and of a long row that a workgroup holds
 constexpr int64_t kMostBlocks = 1 << 22;
 
 struct Rows {
@@ -27,14 +29,22 @@ enum { kValues = 0, kPreference = 1, kPolicy = 2 };
 // what happens to a row once its statistics are known
 struct Finish {
     int kind;
-    float* log_probs;       // values, preference
+    float* out;             // values: log probabilities; preference: log probability - ref
     float2* stats;          // (top, 1 / sum), what the gradient needs (or null)
-    float* weight;          // preference: cleared (rows of no answer keep that), policy: d loss_r / d lp
+    float* weight;          // preference: cleared (rows of no answer keep that), policy: d loss_r / d lp (or null)
     float4* terms;          // policy: surrogate, divergence, clipped, kept
     const float *old, *advantage, *ref;
     int64_t advantage_outer, advantage_inner;
     float low, high, kl;
     uint32_t* ticket;       // cleared for the kernel of sums behind this one (or null)
+};
+
+struct Gradient {
+    const float2* stats;
+    const float* weight;
+    const float *scale, *scale2;    // one number each that every weight is multiplied by (or null)
+    void* grad;                     // rows one behind the other
+    bool unless_one;                // nothing is done where *scale2 is 1
 };
 
 template <class T> __device__ __forceinline__ const T* row_start(const Rows& a, int64_t r) {
@@ -44,6 +54,206 @@ template <class T> __device__ __forceinline__ const T* row_start(const Rows& a, 
 
 __device__ __forceinline__ float finite(float top) { return fmaxf(top, -FLT_MAX); }
 
+// ---- a row's end: one work-item per row ------------------------------------------------------------------------------------
+// What it needs besides (top, sum), loaded before the row is read, so that the loads run beside it.
+struct Given { int64_t label; float at, old, advantage, ref; };
+
+template <class T> __device__ __forceinline__ Given given(const Rows& a, const Finish& e, int64_t r, int64_t label) {
+    Given g{label, __builtin_nanf(""), 0.f, 0.f, 0.f};      // a label that names no class has no log probability
+    if (label == a.ignore) return g;
+    if (label >= 0 && label < a.classes) g.at = Elem<T>::get(row_start<T>(a, r)[label]);
+    if (e.kind == kPolicy) {
+        const uint32_t o = (uint32_t)r / a.inner, i = (uint32_t)r - o * a.inner;
+        g.advantage = e.advantage[o * e.advantage_outer + i * e.advantage_inner];
+        g.old = e.old[r];
+    }
+    if (e.ref) g.ref = e.ref[r];
+    return g;
+}
+
+struct End { float top, inverse, weight; };
+
+__device__ __forceinline__ End finish_row(const Rows& a, const Finish& e, int64_t r, const Given& g, float top, float sum) {
+    const bool kept = g.label != a.ignore;
+    top = finite(top);
+    End end{kept ? top : 0.f, 1.f / sum, 0.f};
+    const float lp = kept ? g.at - top - logf(sum) : 0.f;
+    if (e.stats) e.stats[r] = make_float2(end.top, end.inverse);
+    if (e.kind != kPolicy) {
+        e.out[r] = kept ? lp - g.ref : 0.f;
+        if (e.weight) e.weight[r] = 0.f;
+        return end;
+    }
+    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (kept) {
+        const float ratio = expf(lp - g.old);
+        const float held = ratio < e.low ? e.low : ratio > e.high ? e.high : ratio;
+        const float free = ratio * g.advantage, bounded = held * g.advantage;
+        const bool clipped = bounded < free;
+        t.x = -(clipped ? bounded : free);
+        t.z = clipped ? 1.f : 0.f;
+        t.w = 1.f;
+        end.weight = clipped ? 0.f : -free;
+        if (e.kl != 0.f) {
+            const float apart = g.ref - lp, grown = expm1f(apart);
+            t.y = grown - apart;
+            end.weight -= e.kl * grown;
+        }
+    }
+    e.terms[r] = t;
+    if (e.weight) e.weight[r] = end.weight;
+    return end;
+}
+
+// the weight of a row's gradient
+__device__ __forceinline__ float scaled(const Gradient& g, float w) {
+    if (g.scale) w *= *g.scale;
+    if (g.scale2) w *= *g.scale2;
+    return w;
+}
+
+__device__ __forceinline__ float row_weight(const Rows& a, const Gradient& g, int64_t r, int64_t label) {
+    if (label == a.ignore) return 0.f;
+    if (label < 0 || label >= a.classes) return __builtin_nanf("");
+    return scaled(g, g.weight[r]);
+}
+
+// N values from column c on become their gradients (a label that names no class, whose low half may name one, has w = NaN)
+template <class T, int N> __device__ __forceinline__ void slopes(float (&f)[N], float top, float inverse, float w, int c, int label) {
+    #pragma unroll
+    for (int i = 0; i < N; i++) f[i] = -(Elem<T>::exp(f[i] - top) * inverse) * w;
+    const uint32_t at = (uint32_t)label - (uint32_t)c;
+    if (at < N) {
+        #pragma unroll
+        for (int i = 0; i < N; i++) f[i] += i == (int)at ? w : 0.f;
+    }
+}
+
+// ---- short rows: 2^shift lanes of a wavefront hold a row in registers, NV vectors each ---------------------------------------
+// The last vector of a row of at least one ends with the row and overlaps the one before it; a shorter row is one vector, padded with -inf.
+template <class T, int NV> struct Held {
+    static constexpr int V = Elem<T>::kVec;
+    u32x4 v[NV];
+    int n, vecs, lane, shift;
+
+    __device__ __forceinline__ int index(int k) const { return lane + (k << shift); }
+    __device__ __forceinline__ int column(int i) const { return i * V + V <= n ? i * V : n - V; }     // (n >= V)
+
+    __device__ __forceinline__ void load(const T* p) {
+        if (n >= V) {
+            #pragma unroll
+            for (int k = 0; k < NV; k++)
+                if (index(k) < vecs) v[k] = load16(p + column(index(k)));
+        } else if (lane == 0) {
+            float f[V];
+            #pragma unroll
+            for (int i = 0; i < V; i++) f[i] = i < n ? Elem<T>::get(p[i]) : -INFINITY;
+            v[0] = Elem<T>::pack(f);
+        }
+    }
+    __device__ __forceinline__ float top() const {
+        float t = -INFINITY;
+        #pragma unroll
+        for (int k = 0; k < NV; k++)
+            if (index(k) < vecs) {
+                float f[V];
+                Elem<T>::unpack(v[k], f);
+                #pragma unroll
+                for (int i = 0; i < V; i++) t = fmaxf(t, f[i]);
+            }
+        for (int o = (1 << shift) >> 1; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
+        return t;
+    }
+    __device__ __forceinline__ float sum(float top) const {
+        const float b = finite(top);
+        float s = 0.f;
+        #pragma unroll
+        for (int k = 0; k < NV; k++)
+            if (index(k) < vecs) {
+                const int past = n >= V ? index(k) * V - column(index(k)) : 0;      // values that the vector before has, too
+                float f[V];
+                Elem<T>::unpack(v[k], f);
+                #pragma unroll
+                for (int i = 0; i < V; i++) f[i] = Elem<T>::exp(f[i] - b);
+                if (past > 0) {
+                    #pragma unroll
+                    for (int i = 0; i < V; i++) f[i] = i < past ? 0.f : f[i];
+                }
+                #pragma unroll
+                for (int i = 0; i < V; i++) s += f[i];
+            }
+        for (int o = (1 << shift) >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
+        return s;
+    }
+    // the gradient of weight w; zeros, without a look at the values, where that is 0
+    __device__ __forceinline__ void gradient(T* q, float top, float inverse, float w, int label) const {
+        #pragma unroll
+        for (int k = 0; k < NV; k++)
+            if (index(k) < vecs) {
+                const int c = n >= V ? column(index(k)) : 0;
+                float f[V];
+                if (w == 0.f) {
+                    #pragma unroll
+                    for (int i = 0; i < V; i++) f[i] = 0.f;
+                } else {
+                    Elem<T>::unpack(v[k], f);
+                    slopes<T>(f, top, inverse, w, c, label);
+                }
+                if (n >= V) store16(q + c, Elem<T>::pack(f));
+                else {
+                    #pragma unroll
+                    for (int i = 0; i < V; i++)
+                        if (i < n) q[i] = Elem<T>::put(f[i]);
+                }
+            }
+    }
+};
+
+// FUSED: the gradient leaves with the row (its scale is known before: the reciprocal of the number of rows that count)
+template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) label_rows_kernel(Rows a, Finish e, Gradient g, int shift) {
+    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
+    const int per = 256 >> shift;
+    Held<T, NV> row;
+    row.n = (int)a.classes; row.shift = shift;
+    row.lane = threadIdx.x & ((1 << shift) - 1);
+    row.vecs = (row.n + Elem<T>::kVec - 1) / Elem<T>::kVec;
+    for (int64_t r = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); r < a.rows; r += (int64_t)gridDim.x * per) {
+        const int64_t label = a.labels[r];
+        Given in{label, 0.f, 0.f, 0.f, 0.f};
+        float top = 0.f, sum = 1.f;
+        if (label != a.ignore) {
+            row.load(row_start<T>(a, r));
+            if (row.lane == 0) in = given<T>(a, e, r, label);
+            top = row.top();
+            sum = row.sum(top);
+        }
+        End end{0.f, 0.f, 0.f};
+        if (row.lane == 0) end = finish_row(a, e, r, in, top, sum);
+        if (FUSED) {
+            const int lead = (threadIdx.x & 63) - row.lane;
+            const float w = scaled(g, __shfl(end.weight, lead));
+            row.gradient(static_cast<T*>(g.grad) + r * a.classes, __shfl(end.top, lead), __shfl(end.inverse, lead), w, (int)label);
+        }
+    }
+}
+
+template <class T, int NV> __global__ void __launch_bounds__(256) label_gradient_kernel(Rows a, Gradient g, int shift) {
+    if (g.unless_one && *g.scale2 == 1.f) return;
+    const int per = 256 >> shift;
+    Held<T, NV> row;
+    row.n = (int)a.classes; row.shift = shift;
+    row.lane = threadIdx.x & ((1 << shift) - 1);
+    row.vecs = (row.n + Elem<T>::kVec - 1) / Elem<T>::kVec;
+    for (int64_t r = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); r < a.rows; r += (int64_t)gridDim.x * per) {
+        const int64_t label = a.labels[r];
+        const float w = row_weight(a, g, r, label);
+        const float2 st = g.stats[r];
+        if (w != 0.f) row.load(row_start<T>(a, r));
+        row.gradient(static_cast<T*>(g.grad) + r * a.classes, st.x, st.y, w, (int)label);
+    }
+}
+
+// ---- long rows: a workgroup reads a row, or one of its parts ------------------------------------------------------------------
 // (top, sum) of two parts of a row
 template <class T> __device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2) {
     const float t = fmaxf(top, top2);
@@ -61,6 +271,19 @@ template <class T, int N> __device__ __forceinline__ void take(const float (&f)[
     for (int i = 0; i < N; i++) s += Elem<T>::exp(f[i] - b);
     top = t;
     sum = s;
+}
+
+// of all work-items of a workgroup, to its first
+template <class T, int WAVES> __device__ __forceinline__ void join_workgroup(float& top, float& sum, float2* waves) {
+    for (int o = 32; o > 0; o >>= 1) {
+        const float t = __shfl_xor(top, o), s = __shfl_xor(sum, o);
+        join<T>(top, sum, t, s);
+    }
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(top, sum);
+    __syncthreads();
+    if (threadIdx.x == 0)
+        for (int k = 1; k < WAVES; k++) join<T>(top, sum, waves[k].x, waves[k].y);
+    __syncthreads();        // (waves is written again)
 }
 
 // (top, sum) of this work-item's share of p[0 .. n), which `lanes` work-items read together
@@ -88,148 +311,23 @@ template <class T> __device__ __forceinline__ void scan(const T* p, int64_t n, i
     }
 }
 
-// one work-item per row, with the row's top and sum
-template <class T> __device__ void finish_row(const Rows& a, const Finish& e, int64_t r, float top, float sum) {
-    const int64_t label = a.labels[r];
-    const bool kept = label != a.ignore, known = label >= 0 && label < a.classes;
-    float lp = 0.f;
-    if (kept) {
-        top = finite(top);
-        // a label that names no class has no log probability
-        lp = known ? Elem<T>::get(row_start<T>(a, r)[label]) - top - logf(sum) : __builtin_nanf("");
-    }
-    if (e.stats) e.stats[r] = make_float2(top, 1.f / sum);
-    if (e.kind != kPolicy) {
-        e.log_probs[r] = lp;
-        if (e.weight) e.weight[r] = 0.f;
-        return;
-    }
-    float4 t = make_float4(0.f, 0.f, 0.f, 0.f);
-    float w = 0.f;
-    if (kept) {
-        const uint32_t o = (uint32_t)r / a.inner, i = (uint32_t)r - o * a.inner;
-        const float adv = e.advantage[o * e.advantage_outer + i * e.advantage_inner];
-        const float ratio = expf(lp - e.old[r]);
-        const float held = ratio < e.low ? e.low : ratio > e.high ? e.high : ratio;
-        const float free = ratio * adv, bounded = held * adv;
-        const bool clipped = bounded < free;
-        t.x = -(clipped ? bounded : free);
-        t.z = clipped ? 1.f : 0.f;
-        t.w = 1.f;
-        w = clipped ? 0.f : -free;
-        if (e.kl != 0.f) {
-            const float apart = e.ref[r] - lp, grown = expm1f(apart);
-            t.y = grown - apart;
-            w -= e.kl * grown;
-        }
-    }
-    e.terms[r] = t;
-    if (e.weight) e.weight[r] = w;
-}
-
-// Rows of up to kGroupVecs vectors per lane of a wavefront: 2^shift lanes to a row.
-template <class T> __global__ void __launch_bounds__(256) label_rows_kernel(Rows a, Finish e, int shift) {
-    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
-    const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1), per = 256 >> shift;
-    for (int64_t r = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); r < a.rows; r += (int64_t)gridDim.x * per) {
-        float top = -INFINITY, sum = 0.f;
-        if (a.labels[r] != a.ignore) scan(row_start<T>(a, r), a.classes, lane, lanes, top, sum);
-        else top = 0.f, sum = 1.f;
-        for (int o = lanes >> 1; o > 0; o >>= 1) {
-            const float t = __shfl_xor(top, o), s = __shfl_xor(sum, o);
-            join<T>(top, sum, t, s);
-        }
-        if (lane == 0) finish_row<T>(a, e, r, top, sum);
-    }
-}
-
-// Longer rows: a workgroup per row, or per one of `splits` parts of a row, which then leaves its (top, sum) for join_rows_kernel.
-template <class T> __global__ void __launch_bounds__(256) label_long_rows_kernel(Rows a, Finish e, int splits, int64_t part, float2* parts) {
-    __shared__ float2 waves[4];
-    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
-        const int64_t r = splits == 1 ? b : b / splits, c0 = (b - r * splits) * part;
-        const int64_t n = a.classes - c0 < part ? a.classes - c0 : part;
-        float top = -INFINITY, sum = 0.f;
-        const bool kept = a.labels[r] != a.ignore;      // (the whole workgroup's)
-        if (kept) {
-            scan(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
-            for (int o = 32; o > 0; o >>= 1) {
-                const float t = __shfl_xor(top, o), s = __shfl_xor(sum, o);
-                join<T>(top, sum, t, s);
-            }
-            if (lane == 0) waves[wave] = make_float2(top, sum);
-            __syncthreads();
-            if (threadIdx.x == 0)
-                for (int k = 1; k < 4; k++) join<T>(top, sum, waves[k].x, waves[k].y);
-            __syncthreads();
-        } else top = 0.f, sum = 1.f;
-        if (threadIdx.x == 0) {
-            if (splits == 1) finish_row<T>(a, e, r, top, sum);
-            else parts[b] = make_float2(top, sum);
-        }
-    }
-}
-
-// a wavefront per row joins the parts of label_long_rows_kernel
-template <class T> __global__ void __launch_bounds__(256) join_rows_kernel(Rows a, Finish e, int splits, const float2* parts) {
-    const int lane = threadIdx.x & 63;
-    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
-        float top = -INFINITY, sum = 0.f;
-        if (a.labels[r] != a.ignore) {
-            for (int k = lane; k < splits; k += 64) join<T>(top, sum, parts[r * splits + k].x, parts[r * splits + k].y);
-            for (int o = 32; o > 0; o >>= 1) {
-                const float t = __shfl_xor(top, o), s = __shfl_xor(sum, o);
-                join<T>(top, sum, t, s);
-            }
-        } else top = 0.f, sum = 1.f;
-        if (lane == 0) finish_row<T>(a, e, r, top, sum);
-    }
-}
-
-// ---- gradient ------------------------------------------------------------------------------------------------------------
-struct Gradient {
-    const float2* stats;
-    const float* weight;
-    const float *scale, *scale2;    // one number each that every weight is multiplied by (or null)
-    void* grad;                     // rows one behind the other
-};
-
-__device__ __forceinline__ float row_weight(const Rows& a, const Gradient& g, int64_t r, int64_t label) {
-    if (label == a.ignore) return 0.f;
-    if (label < 0 || label >= a.classes) return __builtin_nanf("");
-    float w = g.weight[r];
-    if (g.scale) w *= *g.scale;
-    if (g.scale2) w *= *g.scale2;
-    return w;
-}
-
-// N values from column c on
-template <class T, int N> __device__ __forceinline__ void slopes(float (&f)[N], float2 st, float w, int64_t c, int64_t label) {
-    #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = -(Elem<T>::exp(f[i] - st.x) * st.y) * w;
-    const uint64_t at = (uint64_t)(label - c);
-    if (at < N) {
-        #pragma unroll
-        for (int i = 0; i < N; i++) f[i] += i == (int)at ? w : 0.f;
-    }
+// zeros in a row of a gradient, by a whole workgroup
+template <class T> __device__ __forceinline__ void clear_row(T* q, int n, int threads) {
+    constexpr int V = Elem<T>::kVec;
+    const int full = n / V;
+    for (int i = threadIdx.x; i < full; i += threads) store16(q + i * V, u32x4{0u, 0u, 0u, 0u});
+    for (int j = full * V + threadIdx.x; j < n; j += threads) q[j] = T{};
 }
 
 // columns [c0, c1) of a row, c0 a multiple of the vector's length; a row of weight 0 (ignored, clipped, or of no answer) is not read
-template <class T> __device__ __forceinline__ void grad_row(const Rows& a, const Gradient& g, int64_t r, int64_t c0, int64_t c1, int lane, int lanes) {
+template <class T> __device__ __forceinline__ void grad_row(const T* src, T* dst, float top, float inverse, float w, int label, int64_t c0, int64_t c1, int lane, int lanes) {
     constexpr int V = Elem<T>::kVec;
-    const int64_t label = a.labels[r];
-    const float w = row_weight(a, g, r, label);
-    const T* src = row_start<T>(a, r);
-    T* dst = static_cast<T*>(g.grad) + r * a.classes;
     const int64_t full = c1 / V;
     if (w == 0.f) {
         for (int64_t i = c0 / V + lane; i < full; i += lanes) store16(dst + i * V, u32x4{0u, 0u, 0u, 0u});
         for (int64_t j = full * V + lane; j < c1; j += lanes) dst[j] = T{};
         return;
     }
-    const float2 st = g.stats[r];
     int64_t i = c0 / V + lane;
     for (; i + (int64_t)(kUnroll - 1) * lanes < full; i += (int64_t)kUnroll * lanes) {
         u32x4 v[kUnroll];
@@ -240,33 +338,144 @@ template <class T> __device__ __forceinline__ void grad_row(const Rows& a, const
             const int64_t c = (i + (int64_t)k * lanes) * V;
             float f[V];
             Elem<T>::unpack(v[k], f);
-            slopes<T>(f, st, w, c, label);
+            slopes<T>(f, top, inverse, w, (int)c, label);
             store16(dst + c, Elem<T>::pack(f));
         }
     }
     for (; i < full; i += lanes) {
         float f[V];
         Elem<T>::unpack(load16(src + i * V), f);
-        slopes<T>(f, st, w, i * V, label);
+        slopes<T>(f, top, inverse, w, (int)(i * V), label);
         store16(dst + i * V, Elem<T>::pack(f));
     }
     for (int64_t j = full * V + lane; j < c1; j += lanes) {
         float f[1] = {Elem<T>::get(src[j])};
-        slopes<T>(f, st, w, j, label);
+        slopes<T>(f, top, inverse, w, (int)j, label);
         dst[j] = Elem<T>::put(f[0]);
     }
 }
 
-template <class T> __global__ void __launch_bounds__(256) label_gradient_kernel(Rows a, Gradient g, int shift) {
-    const int lanes = 1 << shift, lane = threadIdx.x & (lanes - 1), per = 256 >> shift;
-    for (int64_t r = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); r < a.rows; r += (int64_t)gridDim.x * per)
-        grad_row<T>(a, g, r, 0, a.classes, lane, lanes);
+// A workgroup per row, or per one of `splits` parts of a row, which then leaves its (top, sum) for join_rows_kernel.
+template <class T> __global__ void __launch_bounds__(256) label_long_rows_kernel(Rows a, Finish e, int splits, int64_t part, float2* parts) {
+    __shared__ float2 waves[4];
+    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
+    for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
+        const int64_t r = splits == 1 ? b : b / splits, c0 = (b - r * splits) * part;
+        const int64_t n = a.classes - c0 < part ? a.classes - c0 : part;
+        float top = 0.f, sum = 1.f;
+        const int64_t label = a.labels[r];
+        Given in{label, 0.f, 0.f, 0.f, 0.f};
+        if (label != a.ignore) {        // (the whole workgroup's)
+            if (threadIdx.x == 0 && splits == 1) in = given<T>(a, e, r, label);
+            top = -INFINITY; sum = 0.f;
+            scan(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
+            join_workgroup<T, 4>(top, sum, waves);
+        }
+        if (threadIdx.x == 0) {
+            if (splits > 1) parts[b] = make_float2(top, sum);
+            else finish_row(a, e, r, in, top, sum);
+        }
+    }
 }
 
+// FUSED long rows: the workgroup holds the row in its registers, at most 16 vectors per work-item, so that the logits are read once and
+// the gradient leaves with the statistics.  (Reading the row again from the caches instead lost: eight rows of 256 KiB per compute
+// unit are more than the last level holds, 4096 x 131072 bf16 596 us; two passes of their own 515.)
+template <class T, int NV, int THREADS> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
+    constexpr int V = Elem<T>::kVec, kChunk = 16 / V;
+    __shared__ float2 waves[THREADS / 64];
+    __shared__ End row_end;
+    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
+    const int n = (int)a.classes, full = n / V, rest = full * V + (int)threadIdx.x;     // the values behind the last whole vector: one per work-item
+    const T lowest = Elem<T>::put(-INFINITY);
+    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const int64_t label = a.labels[r];
+        T* q = static_cast<T*>(g.grad) + r * a.classes;
+        if (label == a.ignore) {        // (the whole workgroup's)
+            if (threadIdx.x == 0) finish_row(a, e, r, Given{label, 0.f, 0.f, 0.f, 0.f}, 0.f, 1.f);
+            clear_row(q, n, THREADS);
+            continue;
+        }
+        const T* p = row_start<T>(a, r);
+        u32x4 v[NV];
+        const u32x4 none = Elem<T>::splat(lowest);
+        T last = lowest;
+        #pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int i = (int)threadIdx.x + k * THREADS;
+            v[k] = none;
+            if (i < full) v[k] = load16(p + i * V);
+        }
+        if (rest < n) last = p[rest];
+        Given in{label, 0.f, 0.f, 0.f, 0.f};
+        if (threadIdx.x == 0) in = given<T>(a, e, r, label);
+        float top = -INFINITY, sum = 0.f;
+        #pragma unroll
+        for (int c = 0; c < NV; c += kChunk) {
+            float f[kChunk * V];
+            #pragma unroll
+            for (int k = 0; k < kChunk; k++) Elem<T>::unpack(v[c + k], reinterpret_cast<float (&)[V]>(f[k * V]));
+            take<T>(f, top, sum);
+        }
+        const float f1[1] = {Elem<T>::get(last)};
+        take<T>(f1, top, sum);
+        join_workgroup<T, THREADS / 64>(top, sum, waves);
+        if (threadIdx.x == 0) row_end = finish_row(a, e, r, in, top, sum);
+        __syncthreads();
+        const End end = row_end;
+        __syncthreads();    // (row_end is written again)
+        const float w = scaled(g, end.weight);
+        if (w == 0.f) { clear_row(q, n, THREADS); continue; }
+        // What was derived from the vectors above is derived again: kept, it would be twice the registers that there are.
+        int item = threadIdx.x;
+        asm("" : "+v"(item));
+        #pragma unroll
+        for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
+        #pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const int i = item + k * THREADS;
+            float f[V];
+            Elem<T>::unpack(v[k], f);
+            slopes<T>(f, end.top, end.inverse, w, i * V, (int)label);
+            if (i < full) store16(q + i * V, Elem<T>::pack(f));
+        }
+        if (rest < n) {
+            float f[1] = {Elem<T>::get(last)};
+            slopes<T>(f, end.top, end.inverse, w, rest, (int)label);
+            q[rest] = Elem<T>::put(f[0]);
+        }
+    }
+}
+
+// a wavefront per row joins the parts of label_long_rows_kernel
+template <class T> __global__ void __launch_bounds__(256) join_rows_kernel(Rows a, Finish e, int splits, const float2* parts) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
+        const int64_t label = a.labels[r];
+        Given in{label, 0.f, 0.f, 0.f, 0.f};
+        float top = 0.f, sum = 1.f;
+        if (label != a.ignore) {
+            if (lane == 0) in = given<T>(a, e, r, label);
+            top = -INFINITY; sum = 0.f;
+            for (int k = lane; k < splits; k += 64) join<T>(top, sum, parts[r * splits + k].x, parts[r * splits + k].y);
+            for (int o = 32; o > 0; o >>= 1) {
+                const float t = __shfl_xor(top, o), s = __shfl_xor(sum, o);
+                join<T>(top, sum, t, s);
+            }
+        }
+        if (lane == 0) finish_row(a, e, r, in, top, sum);
+    }
+}
+
+// Rows and parts from the last to the first: what the pass before read last is still in the caches.
 template <class T> __global__ void __launch_bounds__(256) label_long_gradient_kernel(Rows a, Gradient g, int splits, int64_t part) {
-    for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
+    if (g.unless_one && *g.scale2 == 1.f) return;
+    for (int64_t b = a.rows * splits - 1 - blockIdx.x; b >= 0; b -= gridDim.x) {
         const int64_t r = b / splits, c0 = (b - r * splits) * part;
-        grad_row<T>(a, g, r, c0, a.classes - c0 < part ? a.classes : c0 + part, threadIdx.x, 256);
+        const int64_t label = a.labels[r];
+        const float2 st = g.stats[r];
+        grad_row<T>(row_start<T>(a, r), static_cast<T*>(g.grad) + r * a.classes, st.x, st.y, row_weight(a, g, r, label), (int)label, c0, a.classes - c0 < part ? a.classes : c0 + part,
+                    threadIdx.x, 256);
     }
 }
 
@@ -293,9 +502,8 @@ __device__ __forceinline__ double published(const double* p) { return __hip_atom
 __device__ __forceinline__ void publish(double* p, double v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
 struct Pairs {
-    const float *log_probs, *ref;
-    const int64_t* labels;
-    int64_t ignore, rows, tokens;
+    const float* ratios;            // log probability - ref of each row, 0 where ignored
+    int64_t rows, tokens;
     const int *offsets32;           // where the answers start and the last one ends; both null: `tokens` rows to an answer
     const int64_t* offsets64;
     int pairs;
@@ -310,48 +518,69 @@ __device__ __forceinline__ int64_t answer_start(const Pairs& a, int64_t k) {
     return at < 0 ? 0 : at > a.rows ? a.rows : at;
 }
 
-// A wavefront per pair: x = beta (chosen - rejected), the sums of lp - ref over the rows of the two answers, in 64 bits; then the
-// pair's loss and the weight of its rows.
-__global__ void __launch_bounds__(256) preference_kernel(Pairs a) {
-    __shared__ double waves[4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// WAVES wavefronts per pair: x = beta (chosen - rejected), the sums of lp - ref over the rows of the two answers, in 64 bits; then the
+// pair's loss and the weight of its rows.  The workgroups' sums are added in order by the last one.
+template <int WAVES> __global__ void __launch_bounds__(256) preference_kernel(Pairs a) {
+    __shared__ double waves[4], sums[2][4];
+    constexpr int kPairs = 4 / WAVES, kLanes = 64 * WAVES;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, item = threadIdx.x & (kLanes - 1);
     double loss = 0.0;
-    for (int64_t pair = (int64_t)blockIdx.x * 4 + wave; pair < a.pairs; pair += (int64_t)gridDim.x * 4) {
-        double reward[2];
-        int64_t from[2], until[2];
-        #pragma unroll
-        for (int k = 0; k < 2; k++) {
-            from[k] = answer_start(a, pair + k * (int64_t)a.pairs);
-            until[k] = answer_start(a, pair + k * (int64_t)a.pairs + 1);
-            double s = 0.0;
-            #pragma unroll 4
-            for (int64_t r = from[k] + lane; r < until[k]; r += 64)
-                if (a.labels[r] != a.ignore) s += (double)(a.log_probs[r] - a.ref[r]);
-            reward[k] = a.beta * wave_total(s);
-            if (lane == 0) a.rewards[pair + k * (int64_t)a.pairs] = (float)reward[k];
-        }
-        const double x = reward[0] - reward[1], small = exp(-fabs(x)), tail = log1p(small);
-        // -log sigma(x) = max(-x, 0) + log(1 + exp(-|x|))
-        double l = (1.0 - a.smoothing) * ((x < 0.0 ? -x : 0.0) + tail);
-        if (a.smoothing != 0.0) l += a.smoothing * ((x > 0.0 ? x : 0.0) + tail);
-        loss += l;
-        const double up = (x < 0.0 ? small : 1.0) / (1.0 + small), down = (x < 0.0 ? 1.0 : small) / (1.0 + small);   // sigma(x), sigma(-x)
-        const float slope = (float)(-a.beta / a.pairs * ((1.0 - a.smoothing) * down - a.smoothing * up));
-        if (a.weight) {
+    for (int64_t p0 = (int64_t)blockIdx.x * kPairs; p0 < a.pairs; p0 += (int64_t)gridDim.x * kPairs) {
+        const int64_t pair = p0 + wave / WAVES;
+        const bool here = pair < a.pairs;
+        double s[2] = {0.0, 0.0};
+        int64_t from[2] = {0, 0}, until[2] = {0, 0};
+        if (here) {
             #pragma unroll
-            for (int k = 0; k < 2; k++)
-                for (int64_t r = from[k] + lane; r < until[k]; r += 64)
-                    if (a.labels[r] != a.ignore) a.weight[r] = k ? -slope : slope;
+            for (int k = 0; k < 2; k++) {
+                from[k] = answer_start(a, pair + k * (int64_t)a.pairs);
+                until[k] = answer_start(a, pair + k * (int64_t)a.pairs + 1);
+            }
+            #pragma unroll
+            for (int k = 0; k < 2; k++) {
+                #pragma unroll 4
+                for (int64_t r = from[k] + item; r < until[k]; r += kLanes) s[k] += (double)a.ratios[r];
+            }
+        }
+        s[0] = wave_total(s[0]); s[1] = wave_total(s[1]);
+        if (WAVES > 1) {
+            if (lane == 0) { sums[0][wave] = s[0]; sums[1][wave] = s[1]; }
+            __syncthreads();
+            #pragma unroll
+            for (int k = 0; k < 2; k++) s[k] = sums[k][0] + sums[k][1] + sums[k][2] + sums[k][3];
+            __syncthreads();
+        }
+        if (here) {
+            const double chosen = a.beta * s[0], rejected = a.beta * s[1];
+            const double x = chosen - rejected, small = exp(-fabs(x)), tail = log1p(small);
+            // -log sigma(x) = max(-x, 0) + log(1 + exp(-|x|))
+            double l = (1.0 - a.smoothing) * ((x < 0.0 ? -x : 0.0) + tail);
+            if (a.smoothing != 0.0) l += a.smoothing * ((x > 0.0 ? x : 0.0) + tail);
+            if (item == 0) {
+                a.rewards[pair] = (float)chosen;
+                a.rewards[pair + a.pairs] = (float)rejected;
+                loss += l;
+            }
+            if (a.weight) {
+                const double up = (x < 0.0 ? small : 1.0) / (1.0 + small), down = (x < 0.0 ? 1.0 : small) / (1.0 + small);   // sigma(x), sigma(-x)
+                const float slope = (float)(-a.beta / a.pairs * ((1.0 - a.smoothing) * down - a.smoothing * up));
+                #pragma unroll
+                for (int k = 0; k < 2; k++)
+                    for (int64_t r = from[k] + item; r < until[k]; r += kLanes) a.weight[r] = k ? -slope : slope;   // (ignored rows have none whatever stands here)
+            }
         }
     }
     if (lane == 0) waves[wave] = loss;
     __syncthreads();
-    if (threadIdx.x == 0) publish(a.parts + blockIdx.x, waves[0] + waves[1] + waves[2] + waves[3]);
-    if (!last_workgroup(a.ticket) || wave != 0) return;
-    double total = 0.0;
-    for (int k = lane; k < (int)gridDim.x; k += 64) total += published(a.parts + k);
-    total = wave_total(total);
-    if (lane == 0) *a.loss = (float)(total / a.pairs);
+    loss = waves[0] + waves[1] + waves[2] + waves[3];
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) publish(a.parts + blockIdx.x, loss);
+        if (!last_workgroup(a.ticket) || wave != 0) return;
+        loss = 0.0;
+        for (int k = lane; k < (int)gridDim.x; k += 64) loss += published(a.parts + k);
+        loss = wave_total(loss);
+    }
+    if (threadIdx.x == 0) *a.loss = (float)(loss / a.pairs);
 }
 
 // Means of the policy's terms over the kept rows (over one where there are none); `scale` = 1 / that number.
@@ -371,24 +600,43 @@ __global__ void __launch_bounds__(256) policy_sums_kernel(const float4* terms, i
         if (lane == 0) waves[wave][k] = s[k];
     }
     __syncthreads();
-    if (threadIdx.x == 0) {
-        #pragma unroll
-        for (int k = 0; k < 4; k++) publish(parts + 4 * blockIdx.x + k, waves[0][k] + waves[1][k] + waves[2][k] + waves[3][k]);
-    }
-    if (!last_workgroup(ticket) || wave != 0) return;
     #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        s[k] = 0.0;
-        for (int b = lane; b < (int)gridDim.x; b += 64) s[k] += published(parts + 4 * b + k);
-        s[k] = wave_total(s[k]);
+    for (int k = 0; k < 4; k++) s[k] = waves[0][k] + waves[1][k] + waves[2][k] + waves[3][k];
+    if (gridDim.x > 1) {
+        if (threadIdx.x == 0) {
+            #pragma unroll
+            for (int k = 0; k < 4; k++) publish(parts + 4 * blockIdx.x + k, s[k]);
+        }
+        if (!last_workgroup(ticket) || wave != 0) return;
+        #pragma unroll
+        for (int k = 0; k < 4; k++) {
+            s[k] = 0.0;
+            for (int b = lane; b < (int)gridDim.x; b += 64) s[k] += published(parts + 4 * b + k);
+            s[k] = wave_total(s[k]);
+        }
     }
-    if (lane == 0) {
+    if (threadIdx.x == 0) {
         const double count = s[3] > 1.0 ? s[3] : 1.0;
         *loss = (float)((s[0] + kl * s[1]) / count);
         stats[0] = (float)(s[0] / count);
         stats[1] = (float)(s[1] / count);
         stats[2] = (float)(s[2] / count);
-        *scale = (float)(1.0 / count);
+        if (scale) *scale = (float)(1.0 / count);
+    }
+}
+
+// `scale` = 1 / the number of rows that count, before the rows are read (sums of whole numbers: the order does not matter)
+__global__ void __launch_bounds__(1024) count_rows_kernel(const int64_t* labels, int64_t rows, int64_t ignore, float* scale) {
+    __shared__ int waves[16];
+    int n = 0;
+    #pragma unroll 8
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) n += labels[r] != ignore ? 1 : 0;
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int k = 1; k < 16; k++) n += waves[k];
+        *scale = (float)(1.0 / (n > 1 ? n : 1));
     }
 }
 
@@ -399,13 +647,27 @@ constexpr int kPairBlocks = 256, kSumBlocks = 128;
 
 int vec_of(int dtype) { return dtype == SD_FLOAT32 ? 4 : 8; }
 
-// lanes of a wavefront that read a row together (as a power of two), or -1: a row is read by whole workgroups
-int group_shift(int64_t classes, int vec) {
+// Lanes of a wavefront that hold a row together (as a power of two) and vectors that each holds; shift = -1: a row is read by whole workgroups.
+// Many rows want few lanes with several vectors each (fewer steps to add up lanes per row), few rows one vector per lane.
+struct Group { int shift, vectors; };
+Group group_of(int64_t rows, int64_t classes, int vec) {
     const int64_t vecs = (classes + vec - 1) / vec;
-    if (vecs > 64 * kGroupVecs) return -1;
-    int s = 0;
-    while (s < 6 && (1 << s) < vecs) s++;
-    return s;
+    if (vecs > 64 * kHeld) return {-1, 0};
+    int shift = 0;
+    while (shift < 6 && (1 << shift) < vecs) shift++;
+    int vectors = 1;
+    while ((int64_t)vectors << shift < vecs) vectors *= 2;
+    while (vectors < 4 && shift > 0 && (rows << shift) > (1 << 16)) { shift--; vectors *= 2; }
+    return {shift, vectors};
+}
+
+template <class F> void with_vectors(int vectors, F&& f) {
+    switch (vectors) {
+        case 1: f(std::integral_constant<int, 1>()); return;
+        case 2: f(std::integral_constant<int, 2>()); return;
+        case 4: f(std::integral_constant<int, 4>()); return;
+        default: f(std::integral_constant<int, kHeld>()); return;
+    }
 }
 
 // Parts of a long row: so many that there are 2048 workgroups (eight for each compute unit), none with less than one vector per work-item.
@@ -437,18 +699,35 @@ int check_rows(const sd_label_rows* in, const char* who, Rows* a) {
 
 int64_t split_floats(const sd_label_rows* in) {
     const int vec = vec_of(in->dtype);
-    if (group_shift(in->classes, vec) >= 0) return 0;
+    if (group_of(in->rows, in->classes, vec).shift >= 0) return 0;
     const int splits = row_splits(in->rows, in->classes, vec);
     return splits > 1 ? 2 * in->rows * splits : 0;
 }
 
-int launch_rows(const sd_label_rows* in, const Rows& a, const Finish& e, float* parts, hipStream_t stream) {
-    const int vec = vec_of(in->dtype), shift = group_shift(a.classes, vec);
+// with `g` the rows' gradients, too (rows that a workgroup can hold)
+int launch_rows(const sd_label_rows* in, const Rows& a, const Finish& e, const Gradient* g, float* parts, hipStream_t stream) {
+    const int vec = vec_of(in->dtype);
+    const Group group = group_of(a.rows, a.classes, vec);
+    const Gradient grad = g ? *g : Gradient{};
     with_dtype(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (shift >= 0) {
-            const int per = 256 >> shift;
-            hipLaunchKernelGGL(label_rows_kernel<T>, dim3(blocks_for((a.rows + per - 1) / per)), dim3(256), 0, stream, a, e, shift);
+        if (group.shift >= 0) {
+            const int per = 256 >> group.shift;
+            const dim3 grid(blocks_for((a.rows + per - 1) / per));
+            with_vectors(group.vectors, [&](auto nv) {
+                if (g) hipLaunchKernelGGL((label_rows_kernel<T, nv.value, true>), grid, dim3(256), 0, stream, a, e, grad, group.shift);
+                else hipLaunchKernelGGL((label_rows_kernel<T, nv.value, false>), grid, dim3(256), 0, stream, a, e, grad, group.shift);
+            });
+            return;
+        }
+        if (g) {
+            const dim3 grid(blocks_for(a.rows));
+            const int64_t vecs = (a.classes + vec - 1) / vec;
+            if (vecs <= 4 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 256>), grid, dim3(256), 0, stream, a, e, grad);
+            else if (vecs <= 8 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 256>), grid, dim3(256), 0, stream, a, e, grad);
+            else if (vecs <= 16 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 256>), grid, dim3(256), 0, stream, a, e, grad);
+            else if (vecs <= 16 * 512) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 512>), grid, dim3(512), 0, stream, a, e, grad);
+            else hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 1024>), grid, dim3(1024), 0, stream, a, e, grad);
             return;
         }
         int splits = row_splits(a.rows, a.classes, vec);
@@ -480,9 +759,9 @@ extern "C" int sd_label_log_probs(const sd_label_rows* in, float* log_probs, flo
     SD_REQUIRE(log_probs && scratch, "label_log_probs: null output or scratch");
     Finish e{};
     e.kind = kValues;
-    e.log_probs = log_probs;
+    e.out = log_probs;
     e.stats = reinterpret_cast<float2*>(stats);
-    return launch_rows(in, a, e, scratch + kSumFloats, static_cast<hipStream_t>(stream));
+    return launch_rows(in, a, e, nullptr, scratch + kSumFloats, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int sd_preference_loss(const sd_label_rows* in, const float* ref, const void* offsets, int offset_bytes, int64_t tokens, int pairs, double beta, double smoothing,
@@ -500,65 +779,90 @@ extern "C" int sd_preference_loss(const sd_label_rows* in, const float* ref, con
     const int64_t parts = split_floats(in);
     Finish e{};
     e.kind = kPreference;
-    e.log_probs = scratch + kSumFloats + parts;
+    e.out = scratch + kSumFloats + parts;
+    e.ref = ref;
     e.stats = reinterpret_cast<float2*>(stats);
     e.weight = weight;
     e.ticket = reinterpret_cast<uint32_t*>(scratch);
-    if (int rc = launch_rows(in, a, e, scratch + kSumFloats, s)) return rc;
-    Pairs p{e.log_probs, ref, a.labels, a.ignore, a.rows, tokens, offset_bytes == 4 ? static_cast<const int*>(offsets) : nullptr,
-            offset_bytes == 8 ? static_cast<const int64_t*>(offsets) : nullptr, pairs, beta, smoothing, weight, rewards, loss,
-            reinterpret_cast<double*>(scratch + 4), e.ticket};
-    const int blocks = (pairs + 3) / 4 < kPairBlocks ? (pairs + 3) / 4 : kPairBlocks;
-    hipLaunchKernelGGL(preference_kernel, dim3(blocks), dim3(256), 0, s, p);
+    if (int rc = launch_rows(in, a, e, nullptr, scratch + kSumFloats, s)) return rc;
+    const Pairs p{e.out, a.rows, tokens, offset_bytes == 4 ? static_cast<const int*>(offsets) : nullptr, offset_bytes == 8 ? static_cast<const int64_t*>(offsets) : nullptr,
+                  pairs, beta, smoothing, weight, rewards, loss, reinterpret_cast<double*>(scratch + 4), e.ticket};
+    // a workgroup per pair where that fills the card no more than once, and answers are long enough for it
+    if (pairs <= kPairBlocks && a.rows >= 64 * (int64_t)pairs) hipLaunchKernelGGL(preference_kernel<4>, dim3(pairs), dim3(256), 0, s, p);
+    else hipLaunchKernelGGL(preference_kernel<1>, dim3((pairs + 3) / 4 < kPairBlocks ? (pairs + 3) / 4 : kPairBlocks), dim3(256), 0, s, p);
     return check_launch("preference_kernel");
 }
 
+// Whether the gradient leaves with the rows: it then costs one reading of the logits less (5.5 TB/s) and a launch more (4 us); a
+// workgroup must be able to hold a row, and there must be rows for all compute units.
+static bool fused_policy(const sd_label_rows* in) {
+    const int vec = vec_of(in->dtype);
+    if (in->rows * in->classes * (16 / vec) < (32ll << 20)) return false;
+    return group_of(in->rows, in->classes, vec).shift >= 0 || (in->rows >= 512 && in->classes <= kHeldLong * vec);
+}
+
+extern "C" int sd_policy_fuses(const sd_label_rows* in) {
+    Rows a;
+    return check_rows(in, "policy_fuses", &a) == SD_OK && fused_policy(in) ? 1 : 0;
+}
+
 extern "C" int sd_policy_loss(const sd_label_rows* in, const float* old_log_probs, const float* advantages, int64_t advantage_outer, int64_t advantage_inner,
-                              const float* ref, double clip_low, double clip_high, double kl, float* stats, float* weight, float* scale, float* loss, float* means,
-                              float* scratch, sd_stream_t stream) {
+                              const float* ref, double clip_low, double clip_high, double kl, float* stats, float* weight, float* scale, void* grad, float* loss,
+                              float* means, float* scratch, sd_stream_t stream) {
     sd::CallGuard call_guard;
     Rows a;
     if (int rc = check_rows(in, "policy_loss", &a)) return rc;
     SD_REQUIRE(old_log_probs && advantages && scale && loss && means && scratch, "policy_loss: null argument");
     SD_REQUIRE(!stats == !weight, "policy_loss: the gradient needs both stats and weight");
+    SD_REQUIRE(!grad || stats, "policy_loss: a gradient that leaves with the rows needs stats and weight, too");
+    SD_REQUIRE(!grad || fused_policy(in), "policy_loss: the gradient of these rows does not leave with them (sd_policy_fuses)");
     SD_REQUIRE(clip_low >= 0.0 && clip_low <= 1.0 && clip_high >= 0.0, "policy_loss: clip=%g, clip_high=%g: need 0 <= clip <= 1 and 0 <= clip_high", clip_low, clip_high);
     SD_REQUIRE(ref || kl == 0.0, "policy_loss: a KL term needs reference log probabilities");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t parts = split_floats(in);
     Finish e{};
     e.kind = kPolicy;
     e.stats = reinterpret_cast<float2*>(stats);
     e.weight = weight;
     e.terms = reinterpret_cast<float4*>(scratch + kSumFloats);          // (16-byte aligned: before the parts)
-    e.old = old_log_probs; e.advantage = advantages; e.ref = ref;
+    e.old = old_log_probs; e.advantage = advantages; e.ref = kl != 0.0 ? ref : nullptr;
     e.advantage_outer = advantage_outer; e.advantage_inner = advantage_inner;
     e.low = (float)(1.0 - clip_low); e.high = (float)(1.0 + clip_high); e.kl = (float)kl;
     e.ticket = reinterpret_cast<uint32_t*>(scratch);
-    if (int rc = launch_rows(in, a, e, scratch + kSumFloats + 4 * a.rows, s)) return rc;
+    Gradient g{};
+    g.scale = scale; g.grad = grad;
+    if (grad) hipLaunchKernelGGL(count_rows_kernel, dim3(1), dim3(1024), 0, s, a.labels, a.rows, a.ignore, scale);
+    if (int rc = launch_rows(in, a, e, grad ? &g : nullptr, scratch + kSumFloats + 4 * a.rows, s)) return rc;
     const int64_t want = (a.rows + 2047) / 2048;
-    hipLaunchKernelGGL(policy_sums_kernel, dim3((unsigned)(want < kSumBlocks ? want : kSumBlocks)), dim3(256), 0, s, e.terms, a.rows, kl, loss, means, scale,
+    hipLaunchKernelGGL(policy_sums_kernel, dim3((unsigned)(want < kSumBlocks ? want : kSumBlocks)), dim3(256), 0, s, e.terms, a.rows, kl, loss, means, grad ? nullptr : scale,
                        reinterpret_cast<double*>(scratch + 4), e.ticket);
     return check_launch("policy_sums_kernel");
 }
 
-extern "C" int sd_label_gradient(const sd_label_rows* in, const float* stats, const float* weight, const float* scale, const float* scale2, void* grad, sd_stream_t stream) {
+extern "C" int sd_label_gradient(const sd_label_rows* in, const float* stats, const float* weight, const float* scale, const float* scale2, int unless_one, void* grad,
+                                 sd_stream_t stream) {
     sd::CallGuard call_guard;
     Rows a;
     if (int rc = check_rows(in, "label_gradient", &a)) return rc;
     SD_REQUIRE(stats && weight && grad, "label_gradient: null argument");
-    const Gradient g{reinterpret_cast<const float2*>(stats), weight, scale, scale2, grad};
+    SD_REQUIRE(!unless_one || scale2, "label_gradient: unless_one needs scale2");
+    const Gradient g{reinterpret_cast<const float2*>(stats), weight, scale, scale2, grad, unless_one != 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int vec = vec_of(in->dtype), shift = group_shift(a.classes, vec);
+    const int vec = vec_of(in->dtype);
+    const Group group = group_of(a.rows, a.classes, vec);
+    // a launch that mostly finds nothing to do has no more workgroups than run at once: each takes time to come and go
+    const auto blocks = [&](int64_t n) { return dim3(unless_one && n > 8 * num_cus() ? (unsigned)(8 * num_cus()) : blocks_for(n)); };
     with_dtype(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (shift >= 0) {
-            const int per = 256 >> shift;
-            hipLaunchKernelGGL(label_gradient_kernel<T>, dim3(blocks_for((a.rows + per - 1) / per)), dim3(256), 0, s, a, g, shift);
+        if (group.shift >= 0) {
+            const int per = 256 >> group.shift;
+            with_vectors(group.vectors, [&](auto nv) {
+                hipLaunchKernelGGL((label_gradient_kernel<T, nv.value>), blocks((a.rows + per - 1) / per), dim3(256), 0, s, a, g, group.shift);
+            });
             return;
         }
         const int64_t part = 256 * vec * kUnroll;
         const int splits = (int)((a.classes + part - 1) / part);
-        hipLaunchKernelGGL(label_long_gradient_kernel<T>, dim3(blocks_for(a.rows * splits)), dim3(256), 0, s, a, g, splits, part);
+        hipLaunchKernelGGL(label_long_gradient_kernel<T>, blocks(a.rows * splits), dim3(256), 0, s, a, g, splits, part);
     });
     return check_launch("label_gradient_kernel");
 }

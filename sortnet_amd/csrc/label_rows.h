@@ -26,6 +26,7 @@ template <> struct Elem<float> {
         for (int i = 0; i < 4; i++) v[i] = __float_as_uint(f[i]);
         return v;
     }
+    static __device__ __forceinline__ u32x4 splat(float v) { const uint32_t w = __float_as_uint(v); return u32x4{w, w, w, w}; }
     static __device__ __forceinline__ float exp(float v) { return expf(v); }
 };
 struct bf16 { uint16_t bits; };
@@ -48,6 +49,7 @@ template <> struct Elem<bf16> {
         for (int i = 0; i < 4; i++) v[i] = (uint32_t)bits(f[2 * i]) | (uint32_t)bits(f[2 * i + 1]) << 16;
         return v;
     }
+    static __device__ __forceinline__ u32x4 splat(bf16 v) { const uint32_t w = v.bits | (uint32_t)v.bits << 16; return u32x4{w, w, w, w}; }
     // results are rounded to 8 bits: the hardware's exp2 of a rounded argument is exact enough (|v| 2^-24 relative)
     static __device__ __forceinline__ float exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 };
@@ -69,6 +71,7 @@ template <> struct Elem<fp16> {
         for (int i = 0; i < 4; i++) v[i] = (uint32_t)bits(f[2 * i]) | (uint32_t)bits(f[2 * i + 1]) << 16;
         return v;
     }
+    static __device__ __forceinline__ u32x4 splat(fp16 v) { const uint32_t w = v.bits | (uint32_t)v.bits << 16; return u32x4{w, w, w, w}; }
     static __device__ __forceinline__ float exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 };
 

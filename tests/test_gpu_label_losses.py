@@ -312,6 +312,64 @@ def test_policy(answers, tokens, classes, kl, shared, dtype):
     assert torch.equal(quiet[0], loss) and torch.equal(quiet[1], stats)
 
 
+@pytest.mark.parametrize("answers, tokens, classes, kl, dtype", [(40000, 1, 230, 0.1, torch.float32), (2000, 42, 203, 0.0, torch.float16), (1030, 1, 9001, 0.05, torch.float32),
+                                                                (60, 20, 16500, 0.1, torch.bfloat16), (1 << 20, 1, 9, 0.0, torch.float32), (1 << 22, 1, 5, 0.1, torch.bfloat16)])
+def test_policy_of_many_rows(answers, tokens, classes, kl, dtype):
+    """Logits of 32 MiB and more, whose gradient is made with the loss: alone, scaled, kept for a second backward, and in a replayed graph."""
+    rows, low, high = answers * tokens, 0.2, 0.28
+    assert rows * classes * torch.finfo(dtype).bits // 8 >= 32 << 20
+    z, labels, g = make(rows, classes, dtype, rows + classes, ignored=0.2)
+    lp = exact_rows(z, labels)[0].float()
+    old = lp - away_from_borders(0.25 * torch.randn(rows, generator=g).cuda(), low, high)
+    ref = lp + 0.3 * torch.randn(rows, generator=g).cuda()
+    adv = torch.randn(answers, 1, generator=g).cuda().expand(answers, tokens)
+    want = exact_policy(z, labels, old, adv.reshape(-1), ref, low, high, kl)
+    shape = (answers, tokens)
+    leaf = z.view(*shape, classes).requires_grad_()
+    call = lambda t: losses.policy_loss(t, labels.view(shape), old.view(shape), adv, ref_log_probs=ref.view(shape) if kl else None, clip=low, clip_high=high, kl_coef=kl)
+    loss, stats = call(leaf)
+    close(loss.detach(), want[0], want[1], "loss")
+    close(stats, want[2], want[3], "stats")
+    check = lambda got, by: check_gradient(got.view(rows, classes), z, labels, by * want[4], abs(by) * (want[5] + 4 * U * want[4].abs()), "gradient")
+    first, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    check(first, 1.0)
+    whole = first.clone()
+    first.zero_()                           # the caller's own
+    second, = torch.autograd.grad(loss, leaf, torch.tensor(-0.375, device="cuda"), retain_graph=True)
+    check(second, -0.375)
+    second.zero_()
+    third, = torch.autograd.grad(loss, leaf)
+    assert torch.equal(third, whole)
+    loss, _ = call(leaf)
+    scaled, = torch.autograd.grad(0.3 * loss, leaf)
+    check(scaled, float(torch.tensor(0.3)))
+    loss, _ = call(leaf)
+    loss.backward()
+    assert torch.equal(leaf.grad, whole)
+    nothing, = torch.autograd.grad(call(leaf)[0], leaf, torch.zeros((), device="cuda"))
+    assert (nothing == 0).all()
+    if classes > 5:
+        static, other = leaf.detach().clone().requires_grad_(), leaf.detach().flip(1 if tokens > 1 else 0).contiguous()
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            torch.autograd.grad(call(static)[0], static)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs = call(static)
+            made, = torch.autograd.grad(outs[0], static)
+        for data in (other, leaf.detach(), other):
+            with torch.no_grad():
+                static.copy_(data)
+            fresh = data.clone().requires_grad_()
+            eager = call(fresh)
+            eager_grad, = torch.autograd.grad(eager[0], fresh)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0], eager[0]) and torch.equal(outs[1], eager[1]) and torch.equal(made, eager_grad)
+
+
 def test_policy_clips_and_defaults():
     """Each side of the clip with either sign of the advantage; clip_high defaults to clip; a clip of 1 and 0."""
     z, labels, _ = make(6, 5, torch.float32, 4, ignored=0.0)

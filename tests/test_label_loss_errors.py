@@ -36,7 +36,7 @@ def test_rows_without_a_meaning(bad):
     rows = _rows(**bad)
     assert _lib.load().sd_label_scratch(rows) == -1
     for name, args in [("sd_label_log_probs", (p, p, p, None)), ("sd_preference_loss", (p, None, 0, 1, 2, 0.1, 0.0, p, p, p, p, p, None)),
-                       ("sd_policy_loss", (p, p, 0, 1, p, 0.2, 0.2, 0.0, p, p, p, p, p, p, None)), ("sd_label_gradient", (p, p, None, None, p, None))]:
+                       ("sd_policy_loss", (p, p, 0, 1, p, 0.2, 0.2, 0.0, p, p, p, None, p, p, p, None)), ("sd_label_gradient", (p, p, None, None, 0, p, None))]:
         with pytest.raises(RuntimeError, match=r"status 1\)"):
             _lib.call(name, rows, *args)
 
@@ -56,7 +56,12 @@ def test_halves_of_the_gradient():
     with pytest.raises(RuntimeError, match="both"):
         _lib.call("sd_preference_loss", _rows(), p, None, 0, 1, 2, 0.1, 0.0, p, None, p, p, p, None)
     with pytest.raises(RuntimeError, match="both"):
-        _lib.call("sd_policy_loss", _rows(), p, p, 0, 1, None, 0.2, 0.2, 0.0, None, p, p, p, p, p, None)
+        _lib.call("sd_policy_loss", _rows(), p, p, 0, 1, None, 0.2, 0.2, 0.0, None, p, p, None, p, p, p, None)
+    assert _lib.load().sd_policy_fuses(_rows()) == 0
+    with pytest.raises(RuntimeError, match="does not leave"):      # too few rows for a gradient that leaves with them
+        _lib.call("sd_policy_loss", _rows(), p, p, 0, 1, None, 0.2, 0.2, 0.0, p, p, p, p, p, p, p, None)
+    with pytest.raises(RuntimeError, match="unless_one"):
+        _lib.call("sd_label_gradient", _rows(), p, p, None, None, 1, p, None)
 
 
 @pytest.mark.parametrize("low, high, kl, ref, match", [(-0.1, 0.2, 0.0, 0, "clip"), (1.1, 0.2, 0.0, 0, "clip"), (0.2, -0.1, 0.0, 0, "clip"), (math.nan, 0.2, 0.0, 0, "clip"),
@@ -64,7 +69,7 @@ def test_halves_of_the_gradient():
 def test_policies_without_a_meaning(low, high, kl, ref, match):
     p = 1 << 20
     with pytest.raises(RuntimeError, match=match):
-        _lib.call("sd_policy_loss", _rows(), p, p, 0, 1, ref or None, low, high, kl, p, p, p, p, p, p, None)
+        _lib.call("sd_policy_loss", _rows(), p, p, 0, 1, ref or None, low, high, kl, p, p, p, None, p, p, p, None)
 
 
 def test_dropout_without_a_meaning():
