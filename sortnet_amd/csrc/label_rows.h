@@ -77,6 +77,9 @@ template <> struct Elem<fp16> {
 
 template <class T> __device__ __forceinline__ u32x4 load16(const T* p) { return reinterpret_cast<const typename Elem<T>::Pack*>(p)->v; }
 template <class T> __device__ __forceinline__ void store16(T* p, u32x4 v) { reinterpret_cast<typename Elem<T>::Pack*>(p)->v = v; }
+// the same for what is not read again soon, past the caches
+template <class T> __device__ __forceinline__ u32x4 stream16(const T* p) { return __builtin_nontemporal_load(&reinterpret_cast<const typename Elem<T>::Pack*>(p)->v); }
+template <class T> __device__ __forceinline__ void put_stream16(T* p, u32x4 v) { __builtin_nontemporal_store(v, &reinterpret_cast<typename Elem<T>::Pack*>(p)->v); }
 
 // calls f with a null pointer of the element type that `dtype` names; false for none
 template <class F> bool with_dtype(int dtype, F&& f) {
