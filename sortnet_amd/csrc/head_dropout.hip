@@ -3,8 +3,10 @@
 // call with the same seed makes the same mask again.
 // One word serves two neighbouring values: pair j = i / 2 stands at column j mod 2^15 of row j / 2^15; the word is mixed with two keys of
 // its row, so that the words of two rows are no shifted copies of each other (one key of 32 bits leaves 2^32 sequences that overlap).
-// Bound by the bytes; the words take about half of the issue slots that the bytes of a 16-bit tensor leave.
+// Bound by the bytes: 2^27 values bf16 82 us, 6.5 TB/s (a copy 99 us), three times 2^26 fp32 284 us, 5.7 TB/s.  Results are stored past the
+// caches (108 -> 82 us, 2^22 values fp32 6.0 -> 4.7), and inputs that the last-level cache cannot hold are read past it (292 -> 284).
 #include <cmath>
+#include <type_traits>
 #include "label_rows.h"
 
 namespace sd {
@@ -20,42 +22,68 @@ struct DropArgs {
 
 __device__ __forceinline__ uint32_t drop_word(uint32_t key, uint32_t other, uint32_t col) { return rng_mix(rng_word(key, col) ^ other); }
 
-// A work-item takes 8 neighbouring values at a time of each of COUNT tensors.
-template <class T, int COUNT> __global__ void __launch_bounds__(256) dropout_kernel(DropArgs a) {
-    constexpr int V = Elem<T>::kVec, P = 8 / V;
+// A workgroup takes 256 UNROLL vectors of 16 bytes of each of COUNT tensors at a time; these lie in one row of the generator (they are a
+// power of two, at most 2^13 values), so the two keys are the workgroup's.
+template <class T, int COUNT, int UNROLL> __global__ void __launch_bounds__(256) dropout_kernel(DropArgs a) {
+    constexpr int V = Elem<T>::kVec, kStep = 256 * UNROLL * V;
+    static_assert(kStep <= 65536 && 65536 % kStep == 0, "a step within one row of the generator");
     const uint32_t seed = a.seeds ? (uint32_t)*a.seeds : a.seed;
-    const int64_t eights = (a.n + 7) / 8;
-    for (int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x; e < eights; e += (int64_t)gridDim.x * 256) {
-        const int64_t i = e * 8;
-        const uint32_t row = (uint32_t)(i >> 16), col = (uint32_t)(i & 0xffff) >> 1;
+    const bool far = a.n * (int64_t)sizeof(T) * COUNT > kCached;
+    for (int64_t base = (int64_t)blockIdx.x * kStep; base < a.n; base += (int64_t)gridDim.x * kStep) {
+        const uint32_t row = (uint32_t)(base >> 16), col = (uint32_t)(base & 0xffff) >> 1;
         const uint32_t key = rng_row_key(seed, 5u, row), other = rng_row_key(seed, 6u, row);
-        bool keep[8];
-        #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const uint32_t w = drop_word(key, other, col + k);
-            keep[2 * k] = (w & 0xffffu) < a.limit;
-            keep[2 * k + 1] = (w >> 16) < a.limit;
-        }
+        u32x4 v[COUNT][UNROLL];
         #pragma unroll
         for (int t = 0; t < COUNT; t++) {
-            const T* x = static_cast<const T*>(a.x[t]) + i;
-            T* y = static_cast<T*>(a.y[t]) + i;
-            if (i + 8 <= a.n) {
-                #pragma unroll
-                for (int p = 0; p < P; p++) {
-                    float f[V];
-                    Elem<T>::unpack(load16(x + p * V), f);
-                    #pragma unroll
-                    for (int k = 0; k < V; k++) f[k] = keep[p * V + k] ? f[k] * a.scale : 0.f;
-                    store16(y + p * V, Elem<T>::pack(f));
+            #pragma unroll
+            for (int u = 0; u < UNROLL; u++) {
+                const int at = (u * 256 + (int)threadIdx.x) * V;
+                if (base + at + V <= a.n) {
+                    const T* x = static_cast<const T*>(a.x[t]) + base + at;
+                    v[t][u] = far ? stream16(x) : load16(x);
                 }
-            } else {
-                #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    if (i + k < a.n) y[k] = keep[k] ? Elem<T>::put(Elem<T>::get(x[k]) * a.scale) : T{};
+            }
+        }
+        #pragma unroll
+        for (int u = 0; u < UNROLL; u++) {
+            const int at = (u * 256 + (int)threadIdx.x) * V;
+            bool keep[V];
+            #pragma unroll
+            for (int k = 0; k < V / 2; k++) {
+                const uint32_t w = drop_word(key, other, col + at / 2 + k);
+                keep[2 * k] = (w & 0xffffu) < a.limit;
+                keep[2 * k + 1] = (w >> 16) < a.limit;
+            }
+            #pragma unroll
+            for (int t = 0; t < COUNT; t++) {
+                if (base + at + V <= a.n) {
+                    float f[V];
+                    Elem<T>::unpack(v[t][u], f);
+                    #pragma unroll
+                    for (int k = 0; k < V; k++) f[k] = keep[k] ? f[k] * a.scale : 0.f;
+                    put_stream16(static_cast<T*>(a.y[t]) + base + at, Elem<T>::pack(f));
+                } else {
+                    const T* x = static_cast<const T*>(a.x[t]) + base + at;
+                    T* y = static_cast<T*>(a.y[t]) + base + at;
+                    #pragma unroll
+                    for (int k = 0; k < V; k++)
+                        if (base + at + k < a.n) y[k] = keep[k] ? Elem<T>::put(Elem<T>::get(x[k]) * a.scale) : T{};
+                }
             }
         }
     }
+}
+
+template <class T, int COUNT, int UNROLL> void launch_dropout(const DropArgs& a, hipStream_t stream) {
+    const int64_t step = 256 * UNROLL * Elem<T>::kVec, want = (a.n + step - 1) / step;
+    hipLaunchKernelGGL((dropout_kernel<T, COUNT, UNROLL>), dim3((unsigned)(want < (1 << 22) ? want : (1 << 22))), dim3(256), 0, stream, a);
+}
+
+// Several vectors of a work-item on their way where there is work for all compute units, one where there is not.
+template <class T, int COUNT> void launch_dropout(const DropArgs& a, hipStream_t stream) {
+    constexpr int kUnroll = COUNT == 1 ? 4 : 2;
+    if (a.n >= (int64_t)num_cus() * 4 * 256 * kUnroll * Elem<T>::kVec) launch_dropout<T, COUNT, kUnroll>(a, stream);
+    else launch_dropout<T, COUNT, 1>(a, stream);
 }
 
 }  // namespace sd
@@ -78,14 +106,12 @@ extern "C" int sd_dropout(const void* x0, const void* x1, const void* x2, int dt
     }
     SD_REQUIRE(dtype == SD_FLOAT32 || dtype == SD_BFLOAT16 || dtype == SD_FLOAT16, "dropout: dtype=%d is none of SD_FLOAT32, SD_BFLOAT16, SD_FLOAT16", dtype);
     if (n == 0 || count == 0) return SD_OK;
-    const int64_t want = ((n + 7) / 8 + 255) / 256;
-    const dim3 grid((unsigned)(want < (1 << 20) ? want : (1 << 20)));
     hipStream_t s = static_cast<hipStream_t>(stream);
     with_dtype(dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
-        if (count == 1) hipLaunchKernelGGL((dropout_kernel<T, 1>), grid, dim3(256), 0, s, a);
-        else if (count == 2) hipLaunchKernelGGL((dropout_kernel<T, 2>), grid, dim3(256), 0, s, a);
-        else hipLaunchKernelGGL((dropout_kernel<T, 3>), grid, dim3(256), 0, s, a);
+        if (count == 1) launch_dropout<T, 1>(a, s);
+        else if (count == 2) launch_dropout<T, 2>(a, s);
+        else launch_dropout<T, 3>(a, s);
     });
     return check_launch("dropout_kernel");
 }

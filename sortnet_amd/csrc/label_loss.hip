@@ -21,10 +21,6 @@ constexpr int kShortBlocks = 4096;      // workgroups of short rows, at most
 // Bytes of a FUSED short row from which its gradient is stored past the caches: us with and without, 262144 x 200 fp32 121 / 142,
 // 65536 x 1000 bf16 62 / 67; 1048576 x 10 fp32, whose rows share cache lines, 178 / 160.
 constexpr int kStreamRow = 512;
-// The last-level cache.  A pass over long rows reads them from the last to the first, the gradient's pass from the first on, so that it finds
-// that many bytes still there; the rows behind them are read past the caches, which leaves these alone and is faster by itself:
-// 4096 x 131072 bf16 forward 183 -> 156 us, both passes 545 -> 495.
-constexpr int64_t kCached = 256ll << 20;
 
 struct Rows {
     const void* logits;
@@ -386,6 +382,9 @@ template <class T, bool STREAM> __device__ __forceinline__ void grad_row(const T
     }
 }
 
+// A pass over long rows reads them from the last to the first, the gradient's pass from the first on, so that it finds
+// what the last-level cache holds still there; the rows behind them are read past the caches, which leaves these alone and is faster by itself:
+// 4096 x 131072 bf16 forward 183 -> 156 us, both passes 545 -> 495.
 template <class T> __device__ __forceinline__ bool beyond_cache(const Rows& a, int64_t r) { return r * a.classes * (int64_t)sizeof(T) >= kCached; }
 
 __device__ __forceinline__ End finish_long_row(const Rows& a, const Finish& e, int64_t r, const Given& g, float top, float sum) {

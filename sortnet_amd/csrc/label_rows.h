@@ -7,6 +7,7 @@
 namespace sd {
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+constexpr int64_t kCached = 256ll << 20;    // bytes of the last-level cache
 
 // 16 bytes of a row at an element's own alignment: rows of an odd number of classes start anywhere, and gfx950 loads and stores
 // such vectors whole.
