@@ -342,8 +342,9 @@ typedef struct {
     int dtype;
 } sd_label_rows;
 
-/* Floats of scratch that the calls below want for these rows (host only), or -1 where they would refuse them. */
-int64_t sd_label_scratch(const sd_label_rows* rows);
+/* Floats of scratch, a multiple of 4, that the calls below want for these rows (host only), or -1 where they would refuse them: loss = 0 for
+ * sd_label_log_probs (scratch may be NULL where this is 0), 1 for the losses. */
+int64_t sd_label_scratch(const sd_label_rows* rows, int loss);
 
 /* log_probs[r] = log softmax(row r)[label], 0 where ignored.  stats (rows, 2; may be NULL) receives what sd_label_gradient needs. */
 int sd_label_log_probs(const sd_label_rows* rows, float* log_probs, float* stats, float* scratch, sd_stream_t stream);

@@ -82,7 +82,7 @@ _OTHER = {
     "sd_mask_threshold8": ([_f], _u),
     "sd_mask_threshold16": ([_f], _u),
     "sd_mask_count": ([_u, _i, _f], _i),
-    "sd_label_scratch": ([_R], _l),
+    "sd_label_scratch": ([_R, _i], _l),
     "sd_policy_fuses": ([_R], _i),
 }
 

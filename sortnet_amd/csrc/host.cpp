@@ -597,23 +597,45 @@ Tensor label_indices(const Tensor& targets, const Tensor& outputs) {
 }
 
 // a constant per row: no gradient flows into it
-Tensor row_constants(const Tensor& t, const char* name, const Tensor& targets) {
+void check_constants(const Tensor& t, const char* name, const Tensor& targets) {
     same_device(t, name, targets);
     if (t.scalar_type() != at::kFloat) throw std::runtime_error(std::string(name) + " must have dtype torch.float32");
     if (t.sizes() != targets.sizes()) throw std::runtime_error(std::string(name) + " must have the sizes of targets");
     if (at::GradMode::is_enabled() && t.requires_grad())
         throw std::runtime_error(std::string(name) + " must not require a gradient: the loss is differentiated with respect to outputs alone");
-    return t;
 }
 
-Tensor label_scratch(const sd_label_rows& a, const Tensor& like) {
-    const int64_t n = sd_label_scratch(&a);
-    if (n < 0) require(SD_ERR_ARG, "sd_label_scratch");
-    return new_floats(like, {n});
-}
+// What a call works in, as one tensor (an allocation is a microsecond of the host): where the gradient is wanted what it needs of the
+// rows - (top, 1 / sum), and for the losses the rows' weights and their scale - and behind it the scratch.
+struct Work {
+    Tensor whole;
+    float *stats = nullptr, *weight = nullptr, *scale = nullptr, *scratch = nullptr;
+    Work() = default;
+    Work(const Tensor& like, const sd_label_rows& a, bool loss, bool grad) {
+        const int64_t n = sd_label_scratch(&a, loss);
+        if (n < 0) require(SD_ERR_ARG, "sd_label_scratch");
+        if (n + floats_of(a.rows, loss, grad) == 0) return;
+        whole = new_floats(like, {n + floats_of(a.rows, loss, grad)});
+        places(whole, a.rows, loss, grad);
+    }
+    // the places in the tensor of a call whose gradient is wanted
+    Work(const Tensor& saved, int64_t rows, bool loss) : whole(saved) { places(whole, rows, loss, true); }
+
+private:
+    static int64_t round4(int64_t n) { return (n + 3) / 4 * 4; }
+    static int64_t floats_of(int64_t rows, bool loss, bool grad) { return (grad ? round4(2 * rows) + (loss ? round4(rows) : 0) : 0) + (loss ? 4 : 0); }
+    void places(const Tensor& t, int64_t rows, bool loss, bool grad) {
+        float* p = floats(t, "work");
+        if (loss) { scale = p; p += 4; }
+        if (grad) { stats = p; p += round4(2 * rows); }
+        if (grad && loss) { weight = p; p += round4(rows); }
+        scratch = p;
+    }
+};
 
 struct LabelNode : Node {
-    SavedVariable logits, labels, stats, weight, scale;   // weight, scale: none for plain log probabilities
+    enum Kind { VALUES, PREFERENCE, POLICY } kind;
+    SavedVariable logits, labels, work;
     Tensor made;            // the gradient for an upstream gradient of 1, where the forward made it
     int64_t ignore = 0;
     bool last = false;      // this backward is the graph's last: `made` may be given away
@@ -622,19 +644,20 @@ struct LabelNode : Node {
         const Locked lock(mutex_);
         variable_list out(1);
         if (!task_should_compute_output(0)) return out;
-        const Tensor z = logits.unpack(), l = labels.unpack(), st = stats.unpack(), w = weight.unpack(), sc = scale.unpack();
+        const Tensor z = logits.unpack(), l = labels.unpack(), wk = work.unpack();
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor g = incoming(*this, grads, 0);
         const c10::DeviceGuard guard(z.device());
         // A gradient that is there already is only written again for another upstream gradient than 1, which the device knows; one that a
         // later backward may want, too, stays as it is.
-        const bool there = made.defined() && last;
+        const bool there = made.defined() && last, loss = kind != VALUES;
         out[0] = there ? std::move(made) : at::empty(z.sizes(), z.options());
         if (out[0].numel() == 0) return out;
         const sd_label_rows a = label_rows(z, l, ignore);
-        const float *gp = floats(g, "grad_output"), *sp = sc.defined() ? floats(sc, "scale") : nullptr;
-        const bool loss = w.defined();      // else the upstream gradient is the rows' weights
-        require(sd_label_gradient(&a, floats(st, "stats"), loss ? floats(w, "weight") : gp, sp, loss ? gp : nullptr, there, out[0].data_ptr(), stream_of(z)), "sd_label_gradient");
+        const Work w(wk, a.rows, loss);
+        const float* gp = floats(g, "grad_output");     // of log probabilities: the rows' weights
+        require(sd_label_gradient(&a, w.stats, loss ? w.weight : gp, kind == POLICY ? w.scale : nullptr, loss ? gp : nullptr, there, out[0].data_ptr(), stream_of(z)),
+                "sd_label_gradient");
         return out;
     }
     void will_release_variables() override {
@@ -643,23 +666,21 @@ struct LabelNode : Node {
     }
     void release_variables() override {
         const Locked lock(mutex_);
-        logits.reset_data(); labels.reset_data(); stats.reset_data(); weight.reset_data(); scale.reset_data();
+        logits.reset_data(); labels.reset_data(); work.reset_data();
         made.reset();
     }
     std::string name() const override { return "LabelNode"; }
 };
 
 // makes y the output of a node over the logits
-void attach_labels(const Tensor& y, const Tensor& outputs, const Tensor& z, const Tensor& labels, int64_t ignore, const Tensor& stats, const Tensor& weight,
-                   const Tensor& scale, const Tensor& made) {
+void attach_labels(const Tensor& y, LabelNode::Kind kind, const Tensor& outputs, const Tensor& z, const Tensor& labels, int64_t ignore, const Tensor& work, const Tensor& made) {
     auto node = new_node<LabelNode>();
     node->set_next_edges(collect_next_edges(outputs));
+    node->kind = kind;
     node->ignore = ignore;
     node->logits = SavedVariable(z, false);
     node->labels = SavedVariable(labels, false);
-    node->stats = SavedVariable(stats, false);
-    if (weight.defined()) node->weight = SavedVariable(weight, false);
-    if (scale.defined()) node->scale = SavedVariable(scale, false);
+    node->work = SavedVariable(work, false);
     node->made = made;
     set_history(y, node);
 }
@@ -667,7 +688,8 @@ void attach_labels(const Tensor& y, const Tensor& outputs, const Tensor& z, cons
 Tensor label_log_probs(const Tensor& outputs, const Tensor& targets, int64_t ignore) {
     reverse_mode_only("label_log_probs", outputs);
     const bool grad = want_grad(outputs);
-    Tensor y, z, labels, stats;
+    Tensor y, z, labels;
+    Work work;
     {
         at::AutoDispatchBelowADInplaceOrView below;
         element_type(outputs, "outputs");
@@ -675,14 +697,13 @@ Tensor label_log_probs(const Tensor& outputs, const Tensor& targets, int64_t ign
         labels = label_indices(targets, outputs);
         z = readable_logits(outputs);
         y = new_floats(z, targets.sizes());
-        if (grad) stats = new_floats(z, {labels.numel(), 2});
         if (y.numel() > 0) {
             const sd_label_rows a = label_rows(z, labels, ignore);
-            const Tensor scratch = label_scratch(a, z);
-            require(sd_label_log_probs(&a, floats(y, "log_probs"), grad ? floats(stats, "stats") : nullptr, floats(scratch, "scratch"), stream_of(z)), "sd_label_log_probs");
-        }
+            work = Work(z, a, false, grad);
+            require(sd_label_log_probs(&a, floats(y, "log_probs"), work.stats, work.scratch, stream_of(z)), "sd_label_log_probs");
+        } else work.whole = y;
     }
-    if (grad) attach_labels(y, outputs, z, labels, ignore, stats, {}, {}, {});
+    if (grad) attach_labels(y, LabelNode::VALUES, outputs, z, labels, ignore, work.whole, {});
     return y;
 }
 
@@ -690,15 +711,17 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& outputs, const Tensor& t
                                           double smoothing, int64_t ignore) {
     reverse_mode_only("preference_loss", outputs);
     const bool grad = want_grad(outputs);
-    Tensor loss, rewards, z, labels, stats, weight;
+    Tensor loss, rewards, z, labels;
+    Work work;
     {
         const bool packed = offsets_in && offsets_in->defined();
         element_type(outputs, "outputs");
-        const Tensor ref = row_constants(ref_in, "ref_log_probs", targets).detach().contiguous();
+        check_constants(ref_in, "ref_log_probs", targets);
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::DeviceGuard guard(outputs.device());
         labels = label_indices(targets, outputs);
         z = readable_logits(outputs);
+        const Tensor ref = ref_in.contiguous();
         Tensor offsets;
         int64_t answers = 0, tokens = 0;
         if (packed) {
@@ -711,21 +734,17 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& outputs, const Tensor& t
             answers = outputs.size(0);
             tokens = answers > 0 ? labels.numel() / answers : 0;
         }
-        if (answers < 2 || answers % 2 != 0)
+        if (answers < 2 || answers % 2 != 0 || answers / 2 > INT32_MAX)
             throw std::runtime_error("preference_loss needs an even number of answers, the chosen ones before the rejected: got " + std::to_string(answers));
         const sd_label_rows a = label_rows(z, labels, ignore);
-        const Tensor scratch = label_scratch(a, z);
+        work = Work(z, a, true, grad);
         loss = new_floats(z, {});
         rewards = new_floats(z, {answers});
-        if (grad) {
-            stats = new_floats(z, {labels.numel(), 2});
-            weight = new_floats(z, {labels.numel()});
-        }
         require(sd_preference_loss(&a, floats(ref, "ref_log_probs"), packed ? offsets.data_ptr() : nullptr, packed ? (int)offsets.element_size() : 0, tokens,
-                                   (int)(answers / 2), beta, smoothing, grad ? floats(stats, "stats") : nullptr, grad ? floats(weight, "weight") : nullptr,
-                                   floats(rewards, "rewards"), floats(loss, "loss"), floats(scratch, "scratch"), stream_of(z)), "sd_preference_loss");
+                                   (int)(answers / 2), beta, smoothing, work.stats, work.weight, floats(rewards, "rewards"), floats(loss, "loss"), work.scratch,
+                                   stream_of(z)), "sd_preference_loss");
     }
-    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, {}, {});
+    if (grad) attach_labels(loss, LabelNode::PREFERENCE, outputs, z, labels, ignore, work.whole, {});
     return {loss, rewards};
 }
 
@@ -733,35 +752,32 @@ std::pair<Tensor, Tensor> policy_loss(const Tensor& outputs, const Tensor& targe
                                       double clip_low, double clip_high, double kl, int64_t ignore) {
     reverse_mode_only("policy_loss", outputs);
     const bool grad = want_grad(outputs);
-    Tensor loss, means, z, labels, stats, weight, scale, made;
+    Tensor loss, means, z, labels, made;
+    Work work;
     {
+        const bool has_ref = ref_in && ref_in->defined();
         element_type(outputs, "outputs");
-        const Tensor old = row_constants(old_in, "old_log_probs", targets).detach().contiguous();
-        const Tensor ref = ref_in && ref_in->defined() ? row_constants(*ref_in, "ref_log_probs", targets).detach().contiguous() : Tensor();
-        Tensor adv = row_constants(advantages, "advantages", targets).detach();
+        check_constants(old_in, "old_log_probs", targets);
+        if (has_ref) check_constants(*ref_in, "ref_log_probs", targets);
+        check_constants(advantages, "advantages", targets);
         at::AutoDispatchBelowADInplaceOrView below;
         const c10::DeviceGuard guard(outputs.device());
         labels = label_indices(targets, outputs);
         z = readable_logits(outputs);
         const sd_label_rows a = label_rows(z, labels, ignore);
-        if (adv.dim() > 2) adv = adv.contiguous();
+        const Tensor old = old_in.contiguous(), ref = has_ref ? ref_in->contiguous() : Tensor(), adv = advantages.dim() > 2 ? advantages.contiguous() : advantages;
         // one advantage for all rows of an answer comes as an expanded tensor, which is read where it is
         const bool two = z.dim() == 3;
         const int64_t outer = two ? adv.stride(0) : 0, inner = two ? adv.stride(1) : adv.dim() == 1 ? adv.stride(0) : 1;
-        const Tensor scratch = label_scratch(a, z);
+        work = Work(z, a, true, grad);
         loss = new_floats(z, {});
         means = new_floats(z, {3});
-        scale = new_floats(z, {1});
-        if (grad) {
-            stats = new_floats(z, {labels.numel(), 2});
-            weight = new_floats(z, {labels.numel()});
-            if (sd_policy_fuses(&a)) made = at::empty(z.sizes(), z.options());
-        }
-        require(sd_policy_loss(&a, floats(old, "old_log_probs"), static_cast<const float*>(adv.data_ptr()), outer, inner, ref.defined() ? floats(ref, "ref_log_probs") : nullptr,
-                               clip_low, clip_high, kl, grad ? floats(stats, "stats") : nullptr, grad ? floats(weight, "weight") : nullptr, floats(scale, "scale"),
-                               made.defined() ? made.data_ptr() : nullptr, floats(loss, "loss"), floats(means, "means"), floats(scratch, "scratch"), stream_of(z)), "sd_policy_loss");
+        if (grad && sd_policy_fuses(&a)) made = at::empty(z.sizes(), z.options());
+        require(sd_policy_loss(&a, floats(old, "old_log_probs"), static_cast<const float*>(adv.data_ptr()), outer, inner, has_ref ? floats(ref, "ref_log_probs") : nullptr,
+                               clip_low, clip_high, kl, work.stats, work.weight, work.scale, made.defined() ? made.data_ptr() : nullptr, floats(loss, "loss"),
+                               floats(means, "means"), work.scratch, stream_of(z)), "sd_policy_loss");
     }
-    if (grad) attach_labels(loss, outputs, z, labels, ignore, stats, weight, scale, made);
+    if (grad) attach_labels(loss, LabelNode::POLICY, outputs, z, labels, ignore, work.whole, made);
     return {loss, means};
 }
 

@@ -795,23 +795,23 @@ int launch_rows(const sd_label_rows* in, const Rows& a, const Finish& e, const G
 
 using namespace sd;
 
-extern "C" int64_t sd_label_scratch(const sd_label_rows* in) {
+extern "C" int64_t sd_label_scratch(const sd_label_rows* in, int loss) {
     Rows a;
     if (check_rows(in, "label_scratch", &a) != SD_OK) return -1;
-    // (the policy's terms are 64-bit numbers, the others' rows one float each)
-    return kSumFloats + 8 * term_count(in) + split_floats(in) + in->rows;
+    // (the policy's terms are 64-bit numbers, the preferences' rows one float each)
+    return (split_floats(in) + (loss ? kSumFloats + 8 * term_count(in) + in->rows : 0) + 3) / 4 * 4;
 }
 
 extern "C" int sd_label_log_probs(const sd_label_rows* in, float* log_probs, float* stats, float* scratch, sd_stream_t stream) {
     sd::CallGuard call_guard;
     Rows a;
     if (int rc = check_rows(in, "label_log_probs", &a)) return rc;
-    SD_REQUIRE(log_probs && scratch, "label_log_probs: null output or scratch");
+    SD_REQUIRE(log_probs && (scratch || split_floats(in) == 0), "label_log_probs: null output or scratch");
     Finish e{};
     e.kind = kValues;
     e.out = log_probs;
     e.stats = reinterpret_cast<float2*>(stats);
-    return launch_rows(in, a, e, nullptr, scratch + kSumFloats, static_cast<hipStream_t>(stream));
+    return launch_rows(in, a, e, nullptr, scratch, static_cast<hipStream_t>(stream));
 }
 
 extern "C" int sd_preference_loss(const sd_label_rows* in, const float* ref, const void* offsets, int offset_bytes, int64_t tokens, int pairs, double beta, double smoothing,

@@ -34,7 +34,7 @@ BAD_ROWS = [dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=1 << 31), dic
 def test_rows_without_a_meaning(bad):
     p = 1 << 20    # no kernel is launched: every call is refused by its sizes
     rows = _rows(**bad)
-    assert _lib.load().sd_label_scratch(rows) == -1
+    assert _lib.load().sd_label_scratch(rows, 0) == -1 and _lib.load().sd_label_scratch(rows, 1) == -1
     for name, args in [("sd_label_log_probs", (p, p, p, None)), ("sd_preference_loss", (p, None, 0, 1, 2, 0.1, 0.0, p, p, p, p, p, None)),
                        ("sd_policy_loss", (p, p, 0, 1, p, 0.2, 0.2, 0.0, p, p, p, None, p, p, p, None)), ("sd_label_gradient", (p, p, None, None, 0, p, None))]:
         with pytest.raises(RuntimeError, match=r"status 1\)"):
