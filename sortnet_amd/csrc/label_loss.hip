@@ -417,10 +417,10 @@ template <class T> __global__ void __launch_bounds__(256) label_long_rows_kernel
     }
 }
 
-// FUSED long rows: the workgroup holds the row in its registers, at most 16 vectors per work-item, so that the logits are read once and
-// the gradient leaves with the statistics.  (Reading the row again from the caches instead lost: eight rows of 256 KiB per compute
+// The workgroup holds a long row in its registers, at most 16 vectors per work-item.  FUSED: the logits are read once and the gradient leaves
+// with the statistics.  (Reading the row again from the caches instead lost: eight rows of 256 KiB per compute
 // unit are more than the last level holds, 4096 x 131072 bf16 596 us; two passes of their own 515.)
-template <class T, int NV, int THREADS> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
+template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
     constexpr int V = Elem<T>::kVec, kChunk = 16 / V;
     __shared__ float2 waves[THREADS / 64];
     __shared__ End row_end;
@@ -434,7 +434,7 @@ template <class T, int NV, int THREADS> __global__ void __launch_bounds__(THREAD
         T* q = static_cast<T*>(g.grad) + r * a.classes;
         if (label == a.ignore) {        // (the whole workgroup's)
             if (threadIdx.x == 0) finish_long_row(a, e, r, Given{label, 0.f, 0.f, 0.f, 0.f}, 0.f, 1.f);
-            clear_row(q, n, THREADS);
+            if (FUSED) clear_row(q, n, THREADS);
             continue;
         }
         const T* p = row_start<T>(a, r);
@@ -462,6 +462,7 @@ template <class T, int NV, int THREADS> __global__ void __launch_bounds__(THREAD
         take<T>(f1, top, sum);
         join_workgroup<T, THREADS / 64>(top, sum, waves);
         if (threadIdx.x == 0) row_end = finish_long_row(a, e, r, in, top, sum);
+        if (!FUSED) continue;
         __syncthreads();
         const End end = row_end;
         __syncthreads();    // (row_end is written again)
@@ -714,6 +715,13 @@ int row_splits(int64_t rows, int64_t classes, int vec) {
     return (int)(want < most ? want : most);
 }
 
+// Few rows: a workgroup of 1024 holds a row (4 or 8 vectors per work-item), which spares the launch that joins parts: 256 x 32000 bf16 10.8 -> 5.9 us,
+// 128 x 65536 10.5 -> 7.6.  A very few rows of more than 4 vectors are faster in parts (16 x 50001 7.3, held 8.2), and so are more rows than
+// compute units, of which each holds one at a time (512 x 8192 9.5, held 9.7; 1024 x 8192 10.5, 17.8).
+bool one_launch(int64_t rows, int64_t classes, int vec) {
+    return rows <= num_cus() && classes <= (rows < 32 ? 4 : 8) * 1024 * vec;
+}
+
 int64_t part_of(int64_t classes, int splits, int vec) {
     const int64_t step = 256 * vec, n = (classes + splits - 1) / splits;
     return (n + step - 1) / step * step;
@@ -742,7 +750,7 @@ int check_rows(const sd_label_rows* in, const char* who, Rows* a) {
 
 int64_t split_floats(const sd_label_rows* in) {
     const int vec = vec_of(in->dtype);
-    if (group_of(in->rows, in->classes, vec).shift >= 0) return 0;
+    if (group_of(in->rows, in->classes, vec).shift >= 0 || one_launch(in->rows, in->classes, vec)) return 0;
     const int splits = row_splits(in->rows, in->classes, vec);
     return splits > 1 ? 2 * in->rows * splits : 0;
 }
@@ -772,11 +780,18 @@ int launch_rows(const sd_label_rows* in, const Rows& a, const Finish& e, const G
         if (g) {
             const dim3 grid(blocks_for(a.rows));
             const int64_t vecs = (a.classes + vec - 1) / vec;
-            if (vecs <= 4 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 256>), grid, dim3(256), 0, stream, a, e, grad);
-            else if (vecs <= 8 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 256>), grid, dim3(256), 0, stream, a, e, grad);
-            else if (vecs <= 16 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 256>), grid, dim3(256), 0, stream, a, e, grad);
-            else if (vecs <= 16 * 512) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 512>), grid, dim3(512), 0, stream, a, e, grad);
-            else hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 1024>), grid, dim3(1024), 0, stream, a, e, grad);
+            if (vecs <= 4 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 256, true>), grid, dim3(256), 0, stream, a, e, grad);
+            else if (vecs <= 8 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 256, true>), grid, dim3(256), 0, stream, a, e, grad);
+            else if (vecs <= 16 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 256, true>), grid, dim3(256), 0, stream, a, e, grad);
+            else if (vecs <= 16 * 512) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 512, true>), grid, dim3(512), 0, stream, a, e, grad);
+            else hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 1024, true>), grid, dim3(1024), 0, stream, a, e, grad);
+            return;
+        }
+        if (one_launch(a.rows, a.classes, vec)) {
+            const dim3 grid((unsigned)a.rows);
+            const int64_t vecs = (a.classes + vec - 1) / vec;
+            if (vecs <= 4 * 1024) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 1024, false>), grid, dim3(1024), 0, stream, a, e, grad);
+            else hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 1024, false>), grid, dim3(1024), 0, stream, a, e, grad);
             return;
         }
         int splits = row_splits(a.rows, a.classes, vec);
