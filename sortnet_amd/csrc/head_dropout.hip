@@ -3,8 +3,7 @@
 // call with the same seed makes the same mask again.
 // One word serves two neighbouring values: pair j = i / 2 stands at column j mod 2^15 of row j / 2^15; the word is mixed with two keys of
 // its row, so that the words of two rows are no shifted copies of each other (one key of 32 bits leaves 2^32 sequences that overlap).
-// Bound by the bytes: 2^27 values bf16 82 us, 6.5 TB/s (a copy 99 us), three times 2^26 fp32 284 us, 5.7 TB/s.  Results are stored past the
-// caches (108 -> 82 us, 2^22 values fp32 6.0 -> 4.7), and inputs that the last-level cache cannot hold are read past it (292 -> 284).
+// Bound by the bytes.  Results are stored past the caches (2^26 values bf16 90 -> 78 us for two tensors in turn).
 #include <cmath>
 #include <type_traits>
 #include "label_rows.h"
@@ -22,68 +21,50 @@ struct DropArgs {
 
 __device__ __forceinline__ uint32_t drop_word(uint32_t key, uint32_t other, uint32_t col) { return rng_mix(rng_word(key, col) ^ other); }
 
-// A workgroup takes 256 UNROLL vectors of 16 bytes of each of COUNT tensors at a time; these lie in one row of the generator (they are a
-// power of two, at most 2^13 values), so the two keys are the workgroup's.
-template <class T, int COUNT, int UNROLL> __global__ void __launch_bounds__(256) dropout_kernel(DropArgs a) {
-    constexpr int V = Elem<T>::kVec, kStep = 256 * UNROLL * V;
-    static_assert(kStep <= 65536 && 65536 % kStep == 0, "a step within one row of the generator");
+// A workgroup takes 256 vectors of 16 bytes of each of COUNT tensors; these lie in one row of the generator, so the two keys are the
+// workgroup's.  (Several vectors per work-item on their way lost: 2^27 values bf16, two tensors in turn, 173 us, four vectors 184.)
+template <class T, int COUNT> __global__ void __launch_bounds__(256) dropout_kernel(DropArgs a) {
+    constexpr int V = Elem<T>::kVec, kStep = 256 * V;
+    static_assert(65536 % kStep == 0, "a step within one row of the generator");
     const uint32_t seed = a.seeds ? (uint32_t)*a.seeds : a.seed;
-    const bool far = a.n * (int64_t)sizeof(T) * COUNT > kCached;
+    const int at = (int)threadIdx.x * V;
     for (int64_t base = (int64_t)blockIdx.x * kStep; base < a.n; base += (int64_t)gridDim.x * kStep) {
+        const bool whole = base + at + V <= a.n;
+        u32x4 v[COUNT];
+        #pragma unroll
+        for (int t = 0; t < COUNT; t++)
+            if (whole) v[t] = load16(static_cast<const T*>(a.x[t]) + base + at);
         const uint32_t row = (uint32_t)(base >> 16), col = (uint32_t)(base & 0xffff) >> 1;
         const uint32_t key = rng_row_key(seed, 5u, row), other = rng_row_key(seed, 6u, row);
-        u32x4 v[COUNT][UNROLL];
+        bool keep[V];
         #pragma unroll
-        for (int t = 0; t < COUNT; t++) {
-            #pragma unroll
-            for (int u = 0; u < UNROLL; u++) {
-                const int at = (u * 256 + (int)threadIdx.x) * V;
-                if (base + at + V <= a.n) {
-                    const T* x = static_cast<const T*>(a.x[t]) + base + at;
-                    v[t][u] = far ? stream16(x) : load16(x);
-                }
-            }
+        for (int k = 0; k < V / 2; k++) {
+            const uint32_t w = drop_word(key, other, col + at / 2 + k);
+            keep[2 * k] = (w & 0xffffu) < a.limit;
+            keep[2 * k + 1] = (w >> 16) < a.limit;
         }
         #pragma unroll
-        for (int u = 0; u < UNROLL; u++) {
-            const int at = (u * 256 + (int)threadIdx.x) * V;
-            bool keep[V];
-            #pragma unroll
-            for (int k = 0; k < V / 2; k++) {
-                const uint32_t w = drop_word(key, other, col + at / 2 + k);
-                keep[2 * k] = (w & 0xffffu) < a.limit;
-                keep[2 * k + 1] = (w >> 16) < a.limit;
-            }
-            #pragma unroll
-            for (int t = 0; t < COUNT; t++) {
-                if (base + at + V <= a.n) {
-                    float f[V];
-                    Elem<T>::unpack(v[t][u], f);
-                    #pragma unroll
-                    for (int k = 0; k < V; k++) f[k] = keep[k] ? f[k] * a.scale : 0.f;
-                    put_stream16(static_cast<T*>(a.y[t]) + base + at, Elem<T>::pack(f));
-                } else {
-                    const T* x = static_cast<const T*>(a.x[t]) + base + at;
-                    T* y = static_cast<T*>(a.y[t]) + base + at;
-                    #pragma unroll
-                    for (int k = 0; k < V; k++)
-                        if (base + at + k < a.n) y[k] = keep[k] ? Elem<T>::put(Elem<T>::get(x[k]) * a.scale) : T{};
-                }
+        for (int t = 0; t < COUNT; t++) {
+            const T* x = static_cast<const T*>(a.x[t]) + base + at;
+            T* y = static_cast<T*>(a.y[t]) + base + at;
+            if (whole) {
+                float f[V];
+                Elem<T>::unpack(v[t], f);
+                #pragma unroll
+                for (int k = 0; k < V; k++) f[k] = keep[k] ? f[k] * a.scale : 0.f;
+                put_stream16(y, Elem<T>::pack(f));
+            } else {
+                #pragma unroll
+                for (int k = 0; k < V; k++)
+                    if (base + at + k < a.n) y[k] = keep[k] ? Elem<T>::put(Elem<T>::get(x[k]) * a.scale) : T{};
             }
         }
     }
 }
 
-template <class T, int COUNT, int UNROLL> void launch_dropout(const DropArgs& a, hipStream_t stream) {
-    const int64_t step = 256 * UNROLL * Elem<T>::kVec, want = (a.n + step - 1) / step;
-    hipLaunchKernelGGL((dropout_kernel<T, COUNT, UNROLL>), dim3((unsigned)(want < (1 << 22) ? want : (1 << 22))), dim3(256), 0, stream, a);
-}
-
-// Several vectors of a work-item on their way where there is work for all compute units, one where there is not.
 template <class T, int COUNT> void launch_dropout(const DropArgs& a, hipStream_t stream) {
-    constexpr int kUnroll = COUNT == 1 ? 4 : 2;
-    if (a.n >= (int64_t)num_cus() * 4 * 256 * kUnroll * Elem<T>::kVec) launch_dropout<T, COUNT, kUnroll>(a, stream);
-    else launch_dropout<T, COUNT, 1>(a, stream);
+    const int64_t step = 256 * Elem<T>::kVec, want = (a.n + step - 1) / step;
+    hipLaunchKernelGGL((dropout_kernel<T, COUNT>), dim3((unsigned)(want < (1 << 22) ? want : (1 << 22))), dim3(256), 0, stream, a);
 }
 
 }  // namespace sd

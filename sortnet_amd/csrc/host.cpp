@@ -709,7 +709,7 @@ Tensor label_log_probs(const Tensor& outputs, const Tensor& targets, int64_t ign
 
 std::pair<Tensor, Tensor> preference_loss(const Tensor& outputs, const Tensor& targets, const Tensor& ref_in, const OptTensor& offsets_in, double beta,
                                           double smoothing, int64_t ignore) {
-    reverse_mode_only("preference_loss", outputs);
+    reverse_mode_only("preference_loss", outputs, ref_in);
     const bool grad = want_grad(outputs);
     Tensor loss, rewards, z, labels;
     Work work;
@@ -750,7 +750,8 @@ std::pair<Tensor, Tensor> preference_loss(const Tensor& outputs, const Tensor& t
 
 std::pair<Tensor, Tensor> policy_loss(const Tensor& outputs, const Tensor& targets, const Tensor& old_in, const Tensor& advantages, const OptTensor& ref_in,
                                       double clip_low, double clip_high, double kl, int64_t ignore) {
-    reverse_mode_only("policy_loss", outputs);
+    reverse_mode_only("policy_loss", outputs, old_in, advantages);
+    if (ref_in && ref_in->defined()) reverse_mode_only("policy_loss", *ref_in);
     const bool grad = want_grad(outputs);
     Tensor loss, means, z, labels, made;
     Work work;

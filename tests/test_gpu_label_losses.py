@@ -62,7 +62,7 @@ def check_gradient(grad, z, labels, weight, weight_error, what):
     assert (grad[labels == IGNORE] == 0).all(), what
 
 
-SHAPES = [(1, 1), (3, 1), (5, 2), (9, 3), (512, 10), (77, 33), (7, 257), (300, 1000), (64, 2048), (13, 2049), (9, 4096), (5, 4097), (3, 16385), (1, 50001), (700, 8200), (2, 131072)]
+SHAPES = [(1, 1), (3, 1), (5, 2), (9, 3), (512, 10), (77, 33), (7, 257), (300, 1000), (64, 2048), (13, 2049), (9, 4096), (5, 4097), (3, 16385), (1, 50001), (700, 8200), (2, 131072), (40, 20000), (33, 60001), (2100, 8200), (70, 131072)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -496,6 +496,81 @@ def test_what_is_refused():
         leaf.mul_(2.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(lp.sum(), leaf)
+
+
+@pytest.mark.parametrize("rows, classes, dtype", [(1100, 131072, torch.bfloat16), (4400, 16389, torch.float32)])
+def test_logits_larger_than_the_caches(rows, classes, dtype):
+    """More than 256 MiB of logits: some rows are read past the caches, with each of the losses."""
+    assert rows * classes * torch.finfo(dtype).bits // 8 > 256 << 20
+    z, labels, g = make(rows, classes, dtype, 77, ignored=0.1)
+    z.requires_grad_()
+    up = torch.randn(rows, generator=g).cuda()
+    lp = losses.label_log_probs(z, labels)
+    want, _, _, tol = exact_rows(z, labels)
+    close(lp.detach(), want, tol, "log probs")
+    check_gradient(torch.autograd.grad(lp, z, up)[0], z, labels, up.double(), torch.zeros_like(up).double(), "gradient")
+    ref = want.float() + 0.3 * torch.randn(rows, generator=g).cuda()
+    pw = exact_preference(z, labels, ref, [0, rows // 3, rows // 2, rows // 2 + 7, rows - 2], 0.1, 0.0)
+    loss, rewards = losses.preference_loss(z, labels, ref, offsets=torch.tensor([0, rows // 3, rows // 2, rows // 2 + 7, rows - 2], device="cuda"))
+    close(loss.detach(), pw[0], pw[1], "loss")
+    close(rewards, pw[2], pw[3], "rewards")
+    check_gradient(torch.autograd.grad(loss, z)[0], z, labels, pw[4], pw[5], "gradient")
+    old = want.float() - away_from_borders(0.25 * torch.randn(rows, generator=g).cuda(), 0.2, 0.2)
+    pol = exact_policy(z, labels, old, up, ref, 0.2, 0.2, 0.1)
+    loss, stats = losses.policy_loss(z, labels, old, up, ref_log_probs=ref, kl_coef=0.1)
+    close(loss.detach(), pol[0], pol[1], "loss")
+    close(stats, pol[2], pol[3], "stats")
+    check_gradient(torch.autograd.grad(loss, z)[0], z, labels, pol[4], pol[5], "gradient")
+
+
+def test_two_threads_and_a_first_call_under_capture():
+    """Calls of two host threads on one stream give what each gives alone; a graph needs no call before it."""
+    import threading
+    data = [make(64, 5000 + 100 * k, torch.float32, 30 + k, ignored=0.0) for k in range(2)]
+    wants = []
+    for z, labels, _ in data:
+        leaf = z.clone().requires_grad_()
+        loss, rewards = losses.preference_loss(leaf, labels, torch.zeros(64, device="cuda"))
+        wants.append((loss.detach(), rewards, torch.autograd.grad(loss, leaf)[0]))
+    wrong = []
+
+    def work(k):
+        z, labels, _ = data[k]
+        for _ in range(20):
+            leaf = z.clone().requires_grad_()
+            loss, rewards = losses.preference_loss(leaf, labels, torch.zeros(64, device="cuda"))
+            got = (loss.detach(), rewards, torch.autograd.grad(loss, leaf)[0])
+            if not all(torch.equal(a, b) for a, b in zip(got, wants[k])):
+                wrong.append(k)
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    z, labels, _ = make(5, 90001, torch.float16, 9)
+    zero = torch.zeros(5, device="cuda")
+    stream, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        outs = [losses.label_log_probs(z, labels), *losses.policy_loss(z, labels, zero, zero)]
+    eager = [losses.label_log_probs(z, labels), *losses.policy_loss(z, labels, zero, zero)]
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, eager))
+
+
+def test_transforms_are_refused():
+    z, labels, _ = make(4, 3, torch.float32, 1, ignored=0.0)
+    r = torch.zeros(4, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual, dual_r = torch.autograd.forward_ad.make_dual(z, torch.ones_like(z)), torch.autograd.forward_ad.make_dual(r, torch.ones_like(r))
+        for bad in (lambda: losses.label_log_probs(dual, labels), lambda: losses.preference_loss(dual, labels, r), lambda: losses.preference_loss(z, labels, dual_r),
+                    lambda: losses.policy_loss(z, labels, dual_r, r), lambda: losses.policy_loss(z, labels, r, dual_r), lambda: losses.policy_loss(z, labels, r, r, ref_log_probs=dual_r)):
+            with pytest.raises(NotImplementedError):
+                bad()
 
 
 def test_rows_beyond_32_bit_offsets():
