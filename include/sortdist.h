@@ -346,7 +346,8 @@ typedef struct {
  * sd_label_log_probs (scratch may be NULL where this is 0), 1 for the losses. */
 int64_t sd_label_scratch(const sd_label_rows* rows, int loss);
 
-/* log_probs[r] = log softmax(row r)[label], 0 where ignored.  stats (rows, 2; may be NULL) receives what sd_label_gradient needs. */
+/* log_probs[r] = log softmax(row r)[label], 0 where ignored.  stats (rows, 2; 8-byte aligned; may be NULL) receives what
+ * sd_label_gradient needs. */
 int sd_label_log_probs(const sd_label_rows* rows, float* log_probs, float* stats, float* scratch, sd_stream_t stream);
 
 /* Paired answers: answer a holds the rows offsets[a] .. offsets[a + 1] (2 pairs + 1 entries of offset_bytes = 4 or 8 bytes, not

@@ -701,7 +701,7 @@ Tensor label_log_probs(const Tensor& outputs, const Tensor& targets, int64_t ign
             const sd_label_rows a = label_rows(z, labels, ignore);
             work = Work(z, a, false, grad);
             require(sd_label_log_probs(&a, floats(y, "log_probs"), work.stats, work.scratch, stream_of(z)), "sd_label_log_probs");
-        } else work.whole = y;
+        } else work.whole = new_floats(z, {0});
     }
     if (grad) attach_labels(y, LabelNode::VALUES, outputs, z, labels, ignore, work.whole, {});
     return y;

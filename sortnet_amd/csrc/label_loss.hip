@@ -715,11 +715,12 @@ int row_splits(int64_t rows, int64_t classes, int vec) {
     return (int)(want < most ? want : most);
 }
 
-// Few rows: a workgroup of 1024 holds a row (4 or 8 vectors per work-item), which spares the launch that joins parts: 256 x 32000 bf16 10.8 -> 5.9 us,
-// 128 x 65536 10.5 -> 7.6.  A very few rows of more than 4 vectors are faster in parts (16 x 50001 7.3, held 8.2), and so are more rows than
-// compute units, of which each holds one at a time (512 x 8192 9.5, held 9.7; 1024 x 8192 10.5, 17.8).
+// Rows that would be read in parts to fill the card: where a workgroup can hold a row it is read whole, which spares the launch that joins
+// the parts: 128 x 8192 bf16 7.1 -> 3.9 us, 512 x 16384 10.2 -> 5.3, 1024 x 32000 18.6 -> 14.3 (from 2048 rows on, that are read whole anyway, it makes
+// no difference).  Rows for a workgroup of 512, of which fewer run at once: 256 x 50001 11.8 -> 8.7, but 16 rows 7.3 -> 8.5 and 1024 23.8 -> 24.0.
 bool one_launch(int64_t rows, int64_t classes, int vec) {
-    return rows <= num_cus() && classes <= (rows < 32 ? 4 : 8) * 1024 * vec;
+    const int64_t vecs = (classes + vec - 1) / vec;
+    return rows < 2048 && (vecs <= 16 * 256 || (vecs <= 16 * 512 && rows >= 32 && rows <= 512));
 }
 
 int64_t part_of(int64_t classes, int splits, int vec) {
@@ -744,7 +745,14 @@ int check_rows(const sd_label_rows* in, const char* who, Rows* a) {
     SD_REQUIRE(in->classes > 0 && in->classes < (1ll << 31), "%s: classes=%lld outside 1..2^31-1", who, (long long)in->classes);
     SD_REQUIRE(in->inner > 0 && in->rows % in->inner == 0 && in->inner < (1ll << 31), "%s: inner=%lld does not divide rows=%lld", who, (long long)in->inner, (long long)in->rows);
     SD_REQUIRE(in->logits && in->labels, "%s: null logits or labels", who);
+    SD_REQUIRE((reinterpret_cast<uintptr_t>(in->logits) & (in->dtype == SD_FLOAT32 ? 3 : 1)) == 0 && (reinterpret_cast<uintptr_t>(in->labels) & 7) == 0,
+               "%s: logits or labels are not aligned to their type", who);
     *a = Rows{in->logits, in->labels, in->rows, in->classes, in->outer_stride, in->inner_stride, in->ignore_index, (uint32_t)in->inner};
+    return SD_OK;
+}
+
+int check_work(const char* who, const float* stats, const float* scratch) {
+    SD_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0 && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "%s: stats must be aligned to 8 bytes, scratch to 16", who);
     return SD_OK;
 }
 
@@ -777,21 +785,17 @@ int launch_rows(const sd_label_rows* in, const Rows& a, const Finish& e, const G
             });
             return;
         }
-        if (g) {
+        if (g || one_launch(a.rows, a.classes, vec)) {
             const dim3 grid(blocks_for(a.rows));
             const int64_t vecs = (a.classes + vec - 1) / vec;
-            if (vecs <= 4 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 256, true>), grid, dim3(256), 0, stream, a, e, grad);
-            else if (vecs <= 8 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 256, true>), grid, dim3(256), 0, stream, a, e, grad);
-            else if (vecs <= 16 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 256, true>), grid, dim3(256), 0, stream, a, e, grad);
-            else if (vecs <= 16 * 512) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 512, true>), grid, dim3(512), 0, stream, a, e, grad);
-            else hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 1024, true>), grid, dim3(1024), 0, stream, a, e, grad);
-            return;
-        }
-        if (one_launch(a.rows, a.classes, vec)) {
-            const dim3 grid((unsigned)a.rows);
-            const int64_t vecs = (a.classes + vec - 1) / vec;
-            if (vecs <= 4 * 1024) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 1024, false>), grid, dim3(1024), 0, stream, a, e, grad);
-            else hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 1024, false>), grid, dim3(1024), 0, stream, a, e, grad);
+            const auto held = [&](auto fused) {
+                if (vecs <= 4 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 256, fused.value>), grid, dim3(256), 0, stream, a, e, grad);
+                else if (vecs <= 8 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 256, fused.value>), grid, dim3(256), 0, stream, a, e, grad);
+                else if (vecs <= 16 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 256, fused.value>), grid, dim3(256), 0, stream, a, e, grad);
+                else if (vecs <= 16 * 512) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 512, fused.value>), grid, dim3(512), 0, stream, a, e, grad);
+                else if constexpr (fused.value) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 1024, true>), grid, dim3(1024), 0, stream, a, e, grad);
+            };
+            if (g) held(std::true_type()); else held(std::false_type());
             return;
         }
         int splits = row_splits(a.rows, a.classes, vec);
@@ -821,6 +825,7 @@ extern "C" int sd_label_log_probs(const sd_label_rows* in, float* log_probs, flo
     sd::CallGuard call_guard;
     Rows a;
     if (int rc = check_rows(in, "label_log_probs", &a)) return rc;
+    if (int rc = check_work("label_log_probs", stats, scratch)) return rc;
     SD_REQUIRE(log_probs && (scratch || split_floats(in) == 0), "label_log_probs: null output or scratch");
     Finish e{};
     e.kind = kValues;
@@ -834,6 +839,7 @@ extern "C" int sd_preference_loss(const sd_label_rows* in, const float* ref, con
     sd::CallGuard call_guard;
     Rows a;
     if (int rc = check_rows(in, "preference_loss", &a)) return rc;
+    if (int rc = check_work("preference_loss", stats, scratch)) return rc;
     SD_REQUIRE(ref && rewards && loss && scratch, "preference_loss: null argument");
     SD_REQUIRE(!stats == !weight, "preference_loss: the gradient needs both stats and weight");
     SD_REQUIRE(pairs > 0, "preference_loss: pairs=%d must be positive", pairs);
@@ -877,6 +883,7 @@ extern "C" int sd_policy_loss(const sd_label_rows* in, const float* old_log_prob
     sd::CallGuard call_guard;
     Rows a;
     if (int rc = check_rows(in, "policy_loss", &a)) return rc;
+    if (int rc = check_work("policy_loss", stats, scratch)) return rc;
     SD_REQUIRE(old_log_probs && advantages && scale && loss && means && scratch, "policy_loss: null argument");
     SD_REQUIRE(!stats == !weight, "policy_loss: the gradient needs both stats and weight");
     SD_REQUIRE(!grad || stats, "policy_loss: a gradient that leaves with the rows needs stats and weight, too");
@@ -916,6 +923,7 @@ extern "C" int sd_label_gradient(const sd_label_rows* in, const float* stats, co
     sd::CallGuard call_guard;
     Rows a;
     if (int rc = check_rows(in, "label_gradient", &a)) return rc;
+    if (int rc = check_work("label_gradient", stats, nullptr)) return rc;
     SD_REQUIRE(stats && weight && grad, "label_gradient: null argument");
     SD_REQUIRE(!unless_one || scale2, "label_gradient: unless_one needs scale2");
     const Gradient g{reinterpret_cast<const float2*>(stats), weight, scale, scale2, grad, unless_one != 0};

@@ -51,6 +51,22 @@ def test_preferences_without_a_meaning(bad, match):
         _lib.call("sd_preference_loss", _rows(), *dict(good, **bad).values(), p, p, p, p, p, None)
 
 
+def test_buffers_out_of_line():
+    p = 1 << 20
+    for rows in (_rows(logits=p + 2), _rows(logits=p + 1, dtype=1), _rows(labels=p + 4)):
+        with pytest.raises(RuntimeError, match="aligned"):
+            _lib.call("sd_label_log_probs", rows, p, p, p, None)
+    for stats, scratch in ((p + 4, p), (p, p + 8)):
+        with pytest.raises(RuntimeError, match="aligned"):
+            _lib.call("sd_label_log_probs", _rows(), p, stats, scratch, None)
+        with pytest.raises(RuntimeError, match="aligned"):
+            _lib.call("sd_preference_loss", _rows(), p, None, 0, 1, 2, 0.1, 0.0, stats, p, p, p, scratch, None)
+        with pytest.raises(RuntimeError, match="aligned"):
+            _lib.call("sd_policy_loss", _rows(), p, p, 0, 1, None, 0.2, 0.2, 0.0, stats, p, p, None, p, p, scratch, None)
+    with pytest.raises(RuntimeError, match="aligned"):
+        _lib.call("sd_label_gradient", _rows(), p + 4, p, None, None, 0, p, None)
+
+
 def test_halves_of_the_gradient():
     p = 1 << 20
     with pytest.raises(RuntimeError, match="both"):
