@@ -622,13 +622,13 @@ template <int WAVES> __global__ void __launch_bounds__(256) preference_kernel(Pa
 }
 
 // Means of the policy's terms over the kept rows (over one where there are none); `scale` = 1 / that number (or null: it has been found).
-__global__ void __launch_bounds__(256) policy_sums_kernel(const double* terms, int64_t count, double kl, float* loss, float* stats, float* scale,
+__global__ void __launch_bounds__(1024) policy_sums_kernel(const double* terms, int64_t count, double kl, float* loss, float* stats, float* scale,
                                                           double* parts, uint32_t* ticket) {
-    __shared__ double waves[4][4];
+    __shared__ double waves[16][4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double s[4] = {0.0, 0.0, 0.0, 0.0};
     #pragma unroll 4
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 1024) {
         const double2 t = reinterpret_cast<const double2*>(terms)[2 * i], u = reinterpret_cast<const double2*>(terms)[2 * i + 1];
         s[0] += t.x; s[1] += t.y; s[2] += u.x; s[3] += u.y;
     }
@@ -639,7 +639,14 @@ __global__ void __launch_bounds__(256) policy_sums_kernel(const double* terms, i
     }
     __syncthreads();
     #pragma unroll
-    for (int k = 0; k < 4; k++) s[k] = waves[0][k] + waves[1][k] + waves[2][k] + waves[3][k];
+    for (int k = 0; k < 4; k++) s[k] = 0.0;
+    if (wave == 0) {
+        #pragma unroll
+        for (int k = 0; k < 4; k++) {
+            s[k] = lane < 16 ? waves[lane][k] : 0.0;
+            for (int o = 8; o > 0; o >>= 1) s[k] += __shfl_xor(s[k], o);
+        }
+    }
     if (gridDim.x > 1) {
         if (threadIdx.x == 0) {
             #pragma unroll
@@ -709,9 +716,10 @@ template <class F> void with_vectors(int vectors, F&& f) {
     }
 }
 
-// Parts of a long row: so many that there are 2048 workgroups (eight for each compute unit), none with less than one vector per work-item.
+// Parts of a long row: so many that there are 704 workgroups (2.75 for each compute unit), none with less than one vector per work-item.  More parts
+// lost: 2000 x 50001 bf16 34.5 us whole, in two parts 37.4; 700 x 131072 30.7 and 34.7; 1000 x 131072 41.7 and 45.
 int row_splits(int64_t rows, int64_t classes, int vec) {
-    const int64_t want = (2048 + rows - 1) / rows, most = (classes + 256 * vec - 1) / (256 * vec);
+    const int64_t want = (704 + rows - 1) / rows, most = (classes + 256 * vec - 1) / (256 * vec);
     return (int)(want < most ? want : most);
 }
 
@@ -912,8 +920,8 @@ extern "C" int sd_policy_loss(const sd_label_rows* in, const float* old_log_prob
         if (blocks > 1) hipLaunchKernelGGL(count_rows_kernel<int>, dim3(1), dim3(1024), 0, s, counts, (int64_t)blocks, (int64_t)0, nullptr, scale);
     }
     if (int rc = launch_rows(in, a, e, grad ? &g : nullptr, scratch + kSumFloats + 8 * terms, s)) return rc;
-    const int64_t want = (terms + 4095) / 4096;
-    hipLaunchKernelGGL(policy_sums_kernel, dim3((unsigned)(want < kSumBlocks ? want : kSumBlocks)), dim3(256), 0, s, e.terms, terms, kl, loss, means, grad ? nullptr : scale,
+    const int64_t want = (terms + 16383) / 16384;
+    hipLaunchKernelGGL(policy_sums_kernel, dim3((unsigned)(want < kSumBlocks ? want : kSumBlocks)), dim3(1024), 0, s, e.terms, terms, kl, loss, means, grad ? nullptr : scale,
                        reinterpret_cast<double*>(scratch + 4), e.ticket);
     return check_launch("policy_sums_kernel");
 }
