@@ -85,8 +85,10 @@ template <class T> __device__ __forceinline__ Given given(const Rows& a, const F
 // a quotient and its remainder, so that only sums are formed in 64 bits.
 // A log probability and its distance from another model's are differences of numbers many times their size; in 32 bits each step of
 // them would be off by up to 2.4e-7 where log probabilities lie between 4 and 8, which the mean over a batch shows.
-__device__ __forceinline__ double log_of_sum(float s) {
+__device__ __forceinline__ double log_of_sum(double sum) {
+    const float s = (float)sum;
     if (!(s > 0.f && s < INFINITY)) return (double)logf(s);
+    const float past = (float)(sum - (double)s);        // log(s + past) = log(s) + past / s, past being 2^-24 of s
     const uint32_t bits = __float_as_uint(s);
     int e = (int)(bits >> 23) - 127;
     float m = __uint_as_float((bits & 0x7fffffu) | 0x3f800000u);
@@ -95,15 +97,15 @@ __device__ __forceinline__ double log_of_sum(float s) {
     const float r = __builtin_amdgcn_rcpf(d), t = f * r, tl = fmaf(-t, dl, fmaf(-t, d, f)) * r, u = t * t;
     float p = 1.f / 13.f;
     p = fmaf(p, u, 1.f / 11.f); p = fmaf(p, u, 1.f / 9.f); p = fmaf(p, u, 1.f / 7.f); p = fmaf(p, u, 1.f / 5.f); p = fmaf(p, u, 1.f / 3.f);
-    return fma((double)e, 0.69314718055994530942, (double)(2.f * t)) + (double)(2.f * fmaf(t * u, p, tl));
+    return fma((double)e, 0.69314718055994530942, (double)(2.f * t)) + (double)fmaf(2.f, fmaf(t * u, p, tl), past * __builtin_amdgcn_rcpf(s));
 }
 
 struct End { float top, inverse, weight, surrogate, divergence, clipped, kept; };
 
-__device__ __forceinline__ End finish_row(const Rows& a, const Finish& e, int64_t r, const Given& g, float top, float sum) {
+__device__ __forceinline__ End finish_row(const Rows& a, const Finish& e, int64_t r, const Given& g, float top, double sum) {
     const bool kept = g.label != a.ignore;
     top = finite(top);
-    End end{kept ? top : 0.f, 1.f / sum, 0.f, 0.f, 0.f, 0.f, 0.f};
+    End end{kept ? top : 0.f, 1.f / (float)sum, 0.f, 0.f, 0.f, 0.f, 0.f};
     const double lp = kept ? (double)g.at - (double)top - log_of_sum(sum) : 0.0;
     if (e.stats) e.stats[r] = make_float2(end.top, end.inverse);
     if (e.kind != kPolicy) {
@@ -158,6 +160,20 @@ template <class T, int N> __device__ __forceinline__ void slopes(float (&f)[N], 
     }
 }
 
+// Sums of a row: exponentials of a few vectors in pairs, in 32 bits, and these sums in 64 (an addition to a sum in 32 bits that has the
+// largest value, 1, in it is off by up to 6e-8, and there are hundreds of them).
+template <int N> __device__ __forceinline__ float tree(const float (&f)[N]) {
+    float s[N];
+    #pragma unroll
+    for (int i = 0; i < N; i++) s[i] = f[i];
+    #pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+        #pragma unroll
+        for (int i = 0; i < o; i++) s[i] += s[i + o];
+    }
+    return s[0];
+}
+
 // ---- short rows: 2^shift lanes of a wavefront hold a row in registers, NV vectors each ---------------------------------------
 // The last vector of a row of at least one ends with the row and overlaps the one before it; a shorter row is one vector, padded with -inf.
 template <class T, int NV> struct Held {
@@ -193,9 +209,9 @@ template <class T, int NV> struct Held {
         for (int o = (1 << shift) >> 1; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
         return t;
     }
-    __device__ __forceinline__ float sum(float top) const {
+    __device__ __forceinline__ double sum(float top) const {
         const float b = finite(top);
-        float s = 0.f;
+        double s = 0.0;
         #pragma unroll
         for (int k = 0; k < NV; k++)
             if (index(k) < vecs) {
@@ -208,8 +224,7 @@ template <class T, int NV> struct Held {
                     #pragma unroll
                     for (int i = 0; i < V; i++) f[i] = i < past ? 0.f : f[i];
                 }
-                #pragma unroll
-                for (int i = 0; i < V; i++) s += f[i];
+                s += (double)tree(f);
             }
         for (int o = (1 << shift) >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
         return s;
@@ -252,7 +267,8 @@ template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) la
     for (int64_t r = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); r < a.rows; r += (int64_t)gridDim.x * per) {
         const int64_t label = a.labels[r];
         Given in{label, 0.f, 0.f, 0.f, 0.f};
-        float top = 0.f, sum = 1.f;
+        float top = 0.f;
+        double sum = 1.0;
         if (label != a.ignore) {
             row.load(row_start<T>(a, r));
             if (row.lane == 0) in = given<T>(a, e, r, label);
@@ -298,40 +314,42 @@ template <class T, int NV> __global__ void __launch_bounds__(256) label_gradient
 }
 
 // ---- long rows: a workgroup reads a row, or one of its parts ------------------------------------------------------------------
+struct Part { float top; double sum; };
+
 // (top, sum) of two parts of a row
-template <class T> __device__ __forceinline__ void join(float& top, float& sum, float top2, float sum2) {
+template <class T> __device__ __forceinline__ void join(float& top, double& sum, float top2, double sum2) {
     const float t = fmaxf(top, top2);
-    sum = sum * Elem<T>::exp(finite(top) - finite(t)) + sum2 * Elem<T>::exp(finite(top2) - finite(t));
+    sum = sum * (double)Elem<T>::exp(finite(top) - finite(t)) + sum2 * (double)Elem<T>::exp(finite(top2) - finite(t));
     top = t;
 }
 
-template <class T, int N> __device__ __forceinline__ void take(const float (&f)[N], float& top, float& sum) {
+template <class T, int N> __device__ __forceinline__ void take(float (&f)[N], float& top, double& sum) {
     float t = top;
     #pragma unroll
     for (int i = 0; i < N; i++) t = fmaxf(t, f[i]);
     const float b = finite(t);
-    float s = sum * Elem<T>::exp(finite(top) - b);
     #pragma unroll
-    for (int i = 0; i < N; i++) s += Elem<T>::exp(f[i] - b);
+    for (int i = 0; i < N; i++) f[i] = Elem<T>::exp(f[i] - b);
+    sum = sum * (double)Elem<T>::exp(finite(top) - b) + (double)tree(f);
     top = t;
-    sum = s;
 }
 
 // of all work-items of a workgroup, to its first
-template <class T, int WAVES> __device__ __forceinline__ void join_workgroup(float& top, float& sum, float2* waves) {
+template <class T, int WAVES> __device__ __forceinline__ void join_workgroup(float& top, double& sum, Part* waves) {
     for (int o = 32; o > 0; o >>= 1) {
-        const float t = __shfl_xor(top, o), s = __shfl_xor(sum, o);
+        const float t = __shfl_xor(top, o);
+        const double s = __shfl_xor(sum, o);
         join<T>(top, sum, t, s);
     }
-    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = make_float2(top, sum);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = Part{top, sum};
     __syncthreads();
     if (threadIdx.x == 0)
-        for (int k = 1; k < WAVES; k++) join<T>(top, sum, waves[k].x, waves[k].y);
+        for (int k = 1; k < WAVES; k++) join<T>(top, sum, waves[k].top, waves[k].sum);
     __syncthreads();        // (waves is written again)
 }
 
 // (top, sum) of this work-item's share of p[0 .. n), which `lanes` work-items read together
-template <class T, bool STREAM> __device__ __forceinline__ void scan(const T* p, int64_t n, int lane, int lanes, float& top, float& sum) {
+template <class T, bool STREAM> __device__ __forceinline__ void scan(const T* p, int64_t n, int lane, int lanes, float& top, double& sum) {
     constexpr int V = Elem<T>::kVec;
     const int64_t full = n / V;
     int64_t i = lane;
@@ -350,7 +368,7 @@ template <class T, bool STREAM> __device__ __forceinline__ void scan(const T* p,
         take<T>(f, top, sum);
     }
     for (int64_t j = full * V + lane; j < n; j += lanes) {
-        const float f[1] = {Elem<T>::get(p[j])};
+        float f[1] = {Elem<T>::get(p[j])};
         take<T>(f, top, sum);
     }
 }
@@ -404,31 +422,32 @@ template <class T, bool STREAM> __device__ __forceinline__ void grad_row(const T
 // 4096 x 131072 bf16 forward 183 -> 156 us, both passes 545 -> 495.
 template <class T> __device__ __forceinline__ bool beyond_cache(const Rows& a, int64_t r) { return r * a.classes * (int64_t)sizeof(T) >= kCached; }
 
-__device__ __forceinline__ End finish_long_row(const Rows& a, const Finish& e, int64_t r, const Given& g, float top, float sum) {
+__device__ __forceinline__ End finish_long_row(const Rows& a, const Finish& e, int64_t r, const Given& g, float top, double sum) {
     const End end = finish_row(a, e, r, g, top, sum);
     if (e.terms) store_terms(e.terms + 4 * r, end.surrogate, end.divergence, end.clipped, end.kept);
     return end;
 }
 
 // A workgroup per row, or per one of `splits` parts of a row, which then leaves its (top, sum) for join_rows_kernel.
-template <class T> __global__ void __launch_bounds__(256) label_long_rows_kernel(Rows a, Finish e, int splits, int64_t part, float2* parts) {
-    __shared__ float2 waves[4];
+template <class T> __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 5) label_long_rows_kernel(Rows a, Finish e, int splits, int64_t part, Part* parts) {
+    __shared__ Part waves[4];
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
     for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
         const int64_t back = splits == 1 ? b : b / splits, s = b - back * splits, r = a.rows - 1 - back, c0 = s * part;
         const int64_t n = a.classes - c0 < part ? a.classes - c0 : part;
-        float top = 0.f, sum = 1.f;
+        float top = 0.f;
+        double sum = 1.0;
         const int64_t label = a.labels[r];
         Given in{label, 0.f, 0.f, 0.f, 0.f};
         if (label != a.ignore) {        // (the whole workgroup's)
             if (threadIdx.x == 0 && splits == 1) in = given<T>(a, e, r, label);
-            top = -INFINITY; sum = 0.f;
+            top = -INFINITY; sum = 0.0;
             if (beyond_cache<T>(a, r)) scan<T, true>(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
             else scan<T, false>(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
             join_workgroup<T, 4>(top, sum, waves);
         }
         if (threadIdx.x == 0) {
-            if (splits > 1) parts[r * splits + s] = make_float2(top, sum);
+            if (splits > 1) parts[r * splits + s] = Part{top, sum};
             else finish_long_row(a, e, r, in, top, sum);
         }
     }
@@ -439,7 +458,7 @@ template <class T> __global__ void __launch_bounds__(256) label_long_rows_kernel
 // unit are more than the last level holds, 4096 x 131072 bf16 596 us; two passes of their own 515.)
 template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
     constexpr int V = Elem<T>::kVec, kChunk = 16 / V;
-    __shared__ float2 waves[THREADS / 64];
+    __shared__ Part waves[THREADS / 64];
     __shared__ End row_end;
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
     const int n = (int)a.classes, full = n / V, rest = full * V + (int)threadIdx.x;     // the values behind the last whole vector: one per work-item
@@ -450,7 +469,7 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
         const int64_t label = a.labels[r];
         T* q = static_cast<T*>(g.grad) + r * a.classes;
         if (label == a.ignore) {        // (the whole workgroup's)
-            if (threadIdx.x == 0) finish_long_row(a, e, r, Given{label, 0.f, 0.f, 0.f, 0.f}, 0.f, 1.f);
+            if (threadIdx.x == 0) finish_long_row(a, e, r, Given{label, 0.f, 0.f, 0.f, 0.f}, 0.f, 1.0);
             if (FUSED) clear_row(q, n, THREADS);
             continue;
         }
@@ -467,7 +486,8 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
         if (rest < n) last = p[rest];
         Given in{label, 0.f, 0.f, 0.f, 0.f};
         if (threadIdx.x == 0) in = given<T>(a, e, r, label);
-        float top = -INFINITY, sum = 0.f;
+        float top = -INFINITY;
+        double sum = 0.0;
         #pragma unroll
         for (int c = 0; c < NV; c += kChunk) {
             float f[kChunk * V];
@@ -475,7 +495,7 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
             for (int k = 0; k < kChunk; k++) Elem<T>::unpack(v[c + k], reinterpret_cast<float (&)[V]>(f[k * V]));
             take<T>(f, top, sum);
         }
-        const float f1[1] = {Elem<T>::get(last)};
+        float f1[1] = {Elem<T>::get(last)};
         take<T>(f1, top, sum);
         join_workgroup<T, THREADS / 64>(top, sum, waves);
         if (threadIdx.x == 0) row_end = finish_long_row(a, e, r, in, top, sum);
@@ -507,18 +527,20 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
 }
 
 // a wavefront per row joins the parts of label_long_rows_kernel
-template <class T> __global__ void __launch_bounds__(256) join_rows_kernel(Rows a, Finish e, int splits, const float2* parts) {
+template <class T> __global__ void __launch_bounds__(256) join_rows_kernel(Rows a, Finish e, int splits, const Part* parts) {
     const int lane = threadIdx.x & 63;
     for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
         const int64_t label = a.labels[r];
         Given in{label, 0.f, 0.f, 0.f, 0.f};
-        float top = 0.f, sum = 1.f;
+        float top = 0.f;
+        double sum = 1.0;
         if (label != a.ignore) {
             if (lane == 0) in = given<T>(a, e, r, label);
-            top = -INFINITY; sum = 0.f;
-            for (int k = lane; k < splits; k += 64) join<T>(top, sum, parts[r * splits + k].x, parts[r * splits + k].y);
+            top = -INFINITY; sum = 0.0;
+            for (int k = lane; k < splits; k += 64) join<T>(top, sum, parts[r * splits + k].top, parts[r * splits + k].sum);
             for (int o = 32; o > 0; o >>= 1) {
-                const float t = __shfl_xor(top, o), s = __shfl_xor(sum, o);
+                const float t = __shfl_xor(top, o);
+                const double s = __shfl_xor(sum, o);
                 join<T>(top, sum, t, s);
             }
         }
@@ -785,7 +807,7 @@ int64_t split_floats(const sd_label_rows* in) {
     const int vec = vec_of(in->dtype);
     if (group_of(in->rows, in->classes, vec).shift >= 0 || one_launch(in->rows, in->classes, vec)) return 0;
     const int splits = row_splits(in->rows, in->classes, vec);
-    return splits > 1 ? 2 * in->rows * splits : 0;
+    return splits > 1 ? (int64_t)(sizeof(Part) / sizeof(float)) * in->rows * splits : 0;
 }
 
 // parts of the policy's terms: one per workgroup of short rows, one per long row
@@ -826,7 +848,7 @@ int launch_rows(const sd_label_rows* in, const Rows& a, const Finish& e, const G
         int splits = row_splits(a.rows, a.classes, vec);
         const int64_t part = part_of(a.classes, splits, vec);
         splits = (int)((a.classes + part - 1) / part);
-        float2* out = reinterpret_cast<float2*>(parts);
+        Part* out = reinterpret_cast<Part*>(parts);
         hipLaunchKernelGGL(label_long_rows_kernel<T>, dim3(blocks_for(a.rows * splits)), dim3(256), 0, stream, a, e, splits, part, out);
         if (splits > 1) hipLaunchKernelGGL(join_rows_kernel<T>, dim3(blocks_for((a.rows + 3) / 4)), dim3(256), 0, stream, a, e, splits, out);
     });
