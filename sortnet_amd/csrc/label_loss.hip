@@ -57,10 +57,7 @@ template <class T> __device__ __forceinline__ const T* row_start(const Rows& a, 
     return static_cast<const T*>(a.logits) + o * a.outer_stride + i * a.inner_stride;
 }
 
-__device__ __forceinline__ double wave_total(double v) {
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-    return v;
-}
+__device__ __forceinline__ double wave_total(double v) { return group_total(v, 6); }
 
 __device__ __forceinline__ float finite(float top) { return fmaxf(top, -FLT_MAX); }
 
@@ -196,6 +193,11 @@ template <class T, int NV> struct Held {
             v[0] = Elem<T>::pack(f);
         }
     }
+    // What was derived from the vectors before is derived again afterwards: kept, it would be twice their registers.
+    __device__ __forceinline__ void again() {
+        #pragma unroll
+        for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
+    }
     __device__ __forceinline__ float top() const {
         float t = -INFINITY;
         #pragma unroll
@@ -206,8 +208,7 @@ template <class T, int NV> struct Held {
                 #pragma unroll
                 for (int i = 0; i < V; i++) t = fmaxf(t, f[i]);
             }
-        for (int o = (1 << shift) >> 1; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor(t, o));
-        return t;
+        return group_max(t, shift);
     }
     __device__ __forceinline__ double sum(float top) const {
         const float b = finite(top);
@@ -226,8 +227,7 @@ template <class T, int NV> struct Held {
                 }
                 s += (double)tree(f);
             }
-        for (int o = (1 << shift) >> 1; o > 0; o >>= 1) s += __shfl_xor(s, o);
-        return s;
+        return group_total(s, shift);
     }
     // the gradient of weight w; zeros, without a look at the values, where that is 0
     __device__ __forceinline__ void gradient(T* q, float top, float inverse, float w, int label, int stream_from) const {
@@ -273,6 +273,7 @@ template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) la
             row.load(row_start<T>(a, r));
             if (row.lane == 0) in = given<T>(a, e, r, label);
             top = row.top();
+            row.again();
             sum = row.sum(top);
         }
         End end{};
@@ -281,6 +282,7 @@ template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) la
             if (e.terms) { terms[0] += end.surrogate; terms[1] += end.divergence; terms[2] += end.clipped; terms[3] += end.kept; }
         }
         if (FUSED) {
+            row.again();
             const int lead = (threadIdx.x & 63) - row.lane;
             const float w = scaled(g, __shfl(end.weight, lead));
             row.gradient(static_cast<T*>(g.grad) + r * a.classes, __shfl(end.top, lead), __shfl(end.inverse, lead), w, (int)label, kStreamRow);
@@ -334,13 +336,16 @@ template <class T, int N> __device__ __forceinline__ void take(float (&f)[N], fl
     top = t;
 }
 
+// of all lanes of a wavefront
+template <class T> __device__ __forceinline__ void join_wave(float& top, double& sum) {
+    const float t = group_max(top, 6);
+    sum = group_total(sum * (double)Elem<T>::exp(finite(top) - finite(t)), 6);
+    top = t;
+}
+
 // of all work-items of a workgroup, to its first
 template <class T, int WAVES> __device__ __forceinline__ void join_workgroup(float& top, double& sum, Part* waves) {
-    for (int o = 32; o > 0; o >>= 1) {
-        const float t = __shfl_xor(top, o);
-        const double s = __shfl_xor(sum, o);
-        join<T>(top, sum, t, s);
-    }
+    join_wave<T>(top, sum);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = Part{top, sum};
     __syncthreads();
     if (threadIdx.x == 0)
@@ -505,7 +510,7 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
         __syncthreads();    // (row_end is written again)
         const float w = scaled(g, end.weight);
         if (w == 0.f) { clear_row(q, n, THREADS); continue; }
-        // What was derived from the vectors above is derived again: kept, it would be twice the registers that there are.
+        // (as in Held::again)
         int item = threadIdx.x;
         asm("" : "+v"(item));
         #pragma unroll
@@ -538,11 +543,7 @@ template <class T> __global__ void __launch_bounds__(256) join_rows_kernel(Rows 
             if (lane == 0) in = given<T>(a, e, r, label);
             top = -INFINITY; sum = 0.0;
             for (int k = lane; k < splits; k += 64) join<T>(top, sum, parts[r * splits + k].top, parts[r * splits + k].sum);
-            for (int o = 32; o > 0; o >>= 1) {
-                const float t = __shfl_xor(top, o);
-                const double s = __shfl_xor(sum, o);
-                join<T>(top, sum, t, s);
-            }
+            join_wave<T>(top, sum);
         }
         if (lane == 0) finish_long_row(a, e, r, in, top, sum);
     }

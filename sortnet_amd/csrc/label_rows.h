@@ -82,6 +82,47 @@ template <class T> __device__ __forceinline__ void store16(T* p, u32x4 v) { rein
 template <class T> __device__ __forceinline__ u32x4 stream16(const T* p) { return __builtin_nontemporal_load(&reinterpret_cast<const typename Elem<T>::Pack*>(p)->v); }
 template <class T> __device__ __forceinline__ void put_stream16(T* p, u32x4 v) { __builtin_nontemporal_store(v, &reinterpret_cast<typename Elem<T>::Pack*>(p)->v); }
 
+// One step of adding up (or the like) the lanes of a wavefront in groups of 2, 4, .. 64: v of this lane and of its partner, which are then in the
+// same group.  Every lane of a group of the step before holds the same value, so a mirrored half will do for an exchanged one: rows of 16 by
+// DPP, wider groups by gfx950's swaps, a few clocks each where a permutation through LDS is about 60.
+template <int STEP, class Op> __device__ __forceinline__ uint32_t lanes_step(uint32_t v, Op op) {
+    if constexpr (STEP == 0) return op(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0xb1, 0xf, 0xf, false));           // neighbours
+    else if constexpr (STEP == 1) return op(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x4e, 0xf, 0xf, false));      // pairs of a quad
+    else if constexpr (STEP == 2) return op(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, false));     // halves of 8
+    else if constexpr (STEP == 3) return op(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, 0x140, 0xf, 0xf, false));     // halves of 16
+    else if constexpr (STEP == 4) { const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false); return op(p[0], p[1]); }
+    else { const auto p = __builtin_amdgcn_permlane32_swap(v, v, false, false); return op(p[0], p[1]); }
+}
+template <int STEP> __device__ __forceinline__ double lanes_add(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    uint32_t lo[2], hi[2];
+    lanes_step<STEP>((uint32_t)bits, [&](uint32_t a, uint32_t b) { lo[0] = a; lo[1] = b; return 0u; });
+    lanes_step<STEP>((uint32_t)(bits >> 32), [&](uint32_t a, uint32_t b) { hi[0] = a; hi[1] = b; return 0u; });
+    return __builtin_bit_cast(double, (uint64_t)hi[0] << 32 | lo[0]) + __builtin_bit_cast(double, (uint64_t)hi[1] << 32 | lo[1]);
+}
+template <int STEP> __device__ __forceinline__ float lanes_max(float v) {
+    return __uint_as_float(lanes_step<STEP>(__float_as_uint(v), [](uint32_t a, uint32_t b) { return __float_as_uint(fmaxf(__uint_as_float(a), __uint_as_float(b))); }));
+}
+// over groups of 2^shift lanes (the same shift in all of them, each group whole or not there at all)
+__device__ __forceinline__ double group_total(double v, int shift) {
+    if (shift > 0) v = lanes_add<0>(v);
+    if (shift > 1) v = lanes_add<1>(v);
+    if (shift > 2) v = lanes_add<2>(v);
+    if (shift > 3) v = lanes_add<3>(v);
+    if (shift > 4) v = lanes_add<4>(v);
+    if (shift > 5) v = lanes_add<5>(v);
+    return v;
+}
+__device__ __forceinline__ float group_max(float v, int shift) {
+    if (shift > 0) v = lanes_max<0>(v);
+    if (shift > 1) v = lanes_max<1>(v);
+    if (shift > 2) v = lanes_max<2>(v);
+    if (shift > 3) v = lanes_max<3>(v);
+    if (shift > 4) v = lanes_max<4>(v);
+    if (shift > 5) v = lanes_max<5>(v);
+    return v;
+}
+
 // calls f with a null pointer of the element type that `dtype` names; false for none
 template <class F> bool with_dtype(int dtype, F&& f) {
     switch (dtype) {

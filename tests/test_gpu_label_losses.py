@@ -62,7 +62,7 @@ def check_gradient(grad, z, labels, weight, weight_error, what):
     assert (grad[labels == IGNORE] == 0).all(), what
 
 
-SHAPES = [(1, 1), (3, 1), (5, 2), (9, 3), (512, 10), (77, 33), (7, 257), (300, 1000), (64, 2048), (13, 2049), (9, 4096), (5, 4097), (3, 16385), (1, 50001), (700, 8200), (2, 131072), (40, 20000), (33, 60001), (2100, 8200), (70, 131072)]
+SHAPES = [(1, 1), (3, 1), (5, 2), (9, 3), (512, 10), (77, 33), (7, 257), (300, 1000), (64, 2048), (13, 2049), (9, 4096), (5, 4097), (3, 16385), (1, 50001), (700, 8200), (2, 131072), (40, 20000), (33, 60001), (2100, 8200), (70, 131072), (13, 100), (21, 200), (6, 15), (31, 60)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
