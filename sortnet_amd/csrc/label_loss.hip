@@ -462,7 +462,7 @@ template <class T> __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 5
 // with the statistics.  (Reading the row again from the caches instead lost: eight rows of 256 KiB per compute
 // unit are more than the last level holds, 4096 x 131072 bf16 596 us; two passes of their own 515.)
 template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
-    constexpr int V = Elem<T>::kVec, kChunk = 16 / V;
+    constexpr int V = Elem<T>::kVec, kChunk = (NV == 16 ? 8 : 16) / V;
     __shared__ Part waves[THREADS / 64];
     __shared__ End row_end;
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
