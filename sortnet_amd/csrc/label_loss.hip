@@ -61,6 +61,11 @@ __device__ __forceinline__ double wave_total(double v) { return group_total(v, 6
 
 __device__ __forceinline__ float finite(float top) { return fmaxf(top, -FLT_MAX); }
 
+// exp of a difference to the largest value of a row (or of a part of it): the hardware's exp2 of a product that is off by |v| 2^-24 and
+// as much again for log2(e), relative errors that shrink with the terms they are in; 1 for 0, so that a row's largest term is exact.
+// expf took twice the instructions in fp32 rows and gave the same errors of the results.
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
+
 // ---- a row's end: one work-item per row ------------------------------------------------------------------------------------
 // What it needs besides (top, sum), loaded before the row is read, so that the loads run beside it.
 struct Given { int64_t label; float at, old, advantage, ref; };
@@ -147,9 +152,10 @@ __device__ __forceinline__ float row_weight(const Rows& a, const Gradient& g, in
 }
 
 // N values from column c on become their gradients (a label that names no class, whose low half may name one, has w = NaN)
-template <class T, int N> __device__ __forceinline__ void slopes(float (&f)[N], float top, float inverse, float w, int c, int label) {
+template <int N> __device__ __forceinline__ void slopes(float (&f)[N], float top, float inverse, float w, int c, int label) {
+    const float by = -(inverse * w);
     #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = -(Elem<T>::exp(f[i] - top) * inverse) * w;
+    for (int i = 0; i < N; i++) f[i] = exp_of(f[i] - top) * by;
     const uint32_t at = (uint32_t)label - (uint32_t)c;
     if (at < N) {
         #pragma unroll
@@ -220,7 +226,7 @@ template <class T, int NV> struct Held {
                 float f[V];
                 Elem<T>::unpack(v[k], f);
                 #pragma unroll
-                for (int i = 0; i < V; i++) f[i] = Elem<T>::exp(f[i] - b);
+                for (int i = 0; i < V; i++) f[i] = exp_of(f[i] - b);
                 if (past > 0) {
                     #pragma unroll
                     for (int i = 0; i < V; i++) f[i] = i < past ? 0.f : f[i];
@@ -241,7 +247,7 @@ template <class T, int NV> struct Held {
                     for (int i = 0; i < V; i++) f[i] = 0.f;
                 } else {
                     Elem<T>::unpack(v[k], f);
-                    slopes<T>(f, top, inverse, w, c, label);
+                    slopes(f, top, inverse, w, c, label);
                 }
                 if (n * (int)sizeof(T) >= stream_from) put_stream16(q + c, Elem<T>::pack(f));
                 else if (n >= V) store16(q + c, Elem<T>::pack(f));
@@ -319,37 +325,40 @@ template <class T, int NV> __global__ void __launch_bounds__(256) label_gradient
 struct Part { float top; double sum; };
 
 // (top, sum) of two parts of a row
-template <class T> __device__ __forceinline__ void join(float& top, double& sum, float top2, double sum2) {
+__device__ __forceinline__ void join(float& top, double& sum, float top2, double sum2) {
     const float t = fmaxf(top, top2);
-    sum = sum * (double)Elem<T>::exp(finite(top) - finite(t)) + sum2 * (double)Elem<T>::exp(finite(top2) - finite(t));
+    sum = sum * (double)exp_of(finite(top) - finite(t)) + sum2 * (double)exp_of(finite(top2) - finite(t));
     top = t;
 }
 
-template <class T, int N> __device__ __forceinline__ void take(float (&f)[N], float& top, double& sum) {
+template <int N> __device__ __forceinline__ void take(float (&f)[N], float& top, double& sum) {
     float t = top;
     #pragma unroll
     for (int i = 0; i < N; i++) t = fmaxf(t, f[i]);
     const float b = finite(t);
     #pragma unroll
-    for (int i = 0; i < N; i++) f[i] = Elem<T>::exp(f[i] - b);
-    sum = sum * (double)Elem<T>::exp(finite(top) - b) + (double)tree(f);
+    for (int i = 0; i < N; i++) f[i] = exp_of(f[i] - b);
+    sum = sum * (double)exp_of(finite(top) - b) + (double)tree(f);
     top = t;
 }
 
 // of all lanes of a wavefront
-template <class T> __device__ __forceinline__ void join_wave(float& top, double& sum) {
+__device__ __forceinline__ void join_wave(float& top, double& sum) {
     const float t = group_max(top, 6);
-    sum = group_total(sum * (double)Elem<T>::exp(finite(top) - finite(t)), 6);
+    sum = group_total(sum * (double)exp_of(finite(top) - finite(t)), 6);
     top = t;
 }
 
 // of all work-items of a workgroup, to its first
-template <class T, int WAVES> __device__ __forceinline__ void join_workgroup(float& top, double& sum, Part* waves) {
-    join_wave<T>(top, sum);
+template <int WAVES> __device__ __forceinline__ void join_workgroup(float& top, double& sum, Part* waves) {
+    join_wave(top, sum);
     if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = Part{top, sum};
     __syncthreads();
-    if (threadIdx.x == 0)
-        for (int k = 1; k < WAVES; k++) join<T>(top, sum, waves[k].top, waves[k].sum);
+    if (threadIdx.x < 64) {     // lanes 0 .. WAVES - 1 of each 16 hold the wavefronts' parts
+        const Part part = waves[threadIdx.x & (WAVES - 1)];
+        top = group_max(part.top, 4);
+        sum = group_total((threadIdx.x & 15) < WAVES ? part.sum * (double)exp_of(finite(part.top) - finite(top)) : 0.0, 4);
+    }
     __syncthreads();        // (waves is written again)
 }
 
@@ -365,16 +374,16 @@ template <class T, bool STREAM> __device__ __forceinline__ void scan(const T* p,
         float f[kUnroll * V];
         #pragma unroll
         for (int k = 0; k < kUnroll; k++) Elem<T>::unpack(v[k], reinterpret_cast<float (&)[V]>(f[k * V]));
-        take<T>(f, top, sum);
+        take(f, top, sum);
     }
     for (; i < full; i += lanes) {
         float f[V];
         Elem<T>::unpack(load16(p + i * V), f);
-        take<T>(f, top, sum);
+        take(f, top, sum);
     }
     for (int64_t j = full * V + lane; j < n; j += lanes) {
         float f[1] = {Elem<T>::get(p[j])};
-        take<T>(f, top, sum);
+        take(f, top, sum);
     }
 }
 
@@ -405,19 +414,19 @@ template <class T, bool STREAM> __device__ __forceinline__ void grad_row(const T
             const int64_t c = (i + (int64_t)k * lanes) * V;
             float f[V];
             Elem<T>::unpack(v[k], f);
-            slopes<T>(f, top, inverse, w, (int)c, label);
+            slopes(f, top, inverse, w, (int)c, label);
             put_stream16(dst + c, Elem<T>::pack(f));
         }
     }
     for (; i < full; i += lanes) {
         float f[V];
         Elem<T>::unpack(load16(src + i * V), f);
-        slopes<T>(f, top, inverse, w, (int)(i * V), label);
+        slopes(f, top, inverse, w, (int)(i * V), label);
         put_stream16(dst + i * V, Elem<T>::pack(f));
     }
     for (int64_t j = full * V + lane; j < c1; j += lanes) {
         float f[1] = {Elem<T>::get(src[j])};
-        slopes<T>(f, top, inverse, w, (int)j, label);
+        slopes(f, top, inverse, w, (int)j, label);
         dst[j] = Elem<T>::put(f[0]);
     }
 }
@@ -434,7 +443,7 @@ __device__ __forceinline__ End finish_long_row(const Rows& a, const Finish& e, i
 }
 
 // A workgroup per row, or per one of `splits` parts of a row, which then leaves its (top, sum) for join_rows_kernel.
-template <class T> __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 5) label_long_rows_kernel(Rows a, Finish e, int splits, int64_t part, Part* parts) {
+template <class T> __global__ void __launch_bounds__(256, 8) label_long_rows_kernel(Rows a, Finish e, int splits, int64_t part, Part* parts) {
     __shared__ Part waves[4];
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
     for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
@@ -449,7 +458,7 @@ template <class T> __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 8 : 5
             top = -INFINITY; sum = 0.0;
             if (beyond_cache<T>(a, r)) scan<T, true>(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
             else scan<T, false>(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
-            join_workgroup<T, 4>(top, sum, waves);
+            join_workgroup<4>(top, sum, waves);
         }
         if (threadIdx.x == 0) {
             if (splits > 1) parts[r * splits + s] = Part{top, sum};
@@ -498,11 +507,11 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
             float f[kChunk * V];
             #pragma unroll
             for (int k = 0; k < kChunk; k++) Elem<T>::unpack(v[c + k], reinterpret_cast<float (&)[V]>(f[k * V]));
-            take<T>(f, top, sum);
+            take(f, top, sum);
         }
         float f1[1] = {Elem<T>::get(last)};
-        take<T>(f1, top, sum);
-        join_workgroup<T, THREADS / 64>(top, sum, waves);
+        take(f1, top, sum);
+        join_workgroup<THREADS / 64>(top, sum, waves);
         if (threadIdx.x == 0) row_end = finish_long_row(a, e, r, in, top, sum);
         if (!FUSED) continue;
         __syncthreads();
@@ -520,12 +529,12 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
             const int i = item + k * THREADS;
             float f[V];
             Elem<T>::unpack(v[k], f);
-            slopes<T>(f, end.top, end.inverse, w, i * V, (int)label);
+            slopes(f, end.top, end.inverse, w, i * V, (int)label);
             if (i < full) put_stream16(q + i * V, Elem<T>::pack(f));
         }
         if (rest < n) {
             float f[1] = {Elem<T>::get(last)};
-            slopes<T>(f, end.top, end.inverse, w, rest, (int)label);
+            slopes(f, end.top, end.inverse, w, rest, (int)label);
             q[rest] = Elem<T>::put(f[0]);
         }
     }
@@ -542,8 +551,8 @@ template <class T> __global__ void __launch_bounds__(256) join_rows_kernel(Rows 
         if (label != a.ignore) {
             if (lane == 0) in = given<T>(a, e, r, label);
             top = -INFINITY; sum = 0.0;
-            for (int k = lane; k < splits; k += 64) join<T>(top, sum, parts[r * splits + k].top, parts[r * splits + k].sum);
-            join_wave<T>(top, sum);
+            for (int k = lane; k < splits; k += 64) join(top, sum, parts[r * splits + k].top, parts[r * splits + k].sum);
+            join_wave(top, sum);
         }
         if (lane == 0) finish_long_row(a, e, r, in, top, sum);
     }

@@ -1,4 +1,4 @@
-// Rows of logits: element types, 16-byte loads and the exponentials of their softmax.
+// Rows of values: element types, 16-byte loads and stores, sums over lanes.
 #pragma once
 #include "common.h"
 #include <hip/hip_bf16.h>
@@ -28,7 +28,6 @@ template <> struct Elem<float> {
         return v;
     }
     static __device__ __forceinline__ u32x4 splat(float v) { const uint32_t w = __float_as_uint(v); return u32x4{w, w, w, w}; }
-    static __device__ __forceinline__ float exp(float v) { return expf(v); }
 };
 struct bf16 { uint16_t bits; };
 template <> struct Elem<bf16> {
@@ -51,8 +50,6 @@ template <> struct Elem<bf16> {
         return v;
     }
     static __device__ __forceinline__ u32x4 splat(bf16 v) { const uint32_t w = v.bits | (uint32_t)v.bits << 16; return u32x4{w, w, w, w}; }
-    // results are rounded to 8 bits: the hardware's exp2 of a rounded argument is exact enough (|v| 2^-24 relative)
-    static __device__ __forceinline__ float exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 };
 struct fp16 { uint16_t bits; };
 template <> struct Elem<fp16> {
@@ -73,7 +70,6 @@ template <> struct Elem<fp16> {
         return v;
     }
     static __device__ __forceinline__ u32x4 splat(fp16 v) { const uint32_t w = v.bits | (uint32_t)v.bits << 16; return u32x4{w, w, w, w}; }
-    static __device__ __forceinline__ float exp(float v) { return __builtin_amdgcn_exp2f(v * 1.44269504f); }
 };
 
 template <class T> __device__ __forceinline__ u32x4 load16(const T* p) { return reinterpret_cast<const typename Elem<T>::Pack*>(p)->v; }

@@ -131,6 +131,39 @@ def test_masked_classes(classes, dtype):
     assert (grad[0, :classes // 2] == 0).all() and (grad[2] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("rows, classes", [(7, 5), (7, 700), (7, 5000), (7, 70000), (3000, 9000), (1100, 8800)])
+def test_values_of_any_size(rows, classes, dtype):
+    """Rows whose largest value lies near the ends of the type's range, on both sides of 1e38, with values next to it, and large offsets: log
+    probabilities and gradients as in 64 bits.  (Softmax at distance d: see the head of this file; the products with an offset of z are exact.)"""
+    z, labels, g = make(rows, classes, dtype, classes, ignored=0.0)
+    big = torch.tensor([3.3e38, 1.01e38, 0.99e38, -0.99e38, -1.01e38, -3.3e38, 1e4], device="cuda")
+    for k, b in enumerate(big.tolist()):
+        for r in (k, rows - 1 - k) if rows > 100 else (k,):
+            if k < 6:
+                z[r] = -torch.finfo(dtype).max if k > 2 else 0.0
+                z[r, classes // 2:] = b
+                z[r, -1] = b * 0.5 if b > 0 else b * 1.02
+                labels[r] = classes // 2
+            else:
+                z[r] = (z[r].float() + 1e4).to(dtype)
+    z.requires_grad_()
+    exact = torch.log_softmax(z.detach().double(), 1)
+    want = exact.gather(1, labels.view(-1, 1)).squeeze(1)
+    lp = losses.label_log_probs(z, labels)
+    close(lp.detach(), want, sum_error(classes) + 4 * U * (want.abs() + math.log(classes)), "log probs")
+    p = exact.exp()
+    hot = torch.zeros_like(p).scatter_(1, labels.view(-1, 1), 1.0)
+    far = (-exact).clamp(max=200.0)
+    off = p * (sum_error(classes) + (1.5 * far + 8) * U) + 4 * U * hot
+    tol = off + (hot - p).abs() * HALF_STEP[dtype] + off * HALF_STEP[dtype] + SMALLEST[dtype]
+    close(torch.autograd.grad(lp, z, torch.ones_like(lp))[0], hot - p, tol, "gradient")
+    one = torch.ones(rows, device="cuda")
+    loss, _ = losses.policy_loss(z, labels, lp.detach(), -one)       # ratio 1: the same gradient over the rows
+    got, = torch.autograd.grad(loss, z)
+    close(got.double() * rows, hot - p, tol + 8 * U + (hot - p).abs() * (HALF_STEP[dtype] + 8 * U) + SMALLEST[dtype] * rows, "gradient of the policy")
+
+
 @pytest.mark.parametrize("classes", [6, 3000 + 7, 40000])
 def test_rows_without_values(classes):
     """Ignored rows hold anything; rows of -inf alone, with +inf or NaN, and labels that name no class give NaN, and touch no other row."""
