@@ -18,8 +18,8 @@ constexpr int kHeld = 8;            // 16-byte vectors of a short row that a lan
 constexpr int kHeldLong = 16 * 1024;    // and of a long row that a workgroup holds
 constexpr int64_t kMostBlocks = 1 << 22;
 constexpr int kShortBlocks = 4096;      // workgroups of short rows, at most
-// Bytes of a FUSED short row from which its gradient is stored past the caches: us with and without, 262144 x 200 fp32 121 / 142,
-// 65536 x 1000 bf16 62 / 67; 1048576 x 10 fp32, whose rows share cache lines, 178 / 160.
+// Bytes of a FUSED short row from which its gradient is stored past the caches: us with and without, 262144 x 200 fp32 82 / 95,
+// 65536 x 1000 bf16 60 / 62; 1048576 x 10 fp32, whose rows share cache lines, 53 / 35.
 constexpr int kStreamRow = 512;
 
 struct Rows {
@@ -433,8 +433,8 @@ template <class T, bool STREAM> __device__ __forceinline__ void grad_row(const T
 
 // A pass over long rows reads them from the last to the first, the gradient's pass from the first on, so that it finds
 // what the last-level cache holds still there; the rows behind them are read past the caches, which leaves these alone and is faster by itself:
-// 4096 x 131072 bf16 forward 183 -> 156 us, both passes 545 -> 495.
-template <class T> __device__ __forceinline__ bool beyond_cache(const Rows& a, int64_t r) { return r * a.classes * (int64_t)sizeof(T) >= kCached; }
+// 4096 x 131072 bf16 forward 180 -> 162 us, both passes 541 -> 484.
+__host__ __device__ __forceinline__ bool beyond_cache(const Rows& a, int64_t r, int64_t size) { return r * a.classes * size >= kCached; }
 
 __device__ __forceinline__ End finish_long_row(const Rows& a, const Finish& e, int64_t r, const Given& g, float top, double sum) {
     const End end = finish_row(a, e, r, g, top, sum);
@@ -456,7 +456,7 @@ template <class T> __global__ void __launch_bounds__(256, 8) label_long_rows_ker
         if (label != a.ignore) {        // (the whole workgroup's)
             if (threadIdx.x == 0 && splits == 1) in = given<T>(a, e, r, label);
             top = -INFINITY; sum = 0.0;
-            if (beyond_cache<T>(a, r)) scan<T, true>(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
+            if (beyond_cache(a, r, sizeof(T))) scan<T, true>(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
             else scan<T, false>(row_start<T>(a, r) + c0, n, threadIdx.x, 256, top, sum);
             join_workgroup<4>(top, sum, waves);
         }
@@ -468,17 +468,16 @@ template <class T> __global__ void __launch_bounds__(256, 8) label_long_rows_ker
 }
 
 // The workgroup holds a long row in its registers, at most 16 vectors per work-item.  FUSED: the logits are read once and the gradient leaves
-// with the statistics.  (Reading the row again from the caches instead lost: eight rows of 256 KiB per compute
-// unit are more than the last level holds, 4096 x 131072 bf16 596 us; two passes of their own 515.)
-template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
+// with the statistics.  FAR: logits that the last-level cache cannot hold are read past it (4096 x 131072 bf16 401 -> 393 us,
+// 4096 x 65536 201 -> 191; 2000 x 50001 fp16, which it holds, 76, past it 95).  (Reading the row again from the caches instead lost: eight rows of 256 KiB
+// per compute unit are more than the last level holds, 4096 x 131072 596 us where two passes of their own took 515.)
+template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
     constexpr int V = Elem<T>::kVec, kChunk = (NV == 16 ? 8 : 16) / V;
     __shared__ Part waves[THREADS / 64];
     __shared__ End row_end;
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
     const int n = (int)a.classes, full = n / V, rest = full * V + (int)threadIdx.x;     // the values behind the last whole vector: one per work-item
     const T lowest = Elem<T>::put(-INFINITY);
-    // logits that the last-level cache cannot hold are read past it: 4096 x 131072 bf16 400 -> 392 us, 4096 x 65536 203 -> 192 (2000 x 50001, which it holds, 79 -> 101)
-    const bool far = beyond_cache<T>(a, a.rows);
     for (int64_t r = a.rows - 1 - blockIdx.x; r >= 0; r -= gridDim.x) {     // (the producer's last rows may be in the caches)
         const int64_t label = a.labels[r];
         T* q = static_cast<T*>(g.grad) + r * a.classes;
@@ -495,7 +494,7 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
         for (int k = 0; k < NV; k++) {
             const int i = (int)threadIdx.x + k * THREADS;
             v[k] = none;
-            if (i < full) v[k] = far ? stream16(p + i * V) : load16(p + i * V);
+            if (i < full) v[k] = FAR ? stream16(p + i * V) : load16(p + i * V);
         }
         if (rest < n) last = p[rest];
         Given in{label, 0.f, 0.f, 0.f, 0.f};
@@ -566,7 +565,7 @@ template <class T> __global__ void __launch_bounds__(256) label_long_gradient_ke
         const float2 st = g.stats[r];
         const float w = row_weight(a, g, r, label);
         T* q = static_cast<T*>(g.grad) + r * a.classes;
-        if (beyond_cache<T>(a, r)) grad_row<T, true>(row_start<T>(a, r), q, st.x, st.y, w, (int)label, c0, c1, threadIdx.x, 256);
+        if (beyond_cache(a, r, sizeof(T))) grad_row<T, true>(row_start<T>(a, r), q, st.x, st.y, w, (int)label, c0, c1, threadIdx.x, 256);
         else grad_row<T, false>(row_start<T>(a, r), q, st.x, st.y, w, (int)label, c0, c1, threadIdx.x, 256);
     }
 }
@@ -765,19 +764,20 @@ template <class F> void with_vectors(int vectors, F&& f) {
     }
 }
 
-// Parts of a long row: so many that there are 704 workgroups (2.75 for each compute unit), none with less than one vector per work-item.  More parts
-// lost: 2000 x 50001 bf16 34.5 us whole, in two parts 37.4; 700 x 131072 30.7 and 34.7; 1000 x 131072 41.7 and 45.
+// Parts of a long row: so many that there are kWholeRows workgroups (2.75 for each compute unit), none with less than one vector per work-item.
+// With 2048: 2000 x 50001 bf16 35.8 us whole, in two parts 38.2; 1000 x 131072 43.6 and 48.2; 1030 x 131072 fp32 90.3 and 86.8.
+constexpr int64_t kWholeRows = 704;
 int row_splits(int64_t rows, int64_t classes, int vec) {
-    const int64_t want = (704 + rows - 1) / rows, most = (classes + 256 * vec - 1) / (256 * vec);
+    const int64_t want = (kWholeRows + rows - 1) / rows, most = (classes + 256 * vec - 1) / (256 * vec);
     return (int)(want < most ? want : most);
 }
 
-// Rows that would be read in parts to fill the card: where a workgroup can hold a row it is read whole, which spares the launch that joins
-// the parts: 128 x 8192 bf16 7.1 -> 3.9 us, 512 x 16384 10.2 -> 5.3, 1024 x 32000 18.6 -> 14.3 (from 2048 rows on, that are read whole anyway, it makes
-// no difference).  Rows for a workgroup of 512, of which fewer run at once: 256 x 50001 11.8 -> 8.7, but 16 rows 7.3 -> 8.5 and 1024 23.8 -> 24.0.
+// Rows that would be read in parts: where a workgroup can hold a row it is read whole, which spares the launch that joins the parts:
+// 128 x 8192 bf16 6.8 -> 4.4 us, 512 x 16384 8.6 -> 5.4, 512 x 32000 11.9 -> 9.3.  Rows for a workgroup of 512, of which fewer run at once: 256 x 50001
+// 10.4 -> 9.0, but 16 rows 7.1 -> 8.4 and 1024 21.2 -> 26.0.
 bool one_launch(int64_t rows, int64_t classes, int vec) {
     const int64_t vecs = (classes + vec - 1) / vec;
-    return rows < 2048 && (vecs <= 16 * 256 || (vecs <= 16 * 512 && rows >= 32 && rows <= 512));
+    return rows < kWholeRows && (vecs <= 16 * 256 || (vecs <= 16 * 512 && rows >= 32 && rows <= 512));
 }
 
 int64_t part_of(int64_t classes, int splits, int vec) {
@@ -845,14 +845,16 @@ int launch_rows(const sd_label_rows* in, const Rows& a, const Finish& e, const G
         if (g || one_launch(a.rows, a.classes, vec)) {
             const dim3 grid(blocks_for(a.rows));
             const int64_t vecs = (a.classes + vec - 1) / vec;
-            const auto held = [&](auto fused) {
-                if (vecs <= 4 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 256, fused.value>), grid, dim3(256), 0, stream, a, e, grad);
-                else if (vecs <= 8 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 256, fused.value>), grid, dim3(256), 0, stream, a, e, grad);
-                else if (vecs <= 16 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 256, fused.value>), grid, dim3(256), 0, stream, a, e, grad);
-                else if (vecs <= 16 * 512) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 512, fused.value>), grid, dim3(512), 0, stream, a, e, grad);
-                else if constexpr (fused.value) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 1024, true>), grid, dim3(1024), 0, stream, a, e, grad);
+            const auto held = [&](auto fused, auto far) {
+                if (vecs <= 4 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 4, 256, fused.value, far.value>), grid, dim3(256), 0, stream, a, e, grad);
+                else if (vecs <= 8 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 8, 256, fused.value, far.value>), grid, dim3(256), 0, stream, a, e, grad);
+                else if (vecs <= 16 * 256) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 256, fused.value, far.value>), grid, dim3(256), 0, stream, a, e, grad);
+                else if (vecs <= 16 * 512) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 512, fused.value, far.value>), grid, dim3(512), 0, stream, a, e, grad);
+                else if constexpr (fused.value) hipLaunchKernelGGL((label_held_rows_kernel<T, 16, 1024, true, far.value>), grid, dim3(1024), 0, stream, a, e, grad);
             };
-            if (g) held(std::true_type()); else held(std::false_type());
+            if (!g) held(std::false_type(), std::false_type());     // (few rows)
+            else if (beyond_cache(a, a.rows, sizeof(T))) held(std::true_type(), std::true_type());
+            else held(std::true_type(), std::false_type());
             return;
         }
         int splits = row_splits(a.rows, a.classes, vec);
