@@ -21,7 +21,7 @@ PEAK = 157.3e12
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--shape", type=int, nargs=3, default=[512, 5120, 5120], metavar=("B", "N", "M"))
-    ap.add_argument("--ops", default="linf,mask,bwd,bound,sort,lp,shift,idx")
+    ap.add_argument("--ops", default="linf,mask,bwd,bound,sort,lp,shift,idx,head")
     ap.add_argument("--reps", type=int, default=5)
     ap.add_argument("--keep", type=float, default=0.3, help="keep probability of the index-list rows")
     ap.add_argument("--data", choices=["config", "unit"], default="config",
@@ -151,6 +151,21 @@ def main():
           None, 4 * (3 * B * cm))
     if "shift" in on:
         t("mean_shift_forward", lambda: ext.mean_shift_forward(y, mean, None, 0.1, y2), None, 4 * (3 * B * M))
+    if "head" in on:
+        # training of a head: B x M logits, one label each; dropout of the B x N features
+        from sortnet_amd import functional as F, losses
+        z = torch.randn(B, M, generator=g).to(dev).requires_grad_()
+        labels = torch.randint(0, M, (B,), generator=g).to(dev)
+        up, adv = torch.ones(B, device=dev), torch.randn(B, generator=g).to(dev)
+        ref = losses.label_log_probs(z.detach(), labels) + 0.1
+        feats = x[..., 0].clone().requires_grad_()
+        backward = lambda out, leaf, grad=None: torch.autograd.grad(out, leaf, grad)
+        t("label_log_probs, fwd + bwd", lambda: backward(losses.label_log_probs(z, labels), z, up), None, 8 * B * M)
+        if B % 2 == 0:
+            t("preference_loss, fwd + bwd", lambda: backward(losses.preference_loss(z, labels, ref)[0], z), None, 8 * B * M)
+        t("policy_loss, fwd + bwd",
+          lambda: backward(losses.policy_loss(z, labels, ref, adv, ref_log_probs=ref, kl_coef=0.05)[0], z), None, 8 * B * M)
+        t("dropout q=0.9, fwd + bwd", lambda: backward(F.dropout(feats, 0.9, 1), feats, x[..., 0]), None, 16 * B * N)
     if args.json:
         print(json.dumps({"shape": {"B": B, "N": N, "M": M}, "rows": rows}))
 
