@@ -61,6 +61,14 @@ sd_stream_t stream_of(const Tensor& t) {
     return c10::hip::getCurrentHIPStream(t.device().index()).stream();
 }
 
+// the graph capture that work on this stream goes into: its number, 0 for none, -1 where the runtime does not say
+int64_t capture_of(sd_stream_t stream) {
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (hipStreamGetCaptureInfo(static_cast<hipStream_t>(stream), &status, &id) != hipSuccess) { (void)hipGetLastError(); return -1; }
+    return status == hipStreamCaptureStatusNone ? 0 : status == hipStreamCaptureStatusActive ? (int64_t)id : -1;
+}
+
 // sizes of a layer call on x (B, C, HW)
 struct Dims {
     int B, CI, HW, CO, G;
@@ -637,6 +645,7 @@ struct LabelNode : Node {
     enum Kind { VALUES, PREFERENCE, POLICY } kind;
     SavedVariable logits, labels, work;
     Tensor made;            // the gradient for an upstream gradient of 1, where the forward made it
+    int64_t capture = 0;    // the graph capture that made it
     int64_t ignore = 0;
     bool last = false;      // this backward is the graph's last: `made` may be given away
 
@@ -649,8 +658,10 @@ struct LabelNode : Node {
         const Tensor g = incoming(*this, grads, 0);
         const c10::DeviceGuard guard(z.device());
         // A gradient that is there already is only written again for another upstream gradient than 1, which the device knows; one that a
-        // later backward may want, too, stays as it is.
-        const bool there = made.defined() && last, loss = kind != VALUES;
+        // later backward may want, too, stays as it is, and so does one of another capture: that graph may run again without the forward that
+        // writes it, after the caller has changed it or with another upstream gradient.
+        const int64_t now = made.defined() && last ? capture_of(stream_of(z)) : -1;
+        const bool there = now >= 0 && now == capture, loss = kind != VALUES;
         out[0] = there ? std::move(made) : at::empty(z.sizes(), z.options());
         if (out[0].numel() == 0) return out;
         const sd_label_rows a = label_rows(z, l, ignore);
@@ -682,6 +693,7 @@ void attach_labels(const Tensor& y, LabelNode::Kind kind, const Tensor& outputs,
     node->labels = SavedVariable(labels, false);
     node->work = SavedVariable(work, false);
     node->made = made;
+    if (made.defined()) node->capture = capture_of(stream_of(z));
     set_history(y, node);
 }
 

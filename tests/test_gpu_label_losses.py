@@ -403,6 +403,41 @@ def test_policy_of_many_rows(answers, tokens, classes, kl, dtype):
             assert torch.equal(outs[0], eager[0]) and torch.equal(outs[1], eager[1]) and torch.equal(made, eager_grad)
 
 
+@pytest.mark.parametrize("forward_captured", [False, True])
+def test_policy_backward_in_a_graph_of_its_own(forward_captured):
+    """A backward captured apart from its forward, which made the gradient: run several times for one forward, with another upstream gradient
+    each time and after the caller has overwritten what it got."""
+    rows, classes = 40000, 230
+    z, labels, g = make(rows, classes, torch.float32, 77, ignored=0.2)
+    assert rows * classes * 4 >= 32 << 20
+    old = exact_rows(z, labels)[0].float() - 0.1
+    adv = torch.randn(rows, generator=g).cuda()
+    call = lambda t: losses.policy_loss(t, labels, old, adv)[0]
+    static, up = z.clone().requires_grad_(), torch.ones((), device="cuda")
+    stream, pool = torch.cuda.Stream(), torch.cuda.graph_pool_handle()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        torch.autograd.grad(call(static), static, up)
+        loss = None if forward_captured else call(static)
+    torch.cuda.synchronize()
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    if forward_captured:
+        with torch.cuda.graph(first, stream=stream, pool=pool):
+            loss = call(static)
+    with torch.cuda.graph(second, stream=stream, pool=pool):
+        made, = torch.autograd.grad(loss, static, up)
+    if forward_captured:
+        first.replay()
+    fresh = z.clone().requires_grad_()
+    eager = call(fresh)
+    for factor in (1.0, -0.5, 1.0, 1.0):
+        up.fill_(factor)
+        second.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(made, torch.autograd.grad(eager, fresh, torch.full((), factor, device="cuda"), retain_graph=True)[0]), factor
+        made.zero_()
+
+
 def test_policy_clips_and_defaults():
     """Each side of the clip with either sign of the advantage; clip_high defaults to clip; a clip of 1 and 0."""
     z, labels, _ = make(6, 5, torch.float32, 4, ignored=0.0)
