@@ -379,7 +379,9 @@ int sd_label_gradient(const sd_label_rows* rows, const float* stats, const float
 /* Dropout of up to three tensors of n values under one mask (inputs that are not wanted are NULL with their outputs): value i is kept
  * where field i of the generator is below L = floor(65536 q + 0.5), and multiplied by 65536 / L.  The fields of values 2j and 2j + 1 are
  * the low and high halves of mix(sd_rng_word(seed, 5, j >> 15, j & 32767) ^ key), mix being the generator's finaliser and key =
- * mix((seed ^ (6 * 0x9e3779b9)) + (j >> 15)).  seed_on_device, if not NULL, holds the seed in its low 32 bits (graphs that draw
+ * mix((seed ^ (6 * 0x9e3779b9)) + (j >> 15)).  The masks of two seeds that differ only in bits 2, 4, 5, 8, 10, 14, 17, 18, 21, 23, 24, 26, 27,
+ * 28, 30 and 31 are the same but for a shift of a number of rows of 2^16 values: callers that draw several masks keep those bits below 2^17
+ * alike, or choose seeds at random.  seed_on_device, if not NULL, holds the seed in its low 32 bits (graphs that draw
  * a new mask in each replay).  The backward is the same call on the gradients. */
 int sd_dropout(const void* x0, const void* x1, const void* x2, int dtype, int64_t n, double q, uint32_t seed, const int64_t* seed_on_device,
                void* y0, void* y1, void* y2, sd_stream_t stream);

@@ -2,7 +2,10 @@
 // round(65536 q), and is then multiplied by the reciprocal of that probability.  The backward is the same kernel on the gradient, and a
 // call with the same seed makes the same mask again.
 // One word serves two neighbouring values: pair j = i / 2 stands at column j mod 2^15 of row j / 2^15; the word is mixed with two keys of
-// its row, so that the words of two rows are no shifted copies of each other (one key of 32 bits leaves 2^32 sequences that overlap).
+// its row, so that the words of two rows of a mask are no shifted copies of each other (one key of 32 bits leaves 2^32 sequences that
+// overlap).  Rows of two masks are the same where both keys are: with x = seed ^ c and m = c ^ d, c and d being the streams' constants, where
+// (x + n) ^ m = (x ^ m) + n for a distance of n rows, and that holds where x and x + n differ in no bit of m below 2^31.  Seeds that
+// count up are spread so that this is so for no n below 2^17 (functional.dropout_seed).
 // Bound by the bytes.  Results are stored past the caches (2^26 values bf16 90 -> 78 us for two tensors in turn).
 #include <cmath>
 #include <type_traits>

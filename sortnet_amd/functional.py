@@ -20,6 +20,7 @@ __all__ = [
     "NormDistF", "NormDistDropoutF", "SortNeuronF", "BoundInfDistF", "MaskedInfDistF",
     "norm_dist", "norm_dist_dropout", "sort_neuron", "bound_sort_neuron", "bound_inf_dist", "masked_inf_dist",
     "MeanShiftF", "mean_shift", "MeanShiftIndexF", "mean_shift_index", "dropout", "bound_dropout",
+    "dropout_seed",
 ]
 
 
@@ -284,6 +285,20 @@ def masked_inf_dist(input, weight, q, seed, groups=1, mode=_C.MASK_TERM, tag=Non
     return MaskedInfDistF.apply(input, weight, groups, q, seed, mode)
 
 
+def dropout_seed(number):
+    """The seed of `dropout` for the number-th mask of a run: seeds that count up go through here.
+
+    Rows of 2^16 values have two keys each, made of (seed ^ c) + row and (seed ^ d) + row with constants c and d.  Seeds that differ only in
+    bits that c and d have in common move both by the same number of rows, so that one mask is the other one shifted (seeds 1 and 5: by
+    four rows); seeds that differ in a bit that c and d do not share, the highest aside, have no row in common.  Here the number's low 26
+    bits go to all places but 2, 4, 5, 8, 10 and 14, those of the common bits below 2^17, and its high ones to these: any two of 2^23
+    numbers in a row have masks that are no copies of each other within 2^17 rows, tensors of up to 2^33 values.  A permutation of
+    the 32 bits: other numbers have other seeds.  `number` may be a whole number or a tensor of int64."""
+    n = number & 0xFFFFFFFF
+    return ((n & 3) | (n & 4) << 1 | (n & 0x18) << 3 | (n & 0x20) << 4 | (n & 0x1C0) << 5 | (n & 0x3FFFE00) << 6 |
+            (n >> 24 & 4) | (n >> 23 & 0x30) | (n >> 21 & 0x100) | (n >> 20 & 0x400) | (n >> 17 & 0x4000))
+
+
 def _dropped(tensors, q, seed):
     on_device = isinstance(seed, torch.Tensor)
     return _C.host().dropout(tensors, q, 0 if on_device else seed & 0xFFFFFFFF, seed if on_device else None)
@@ -294,7 +309,8 @@ def dropout(input, q, seed):
     stays by that probability; the mask is a function of (seed, row-major index) and is never stored: the backward makes it
     again, and so does a call with the same seed.  `seed` is a whole number or one int64 on the input's device; a captured
     graph replays the mask of a number, and reads a device seed in each replay (change it between replays, not between a
-    forward and its backward).  Dropped values are 0 whatever they were.  q = 1 or None returns the input."""
+    forward and its backward).  Seeds that count up are to be taken through `dropout_seed`: their masks are else shifted copies of
+    each other above 2^18 values.  Dropped values are 0 whatever they were.  q = 1 or None returns the input."""
     if q is None or q == 1.0:
         return input
     return _dropped([input], q, seed)[0]

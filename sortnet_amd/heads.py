@@ -32,10 +32,10 @@ class BoundTanh(nn.Tanh):
 class BoundDropout(nn.Module):
     """Dropout of a dense head's features (no counterpart in the reference): in training, values and bounds keep the same entries,
     each with probability `q`, divided by it; in evaluation, or with q = 1 or None, nothing changes.  The mask is a function of a
-    seed and is never stored.  Seeds come from the registry that the distance layers' lists come from
-    (`layers.set_mask_seed` makes a run reproducible); `last_seed` is that of the latest pass, with which `functional.bound_dropout` makes the
-    same mask again.  A captured graph would replay one mask: `seed`, one int64 on the GPU, is then read in each replay, and is the caller's
-    to change between them."""
+    seed and is never stored.  Seeds are those of the numbers (`functional.dropout_seed`) of the registry that the distance layers' lists come
+    from (`layers.set_mask_seed` makes a run reproducible); `last_seed` is that of the latest pass, with which `functional.bound_dropout` makes
+    the same mask again.  A captured graph would replay one mask: `seed`, one int64 on the GPU, is then read in each replay, and is the caller's
+    to change between them, to `functional.dropout_seed` of a number that counts up."""
 
     def __init__(self, q, registry=None, seed=None):
         super().__init__()
@@ -46,7 +46,7 @@ class BoundDropout(nn.Module):
     def forward(self, x=None, lower=None, upper=None):
         if not self.training or self.q is None or self.q == 1.0:
             return x, lower, upper
-        self.last_seed = self.registry.next_seed() if self.seed is None else self.seed
+        self.last_seed = F.dropout_seed(self.registry.next_seed()) if self.seed is None else self.seed
         return F.bound_dropout(x, lower, upper, self.q, self.last_seed)
 
     def extra_repr(self):

@@ -232,3 +232,18 @@ def test_a_hybrid_model_trains(kind):
         if a is not None:
             assert (a - b).abs().max().item() <= 2e-3 * max(b.abs().max().item(), 1e-6)
     assert any(a is not None and (a != 0).any() for a in grads)
+
+
+def test_masks_of_several_passes_are_unlike_at_any_shift():
+    """The masks of the first 32 passes of a layer, each against each, shifted by up to 16 rows of 2^16 values: kept together as often as chance has it,
+    within seven standard deviations (33 x 496 pairs)."""
+    layer = heads.BoundDropout(0.5, registry=DropoutRegistry(seed=0))
+    x = torch.ones(24, 65536, device="cuda")
+    masks = torch.stack([layer(x)[0] != 0 for _ in range(32)]).to(torch.bfloat16)
+    for shift in range(17):
+        n = 24 - shift
+        a, b = masks[:, shift:].reshape(32, -1), masks[:, :n].reshape(32, -1)
+        both = sum(torch.mm(a[:, k:k + 65536].float(), b[:, k:k + 65536].float().t()) for k in range(0, n * 65536, 65536)) / (n * 65536)
+        if shift == 0:
+            both.fill_diagonal_(0.25)
+        assert (both - 0.25).abs().max().item() <= 7 * math.sqrt(0.25 * 0.75 / (n * 65536)), shift
