@@ -814,11 +814,30 @@ struct DropNode : Node {
     double q = 1.0;
     uint32_t seed = 0;
 
+    // Under create_graph the results depend on the incoming gradients as the outputs do on the inputs: their node, or none.
+    std::shared_ptr<DropNode> of_gradients(const variable_list& grads, const Tensor& sd) {
+        torch::autograd::edge_list edges(grads.size());
+        bool any = false;
+        for (size_t k = 0; k < grads.size(); k++)
+            if (at::GradMode::is_enabled() && task_should_compute_output(k) && grads[k].defined() && grads[k].requires_grad()) {
+                edges[k] = torch::autograd::impl::gradient_edge(grads[k]);
+                any = true;
+            }
+        if (!any) return nullptr;
+        auto node = new_node<DropNode>();
+        node->set_next_edges(std::move(edges));
+        node->q = q;
+        node->seed = seed;
+        if (sd.defined()) node->seeds = SavedVariable(sd, false);
+        return node;
+    }
+
     variable_list apply(variable_list&& grads) override {
         const Locked lock(mutex_);
         const int count = (int)grads.size();
         variable_list out(count);
         const Tensor sd = seeds.unpack();
+        const std::shared_ptr<DropNode> again = of_gradients(grads, sd);
         at::AutoDispatchBelowADInplaceOrView below;
         std::array<Tensor, 3> g, gx;
         c10::OptionalDeviceGuard guard;
@@ -829,6 +848,7 @@ struct DropNode : Node {
             out[k] = gx[k] = at::empty(g[k].sizes(), g[k].options());
         }
         drop(g, gx, q, seed, sd);
+        if (again) set_history(out, again);
         return out;
     }
     void release_variables() override {

@@ -247,3 +247,37 @@ def test_masks_of_several_passes_are_unlike_at_any_shift():
         if shift == 0:
             both.fill_diagonal_(0.25)
         assert (both - 0.25).abs().max().item() <= 7 * math.sqrt(0.25 * 0.75 / (n * 65536)), shift
+
+
+def test_second_derivatives():
+    """A penalty on a gradient that went through the dropout, against the mask multiplied in in 64 bits.  Every value is a product of at most 16 numbers, each
+    rounded once, and sums of two of one sign: off by at most 32 half steps of fp32."""
+    g = torch.Generator().manual_seed(4)
+    x, lower, w, v = [torch.randn(33, 70, generator=g).cuda().requires_grad_() for _ in range(4)]
+    m = kept(x.numel(), 0.6, 21).view(x.shape).double() * (65536 / limit_of(0.6))
+
+    def penalty(x, lower, w, v, drop):
+        a, b = drop(x, lower)
+        gx, gl = torch.autograd.grad((a * w).pow(2).sum() + (b * v).pow(2).sum(), (x, lower), create_graph=True)
+        return torch.autograd.grad(gx.pow(2).sum() + gl.pow(2).sum(), (x, w, lower, v))
+
+    def one(x, lower):
+        return F.dropout(x, 0.6, 21), F.dropout(lower, 0.6, torch.tensor(21, device="cuda"))
+
+    want = penalty(*[t.detach().double().requires_grad_() for t in (x, lower, w, v)], lambda a, b: (a * m, b * m))
+    for drop in (one, lambda a, b: F.bound_dropout(a, b, None, 0.6, 21)[:2]):
+        for got, exact in zip(penalty(x, lower, w, v, drop), want):
+            assert ((got.double() - exact).abs() <= 32 * 2.0 ** -24 * exact.abs()).all()
+    # one of two tensors alone, and a gradient that depends on nothing
+    a, b, _ = F.bound_dropout(x, lower, None, 0.6, 21)
+    gl, = torch.autograd.grad((a * b * v).sum(), lower, create_graph=True)
+    got, exact = torch.autograd.grad(gl.pow(2).sum(), (x, v)), (2 * (m * m * x * v) * m * m * v, 2 * (m * m * x * v) * m * m * x)
+    assert all(((p.double() - q).abs() <= 32 * 2.0 ** -24 * q.abs()).all() for p, q in zip(got, exact))
+    gx, = torch.autograd.grad(F.dropout(x, 0.6, 21), x, torch.ones_like(x), create_graph=True)
+    assert not gx.requires_grad
+    # and a third derivative
+    y = F.dropout(x, 0.6, 21)
+    first, = torch.autograd.grad(y.pow(3).sum(), x, create_graph=True)
+    second, = torch.autograd.grad(first.sum(), x, create_graph=True)
+    third, = torch.autograd.grad(second.sum(), x)
+    assert ((third.double() - 6 * m ** 3).abs() <= 32 * 2.0 ** -24 * 6 * m ** 3).all()
