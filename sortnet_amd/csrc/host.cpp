@@ -641,6 +641,15 @@ private:
     }
 };
 
+// Stands behind a gradient that create_graph asked for: the first derivative is right, a second one would be more than these
+// kernels know.
+struct OnceNode : Node {
+    variable_list apply(variable_list&&) override {
+        throw std::runtime_error("sortnet_amd: label_log_probs, preference_loss and policy_loss can be differentiated once: their gradients have no derivatives");
+    }
+    std::string name() const override { return "OnceNode"; }
+};
+
 struct LabelNode : Node {
     enum Kind { VALUES, PREFERENCE, POLICY } kind;
     SavedVariable logits, labels, work;
@@ -654,6 +663,11 @@ struct LabelNode : Node {
         variable_list out(1);
         if (!task_should_compute_output(0)) return out;
         const Tensor z = logits.unpack(), l = labels.unpack(), wk = work.unpack();
+        std::shared_ptr<OnceNode> once;
+        if (at::GradMode::is_enabled()) {
+            once = new_node<OnceNode>();
+            once->set_next_edges({next_edge(0), grads[0].defined() ? torch::autograd::impl::gradient_edge(grads[0]) : torch::autograd::Edge()});
+        }
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor g = incoming(*this, grads, 0);
         const c10::DeviceGuard guard(z.device());
@@ -663,12 +677,14 @@ struct LabelNode : Node {
         const int64_t now = made.defined() && last ? capture_of(stream_of(z)) : -1;
         const bool there = now >= 0 && now == capture, loss = kind != VALUES;
         out[0] = there ? std::move(made) : at::empty(z.sizes(), z.options());
-        if (out[0].numel() == 0) return out;
-        const sd_label_rows a = label_rows(z, l, ignore);
-        const Work w(wk, a.rows, loss);
-        const float* gp = floats(g, "grad_output");     // of log probabilities: the rows' weights
-        require(sd_label_gradient(&a, w.stats, loss ? w.weight : gp, kind == POLICY ? w.scale : nullptr, loss ? gp : nullptr, there, out[0].data_ptr(), stream_of(z)),
-                "sd_label_gradient");
+        if (out[0].numel() > 0) {
+            const sd_label_rows a = label_rows(z, l, ignore);
+            const Work w(wk, a.rows, loss);
+            const float* gp = floats(g, "grad_output");     // of log probabilities: the rows' weights
+            require(sd_label_gradient(&a, w.stats, loss ? w.weight : gp, kind == POLICY ? w.scale : nullptr, loss ? gp : nullptr, there, out[0].data_ptr(), stream_of(z)),
+                    "sd_label_gradient");
+        }
+        if (once) set_history(out[0], once);
         return out;
     }
     void will_release_variables() override {

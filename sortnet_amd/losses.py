@@ -9,7 +9,7 @@ a plain function; the classes below carry the reference's names, constructor arg
 Beside them stand losses for heads that learn from answers, preferences and rewards instead of one right label
 (no counterpart in the reference): `label_log_probs`, `preference_loss` and `policy_loss`, as HIP kernels.  They take
 logits in fp32, bf16 or fp16 on the GPU; of `worst_outputs` in the place of `outputs` they take the certified lower bounds of the
-log probabilities, as the cross entropies above do.
+log probabilities, as the cross entropies above do.  They are differentiated once: a derivative of their gradients raises an error.
 """
 import math
 

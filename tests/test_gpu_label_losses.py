@@ -657,3 +657,47 @@ def test_rows_beyond_32_bit_offsets():
     grad, = torch.autograd.grad(lp.sum(), z)
     check_gradient(grad[-1:], z[-1:], labels[-1:], torch.ones(1, device="cuda", dtype=torch.float64), torch.zeros(1, device="cuda", dtype=torch.float64), "gradient")
     assert (grad[1:3] == 0).all() and (grad[-2] == 0).all()
+
+
+def test_second_derivatives_are_refused():
+    """A gradient under create_graph is the gradient; whatever asks for its derivative raises, and what does not, does not."""
+    z, labels, g = make(8, 30, torch.float32, 3)
+    ref, adv = exact_rows(z, labels)[0].float() + 0.1, torch.randn(8, generator=g).cuda()
+    up = torch.randn(8, generator=g).cuda().requires_grad_()
+    leaf = z.requires_grad_()
+    wide = (torch.randn(30, 8, generator=g).cuda().requires_grad_(), lambda t: t.t())       # logits that are copied
+    for start, view in ((leaf, lambda t: t), (leaf, lambda t: torch.tanh(t) * 3), wide):
+        for call in (lambda t: (losses.label_log_probs(t, labels) * up).sum(), lambda t: losses.preference_loss(t, labels, ref)[0],
+                     lambda t: losses.policy_loss(t, labels, ref, adv, ref_log_probs=ref, kl_coef=0.1)[0]):
+            plain, = torch.autograd.grad(call(view(start)), start)
+            loss = call(view(start))
+            grad, = torch.autograd.grad(loss, start, create_graph=True)
+            assert torch.equal(grad, plain) and grad.requires_grad
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                torch.autograd.grad(grad.pow(2).sum(), start, retain_graph=True)
+            with pytest.raises(RuntimeError, match="differentiated once"):
+                (loss + grad.pow(2).sum()).backward(retain_graph=True)
+            again, = torch.autograd.grad(loss + grad.detach().sum(), start)
+            assert torch.equal(again, plain)
+    loss = (losses.label_log_probs(leaf, labels) * up).sum()
+    grad, = torch.autograd.grad(loss, leaf, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated once"):
+        torch.autograd.grad(grad.sum(), up)
+    empty = z[:0].detach().requires_grad_()
+    grad, = torch.autograd.grad(losses.label_log_probs(empty, labels[:0]).sum(), empty, create_graph=True)
+    assert grad.shape == (0, 30)
+
+
+def test_second_derivatives_of_a_gradient_made_with_the_loss():
+    """The same where the policy's forward made the gradient (32 MiB of logits and more)."""
+    rows, classes = 40000, 230
+    z, labels, g = make(rows, classes, torch.float32, 78)
+    old, adv = exact_rows(z, labels)[0].float(), torch.randn(rows, generator=g).cuda()
+    z.requires_grad_()
+    plain, = torch.autograd.grad(losses.policy_loss(z, labels, old, adv)[0], z)
+    for retain in (True, False):
+        loss = losses.policy_loss(z, labels, old, adv)[0]
+        grad, = torch.autograd.grad(loss, z, create_graph=True, retain_graph=retain)
+        assert torch.equal(grad, plain)
+        with pytest.raises(RuntimeError, match="differentiated once"):
+            torch.autograd.grad(grad.sum(), z)
