@@ -55,3 +55,23 @@ def test_rewards_of_long_answers(dtype):
     _, rewards = losses.preference_loss(z.view(4, 1024, -1), labels.view(4, 1024), ref.view(4, 1024), beta=0.1)
     exact = 0.1 * (want - ref.double()).view(4, 1024).sum(1)
     assert ((rewards.double() - exact).abs() <= 0.1 * (1024 * 0.25 + 6 * math.sqrt(1024) * 1.2) * U + U * exact.abs()).all()
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_divergence_of_near_policies(rows):
+    """exp(a) - 1 - a of reference and policy, a from 1e-6 to 20 of either sign.  Rows of one class that can be chosen have the log probability 0, so a is the
+    reference's: below 1/2 the power series rounds a, its square, eight steps of which the last two count, and the result: 8 u.  Beyond, expm1 is off by
+    2 u of its value, and its argument, rounded already, by nothing; that is 2 u (1 - exp(-1/2)) / (exp(-1/2) - 1/2) = 7.4 u of the result at -1/2 and 8.8 u
+    at 1/2, less further out; and 2 u for the results, stored twice."""
+    z = torch.full((rows, 5), -math.inf, device="cuda")
+    z[:, 3] = 1.25
+    labels = torch.full((rows,), 3, device="cuda")
+    zero, one = torch.zeros(rows, device="cuda"), torch.ones(rows, device="cuda")
+    for size in (1e-6, 1e-5, 1e-4, 1e-3, 1e-2, 0.1, 0.3, 0.4999, 0.5, 0.5001, 0.7, 1.0, 3.0, 20.0):
+        for a in (size, -size):
+            ref = torch.full((rows,), a, device="cuda")
+            d = ref[0].double().item()
+            exact = d * d / 2 * (1 + d / 3 * (1 + d / 4 * (1 + d / 5))) if size < 0.005 else math.expm1(d) - d
+            z.requires_grad_()
+            loss, stats = losses.policy_loss(z, labels, zero, zero, ref_log_probs=ref, kl_coef=1.0)
+            assert abs(stats[1].item() - exact) <= 11 * U * exact and abs(loss.item() - exact) <= 11 * U * exact, a
