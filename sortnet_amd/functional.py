@@ -299,6 +299,11 @@ def dropout_seed(number):
             (n >> 24 & 4) | (n >> 23 & 0x30) | (n >> 21 & 0x100) | (n >> 20 & 0x400) | (n >> 17 & 0x4000))
 
 
+def _keeps_all(q):
+    """Whether `dropout` keeps every value at q: None, 1 and what is rounded to 1."""
+    return q is None or 1.0 - 2.0 ** -17 <= q <= 1.0
+
+
 def _dropped(tensors, q, seed):
     on_device = isinstance(seed, torch.Tensor)
     return _C.host().dropout(tensors, q, 0 if on_device else seed & 0xFFFFFFFF, seed if on_device else None)
@@ -310,8 +315,9 @@ def dropout(input, q, seed):
     again, and so does a call with the same seed.  `seed` is a whole number or one int64 on the input's device; a captured
     graph replays the mask of a number, and reads a device seed in each replay (change it between replays, not between a
     forward and its backward).  Seeds that count up are to be taken through `dropout_seed`: their masks are else shifted copies of
-    each other above 2^18 values.  Dropped values are 0 whatever they were.  q = 1 or None returns the input."""
-    if q is None or q == 1.0:
+    each other above 2^18 values.  Dropped values are 0 whatever they were.  None, and a q that is rounded to 1, return the
+    input; one that is rounded to 0 (below 2^-17) keeps nothing."""
+    if _keeps_all(q):
         return input
     return _dropped([input], q, seed)[0]
 
@@ -319,7 +325,7 @@ def dropout(input, q, seed):
 def bound_dropout(x, lower, upper, q, seed):
     """`dropout` of values and their bounds under one mask, in one launch (None stays None): what stays is scaled by a positive
     number, so bounds of the input are bounds of the result."""
-    if q is None or q == 1.0:
+    if _keeps_all(q):
         return x, lower, upper
     there = [t for t in (x, lower, upper) if t is not None]
     done = iter(_dropped(there, q, seed) if there else ())

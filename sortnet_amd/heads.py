@@ -31,7 +31,7 @@ class BoundTanh(nn.Tanh):
 
 class BoundDropout(nn.Module):
     """Dropout of a dense head's features (no counterpart in the reference): in training, values and bounds keep the same entries,
-    each with probability `q`, divided by it; in evaluation, or with q = 1 or None, nothing changes.  The mask is a function of a
+    each with probability `q`, divided by it (rounded to 1/65536); in evaluation, or with q = 1 or None, nothing changes.  The mask is a function of a
     seed and is never stored.  Seeds are those of the numbers (`functional.dropout_seed`) of the registry that the distance layers' lists come
     from (`layers.set_mask_seed` makes a run reproducible); `last_seed` is that of the latest pass, with which `functional.bound_dropout` makes
     the same mask again.  A captured graph would replay one mask: `seed`, one int64 on the GPU, is then read in each replay, and is the caller's
@@ -39,12 +39,12 @@ class BoundDropout(nn.Module):
 
     def __init__(self, q, registry=None, seed=None):
         super().__init__()
-        if q is not None and not 0.0 < q <= 1.0:
-            raise ValueError("BoundDropout: keep probability q=%s outside 0..1" % (q,))
+        if q is not None and not 2.0 ** -17 <= q <= 1.0:     # (a smaller one is rounded to 0: nothing would be left to train)
+            raise ValueError("BoundDropout: keep probability q=%s outside 2^-17..1" % (q,))
         self.q, self.registry, self.seed, self.last_seed = q, DEFAULT_REGISTRY if registry is None else registry, seed, None
 
     def forward(self, x=None, lower=None, upper=None):
-        if not self.training or self.q is None or self.q == 1.0:
+        if not self.training or F._keeps_all(self.q):
             return x, lower, upper
         self.last_seed = F.dropout_seed(self.registry.next_seed()) if self.seed is None else self.seed
         return F.bound_dropout(x, lower, upper, self.q, self.last_seed)

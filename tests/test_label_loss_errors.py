@@ -124,3 +124,22 @@ def test_seeds_of_layers_continue_the_registry():
 def test_losses_keep_their_registry():
     assert set(losses.LOSSES) == {"hinge", "crossentropy", "mixture", "ce_hinge", "ce_mixture"}
     assert ext.host().label_log_probs is not None
+
+
+def test_keep_probabilities_that_are_rounded_to_the_ends():
+    """q is rounded to 1/65536: a layer that would keep nothing is refused, one that would keep everything draws no seed and runs no kernel."""
+    x = torch.randn(3, 4)
+    for q in (1e-300, 1e-6, 2.0 ** -17 * (1 - 2.0 ** -50)):
+        with pytest.raises(ValueError):
+            heads.BoundDropout(q)
+    for q in (2.0 ** -17, 2.0 ** -16):
+        assert heads.BoundDropout(q).q == q
+    for q in (1.0 - 2.0 ** -17, 1.0 - 1e-9, 1.0):
+        layer = heads.BoundDropout(q, registry=DropoutRegistry(seed=1))
+        assert layer(x, None, x) == (x, None, x) and layer.last_seed is None and layer.registry.draws == 0
+        assert F.dropout(x, q, 3) is x and F.bound_dropout(x, x, None, q, 3) == (x, x, None)
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        F.dropout(x, 1.0 - 2.0 ** -17 - 1e-9, 3)
+    for q in (1.0 + 1e-9, math.inf, math.nan, -1e-9):
+        with pytest.raises(ValueError):
+            heads.BoundDropout(q)
