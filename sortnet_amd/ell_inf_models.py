@@ -82,7 +82,8 @@ class _HybridNet(_SortNet):
 
     def _build_head(self, features, hidden, num_classes, scalar, head_dropout, registry):
         self.fc_linear = BoundSequential(BoundLinear(features, hidden, bias=True), BoundTanh())
-        self.head_drop = BoundDropout(head_dropout, registry)
+        if head_dropout is not None:
+            self.head_drop = BoundDropout(head_dropout, registry)
         self.fc_final = BoundFinalLinear(hidden, num_classes, bias=True)
         self.scalar = _make_scalar(scalar)
 
@@ -90,7 +91,10 @@ class _HybridNet(_SortNet):
         paras = apply_if_not_none(self._distance_features(x, eps, up, down), self._pool)
         if targets is not None and (paras[1] is None or paras[2] is None):
             paras = paras[0], paras[0] - eps, paras[0] + eps
-        paras = self.head_drop(*self.fc_linear(paras))
+        paras = self.fc_linear(paras)
+        drop = self._modules.get("head_drop")       # (models without one, those that were saved before there was one among them)
+        if drop is not None:
+            paras = drop(*paras)
         out = self.fc_final(*paras, targets=targets)
         if targets is None:
             return out * self.scalar
