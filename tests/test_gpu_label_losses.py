@@ -701,3 +701,9 @@ def test_second_derivatives_of_a_gradient_made_with_the_loss():
         assert torch.equal(grad, plain)
         with pytest.raises(RuntimeError, match="differentiated once"):
             torch.autograd.grad(grad.sum(), z)
+
+
+@pytest.mark.parametrize("bits", [torch.int32, torch.int64], ids=str)
+@pytest.mark.parametrize("classes", [7, 5000, 40001])
+def test_preference_of_packed_answers_in_half_precision(classes, bits):
+    test_preference_of_packed_answers(classes, bits, torch.float16)
