@@ -487,8 +487,8 @@ template <class T> __global__ void __launch_bounds__(256, 8) label_long_rows_ker
 }
 
 // The workgroup holds a long row in its registers, at most 16 vectors per work-item.  FUSED: the logits are read once and the gradient leaves
-// with the statistics.  FAR: logits that the last-level cache cannot hold are read past it (4096 x 131072 bf16 401 -> 393 us,
-// 4096 x 65536 201 -> 191; 2000 x 50001 fp16, which it holds, 76, past it 95).  (Reading the row again from the caches instead lost: eight rows of 256 KiB
+// with the statistics.  FAR: logits that the last-level cache cannot hold are read past it (4096 x 131072 bf16 437 -> 432 us with
+// the launches beside it, 4096 x 65536 206 -> 197; 2000 x 50001 fp16, which it holds, 76, past it 95).  (Reading the row again from the caches instead lost: eight rows of 256 KiB
 // per compute unit are more than the last level holds, 4096 x 131072 596 us where two passes of their own took 515.)
 template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __launch_bounds__(THREADS, 4) label_held_rows_kernel(Rows a, Finish e, Gradient g) {
     constexpr int V = Elem<T>::kVec, kChunk = (NV == 16 ? 8 : 16) / V;

@@ -63,7 +63,7 @@ def label_log_probs(outputs, targets, ignore_index=-100):
 
     outputs (..., classes); targets int64 or int32 with the sizes before the classes.  Rows whose target is `ignore_index` are not
     read: 0, with a gradient of zeros, whatever they hold.  A target that names no class gives NaN.  Rows may be strided (a padded vocabulary, a
-    part of a batch); logits of -inf are classes that cannot be chosen."""
+    part of a batch); logits of -inf are classes that cannot be chosen.  A batch of no rows gives no values."""
     return ext.host().label_log_probs(outputs, targets, ignore_index)
 
 
@@ -76,7 +76,7 @@ def preference_loss(outputs, targets, ref_log_probs, offsets=None, beta=0.1, lab
     the tokens (`ignore_index` for prompts and padding), `ref_log_probs` what label_log_probs gives for the reference model.
 
     rewards[a] = beta sum over the rows of a of (log prob - ref), without a gradient; x = chosen's - rejected's reward;
-    loss = mean of -(1 - s) log sigma(x) - s log sigma(-x) with s = label_smoothing below 1/2."""
+    loss = mean of -(1 - s) log sigma(x) - s log sigma(-x) with s = label_smoothing below 1/2.  A batch of no pairs, or of no rows, is refused."""
     return ext.host().preference_loss(outputs, targets, ref_log_probs, offsets, beta, label_smoothing, ignore_index)
 
 
@@ -85,9 +85,10 @@ def policy_loss(outputs, targets, old_log_probs, advantages, ref_log_probs=None,
 
     Per row, with ratio = exp(log prob - old) of the action `targets` and advantage A:
         -min(ratio A, clip(ratio, 1 - clip, 1 + clip_high) A) + kl_coef (exp(ref - log prob) - (ref - log prob) - 1)
-    and the mean over the rows that are not ignored (0 where all are).  clip_high defaults to clip.  `old_log_probs`, `advantages` and
+    and the mean over the rows that are not ignored (0 where all are; a batch of no rows is refused).  clip_high defaults to clip.  `old_log_probs`, `advantages` and
     `ref_log_probs` have the sizes of `targets` and get no gradient; one advantage per answer is given as `a[:, None].expand(...)`, which is
-    not copied.  stats: the first term, the divergence (without kl_coef; 0 where that is 0) and the share of clipped rows."""
+    not copied.  From 32 MiB of logits on the gradient is made with the loss, for an upstream gradient of 1: a positive factor on the loss is cheaper
+    as one on `advantages` and `kl_coef`.  stats: the first term, the divergence (without kl_coef; 0 where that is 0) and the share of clipped rows."""
     return ext.host().policy_loss(outputs, targets, old_log_probs, advantages, ref_log_probs, clip, clip if clip_high is None else clip_high,
                                   kl_coef, ignore_index)
 

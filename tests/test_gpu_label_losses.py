@@ -707,3 +707,16 @@ def test_second_derivatives_of_a_gradient_made_with_the_loss():
 @pytest.mark.parametrize("classes", [7, 5000, 40001])
 def test_preference_of_packed_answers_in_half_precision(classes, bits):
     test_preference_of_packed_answers(classes, bits, torch.float16)
+
+
+def test_policy_scaled_by_its_inputs():
+    """A positive factor, a power of two, on advantages and kl_coef is one on the loss: the same bits, its sizes and the gradient made with the loss included."""
+    for rows, classes in ((64, 30), (40000, 230)):
+        z, labels, g = make(rows, classes, torch.float32, 11)
+        lp = exact_rows(z, labels)[0].float()
+        old, ref, adv = lp - 0.2 * torch.randn(rows, generator=g).cuda(), lp + 0.2, torch.randn(rows, generator=g).cuda()
+        z.requires_grad_()
+        loss, _ = losses.policy_loss(z, labels, old, adv, ref_log_probs=ref, kl_coef=0.5)
+        scaled, _ = losses.policy_loss(z, labels, old, 8 * adv, ref_log_probs=ref, kl_coef=4.0)
+        assert torch.equal(8 * loss, scaled)
+        assert torch.equal(torch.autograd.grad(8 * loss, z)[0], torch.autograd.grad(scaled, z)[0])
