@@ -35,7 +35,8 @@ class BoundDropout(nn.Module):
     seed and is never stored.  Seeds are those of the numbers (`functional.dropout_seed`) of the registry that the distance layers' lists come
     from (`layers.set_mask_seed` makes a run reproducible); `last_seed` is that of the latest pass, with which `functional.bound_dropout` makes
     the same mask again.  A captured graph would replay one mask: `seed`, one int64 on the GPU, is then read in each replay, and is the caller's
-    to change between them, to `functional.dropout_seed` of a number that counts up."""
+    to change between them, to `functional.dropout_seed` of a number that counts up.  A forward that is run again for the backward (activation
+    checkpointing) would draw another mask: give the layer a `seed` there, too, or call `functional.bound_dropout` with one."""
 
     def __init__(self, q, registry=None, seed=None):
         super().__init__()

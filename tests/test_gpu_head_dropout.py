@@ -281,3 +281,26 @@ def test_second_derivatives():
     second, = torch.autograd.grad(first.sum(), x, create_graph=True)
     third, = torch.autograd.grad(second.sum(), x)
     assert ((third.double() - 6 * m ** 3).abs() <= 32 * 2.0 ** -24 * 6 * m ** 3).all()
+
+
+def test_activation_checkpointing():
+    """A step whose forward runs again for the backward: the gradients of the step itself, with the functions and with a layer that has a seed of its own."""
+    from torch.utils.checkpoint import checkpoint
+    g = torch.Generator().manual_seed(9)
+    x, w = torch.randn(64, 40, generator=g).cuda().requires_grad_(), torch.randn(40, 30, generator=g).cuda().requires_grad_()
+    t = torch.randint(0, 30, (64,), generator=g).cuda()
+    ref, adv = torch.full((64,), -3.0, device="cuda"), torch.randn(64, generator=g).cuda()
+    layer = heads.BoundDropout(0.7, seed=torch.tensor(F.dropout_seed(3), device="cuda"))
+    for drop in (lambda v: F.dropout(v, 0.7, 9), lambda v: layer(v)[0]):
+        for loss in (lambda z: losses.label_log_probs(z, t).sum(), lambda z: losses.preference_loss(z, t, ref)[0],
+                     lambda z: losses.policy_loss(z, t, ref, adv, ref_log_probs=ref, kl_coef=0.1)[0]):
+            step = lambda x, w: loss(drop(torch.tanh(x)) @ w)
+            want = torch.autograd.grad(step(x, w), (x, w))
+            for reentrant in (False, True):
+                if reentrant:       # (serves .backward() alone)
+                    x.grad = w.grad = None
+                    checkpoint(step, x, w, use_reentrant=True).backward()
+                    got = x.grad, w.grad
+                else:
+                    got = torch.autograd.grad(checkpoint(step, x, w, use_reentrant=False), (x, w))
+                assert all(torch.equal(a, b) for a, b in zip(got, want))
