@@ -376,6 +376,45 @@ int sd_policy_loss(const sd_label_rows* rows, const float* old_log_probs, const 
 int sd_label_gradient(const sd_label_rows* rows, const float* stats, const float* weight, const float* scale, const float* scale2,
                       int unless_one, void* grad, sd_stream_t stream);
 
+/* ---- answering with a head's logits, learning from another model's (no reference launchers) ----
+ * As above: fp32, bf16 or fp16, everything per row in 32 bits or more, scratch from the caller. */
+
+/* Rows of logits, laid out as in sd_label_rows. */
+typedef struct {
+    const void* logits;
+    int64_t rows, inner, classes, outer_stride, inner_stride;
+    int dtype;
+} sd_logit_rows;
+
+/* What constrains the choice of a class.  Rows of the history, the bias and the allowed classes lie as those of the logits, (r / inner) *
+ * outer + (r % inner) * inner entries behind their pointer; strides may be 0.
+ *   history (NULL: none): history_length classes of history_bytes = 4 or 8 each, of which row r's first lengths[r] count (NULL: all; of
+ *     length_bytes; taken as 0..history_length); entries outside 0..classes-1 are no class.
+ *   repetition_rows, presence_rows, frequency_rows: one number for each row, or NULL: the number that follows.
+ *   bias (NULL: none): fp32, one for each class.
+ *   allowed (NULL: all): SD_ALLOWED_FLAGS one byte for each class, or SD_ALLOWED_BITS, bit v % 32 of the 32-bit word v / 32; strides in bytes
+ *     and in words. */
+#define SD_ALLOWED_FLAGS 1
+#define SD_ALLOWED_BITS 2
+typedef struct {
+    const void* history;
+    const void* lengths;
+    const float* repetition_rows;
+    const float* presence_rows;
+    const float* frequency_rows;
+    const float* bias;
+    const void* allowed;
+    double repetition, presence, frequency;
+    int64_t history_length, history_outer, history_inner, bias_outer, bias_inner, allowed_outer, allowed_inner;
+    int history_bytes, length_bytes, allowed_kind;
+} sd_constraints;
+
+/* out[r, v], rows of `classes` values one behind the other in the logits' type: with n = how often v stands in row r's history, z where n = 0, else
+ * (z > 0 ? z / repetition : z * repetition) - frequency n - presence; plus bias; -inf where v is not allowed.  The gradient reads the
+ * logits only where n > 0. */
+int sd_constrain_logits(const sd_logit_rows* rows, const sd_constraints* constraints, void* out, sd_stream_t stream);
+int sd_constrain_gradient(const sd_logit_rows* rows, const sd_constraints* constraints, const void* grad_output, void* grad, sd_stream_t stream);
+
 /* Dropout of up to three tensors of n values under one mask (inputs that are not wanted are NULL with their outputs): value i is kept
  * where field i of the generator is below L = floor(65536 q + 0.5), and multiplied by 65536 / L.  The fields of values 2j and 2j + 1 are
  * the low and high halves of mix(sd_rng_word(seed, 5, j >> 15, j & 32767) ^ key), mix being the generator's finaliser and key =

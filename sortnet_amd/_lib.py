@@ -25,7 +25,22 @@ class LabelRows(ctypes.Structure):
                 ("inner_stride", _l), ("ignore_index", _l), ("dtype", _i)]
 
 
+class LogitRows(ctypes.Structure):
+    """sd_logit_rows of include/sortdist.h."""
+    _fields_ = [("logits", _F), ("rows", _l), ("inner", _l), ("classes", _l), ("outer_stride", _l), ("inner_stride", _l), ("dtype", _i)]
+
+
+class Constraints(ctypes.Structure):
+    """sd_constraints of include/sortdist.h."""
+    _fields_ = [("history", _I), ("lengths", _I), ("repetition_rows", _F), ("presence_rows", _F), ("frequency_rows", _F), ("bias", _F), ("allowed", _I),
+                ("repetition", _d), ("presence", _d), ("frequency", _d), ("history_length", _l), ("history_outer", _l), ("history_inner", _l),
+                ("bias_outer", _l), ("bias_inner", _l), ("allowed_outer", _l), ("allowed_inner", _l), ("history_bytes", _i), ("length_bytes", _i),
+                ("allowed_kind", _i)]
+
+
 _R = ctypes.POINTER(LabelRows)
+_Z = ctypes.POINTER(LogitRows)
+_C = ctypes.POINTER(Constraints)
 
 # name -> argument types, in the order of include/sortdist.h
 SIGNATURES = {
@@ -63,6 +78,8 @@ SIGNATURES = {
     "sd_preference_loss": [_R, _F, _I, _i, _l, _i, _d, _d, _F, _F, _F, _F, _F, _S],
     "sd_policy_loss": [_R, _F, _F, _l, _l, _F, _d, _d, _d, _F, _F, _F, _F, _F, _F, _F, _S],
     "sd_label_gradient": [_R, _F, _F, _F, _F, _i, _F, _S],
+    "sd_constrain_logits": [_Z, _C, _F, _S],
+    "sd_constrain_gradient": [_Z, _C, _F, _F, _S],
     "sd_dropout": [_F, _F, _F, _i, _l, _d, _u, _I, _F, _F, _F, _S],
 }
 _OTHER = {

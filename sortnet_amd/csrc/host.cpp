@@ -915,6 +915,195 @@ std::vector<Tensor> dropout(const std::vector<Tensor>& inputs, double q, int64_t
     return out;
 }
 
+// ---- logits as they stand when a class is chosen -------------------------------------------------------------------------
+// rows of logits that readable_logits has made readable
+sd_logit_rows logit_rows(const Tensor& z) {
+    sd_logit_rows a{};
+    a.dtype = element_type(z, "outputs");
+    a.logits = z.data_ptr();
+    a.classes = z.size(-1);
+    a.rows = a.classes > 0 ? z.numel() / a.classes : 0;
+    if (z.dim() == 3) {
+        a.inner = z.size(1);
+        a.outer_stride = z.stride(0); a.inner_stride = z.stride(1);
+    } else {
+        a.inner = a.rows;
+        a.inner_stride = z.dim() == 2 ? z.stride(0) : a.classes;
+    }
+    return a;
+}
+
+void check_outputs(const Tensor& outputs) {
+    element_type(outputs, "outputs");
+    if (outputs.dim() < 2 || outputs.size(-1) < 1) throw std::runtime_error("outputs must have the sizes (..., classes), with one class at least");
+}
+
+// What stands beside the rows of logits: entries of a row next to each other, rows with the strides of the logits' dimensions, or one row for all
+// (its only dimension).
+struct Beside {
+    Tensor t;
+    int64_t outer = 0, inner = 0;
+    Beside() = default;
+    Beside(const Tensor& given, const char* name, const Tensor& z, bool may_be_shared, int64_t entries) : t(given) {
+        same_device(t, name, z);
+        const bool shared = may_be_shared && t.dim() == 1;
+        if (!shared && (t.dim() != z.dim() || t.sizes().slice(0, t.dim() - 1) != z.sizes().slice(0, z.dim() - 1)))
+            throw std::runtime_error(std::string(name) + " must have the sizes of outputs before the classes");
+        if (entries >= 0 && t.size(-1) != entries) throw std::runtime_error(std::string(name) + " must have " + std::to_string(entries) + " entries for each row, not " + std::to_string(t.size(-1)));
+        if ((t.size(-1) > 1 && t.stride(-1) != 1) || t.dim() > 3) t = t.contiguous();
+        if (shared) return;
+        if (t.dim() == 3) outer = t.stride(0);
+        inner = t.dim() <= 3 ? t.stride(-2) : t.size(-1);
+    }
+};
+
+void no_gradient(const Tensor& t, const char* name) {
+    if (at::GradMode::is_enabled() && t.requires_grad()) throw std::runtime_error(std::string(name) + " must not require a gradient: the result is differentiated with respect to outputs alone");
+}
+
+struct Constraints {
+    Tensor z;       // the logits
+    Beside history, bias, allowed;
+    Tensor lengths, rows[3];
+    double numbers[3] = {1.0, 0.0, 0.0};    // repetition, presence, frequency, where there is no tensor of them
+
+    bool narrow() const { return history.t.defined() || allowed.t.defined(); }   // (else the gradient passes as it is)
+    void call(const Tensor* grad, const Tensor& out) const {
+        if (out.numel() == 0) return;
+        const sd_logit_rows a = logit_rows(z);
+        sd_constraints c{};
+        if (history.t.defined()) {
+            c.history = history.t.data_ptr();
+            c.history_bytes = (int)history.t.element_size();
+            c.history_length = history.t.size(-1);
+            c.history_outer = history.outer; c.history_inner = history.inner;
+            if (lengths.defined()) { c.lengths = lengths.data_ptr(); c.length_bytes = (int)lengths.element_size(); }
+            if (rows[0].defined()) c.repetition_rows = floats(rows[0], "repetition");
+            if (rows[1].defined()) c.presence_rows = floats(rows[1], "presence");
+            if (rows[2].defined()) c.frequency_rows = floats(rows[2], "frequency");
+        }
+        c.repetition = numbers[0]; c.presence = numbers[1]; c.frequency = numbers[2];
+        if (bias.t.defined()) { c.bias = static_cast<const float*>(bias.t.data_ptr()); c.bias_outer = bias.outer; c.bias_inner = bias.inner; }
+        if (allowed.t.defined()) {
+            c.allowed = allowed.t.data_ptr();
+            c.allowed_kind = allowed.t.scalar_type() == at::kBool ? SD_ALLOWED_FLAGS : SD_ALLOWED_BITS;
+            c.allowed_outer = allowed.outer; c.allowed_inner = allowed.inner;
+        }
+        if (grad) require(sd_constrain_gradient(&a, &c, grad->data_ptr(), out.data_ptr(), stream_of(z)), "sd_constrain_gradient");
+        else require(sd_constrain_logits(&a, &c, out.data_ptr(), stream_of(z)), "sd_constrain_logits");
+    }
+};
+
+// The results are linear in the gradients, with one factor each: the derivative of this node's is the node again.
+struct ConstrainNode : Node {
+    SavedVariable logits, history, bias, allowed, lengths, rows[3];
+    Constraints given;      // all but the tensors
+
+    void save(const Constraints& c) {
+        given = c;
+        given.z = given.history.t = given.bias.t = given.allowed.t = given.lengths = Tensor();
+        for (Tensor& t : given.rows) t = Tensor();
+        logits = SavedVariable(c.z, false);
+        const auto keep = [](SavedVariable& v, const Tensor& t) { if (t.defined()) v = SavedVariable(t, false); };
+        keep(history, c.history.t); keep(allowed, c.allowed.t); keep(lengths, c.lengths);
+        for (int k = 0; k < 3; k++) keep(rows[k], c.rows[k]);
+    }
+    variable_list apply(variable_list&& grads) override {
+        const Locked lock(mutex_);
+        variable_list out(1);
+        if (!task_should_compute_output(0)) return out;
+        Constraints c = given;
+        c.z = logits.unpack(); c.history.t = history.unpack(); c.allowed.t = allowed.unpack(); c.lengths = lengths.unpack();
+        for (int k = 0; k < 3; k++) c.rows[k] = rows[k].unpack();
+        const bool again = at::GradMode::is_enabled() && grads[0].defined() && grads[0].requires_grad();
+        std::shared_ptr<ConstrainNode> next;
+        if (again) {
+            next = new_node<ConstrainNode>();
+            next->set_next_edges({torch::autograd::impl::gradient_edge(grads[0])});
+            next->save(c);
+        }
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor g = incoming(*this, grads, 0);
+        const c10::DeviceGuard guard(c.z.device());
+        out[0] = at::empty(c.z.sizes(), c.z.options());
+        c.call(&g, out[0]);
+        if (again) set_history(out[0], next);
+        return out;
+    }
+    void release_variables() override {
+        const Locked lock(mutex_);
+        for (SavedVariable* v : {&logits, &history, &bias, &allowed, &lengths, &rows[0], &rows[1], &rows[2]}) v->reset_data();
+    }
+    std::string name() const override { return "ConstrainNode"; }
+};
+
+struct PassNode : Node {       // a bias alone: the gradient as it is
+    variable_list apply(variable_list&& grads) override { return {task_should_compute_output(0) ? grads[0] : Tensor()}; }
+    std::string name() const override { return "PassNode"; }
+};
+
+Tensor constrain_logits(const Tensor& outputs, const OptTensor& history, const OptTensor& lengths, double repetition, double presence, double frequency,
+                        const OptTensor& repetitions, const OptTensor& presences, const OptTensor& frequencies, const OptTensor& bias, const OptTensor& allowed) {
+    reverse_mode_only("constrain_logits", outputs);
+    const auto there = [](const OptTensor& t) { return t && t->defined(); };
+    check_outputs(outputs);
+    const bool grad = want_grad(outputs);
+    const OptTensor* of_rows[3] = {&repetitions, &presences, &frequencies};
+    const char* names[3] = {"repetition", "presence", "frequency"};
+    for (int k = 0; k < 3; k++)
+        if (there(*of_rows[k])) { reverse_mode_only("constrain_logits", **of_rows[k]); no_gradient(**of_rows[k], names[k]); }
+    if (there(bias)) { reverse_mode_only("constrain_logits", *bias); no_gradient(*bias, "bias"); }
+    Constraints c;
+    Tensor out;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const c10::DeviceGuard guard(outputs.device());
+        const auto whole = [](const Tensor& t) { return t.scalar_type() == at::kLong || t.scalar_type() == at::kInt; };
+        c.numbers[0] = repetition; c.numbers[1] = presence; c.numbers[2] = frequency;
+        for (int k = 0; k < 3; k++) {
+            if (!there(*of_rows[k])) continue;
+            const Tensor& t = **of_rows[k];
+            same_device(t, names[k], outputs);
+            if (t.scalar_type() != at::kFloat) throw std::runtime_error(std::string(names[k]) + " must have dtype torch.float32");
+            if (t.sizes() != outputs.sizes().slice(0, outputs.dim() - 1)) throw std::runtime_error(std::string(names[k]) + " must be a number or have the sizes of outputs before the classes");
+            c.rows[k] = t.contiguous();
+        }
+        if (there(history)) {
+            if (!whole(*history)) throw std::runtime_error("history must have dtype torch.int64 or torch.int32");
+            c.history = Beside(*history, "history", outputs, false, -1);
+        }
+        if (there(lengths)) {
+            if (!there(history)) throw std::runtime_error("lengths are those of a history: none was given");
+            same_device(*lengths, "lengths", outputs);
+            if (!whole(*lengths)) throw std::runtime_error("lengths must have dtype torch.int64 or torch.int32");
+            if (lengths->sizes() != outputs.sizes().slice(0, outputs.dim() - 1)) throw std::runtime_error("lengths must have the sizes of outputs before the classes");
+            c.lengths = lengths->contiguous();
+        }
+        if (there(bias)) {
+            if (bias->scalar_type() != at::kFloat) throw std::runtime_error("bias must have dtype torch.float32");
+            c.bias = Beside(*bias, "bias", outputs, true, outputs.size(-1));
+        }
+        if (there(allowed)) {
+            if (allowed->scalar_type() != at::kBool && allowed->scalar_type() != at::kInt) throw std::runtime_error("allowed must have dtype torch.bool, or torch.int32 with a bit for each class");
+            c.allowed = Beside(*allowed, "allowed", outputs, true, allowed->scalar_type() == at::kBool ? outputs.size(-1) : (outputs.size(-1) + 31) / 32);
+        }
+        c.z = readable_logits(outputs);
+        out = at::empty(c.z.sizes(), c.z.options());
+        c.call(nullptr, out);
+    }
+    if (grad) {
+        std::shared_ptr<Node> node;
+        if (c.narrow()) {
+            auto full = new_node<ConstrainNode>();
+            full->save(c);
+            node = full;
+        } else node = new_node<PassNode>();
+        node->set_next_edges(collect_next_edges(outputs));
+        set_history(out, node);
+    }
+    return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -940,4 +1129,5 @@ PYBIND11_MODULE(_host, m) {
     m.def("preference_loss", &preference_loss, released());
     m.def("policy_loss", &policy_loss, released());
     m.def("dropout", &dropout, released());
+    m.def("constrain_logits", &constrain_logits, released());
 }

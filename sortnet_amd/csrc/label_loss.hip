@@ -16,7 +16,6 @@ namespace sd {
 constexpr int kUnroll = 4;          // 16-byte loads of a work-item of a long row that are on their way together
 constexpr int kHeld = 8;            // 16-byte vectors of a short row that a lane holds, at most
 constexpr int kHeldLong = 16 * 1024;    // and of a long row that a workgroup holds
-constexpr int64_t kMostBlocks = 1 << 22;
 constexpr int kShortBlocks = 4096;      // workgroups of short rows, at most
 // Bytes of a FUSED short row from which its gradient is stored past the caches: us with and without, 262144 x 200 fp32 82 / 95,
 // 65536 x 1000 bf16 60 / 62; 1048576 x 10 fp32, whose rows share cache lines, 53 / 35.
@@ -52,20 +51,6 @@ struct Gradient {
     bool unless_one;                // nothing is done where *scale2 is 1
 };
 
-template <class T> __device__ __forceinline__ const T* row_start(const Rows& a, int64_t r) {
-    const uint32_t o = (uint32_t)r / a.inner, i = (uint32_t)r - o * a.inner;
-    return static_cast<const T*>(a.logits) + o * a.outer_stride + i * a.inner_stride;
-}
-
-__device__ __forceinline__ double wave_total(double v) { return group_total(v, 6); }
-
-__device__ __forceinline__ float finite(float top) { return fmaxf(top, -FLT_MAX); }
-
-// exp of a difference to the largest value of a row (or of a part of it): the hardware's exp2 of v log2(e), 1 for 0, so that a row's largest
-// term is exact.  log2(e) is the sum of two numbers (both positive: -inf stays -inf): of one it would be off by 1.3e-8 of v to one side, which the sum
-// over a row and the sum over an answer's rows add up.  As it is the product is rounded once, off by up to |v| 2^-24 of the result to either side,
-// and the hardware's exp2 by up to 1.4 2^-24, 0.06 2^-24 below on average (measured over 2^24 values a binade; expf 0.04).
-__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(fmaf(v, 1.44269504f, v * 1.92596299e-8f)); }
 // The same for what is stored in T: one product will do where that has 16 bits, whose half step is 2^-11 of a value at least.  (4096 x 131072 bf16,
 // policy with its gradient: 437 us with two everywhere, 425 so, 413 with one in the sums, too.)
 template <class T> __device__ __forceinline__ float exp_to(float v) {
@@ -180,20 +165,6 @@ template <class T, int N> __device__ __forceinline__ void slopes(float (&f)[N], 
         #pragma unroll
         for (int i = 0; i < N; i++) f[i] += i == (int)at ? w : 0.f;
     }
-}
-
-// Sums of a row: exponentials of a few vectors in pairs, in 32 bits, and these sums in 64 (an addition to a sum in 32 bits that has the
-// largest value, 1, in it is off by up to 6e-8, and there are hundreds of them).
-template <int N> __device__ __forceinline__ float tree(const float (&f)[N]) {
-    float s[N];
-    #pragma unroll
-    for (int i = 0; i < N; i++) s[i] = f[i];
-    #pragma unroll
-    for (int o = N / 2; o > 0; o >>= 1) {
-        #pragma unroll
-        for (int i = 0; i < o; i++) s[i] += s[i + o];
-    }
-    return s[0];
 }
 
 // ---- short rows: 2^shift lanes of a wavefront hold a row in registers, NV vectors each ---------------------------------------
@@ -406,14 +377,6 @@ template <class T, bool STREAM> __device__ __forceinline__ void scan(const T* p,
     }
 }
 
-// zeros in a row of a gradient, by a whole workgroup
-template <class T> __device__ __forceinline__ void clear_row(T* q, int n, int threads) {
-    constexpr int V = Elem<T>::kVec;
-    const int full = n / V;
-    for (int i = threadIdx.x; i < full; i += threads) put_stream16(q + i * V, u32x4{0u, 0u, 0u, 0u});
-    for (int j = full * V + threadIdx.x; j < n; j += threads) q[j] = T{};
-}
-
 // columns [c0, c1) of a row, c0 a multiple of the vector's length; a row of weight 0 (ignored, clipped, or of no answer) is not read
 template <class T, bool STREAM> __device__ __forceinline__ void grad_row(const T* src, T* dst, float top, float inverse, float w, int label, int64_t c0, int64_t c1, int lane, int lanes) {
     constexpr int V = Elem<T>::kVec;
@@ -590,22 +553,6 @@ template <class T> __global__ void __launch_bounds__(256) label_long_gradient_ke
 }
 
 // ---- sums over rows ---------------------------------------------------------------------------------------------------------
-// Whether this workgroup is the last to have stored its part, which its first work-item did before; the parts of all are then
-// visible to it.  The counter is the call's own and was cleared by the kernel before this one.
-__device__ __forceinline__ bool last_workgroup(uint32_t* ticket) {
-    __shared__ int last;
-    if (threadIdx.x == 0) {
-        __threadfence();
-        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
-        __threadfence();
-    }
-    __syncthreads();
-    return last != 0;
-}
-
-__device__ __forceinline__ double published(const double* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-__device__ __forceinline__ void publish(double* p, double v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
-
 struct Pairs {
     const float* ratios;            // log probability - ref of each row, 0 where ignored
     int64_t rows, tokens;
@@ -758,8 +705,6 @@ namespace {
 
 constexpr int kPairBlocks = 256, kSumBlocks = 128;
 
-int vec_of(int dtype) { return dtype == SD_FLOAT32 ? 4 : 8; }
-
 // Lanes of a wavefront that hold a row together (as a power of two) and vectors that each holds; shift = -1: a row is read by whole workgroups.
 // Many rows want few lanes with several vectors each (fewer steps to add up lanes per row), few rows one vector per lane.
 struct Group { int shift, vectors; };
@@ -808,8 +753,6 @@ unsigned short_blocks(int64_t rows, int per) {
     const int64_t n = (rows + per - 1) / per;
     return (unsigned)(n < kShortBlocks ? n : kShortBlocks);
 }
-
-unsigned blocks_for(int64_t n) { return (unsigned)(n < kMostBlocks ? n : kMostBlocks); }
 
 // scratch of a call: the ticket, sums of workgroups, and then what follows
 constexpr int64_t kSumFloats = 4 + 2 * (kPairBlocks > 4 * kSumBlocks ? kPairBlocks : 4 * kSumBlocks);

@@ -1,5 +1,6 @@
 // Rows of values: element types, 16-byte loads and stores, sums over lanes.
 #pragma once
+#include <cfloat>
 #include "common.h"
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -119,6 +120,60 @@ __device__ __forceinline__ float group_max(float v, int shift) {
     return v;
 }
 
+// where row r of logits begins whose rows lie `outer_stride` apart in blocks of `inner` rows that lie `inner_stride` apart
+template <class T, class R> __device__ __forceinline__ const T* row_start(const R& a, int64_t r) {
+    const uint32_t o = (uint32_t)r / a.inner, i = (uint32_t)r - o * a.inner;
+    return static_cast<const T*>(a.logits) + o * a.outer_stride + i * a.inner_stride;
+}
+
+__device__ __forceinline__ double wave_total(double v) { return group_total(v, 6); }
+
+__device__ __forceinline__ float finite(float top) { return fmaxf(top, -FLT_MAX); }
+
+// exp of a difference to the largest value of a row (or of a part of it): the hardware's exp2 of v log2(e), 1 for 0, so that a row's largest
+// term is exact.  log2(e) is the sum of two numbers (both positive: -inf stays -inf): of one it would be off by 1.3e-8 of v to one side, which the sum
+// over a row and the sum over an answer's rows add up.  As it is the product is rounded once, off by up to |v| 2^-24 of the result to either side,
+// and the hardware's exp2 by up to 1.4 2^-24, 0.06 2^-24 below on average (measured over 2^24 values a binade; expf 0.04).
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(fmaf(v, 1.44269504f, v * 1.92596299e-8f)); }
+
+// Sums of a row: exponentials of a few vectors in pairs, in 32 bits, and these sums in 64 (an addition to a sum in 32 bits that has the
+// largest value, 1, in it is off by up to 6e-8, and there are hundreds of them).
+template <int N> __device__ __forceinline__ float tree(const float (&f)[N]) {
+    float s[N];
+    #pragma unroll
+    for (int i = 0; i < N; i++) s[i] = f[i];
+    #pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) {
+        #pragma unroll
+        for (int i = 0; i < o; i++) s[i] += s[i + o];
+    }
+    return s[0];
+}
+
+// zeros in a row of a gradient, by a whole workgroup
+template <class T> __device__ __forceinline__ void clear_row(T* q, int n, int threads) {
+    constexpr int V = Elem<T>::kVec;
+    const int full = n / V;
+    for (int i = threadIdx.x; i < full; i += threads) put_stream16(q + i * V, u32x4{0u, 0u, 0u, 0u});
+    for (int j = full * V + threadIdx.x; j < n; j += threads) q[j] = T{};
+}
+
+// Whether this workgroup is the last to have stored its part, which its first work-item did before; the parts of all are then
+// visible to it.  The counter is the call's own and was cleared by the kernel before this one.
+__device__ __forceinline__ bool last_workgroup(uint32_t* ticket) {
+    __shared__ int last;
+    if (threadIdx.x == 0) {
+        __threadfence();
+        last = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1;
+        __threadfence();
+    }
+    __syncthreads();
+    return last != 0;
+}
+
+__device__ __forceinline__ double published(const double* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+__device__ __forceinline__ void publish(double* p, double v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+
 // calls f with a null pointer of the element type that `dtype` names; false for none
 template <class F> bool with_dtype(int dtype, F&& f) {
     switch (dtype) {
@@ -128,5 +183,9 @@ template <class F> bool with_dtype(int dtype, F&& f) {
     }
     return false;
 }
+
+constexpr int64_t kMostBlocks = 1 << 22;
+inline unsigned blocks_for(int64_t n) { return (unsigned)(n < kMostBlocks ? n : kMostBlocks); }
+inline int vec_of(int dtype) { return dtype == SD_FLOAT32 ? 4 : 8; }
 
 }  // namespace sd

@@ -20,7 +20,7 @@ __all__ = [
     "NormDistF", "NormDistDropoutF", "SortNeuronF", "BoundInfDistF", "MaskedInfDistF",
     "norm_dist", "norm_dist_dropout", "sort_neuron", "bound_sort_neuron", "bound_inf_dist", "masked_inf_dist",
     "MeanShiftF", "mean_shift", "MeanShiftIndexF", "mean_shift_index", "dropout", "bound_dropout",
-    "dropout_seed",
+    "dropout_seed", "constrain_logits",
 ]
 
 
@@ -330,3 +330,23 @@ def bound_dropout(x, lower, upper, q, seed):
     there = [t for t in (x, lower, upper) if t is not None]
     done = iter(_dropped(there, q, seed) if there else ())
     return tuple(None if t is None else next(done) for t in (x, lower, upper))
+
+
+def constrain_logits(outputs, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):
+    """The logits from which a class is chosen, in a new tensor of the type of `outputs` (..., classes; fp32, bf16 or fp16).  With n = how
+    often class v stands in the row's history:
+        where n > 0:  z / repetition (z > 0) or z * repetition, minus frequency n, minus presence;  plus bias[v];  -inf where v is not allowed.
+
+    history  (..., places) int32 or int64: the classes chosen before; of row r the first lengths[r] places (all without `lengths`) that hold a
+             class, others (a padding of -1) are none.
+    repetition, presence, frequency: numbers, or fp32 with one for each row.
+    bias     (classes) or the sizes of `outputs`, fp32.
+    allowed  bool (classes) or the sizes of `outputs`; or int32 (words) or (..., words) with words = ceil(classes / 32), class v being bit
+             v % 32 of word v // 32.  A row with nothing allowed is -inf all over.
+    Rows of all of them may be strided or expanded.  Gradients flow to `outputs` alone, and may be differentiated again; a class that is not allowed has 0."""
+    numbers, rows = [], []
+    for value in (repetition, presence, frequency):
+        on_device = isinstance(value, torch.Tensor)
+        numbers.append(1.0 if on_device else float(value))
+        rows.append(value if on_device else None)
+    return _C.host().constrain_logits(outputs, history, lengths, *numbers, *rows, bias, allowed)

@@ -1,0 +1,67 @@
+"""Calls of the operators that answer with logits or learn from another model's, refused before any device work."""
+import math
+
+import pytest
+import torch
+
+from sortnet_amd import _lib
+from sortnet_amd import functional as F
+
+P = 1 << 20     # an address: no kernel is launched, every call is refused by its sizes
+Z = torch.zeros(4, 3)
+
+
+def _rows(**kw):
+    rows = _lib.LogitRows()
+    for k, v in dict(dict(logits=P, rows=4, inner=4, classes=3, outer_stride=0, inner_stride=3, dtype=0), **kw).items():
+        setattr(rows, k, v)
+    return rows
+
+
+def _constraints(**kw):
+    c = _lib.Constraints()
+    for k, v in dict(dict(repetition=1.0), **kw).items():
+        setattr(c, k, v)
+    return c
+
+
+BAD_ROWS = [dict(dtype=3), dict(dtype=-1), dict(rows=0), dict(rows=1 << 31), dict(classes=0), dict(classes=1 << 31), dict(inner=0), dict(inner=3), dict(logits=0),
+            dict(logits=P + 2), dict(logits=P + 1, dtype=1)]
+
+
+@pytest.mark.parametrize("bad", BAD_ROWS, ids=str)
+def test_rows_without_a_meaning(bad):
+    for name, args in (("sd_constrain_logits", (P,)), ("sd_constrain_gradient", (P, P))):
+        with pytest.raises(RuntimeError, match=r"status 1\)"):
+            _lib.call(name, _rows(**bad), _constraints(), *args, None)
+
+
+@pytest.mark.parametrize("bad, match", [
+    (dict(history=P, history_bytes=2, history_length=3), "history of"), (dict(history=P, history_bytes=8, history_length=-1), "history_length"),
+    (dict(history=P, history_bytes=8, history_length=1 << 32), "history_length"), (dict(history=P + 4, history_bytes=8, history_length=3), "aligned"),
+    (dict(lengths=P, length_bytes=4), "without a history"), (dict(history=P, history_bytes=4, history_length=3, lengths=P, length_bytes=3), "lengths of"),
+    (dict(history=P, history_bytes=4, history_length=3, lengths=P + 2, length_bytes=4), "aligned"),
+    (dict(repetition=0.0), "repetition"), (dict(repetition=-1.0), "repetition"), (dict(repetition=math.nan), "repetition"), (dict(repetition=math.inf), "repetition"),
+    (dict(repetition=1e-60), "repetition"), (dict(presence=math.nan), "presence"), (dict(presence=math.inf), "presence"), (dict(frequency=-math.inf), "frequency"),
+    (dict(allowed=P, allowed_kind=0), "allowed_kind"), (dict(allowed=P, allowed_kind=3), "allowed_kind"), (dict(allowed=P + 2, allowed_kind=2), "aligned"),
+    (dict(bias=P + 1), "aligned"), (dict(presence_rows=P + 2), "aligned")], ids=str)
+def test_constraints_without_a_meaning(bad, match):
+    with pytest.raises(RuntimeError, match=match):
+        _lib.call("sd_constrain_logits", _rows(), _constraints(**bad), P, None)
+    with pytest.raises(RuntimeError, match=match):
+        _lib.call("sd_constrain_gradient", _rows(), _constraints(**bad), P, P, None)
+
+
+def test_results_out_of_line():
+    for out in (None, P + 2):
+        with pytest.raises(RuntimeError):
+            _lib.call("sd_constrain_logits", _rows(), _constraints(), out, None)
+    for grad in (None, P + 1):
+        with pytest.raises(RuntimeError):
+            _lib.call("sd_constrain_gradient", _rows(), _constraints(), grad, P, None)
+
+
+@pytest.mark.parametrize("call", [lambda: F.constrain_logits(Z), lambda: F.constrain_logits(Z, torch.zeros(4, 2, dtype=torch.int64), presence=1.0)])
+def test_tensors_on_the_host(call):
+    with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
+        call()
