@@ -386,6 +386,32 @@ typedef struct {
     int dtype;
 } sd_logit_rows;
 
+/* A teacher's top logits: k entries for each row (1..SD_MOST_TOP; row r's from r * k on), logits `values` in the type that dtype names and
+ * `classes` of class_bytes = 4 or 8.  A negative class is no entry; one of `classes` and more gives the row a divergence and gradient of NaN.  rest (rows,
+ * or NULL: -inf): log of the sum of exp(logit / temperature) over the teacher's other classes. */
+#define SD_MOST_TOP 256
+typedef struct {
+    const void* values;
+    const void* classes;
+    const float* rest;
+    int64_t k;
+    int dtype, class_bytes;
+} sd_top_lists;
+
+/* Divergence of the student's softmax at `temperature` (1e-4..1e4) from the teacher's, over the classes of the entries and, as one more outcome,
+ * all others: divergences[r] = sum_j q_j (log q_j - log p_j) (terms with q_j = 0 are 0); 0 for rows that do not count: those without an
+ * entry, and those whose entries and rest are all -inf.  loss = weight temperature^2 mean over the rows that count (0 where there are none).
+ * A class in several entries is one class.  stats (rows, 2), entries (rows, k) and scale (1), all or none NULL, are what sd_distill_gradient
+ * needs; scratch: sd_distill_scratch() floats (host only, -1 for what would be refused), 16-byte aligned, any contents. */
+int64_t sd_distill_scratch(const sd_logit_rows* rows, int64_t k);
+int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, double weight, float* stats, float* entries,
+                    float* scale, float* loss, float* divergences, float* scratch, sd_stream_t stream);
+
+/* grad = scale scale2 times the gradient of the sum of divergences by logit / temperature, rows of `classes` values one behind the other in the
+ * logits' type; scale2 (one float on the device) may be NULL. */
+int sd_distill_gradient(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, const float* stats, const float* entries,
+                        const float* scale, const float* scale2, void* grad, sd_stream_t stream);
+
 /* What constrains the choice of a class.  Rows of the history, the bias and the allowed classes lie as those of the logits, (r / inner) *
  * outer + (r % inner) * inner entries behind their pointer; strides may be 0.
  *   history (NULL: none): history_length classes of history_bytes = 4 or 8 each, of which row r's first lengths[r] count (NULL: all; of

@@ -30,6 +30,11 @@ class LogitRows(ctypes.Structure):
     _fields_ = [("logits", _F), ("rows", _l), ("inner", _l), ("classes", _l), ("outer_stride", _l), ("inner_stride", _l), ("dtype", _i)]
 
 
+class TopLists(ctypes.Structure):
+    """sd_top_lists of include/sortdist.h."""
+    _fields_ = [("values", _F), ("classes", _I), ("rest", _F), ("k", _l), ("dtype", _i), ("class_bytes", _i)]
+
+
 class Constraints(ctypes.Structure):
     """sd_constraints of include/sortdist.h."""
     _fields_ = [("history", _I), ("lengths", _I), ("repetition_rows", _F), ("presence_rows", _F), ("frequency_rows", _F), ("bias", _F), ("allowed", _I),
@@ -40,6 +45,7 @@ class Constraints(ctypes.Structure):
 
 _R = ctypes.POINTER(LabelRows)
 _Z = ctypes.POINTER(LogitRows)
+_T = ctypes.POINTER(TopLists)
 _C = ctypes.POINTER(Constraints)
 
 # name -> argument types, in the order of include/sortdist.h
@@ -78,6 +84,8 @@ SIGNATURES = {
     "sd_preference_loss": [_R, _F, _I, _i, _l, _i, _d, _d, _F, _F, _F, _F, _F, _S],
     "sd_policy_loss": [_R, _F, _F, _l, _l, _F, _d, _d, _d, _F, _F, _F, _F, _F, _F, _F, _S],
     "sd_label_gradient": [_R, _F, _F, _F, _F, _i, _F, _S],
+    "sd_distill_loss": [_Z, _T, _d, _d, _F, _F, _F, _F, _F, _F, _S],
+    "sd_distill_gradient": [_Z, _T, _d, _F, _F, _F, _F, _F, _S],
     "sd_constrain_logits": [_Z, _C, _F, _S],
     "sd_constrain_gradient": [_Z, _C, _F, _F, _S],
     "sd_dropout": [_F, _F, _F, _i, _l, _d, _u, _I, _F, _F, _F, _S],
@@ -100,6 +108,7 @@ _OTHER = {
     "sd_mask_threshold16": ([_f], _u),
     "sd_mask_count": ([_u, _i, _f], _i),
     "sd_label_scratch": ([_R, _i], _l),
+    "sd_distill_scratch": ([_Z, _l], _l),
     "sd_policy_fuses": ([_R], _i),
 }
 

@@ -645,7 +645,7 @@ private:
 // kernels know.
 struct OnceNode : Node {
     variable_list apply(variable_list&&) override {
-        throw std::runtime_error("sortnet_amd: label_log_probs, preference_loss and policy_loss can be differentiated once: their gradients have no derivatives");
+        throw std::runtime_error("sortnet_amd: label_log_probs, preference_loss, policy_loss and distill_loss can be differentiated once: their gradients have no derivatives");
     }
     std::string name() const override { return "OnceNode"; }
 };
@@ -1104,6 +1104,123 @@ Tensor constrain_logits(const Tensor& outputs, const OptTensor& history, const O
     return out;
 }
 
+// ---- distillation from a teacher's top logits ----------------------------------------------------------------------------
+// k entries for each row, one behind the other
+struct Lists {
+    Tensor values, classes, rest;
+    double temperature = 1.0;
+    sd_top_lists call() const {
+        sd_top_lists l{};
+        l.values = values.data_ptr();
+        l.classes = classes.data_ptr();
+        l.rest = rest.defined() ? floats(rest, "top_rest") : nullptr;
+        l.k = values.size(-1);
+        l.dtype = element_type(values, "top_values");
+        l.class_bytes = (int)classes.element_size();
+        return l;
+    }
+};
+
+// What a call works in, as one tensor: where the gradient is wanted what it needs, behind it the scratch (of nothing else the start).
+struct DistillWork {
+    float *scale = nullptr, *stats = nullptr, *entries = nullptr, *scratch = nullptr;
+    static int64_t floats_of(int64_t rows, int64_t k) { return 4 + (2 * rows + 3) / 4 * 4 + (rows * k + 3) / 4 * 4; }
+    DistillWork(const Tensor& whole, int64_t rows, int64_t k, bool grad) {
+        float* p = floats(whole, "work");
+        scratch = p;
+        if (!grad) return;
+        scale = p; stats = p + 4; entries = stats + (2 * rows + 3) / 4 * 4;
+        scratch = p + floats_of(rows, k);
+    }
+};
+
+struct DistillNode : Node {
+    SavedVariable logits, values, classes, rest, work;
+    double temperature = 1.0;
+
+    variable_list apply(variable_list&& grads) override {
+        const Locked lock(mutex_);
+        variable_list out(1);
+        if (!task_should_compute_output(0)) return out;
+        const Tensor z = logits.unpack(), wk = work.unpack();
+        Lists l;
+        l.values = values.unpack(); l.classes = classes.unpack(); l.rest = rest.unpack();
+        std::shared_ptr<OnceNode> once;
+        if (at::GradMode::is_enabled()) {
+            once = new_node<OnceNode>();
+            once->set_next_edges({next_edge(0), grads[0].defined() ? torch::autograd::impl::gradient_edge(grads[0]) : torch::autograd::Edge()});
+        }
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Tensor g = incoming(*this, grads, 0);
+        const c10::DeviceGuard guard(z.device());
+        out[0] = at::empty(z.sizes(), z.options());
+        const sd_logit_rows a = logit_rows(z);
+        const sd_top_lists lists = l.call();
+        const DistillWork w(wk, a.rows, lists.k, true);
+        require(sd_distill_gradient(&a, &lists, temperature, w.stats, w.entries, w.scale, floats(g, "grad_output"), out[0].data_ptr(), stream_of(z)), "sd_distill_gradient");
+        if (once) set_history(out[0], once);
+        return out;
+    }
+    void release_variables() override {
+        const Locked lock(mutex_);
+        for (SavedVariable* v : {&logits, &values, &classes, &rest, &work}) v->reset_data();
+    }
+    std::string name() const override { return "DistillNode"; }
+};
+
+std::pair<Tensor, Tensor> distill_loss(const Tensor& outputs, const Tensor& values, const Tensor& classes, const OptTensor& rest, double temperature, double weight) {
+    reverse_mode_only("distill_loss", outputs, values);
+    const bool has_rest = rest && rest->defined();
+    if (has_rest) reverse_mode_only("distill_loss", *rest);
+    const bool grad = want_grad(outputs);
+    check_outputs(outputs);
+    const auto rows_of = [&](const Tensor& t, const char* name, bool entries) {
+        same_device(t, name, outputs);
+        if (t.dim() != outputs.dim() - !entries || t.sizes().slice(0, outputs.dim() - 1) != outputs.sizes().slice(0, outputs.dim() - 1))
+            throw std::runtime_error(std::string(name) + (entries ? " must have the sizes of outputs before the classes, and entries" : " must have the sizes of outputs before the classes"));
+        if (at::GradMode::is_enabled() && t.requires_grad())
+            throw std::runtime_error(std::string(name) + " must not require a gradient: the loss is differentiated with respect to outputs alone");
+    };
+    rows_of(values, "top_values", true);
+    rows_of(classes, "top_classes", true);
+    if (has_rest) rows_of(*rest, "top_rest", false);
+    element_type(values, "top_values");
+    if (classes.scalar_type() != at::kLong && classes.scalar_type() != at::kInt) throw std::runtime_error("top_classes must have dtype torch.int64 or torch.int32");
+    if (classes.sizes() != values.sizes()) throw std::runtime_error("top_classes must have the sizes of top_values");
+    if (has_rest && rest->scalar_type() != at::kFloat) throw std::runtime_error("top_rest must have dtype torch.float32");
+    Tensor loss, divergences, z, work;
+    Lists l;
+    {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const c10::DeviceGuard guard(outputs.device());
+        z = readable_logits(outputs);
+        const sd_logit_rows a = logit_rows(z);
+        l.values = values.contiguous(); l.classes = classes.contiguous();
+        if (has_rest) l.rest = rest->contiguous();
+        const sd_top_lists lists = l.call();
+        const int64_t n = sd_distill_scratch(&a, lists.k);
+        if (n < 0) require(SD_ERR_ARG, "sd_distill_loss");
+        work = new_floats(z, {n + (grad ? DistillWork::floats_of(a.rows, lists.k) : 0)});
+        const DistillWork w(work, a.rows, lists.k, grad);
+        loss = new_floats(z, {});
+        divergences = new_floats(z, outputs.sizes().slice(0, outputs.dim() - 1));
+        require(sd_distill_loss(&a, &lists, temperature, weight, w.stats, w.entries, w.scale, floats(loss, "loss"), floats(divergences, "divergences"), w.scratch, stream_of(z)),
+                "sd_distill_loss");
+    }
+    if (grad) {
+        auto node = new_node<DistillNode>();
+        node->set_next_edges(collect_next_edges(outputs));
+        node->logits = SavedVariable(z, false);
+        node->values = SavedVariable(l.values, false);
+        node->classes = SavedVariable(l.classes, false);
+        if (has_rest) node->rest = SavedVariable(l.rest, false);
+        node->work = SavedVariable(work, false);
+        node->temperature = temperature;
+        set_history(loss, node);
+    }
+    return {loss, divergences};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_host, m) {
@@ -1130,4 +1247,5 @@ PYBIND11_MODULE(_host, m) {
     m.def("policy_loss", &policy_loss, released());
     m.def("dropout", &dropout, released());
     m.def("constrain_logits", &constrain_logits, released());
+    m.def("distill_loss", &distill_loss, released());
 }

@@ -184,6 +184,25 @@ template <class F> bool with_dtype(int dtype, F&& f) {
     return false;
 }
 
+// rows of logits without labels (sd_logit_rows)
+struct LogitRows {
+    const void* logits;
+    int64_t rows, classes, outer_stride, inner_stride;
+    uint32_t inner;
+};
+
+inline int check_logits(const sd_logit_rows* in, const char* who, LogitRows* a) {
+    SD_REQUIRE(in, "%s: null rows", who);
+    SD_REQUIRE(in->dtype == SD_FLOAT32 || in->dtype == SD_BFLOAT16 || in->dtype == SD_FLOAT16, "%s: dtype=%d is none of SD_FLOAT32, SD_BFLOAT16, SD_FLOAT16", who, in->dtype);
+    SD_REQUIRE(in->rows > 0 && in->rows < (1ll << 31), "%s: rows=%lld outside 1..2^31-1", who, (long long)in->rows);
+    SD_REQUIRE(in->classes > 0 && in->classes < (1ll << 31), "%s: classes=%lld outside 1..2^31-1", who, (long long)in->classes);
+    SD_REQUIRE(in->inner > 0 && in->rows % in->inner == 0 && in->inner < (1ll << 31), "%s: inner=%lld does not divide rows=%lld", who, (long long)in->inner, (long long)in->rows);
+    SD_REQUIRE(in->logits, "%s: null logits", who);
+    SD_REQUIRE((reinterpret_cast<uintptr_t>(in->logits) & (in->dtype == SD_FLOAT32 ? 3 : 1)) == 0, "%s: logits are not aligned to their type", who);
+    *a = LogitRows{in->logits, in->rows, in->classes, in->outer_stride, in->inner_stride, (uint32_t)in->inner};
+    return SD_OK;
+}
+
 constexpr int64_t kMostBlocks = 1 << 22;
 inline unsigned blocks_for(int64_t n) { return (unsigned)(n < kMostBlocks ? n : kMostBlocks); }
 inline int vec_of(int dtype) { return dtype == SD_FLOAT32 ? 4 : 8; }

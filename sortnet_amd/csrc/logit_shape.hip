@@ -3,7 +3,6 @@
 // in 32 bits and in this order, rounded once.  The gradient is 0 where v is not allowed, g / repetition or g * repetition where n > 0, else g.
 // Bound by the bytes of the logits in and out.  The counts of a workgroup's columns stand in its LDS, for which it reads the whole history of
 // its rows: no scratch, nothing to sort, and any number of repeated classes.
-#include <climits>
 #include <type_traits>
 #include "label_rows.h"
 
@@ -11,12 +10,6 @@ namespace sd {
 
 constexpr int kShapeCounts = 8192;      // columns whose counts a workgroup holds (32 KiB)
 enum { kAll = 0, kFlags = SD_ALLOWED_FLAGS, kBits = SD_ALLOWED_BITS };
-
-struct LogitRows {
-    const void* logits;
-    int64_t rows, classes, outer_stride, inner_stride;
-    uint32_t inner;
-};
 
 struct Shape {
     const void *history, *lengths;
@@ -147,22 +140,6 @@ template <class T, int ALLOWED, bool HISTORY, bool GRAD> __global__ void __launc
         }
     }
 }
-
-namespace {
-
-int check_logits(const sd_logit_rows* in, const char* who, LogitRows* a) {
-    SD_REQUIRE(in, "%s: null rows", who);
-    SD_REQUIRE(in->dtype == SD_FLOAT32 || in->dtype == SD_BFLOAT16 || in->dtype == SD_FLOAT16, "%s: dtype=%d is none of SD_FLOAT32, SD_BFLOAT16, SD_FLOAT16", who, in->dtype);
-    SD_REQUIRE(in->rows > 0 && in->rows < (1ll << 31), "%s: rows=%lld outside 1..2^31-1", who, (long long)in->rows);
-    SD_REQUIRE(in->classes > 0 && in->classes < (1ll << 31), "%s: classes=%lld outside 1..2^31-1", who, (long long)in->classes);
-    SD_REQUIRE(in->inner > 0 && in->rows % in->inner == 0 && in->inner < (1ll << 31), "%s: inner=%lld does not divide rows=%lld", who, (long long)in->inner, (long long)in->rows);
-    SD_REQUIRE(in->logits, "%s: null logits", who);
-    SD_REQUIRE((reinterpret_cast<uintptr_t>(in->logits) & (in->dtype == SD_FLOAT32 ? 3 : 1)) == 0, "%s: logits are not aligned to their type", who);
-    *a = LogitRows{in->logits, in->rows, in->classes, in->outer_stride, in->inner_stride, (uint32_t)in->inner};
-    return SD_OK;
-}
-
-}  // namespace
 
 static int shape_logits(const char* who, const sd_logit_rows* in, const sd_constraints* c, const void* grad, void* out, hipStream_t stream) {
     LogitRows a;

@@ -93,6 +93,22 @@ def policy_loss(outputs, targets, old_log_probs, advantages, ref_log_probs=None,
                                   kl_coef, ignore_index)
 
 
+def distill_loss(outputs, top_values, top_classes, top_rest=None, temperature=1.0, weight=1.0):
+    """Distillation from a teacher's top logits: (loss, divergences).
+
+    For each row of `outputs` (..., classes) the teacher gives `top_values` (..., k; fp32, bf16 or fp16; k up to 256) of `top_classes` (..., k;
+    int32 or int64, a negative one being no entry) and `top_rest` (...; fp32), the log of the sum of exp(logit / temperature) over its
+    other classes: what `functional.top_logits` gives for the teacher's logits at the same temperature.  The k classes and, as one more outcome, all
+    the others together have the teacher's probabilities q and, by `outputs` / temperature, the student's p:
+        divergences = sum of q (log q - log p) over the k + 1 outcomes,    loss = weight temperature^2 mean of them.
+    Without `top_rest` the teacher gives the others nothing: q is the softmax of its entries.
+
+    A row without an entry, or whose entries and rest are all -inf, is not read, whatever it holds, does not count in the mean, and gets zeros.
+    A class in several entries is one class.  A class past the end gives NaN.  Only `outputs` gets a gradient; `divergences` has none.  From 32 MiB of
+    logits on the gradient is made with the loss, for an upstream gradient of 1: a known factor is cheaper as `weight`."""
+    return ext.host().distill_loss(outputs, top_values, top_classes, top_rest, float(temperature), float(weight))
+
+
 class hinge:
     def __init__(self, mix=0.25):
         self.mix = mix

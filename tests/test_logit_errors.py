@@ -65,3 +65,55 @@ def test_results_out_of_line():
 def test_tensors_on_the_host(call):
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         call()
+
+
+def _lists(**kw):
+    lists = _lib.TopLists()
+    for k, v in dict(dict(values=P, classes=P, rest=None, k=2, dtype=0, class_bytes=4), **kw).items():
+        setattr(lists, k, v)
+    return lists
+
+
+def _distill(rows=None, lists=None, temperature=1.0, weight=1.0, stats=P, entries=P, scale=P, loss=P, divergences=P, scratch=P):
+    return _lib.call("sd_distill_loss", rows or _rows(), lists or _lists(), temperature, weight, stats, entries, scale, loss, divergences, scratch, None)
+
+
+@pytest.mark.parametrize("bad", BAD_ROWS, ids=str)
+def test_rows_without_a_meaning_to_the_teacher(bad):
+    assert _lib.load().sd_distill_scratch(_rows(**bad), 2) == -1
+    with pytest.raises(RuntimeError, match=r"status 1\)"):
+        _distill(_rows(**bad))
+    with pytest.raises(RuntimeError, match=r"status 1\)"):
+        _lib.call("sd_distill_gradient", _rows(**bad), _lists(), 1.0, P, P, P, None, P, None)
+
+
+@pytest.mark.parametrize("bad, match", [(dict(values=0), "null"), (dict(classes=0), "null"), (dict(k=0), "k=0"), (dict(k=257), "k=257"), (dict(k=-1), "k=-1"), (dict(dtype=5), "dtype"),
+                                        (dict(class_bytes=2), "classes of"), (dict(values=P + 2), "aligned"), (dict(classes=P + 4, class_bytes=8), "aligned"), (dict(rest=P + 1), "aligned")], ids=str)
+def test_lists_without_a_meaning(bad, match):
+    with pytest.raises(RuntimeError, match=match):
+        _distill(lists=_lists(**bad))
+    with pytest.raises(RuntimeError, match=match):
+        _lib.call("sd_distill_gradient", _rows(), _lists(**bad), 1.0, P, P, P, None, P, None)
+
+
+def test_distillation_without_a_meaning():
+    for k in (0, 257):
+        assert _lib.load().sd_distill_scratch(_rows(), k) == -1
+    for t in (0.0, -1.0, 1e-5, 1e5, math.nan, math.inf):
+        with pytest.raises(RuntimeError, match="temperature"):
+            _distill(temperature=t)
+        with pytest.raises(RuntimeError, match="temperature"):
+            _lib.call("sd_distill_gradient", _rows(), _lists(), t, P, P, P, None, P, None)
+    for w in (math.nan, math.inf, -math.inf, 1e39):
+        with pytest.raises(RuntimeError, match="weight"):
+            _distill(weight=w)
+    for missing in ("loss", "divergences", "scratch"):
+        with pytest.raises(RuntimeError, match="null"):
+            _distill(**{missing: None})
+    for missing in ("stats", "entries", "scale"):
+        with pytest.raises(RuntimeError, match="needs stats"):
+            _distill(**{missing: None})
+    with pytest.raises(RuntimeError, match="aligned"):
+        _distill(stats=P + 4)
+    with pytest.raises(RuntimeError, match="aligned"):
+        _distill(scratch=P + 8)
