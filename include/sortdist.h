@@ -379,6 +379,8 @@ int sd_label_gradient(const sd_label_rows* rows, const float* stats, const float
 /* ---- answering with a head's logits, learning from another model's (no reference launchers) ----
  * As above: fp32, bf16 or fp16, everything per row in 32 bits or more, scratch from the caller. */
 
+#define SD_MOST_TOP 256
+
 /* Rows of logits, laid out as in sd_label_rows. */
 typedef struct {
     const void* logits;
@@ -386,10 +388,17 @@ typedef struct {
     int dtype;
 } sd_logit_rows;
 
+/* The k largest logits of each row (1..SD_MOST_TOP, at most `classes`), of equal ones the lower class first, NaN above all: values (rows, k) in
+ * the logits' type, classes (rows, k), and rest (rows), the log of the sum of exp(logit / temperature) over the row's other classes (-inf where
+ * there are none; NaN in a row that has one).  temperature: 1e-4..1e4.  scratch: sd_top_scratch() floats (host only, -1 for what would be
+ * refused), 16-byte aligned, any contents; may be NULL where that is 0. */
+int64_t sd_top_scratch(const sd_logit_rows* rows, int64_t k);
+int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temperature, void* values, int* classes, float* rest, float* scratch,
+                  sd_stream_t stream);
+
 /* A teacher's top logits: k entries for each row (1..SD_MOST_TOP; row r's from r * k on), logits `values` in the type that dtype names and
  * `classes` of class_bytes = 4 or 8.  A negative class is no entry; one of `classes` and more gives the row a divergence and gradient of NaN.  rest (rows,
  * or NULL: -inf): log of the sum of exp(logit / temperature) over the teacher's other classes. */
-#define SD_MOST_TOP 256
 typedef struct {
     const void* values;
     const void* classes;

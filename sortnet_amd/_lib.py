@@ -84,6 +84,7 @@ SIGNATURES = {
     "sd_preference_loss": [_R, _F, _I, _i, _l, _i, _d, _d, _F, _F, _F, _F, _F, _S],
     "sd_policy_loss": [_R, _F, _F, _l, _l, _F, _d, _d, _d, _F, _F, _F, _F, _F, _F, _F, _S],
     "sd_label_gradient": [_R, _F, _F, _F, _F, _i, _F, _S],
+    "sd_top_logits": [_Z, _l, _d, _F, _I, _F, _F, _S],
     "sd_distill_loss": [_Z, _T, _d, _d, _F, _F, _F, _F, _F, _F, _S],
     "sd_distill_gradient": [_Z, _T, _d, _F, _F, _F, _F, _F, _S],
     "sd_constrain_logits": [_Z, _C, _F, _S],
@@ -108,6 +109,7 @@ _OTHER = {
     "sd_mask_threshold16": ([_f], _u),
     "sd_mask_count": ([_u, _i, _f], _i),
     "sd_label_scratch": ([_R, _i], _l),
+    "sd_top_scratch": ([_Z, _l], _l),
     "sd_distill_scratch": ([_Z, _l], _l),
     "sd_policy_fuses": ([_R], _i),
 }

@@ -1104,6 +1104,30 @@ Tensor constrain_logits(const Tensor& outputs, const OptTensor& history, const O
     return out;
 }
 
+// ---- the largest logits ----------------------------------------------------------------------------------------------------
+std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& outputs, int64_t k, double temperature) {
+    reverse_mode_only("top_logits", outputs);
+    check_outputs(outputs);
+    at::AutoDispatchBelowADInplaceOrView below;
+    const c10::DeviceGuard guard(outputs.device());
+    if (k < 1 || k > SD_MOST_TOP || k > outputs.size(-1))
+        throw std::runtime_error("top_logits: k=" + std::to_string(k) + " of " + std::to_string(outputs.size(-1)) + " classes: 1.." + std::to_string(SD_MOST_TOP) + " are possible");
+    const Tensor z = readable_logits(outputs);
+    std::vector<int64_t> sizes(outputs.sizes().begin(), outputs.sizes().end() - 1);
+    const Tensor rest = new_floats(z, sizes);
+    sizes.push_back(k);
+    const Tensor values = at::empty(sizes, z.options()), classes = new_ints(z, sizes);
+    if (rest.numel() > 0) {
+        const sd_logit_rows a = logit_rows(z);
+        const int64_t n = sd_top_scratch(&a, k);
+        if (n < 0) require(SD_ERR_ARG, "sd_top_logits");
+        const Tensor scratch = n > 0 ? new_floats(z, {n}) : Tensor();
+        require(sd_top_logits(&a, k, temperature, values.data_ptr(), ints(classes, "classes"), floats(rest, "rest"), n > 0 ? floats(scratch, "scratch") : nullptr, stream_of(z)),
+                "sd_top_logits");
+    }
+    return {values, classes, rest};
+}
+
 // ---- distillation from a teacher's top logits ----------------------------------------------------------------------------
 // k entries for each row, one behind the other
 struct Lists {
@@ -1247,5 +1271,6 @@ PYBIND11_MODULE(_host, m) {
     m.def("policy_loss", &policy_loss, released());
     m.def("dropout", &dropout, released());
     m.def("constrain_logits", &constrain_logits, released());
+    m.def("top_logits", &top_logits, released());
     m.def("distill_loss", &distill_loss, released());
 }

@@ -20,7 +20,7 @@ __all__ = [
     "NormDistF", "NormDistDropoutF", "SortNeuronF", "BoundInfDistF", "MaskedInfDistF",
     "norm_dist", "norm_dist_dropout", "sort_neuron", "bound_sort_neuron", "bound_inf_dist", "masked_inf_dist",
     "MeanShiftF", "mean_shift", "MeanShiftIndexF", "mean_shift_index", "dropout", "bound_dropout",
-    "dropout_seed", "constrain_logits",
+    "dropout_seed", "top_logits", "constrain_logits",
 ]
 
 
@@ -330,6 +330,16 @@ def bound_dropout(x, lower, upper, q, seed):
     there = [t for t in (x, lower, upper) if t is not None]
     done = iter(_dropped(there, q, seed) if there else ())
     return tuple(None if t is None else next(done) for t in (x, lower, upper))
+
+
+def top_logits(outputs, k, temperature=1.0):
+    """The k (up to 256) largest logits of each row of `outputs` (..., classes; fp32, bf16 or fp16) and what is left: (values, classes, rest).
+
+    values (..., k) in the type of `outputs`, from the largest on, of equal ones the lower class first (NaN above all, -0 as 0; classes masked by -inf come
+    last, and are given where there are not k others); classes (..., k) int32; rest (...) fp32, the log of the sum of exp(logit / temperature) over the other
+    classes: -inf where there are none, NaN in a row that has one.  What `losses.distill_loss` learns from; with it the log
+    probabilities at the temperature are values / temperature - logaddexp(logsumexp(values / temperature), rest).  No gradient flows through it."""
+    return _C.host().top_logits(outputs, k, float(temperature))
 
 
 def constrain_logits(outputs, history=None, lengths=None, repetition=1.0, presence=0.0, frequency=0.0, bias=None, allowed=None):

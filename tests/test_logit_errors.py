@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from sortnet_amd import _lib
+from sortnet_amd import _lib, losses
 from sortnet_amd import functional as F
 
 P = 1 << 20     # an address: no kernel is launched, every call is refused by its sizes
@@ -61,7 +61,8 @@ def test_results_out_of_line():
             _lib.call("sd_constrain_gradient", _rows(), _constraints(), grad, P, None)
 
 
-@pytest.mark.parametrize("call", [lambda: F.constrain_logits(Z), lambda: F.constrain_logits(Z, torch.zeros(4, 2, dtype=torch.int64), presence=1.0)])
+@pytest.mark.parametrize("call", [lambda: F.constrain_logits(Z), lambda: F.constrain_logits(Z, torch.zeros(4, 2, dtype=torch.int64), presence=1.0),
+                                  lambda: F.top_logits(Z, 1), lambda: losses.distill_loss(Z, Z[:, :2], torch.zeros(4, 2, dtype=torch.int32))])
 def test_tensors_on_the_host(call):
     with pytest.raises(RuntimeError, match="must be a CUDA tensor"):
         call()
@@ -76,6 +77,26 @@ def _lists(**kw):
 
 def _distill(rows=None, lists=None, temperature=1.0, weight=1.0, stats=P, entries=P, scale=P, loss=P, divergences=P, scratch=P):
     return _lib.call("sd_distill_loss", rows or _rows(), lists or _lists(), temperature, weight, stats, entries, scale, loss, divergences, scratch, None)
+
+
+@pytest.mark.parametrize("bad", BAD_ROWS, ids=str)
+def test_rows_without_a_largest_logit(bad):
+    assert _lib.load().sd_top_scratch(_rows(**bad), 1) == -1
+    with pytest.raises(RuntimeError, match=r"status 1\)"):
+        _lib.call("sd_top_logits", _rows(**bad), 1, 1.0, P, P, P, P, None)
+
+
+def test_largest_logits_without_a_meaning():
+    for k in (0, -1, 4, 257):
+        assert _lib.load().sd_top_scratch(_rows(), k) == -1
+        with pytest.raises(RuntimeError, match="k="):
+            _lib.call("sd_top_logits", _rows(), k, 1.0, P, P, P, P, None)
+    for t in (0.0, -1.0, 1e-5, 1e5, math.nan, math.inf):
+        with pytest.raises(RuntimeError, match="temperature"):
+            _lib.call("sd_top_logits", _rows(), 2, t, P, P, P, P, None)
+    for values, classes, rest, match in ((None, P, P, "null"), (P, None, P, "null"), (P, P, None, "null"), (P + 2, P, P, "aligned"), (P, P + 1, P, "aligned"), (P, P, P + 2, "aligned")):
+        with pytest.raises(RuntimeError, match=match):
+            _lib.call("sd_top_logits", _rows(), 2, 1.0, values, classes, rest, P, None)
 
 
 @pytest.mark.parametrize("bad", BAD_ROWS, ids=str)
