@@ -39,7 +39,7 @@ def check(z, k, temperature=1.0):
 
 
 SHAPES = [(1, 1, 1), (4, 2, 1), (4, 2, 2), (512, 10, 3), (7, 33, 33), (65, 64, 5), (65, 65, 64), (9, 200, 200), (300, 256, 256), (40, 1000, 5), (40, 1000, 200), (5, 1025, 64), (12, 2049, 65),
-          (7, 4099, 17), (3, 8192, 256), (6, 16385, 1), (2, 20001, 100), (1, 65537, 256), (1, 131072, 50), (300, 50001, 200), (1030, 9001, 8), (2, 300001, 256), (2100, 17000, 33)]
+          (7, 4099, 17), (3, 8192, 256), (6, 16385, 1), (2, 20001, 100), (1, 65537, 256), (1, 131072, 50), (300, 50001, 200), (1030, 9001, 8), (2, 300001, 256), (2100, 17000, 33), (2, 131073, 9), (1, 8193, 5), (3, 4097, 256)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
@@ -89,6 +89,19 @@ def test_infinities_and_nan(classes):
     values, chosen, rest = F.top_logits(z[3:], 3)
     assert torch.isnan(rest).all() and torch.isnan(values[0, 0]) and chosen[0, 0] == 4 and chosen[1].tolist() == [1, 2, 3] and chosen[2].tolist() == [0, 1, 2]
     assert torch.equal(values[0, 1:], torch.cat((z[3, :4], z[3, 5:])).sort(descending=True).values[:2])
+
+
+@pytest.mark.parametrize("classes", [9, 500, 20000, 140000])
+def test_the_largest_far_above_the_others(classes):
+    """What is left keeps its size however far it lies below the k largest."""
+    z = make(4, classes, torch.float32, classes)
+    z[0, 3], z[0, 5] = 400.0, 300.0
+    z[1, 1] = z[1, 2] = math.inf
+    z[2, ::3] += 1000.0
+    z[3] -= 3000.0
+    z[3, 4], z[3, 8] = 0.0, 1e30
+    check(z, 2)
+    check(z, 2, 0.01)
 
 
 @pytest.mark.parametrize("classes", [10, 1000, 30000])
