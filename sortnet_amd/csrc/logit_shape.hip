@@ -8,7 +8,12 @@
 
 namespace sd {
 
-constexpr int kShapeCounts = 8192;      // columns whose counts a workgroup holds (32 KiB)
+// What a workgroup counts in (16 KiB): 8192 columns by 16 bits, or 4096 by 32 where a history has more places than 16 bits count.  Against 32 bits for 8192 columns:
+// 4096 x 65536 bf16 with 1024 places and a bit mask 237 -> 229 us, its gradient 315 -> 282.
+constexpr int kCountWords = 4096;
+constexpr int kShapeVectors = 4;        // 16-byte vectors of a work-item that are on their way together
+enum { kPlain, kBiased, kGradient };
+enum { kNone, kShort, kLong };          // histories: none, of fewer than 2^16 places, of more
 enum { kAll = 0, kFlags = SD_ALLOWED_FLAGS, kBits = SD_ALLOWED_BITS };
 
 struct Shape {
@@ -16,7 +21,7 @@ struct Shape {
     int64_t length, history_outer, history_inner;
     int wide_history, wide_lengths;             // int64 instead of int32
     const float *repetition_rows, *presence_rows, *frequency_rows;
-    float repetition, presence, frequency;
+    float repetition, inverse, presence, frequency;
     const float* bias;
     int64_t bias_outer, bias_inner;
     const void* allowed;
@@ -24,6 +29,7 @@ struct Shape {
     const void* grad;                           // backward: what flows into the result, rows one behind the other
     void* out;
     int64_t part;                               // columns of a workgroup, a multiple of 8
+    bool far;                                   // results that the last-level cache cannot hold are stored past it
     int parts, group;                           // parts of a row, or (with one part) rows of a workgroup
 };
 
@@ -52,23 +58,127 @@ template <int ALLOWED> __device__ __forceinline__ bool allowed_one(const void* r
     else return static_cast<const uint8_t*>(row)[c] != 0;
 }
 
-__device__ __forceinline__ float penalised(float z, float n, float repetition, float presence, float frequency) {
-    return (z > 0.f ? z / repetition : z * repetition) - frequency * n - presence;
+// What classes of the history pay: a positive logit times `inverse`, another one times `repetition`.
+struct Penalties { float repetition, inverse, presence, frequency; };
+__device__ __forceinline__ Penalties penalties_of(const Shape& s, int64_t r) {
+    Penalties p{s.repetition, s.inverse, s.presence, s.frequency};
+    if (s.repetition_rows) { p.repetition = s.repetition_rows[r]; p.inverse = 1.f / p.repetition; }
+    if (s.presence_rows) p.presence = s.presence_rows[r];
+    if (s.frequency_rows) p.frequency = s.frequency_rows[r];
+    return p;
 }
-__device__ __forceinline__ float penalised_slope(float g, float z, float repetition) { return z > 0.f ? g / repetition : g * repetition; }
+__device__ __forceinline__ float penalised(float z, uint32_t n, const Penalties& p) {
+    return n ? z * (z > 0.f ? p.inverse : p.repetition) - p.frequency * (float)n - p.presence : z;
+}
+__device__ __forceinline__ float penalised_slope(float g, float z, uint32_t n, const Penalties& p) { return n ? g * (z > 0.f ? p.inverse : p.repetition) : g; }
 
-template <class T, int ALLOWED, bool HISTORY, bool GRAD> __global__ void __launch_bounds__(256) shape_kernel(LogitRows a, Shape s) {
-    constexpr int V = Elem<T>::kVec;
-    __shared__ __align__(16) uint32_t counts[HISTORY ? kShapeCounts : 4];
+// the count of column `at`
+template <int HISTORY> __device__ __forceinline__ void count_one(uint32_t* counts, uint32_t at) {
+    if constexpr (HISTORY == kLong) atomicAdd(&counts[at], 1u);
+    else atomicAdd(&counts[at >> 1], 1u << (16 * (at & 1)));
+}
+template <int HISTORY> __device__ __forceinline__ uint32_t count_of(const uint32_t* counts, int at) {
+    if constexpr (HISTORY == kLong) return counts[at];
+    else return counts[at >> 1] >> (16 * (at & 1)) & 0xffffu;
+}
+
+// 16 bytes of a row's history, 4 places of 32 bits or 2 of 64
+struct Places { u32x4 v; };
+template <bool WIDE> __device__ __forceinline__ Places load_places(const void* past, int64_t pack) {
+    if constexpr (WIDE) {
+        struct __attribute__((packed, aligned(8))) Pack { u32x4 v; };
+        return Places{static_cast<const Pack*>(past)[pack].v};
+    } else return Places{load16(static_cast<const float*>(past) + 4 * pack)};
+}
+// adds those of the places from `first` on that are below n to the counts of columns [c0, c0 + columns)
+template <bool WIDE, int HISTORY> __device__ __forceinline__ void count_places(uint32_t* counts, const Places& p, int64_t first, int64_t n, uint32_t c0, uint32_t columns) {
+    #pragma unroll
+    for (int i = 0; i < (WIDE ? 2 : 4); i++) {
+        const uint32_t at = (WIDE ? p.v[2 * i] : p.v[i]) - c0;
+        if (first + i < n && at < columns && (!WIDE || p.v[2 * i + 1] == 0u)) count_one<HISTORY>(counts, at);
+    }
+}
+// the first places of a history, which are on their way before it is known how many of them count
+constexpr int kAhead = 2;
+template <bool WIDE> __device__ __forceinline__ void load_ahead(Places (&p)[kAhead], const void* past, int64_t length) {
+    constexpr int kPer = WIDE ? 2 : 4;
+    #pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+        const int64_t pack = (int)threadIdx.x + k * 256;
+        if ((pack + 1) * kPer <= length) p[k] = load_places<WIDE>(past, pack);
+    }
+}
+template <bool WIDE, int HISTORY> __device__ __forceinline__ void count_history(uint32_t* counts, const Places (&ahead)[kAhead], bool with_ahead, const void* past, int64_t length, int64_t n,
+                                                                  uint32_t c0, uint32_t columns) {
+    constexpr int kPer = WIDE ? 2 : 4;
+    int64_t from = 0;
+    if (with_ahead) {
+        #pragma unroll
+        for (int k = 0; k < kAhead; k++) {
+            const int64_t pack = (int)threadIdx.x + k * 256;
+            if ((pack + 1) * kPer <= length) count_places<WIDE, HISTORY>(counts, ahead[k], pack * kPer, n, c0, columns);
+        }
+        from = kAhead * 256;
+    }
+    const int64_t packs = n / kPer;
+    #pragma unroll 2
+    for (int64_t pack = from + threadIdx.x; pack < packs; pack += 256) count_places<WIDE, HISTORY>(counts, load_places<WIDE>(past, pack), pack * kPer, n, c0, columns);
+    // the places behind the last whole 16 bytes, unless they were among those
+    int64_t j = packs * kPer + threadIdx.x;
+    if (with_ahead && packs < from && (packs + 1) * kPer <= length) return;
+    if (j < n) {
+        const uint32_t* word = static_cast<const uint32_t*>(past) + (WIDE ? 2 * j : j);
+        const uint32_t at = word[0] - c0;
+        if (at < columns && (!WIDE || word[1] == 0u)) count_one<HISTORY>(counts, at);
+    }
+}
+
+// A workgroup shapes `part` columns of a row, or `group` whole rows.  A work-item's vectors are on their way together, the first of them while the
+// history is counted.
+template <class T, int ALLOWED, int HISTORY, int KIND> __global__ void __launch_bounds__(256, KIND == kBiased ? (HISTORY == kNone ? 6 : 4) : HISTORY == kNone ? 8 : 6) shape_kernel(LogitRows a, Shape s) {
+    constexpr bool GRAD = KIND == kGradient, BIAS = KIND == kBiased;
+    constexpr int V = Elem<T>::kVec, kAny = ALLOWED == kAll ? kBits : ALLOWED, kPer = HISTORY == kLong ? 1 : 2;     // (kPer: columns of a word of counts)
+    __shared__ __align__(16) uint32_t counts[HISTORY ? kCountWords : 4];
     const int64_t r0 = (int64_t)(blockIdx.x / s.parts) * s.group, c0 = (int64_t)(blockIdx.x % s.parts) * s.part;
     const int rows = (int)(a.rows - r0 < s.group ? a.rows - r0 : s.group);
-    const int columns = (int)(a.classes - c0 < s.part ? a.classes - c0 : s.part), width = (columns + 7) & ~7, vecs = (columns + V - 1) / V;
+    const int columns = (int)(a.classes - c0 < s.part ? a.classes - c0 : s.part), width = (columns + 7) & ~7, vecs = columns / V, items = rows * vecs;
     const auto place = [&](int64_t r, int64_t outer, int64_t inner) {
         const uint32_t o = (uint32_t)r / a.inner, i = (uint32_t)r - o * a.inner;
         return o * outer + i * inner;
     };
+    const auto allowed_row = [&](int64_t r) { return static_cast<const uint8_t*>(s.allowed) + (ALLOWED == kBits ? 4 : 1) * place(r, s.allowed_outer, s.allowed_inner); };
+    const auto split = [&](int item, int per, int& i) { i = rows == 1 ? 0 : item / per; return item - i * per; };
+    u32x4 v[kShapeVectors], b[BIAS ? kShapeVectors : 1][V / 4];
+    uint32_t bits[kShapeVectors];
+    const auto load = [&](int first) {
+        #pragma unroll
+        for (int k = 0; k < kShapeVectors; k++) {
+            const int item = first + k * 256 + (int)threadIdx.x;
+            if (item >= items) continue;
+            int i;
+            const int c = split(item, vecs, i) * V;
+            const int64_t r = r0 + i;
+            v[k] = load16(GRAD ? static_cast<const T*>(s.grad) + r * a.classes + c0 + c : row_start<T>(a, r) + c0 + c);
+            if constexpr (BIAS) {
+                const float* bias = s.bias + place(r, s.bias_outer, s.bias_inner) + c0 + c;
+                #pragma unroll
+                for (int m = 0; m < V / 4; m++) b[k][m] = load16(bias + 4 * m);
+            }
+            if (ALLOWED != kAll) bits[k] = allowed_bits<V, kAny>(allowed_row(r), (int)c0 + c);
+        }
+    };
+    // (loads arrive in their order: the history's first)
+    Places ahead[kAhead];
+    const bool with_ahead = HISTORY != kNone && rows == 1;
+    const void* past = nullptr;
+    if (with_ahead) {
+        past = static_cast<const uint8_t*>(s.history) + place(r0, s.history_outer, s.history_inner) * (s.wide_history ? 8 : 4);
+        if (s.wide_history) load_ahead<true>(ahead, past, s.length);
+        else load_ahead<false>(ahead, past, s.length);
+    }
+    load(0);
     if (HISTORY) {
-        for (int i = threadIdx.x; i < rows * width / 4; i += 256) reinterpret_cast<u32x4*>(counts)[i] = u32x4{0u, 0u, 0u, 0u};
+        for (int i = threadIdx.x; i < rows * width / (4 * kPer); i += 256) reinterpret_cast<u32x4*>(counts)[i] = u32x4{0u, 0u, 0u, 0u};
         __syncthreads();
         for (int i = 0; i < rows; i++) {
             const int64_t r = r0 + i;
@@ -77,67 +187,82 @@ template <class T, int ALLOWED, bool HISTORY, bool GRAD> __global__ void __launc
                 const int64_t given = s.wide_lengths ? static_cast<const int64_t*>(s.lengths)[r] : static_cast<const int*>(s.lengths)[r];
                 n = given < 0 ? 0 : given < n ? given : n;
             }
-            const int64_t at = place(r, s.history_outer, s.history_inner);
-            for (int64_t j = threadIdx.x; j < n; j += 256) {
-                const int64_t token = s.wide_history ? static_cast<const int64_t*>(s.history)[at + j] : static_cast<const int*>(s.history)[at + j];
-                if (token >= c0 && token < c0 + columns) atomicAdd(&counts[i * width + (int)(token - c0)], 1u);
-            }
+            if (!with_ahead) past = static_cast<const uint8_t*>(s.history) + place(r, s.history_outer, s.history_inner) * (s.wide_history ? 8 : 4);
+            if (s.wide_history) count_history<true, HISTORY>(counts + i * width / kPer, ahead, with_ahead, past, s.length, n, (uint32_t)c0, (uint32_t)columns);
+            else count_history<false, HISTORY>(counts + i * width / kPer, ahead, with_ahead, past, s.length, n, (uint32_t)c0, (uint32_t)columns);
         }
         __syncthreads();
     }
-    for (int item = threadIdx.x; item < rows * vecs; item += 256) {
-        const int i = item / vecs, c = (item - i * vecs) * V;
-        const int64_t r = r0 + i;
-        const T* z = row_start<T>(a, r) + c0 + c;
-        const T* g = GRAD ? static_cast<const T*>(s.grad) + r * a.classes + c0 + c : nullptr;
-        T* q = static_cast<T*>(s.out) + r * a.classes + c0 + c;
-        const float* bias = !GRAD && s.bias ? s.bias + place(r, s.bias_outer, s.bias_inner) + c0 + c : nullptr;
-        const uint8_t* allowed = ALLOWED == kAll ? nullptr
-            : static_cast<const uint8_t*>(s.allowed) + (ALLOWED == kBits ? 4 : 1) * place(r, s.allowed_outer, s.allowed_inner);
-        float repetition = 1.f, presence = 0.f, frequency = 0.f;
+    Penalties paid{};
+    if (HISTORY && rows == 1) paid = penalties_of(s, r0);
+    for (int first = 0; first < items; first += kShapeVectors * 256) {
+        if (first > 0) load(first);
+        uint32_t seen = 0;          // bit k: a class of vector k is in the history
+        u32x4 z[GRAD && HISTORY ? kShapeVectors : 1];
         if (HISTORY) {
-            repetition = s.repetition_rows ? s.repetition_rows[r] : s.repetition;
-            presence = s.presence_rows ? s.presence_rows[r] : s.presence;
-            frequency = s.frequency_rows ? s.frequency_rows[r] : s.frequency;
-        }
-        if (c + V <= columns) {
-            float f[V];
-            Elem<T>::unpack(load16(GRAD ? g : z), f);
-            if (HISTORY) {
-                uint32_t n[V], any = 0;
+            #pragma unroll
+            for (int k = 0; k < kShapeVectors; k++) {
+                const int item = first + k * 256 + (int)threadIdx.x;
+                if (item >= items) continue;
+                int i;
+                const int c = split(item, vecs, i) * V;
+                uint32_t any = 0;
                 #pragma unroll
-                for (int k = 0; k < V; k++) { n[k] = counts[i * width + c + k]; any |= n[k]; }
+                for (int m = 0; m < V / kPer; m++) any |= counts[(i * width + c) / kPer + m];
                 if (any) {
-                    #pragma unroll
-                    for (int k = 0; k < V; k++)
-                        if (n[k]) f[k] = GRAD ? penalised_slope(f[k], Elem<T>::get(z[k]), repetition) : penalised(f[k], (float)n[k], repetition, presence, frequency);
+                    seen |= 1u << k;
+                    if constexpr (GRAD && HISTORY) z[k] = load16(row_start<T>(a, r0 + i) + c0 + c);
                 }
             }
-            if (!GRAD && bias) {
+        }
+        #pragma unroll
+        for (int k = 0; k < kShapeVectors; k++) {
+            const int item = first + k * 256 + (int)threadIdx.x;
+            if (item >= items) continue;
+            int i;
+            const int c = split(item, vecs, i) * V;
+            const int64_t r = r0 + i;
+            float f[V];
+            Elem<T>::unpack(v[k], f);
+            if (HISTORY && seen >> k & 1) {
+                if (rows > 1) paid = penalties_of(s, r);
+                float zf[V];
+                if constexpr (GRAD && HISTORY) Elem<T>::unpack(z[k], zf);
                 #pragma unroll
-                for (int k = 0; k < V; k += 4) {
-                    float b[4];
-                    Elem<float>::unpack(load16(bias + k), b);
-                    #pragma unroll
-                    for (int m = 0; m < 4; m++) f[k + m] += b[m];
+                for (int m = 0; m < V; m++) {
+                    const uint32_t n = count_of<HISTORY>(counts, i * width + c + m);
+                    f[m] = GRAD ? penalised_slope(f[m], zf[m], n, paid) : penalised(f[m], n, paid);
                 }
+            }
+            if constexpr (BIAS) {
+                #pragma unroll
+                for (int m = 0; m < V; m++) f[m] += __uint_as_float(b[k][m / 4][m % 4]);
             }
             if (ALLOWED != kAll) {
-                const uint32_t bits = allowed_bits<V, ALLOWED == kAll ? kBits : ALLOWED>(allowed, (int)c0 + c);
                 #pragma unroll
-                for (int k = 0; k < V; k++) f[k] = bits >> k & 1 ? f[k] : GRAD ? 0.f : -INFINITY;
+                for (int m = 0; m < V; m++) f[m] = bits[k] >> m & 1 ? f[m] : GRAD ? 0.f : -INFINITY;
             }
-            store16(q, Elem<T>::pack(f));
-        } else {
-            for (int k = 0; k < columns - c; k++) {
-                float f = Elem<T>::get(GRAD ? g[k] : z[k]);
-                const uint32_t n = HISTORY ? counts[i * width + c + k] : 0u;
-                if (n) f = GRAD ? penalised_slope(f, Elem<T>::get(z[k]), repetition) : penalised(f, (float)n, repetition, presence, frequency);
-                if (!GRAD && bias) f += bias[k];
-                if (ALLOWED != kAll && !allowed_one<ALLOWED == kAll ? kBits : ALLOWED>(allowed, (int)c0 + c + k)) f = GRAD ? 0.f : -INFINITY;
-                q[k] = Elem<T>::put(f);
-            }
+            T* to = static_cast<T*>(s.out) + r * a.classes + c0 + c;
+            if (s.far) put_stream16(to, Elem<T>::pack(f));
+            else store16(to, Elem<T>::pack(f));
         }
+    }
+    // the values behind the last whole vector of each row
+    const int rest = columns - vecs * V;
+    for (int item = threadIdx.x; item < rows * rest; item += 256) {
+        int i;
+        const int c = vecs * V + split(item, rest, i);
+        const int64_t r = r0 + i;
+        const T z = row_start<T>(a, r)[c0 + c];
+        float f = Elem<T>::get(GRAD ? static_cast<const T*>(s.grad)[r * a.classes + c0 + c] : z);
+        if (HISTORY) {
+            const uint32_t n = count_of<HISTORY>(counts, i * width + c);
+            if (rows > 1) paid = penalties_of(s, r);
+            f = GRAD ? penalised_slope(f, Elem<T>::get(z), n, paid) : penalised(f, n, paid);
+        }
+        if (BIAS) f += s.bias[place(r, s.bias_outer, s.bias_inner) + c0 + c];
+        if (ALLOWED != kAll && !allowed_one<kAny>(allowed_row(r), (int)c0 + c)) f = GRAD ? 0.f : -INFINITY;
+        static_cast<T*>(s.out)[r * a.classes + c0 + c] = Elem<T>::put(f);
     }
 }
 
@@ -167,21 +292,22 @@ static int shape_logits(const char* who, const sd_logit_rows* in, const sd_const
         s.length = c->history_length; s.history_outer = c->history_outer; s.history_inner = c->history_inner;
         s.wide_history = c->history_bytes == 8; s.wide_lengths = c->length_bytes == 8;
         s.repetition_rows = c->repetition_rows; s.presence_rows = c->presence_rows; s.frequency_rows = c->frequency_rows;
-        s.repetition = (float)c->repetition; s.presence = (float)c->presence; s.frequency = (float)c->frequency;
+        s.repetition = (float)c->repetition; s.inverse = (float)(1.0 / c->repetition); s.presence = (float)c->presence; s.frequency = (float)c->frequency;
     }
     s.bias = c->bias; s.bias_outer = c->bias_outer; s.bias_inner = c->bias_inner;
     s.allowed = c->allowed; s.allowed_outer = c->allowed_outer; s.allowed_inner = c->allowed_inner;
     s.grad = grad; s.out = out;
-    const int64_t width = (a.classes + 7) / 8 * 8;
-    if (width <= kShapeCounts) {
-        const int64_t most = kShapeCounts / width, want = (a.rows + 1023) / 1024;
-        s.group = (int)(want < most ? want : most);
+    s.far = a.rows * a.classes * (16 / vec_of(in->dtype)) > kCached;
+    const int64_t width = (a.classes + 7) / 8 * 8, most = s.length >= 1 << 16 ? kCountWords : 2 * kCountWords;
+    if (width <= most) {
+        const int64_t fit = most / width, want = (a.rows + 1023) / 1024;
+        s.group = (int)(want < fit ? want : fit);
         s.parts = 1;
         s.part = width;
     } else {
         const int64_t want = (a.classes * a.rows / 1024 + 2047) / 2048 * 2048;
         s.group = 1;
-        s.part = want < 2048 ? 2048 : want < kShapeCounts ? want : kShapeCounts;
+        s.part = want < 2048 ? 2048 : want < most ? want : most;
         s.parts = (int)((a.classes + s.part - 1) / s.part);
     }
     const int64_t blocks = (a.rows + s.group - 1) / s.group * s.parts;
@@ -189,10 +315,15 @@ static int shape_logits(const char* who, const sd_logit_rows* in, const sd_const
     with_dtype(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const auto launch = [&](auto allowed, auto with_history) {
-            if (grad) hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, true>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
-            else hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, false>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
+            if (grad) hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kGradient>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
+            else if (s.bias) hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kBiased>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
+            else hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kPlain>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
         };
-        const auto with = [&](auto allowed) { history ? launch(allowed, std::true_type()) : launch(allowed, std::false_type()); };
+        const auto with = [&](auto allowed) {
+            if (!history) launch(allowed, std::integral_constant<int, kNone>());
+            else if (s.length < 1 << 16) launch(allowed, std::integral_constant<int, kShort>());
+            else launch(allowed, std::integral_constant<int, kLong>());
+        };
         if (!s.allowed) with(std::integral_constant<int, kAll>());
         else if (c->allowed_kind == kFlags) with(std::integral_constant<int, kFlags>());
         else with(std::integral_constant<int, kBits>());

@@ -150,6 +150,17 @@ def test_places_that_hold_no_class():
     close(out, z[:1].double().cpu() - torch.nn.functional.one_hot(torch.tensor([5]), 9) * (100 - 1), torch.full((1, 9), 6 * U * 110, dtype=torch.float64), "often")
 
 
+@pytest.mark.parametrize("places, classes", [(65535, 7), (65536, 7), (65540, 5000), (70001, 9001), (131073, 30000)])
+def test_long_histories(places, classes):
+    """Histories of more places than 16 bits count: one class all along, then another."""
+    history = torch.full((2, places), 3, device="cuda", dtype=torch.int32)
+    history[1, 5:] = classes - 1
+    history[1, -1] = 0
+    z = torch.randn(2, classes, device="cuda")
+    for past in (history, history.long()):
+        check(z, history=past, repetition=1.25, frequency=2.0 ** -10, presence=1.0)
+
+
 @pytest.mark.parametrize("classes", [10, 500, 9001])
 def test_strides(classes):
     """Padded vocabularies, parts and transposes of batches, expanded histories and masks: the results of contiguous copies."""
