@@ -3,12 +3,14 @@
 // Values are compared by whole numbers in their order (order_of): NaN above all, -0 as 0.  With the class behind it, upside down, every logit
 // has a number of its own, so the k largest are the same in every call.
 //
-// A row is read once.  A bound that at least k of its logits reach comes from the work-items' own maxima over its first vectors: the least of the
-// wavefronts' (k / wavefronts)-th largest ones.  What reaches the bound is put on a list in LDS, about 1.3 k of the first vectors' logits and with
-// each further part of the row as many again; of what does not, the exponentials are summed (relative to the largest of them).  A list that gets long is cut
-// to the k largest numbers, the last of which becomes the bound.  At the end the list is sorted by counting.  Few rows are read in parts, whose
-// lists a second kernel joins.  Bound by the bytes of the logits where there are many, else by the steps of a row, which other rows' loads hide.
-// Logits of -inf are never listed: where there are not k others the first classes that are -inf follow, which are among the row's first k.
+// A row is read once, in vectors of 16 bytes, whose largest logits decide: the k largest logits of a row lie in the k vectors that are first by their largest
+// logit and place, since any other logit has those k before it.  Vectors that reach a bound which k of them are known to reach are put on a list in LDS; of the
+// others the exponentials are summed.  The first bound comes from the work-items' own maxima over their first vectors: the least of the wavefronts'
+// (k / wavefronts)-th largest ones, reached by about 1.3 k vectors; a list that gets long is cut to k vectors, the last of which is the new bound (what is
+// cut is read again and summed).  At the end the listed vectors' logits are chosen from in the same way and sorted by counting.  Few rows are read in
+// parts, whose results a second kernel joins.  Logits of -inf are never listed: where there are not k others the first classes that are -inf follow,
+// which are among the row's first k.
+// Bound by the instructions of a logit, of which the exponential is half (it takes the time of four), and by the bytes of the logits.
 #include <climits>
 #include <type_traits>
 #include "label_rows.h"
@@ -26,180 +28,241 @@ __device__ __forceinline__ float value_of(uint32_t order) {
     return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
 constexpr uint32_t kLowestOrder = 0x00800000u;      // of -FLT_MAX; that of -inf is one less
+constexpr uint32_t kInfiniteOrder = 0xff800000u;
 
 typedef unsigned long long Number;      // order << 32 | ~class; 0: none
-__device__ __forceinline__ Number number_of(float v, int cls) { return (Number)order_of(v) << 32 | (uint32_t)~cls; }
-__device__ __forceinline__ float number_value(Number x) { return value_of((uint32_t)(x >> 32)); }
+__device__ __forceinline__ Number number_of(uint32_t order, int cls) { return (Number)order << 32 | (uint32_t)~cls; }
+__device__ __forceinline__ uint32_t number_order(Number x) { return (uint32_t)(x >> 32); }
 __device__ __forceinline__ int number_class(Number x) { return (int)~(uint32_t)x; }
 
 struct Top {
     int k;
-    double inverse;         // 1 / temperature
-    float high, low;        // log2(e) / temperature in two positive parts (see exp_of)
+    float by;               // log2(e) / temperature
     void* values;
     int* classes;
     float* rest;
 };
-__device__ __forceinline__ float exp_at(float v, const Top& t) { return __builtin_amdgcn_exp2f(fmaf(v, t.high, v * t.low)); }
 
-struct Others { float top; double sum; };       // sum of exp((v - top) / T)
-// two of them as one; `top` may be infinite
+// Sums of exp(v / T) are kept as multiples of 2 to the power of what this gives for the largest v in them: a number of fp32, so that v `by` minus it is
+// rounded once, and 2^4 at most where v is the largest; beyond 2^28, where the rounding of the power itself would be more, in 64 bits.
+constexpr float kNear = 0x1p28f;
+__device__ __forceinline__ double power_of(float top, const Top& t) {
+    const float p = top * t.by;
+    return fabsf(p) <= kNear ? (double)p : (double)top * (double)t.by;
+}
+struct Others { float top; double sum; };       // (top: -inf where there are none, never +inf)
+__device__ __forceinline__ double in_powers(float top, float of, const Top& t) { return top == of ? 1.0 : (double)__builtin_amdgcn_exp2f((float)(power_of(top, t) - power_of(of, t))); }
 __device__ __forceinline__ void join(Others& o, float top, double sum, const Top& t) {
+    if (sum == 0.0) return;
     if (top > o.top) {
-        o.sum *= (double)exp_at(o.top - top, t);
+        if (o.sum != 0.0) o.sum *= in_powers(o.top, top, t);
         o.top = top;
     }
-    o.sum += sum * (top == o.top ? 1.0 : (double)exp_at(top - o.top, t));
+    o.sum += sum * in_powers(top, o.top, t);
 }
 
-// The parts of a row: the k largest numbers in order (0 where there are fewer) and the others of each; the sum is NaN in a part that has a NaN.
+template <int V> __device__ __forceinline__ float largest(const float (&f)[V]) {
+    float m = f[0];
+    #pragma unroll
+    for (int i = 1; i < V; i++) m = fmaxf(m, f[i]);
+    return m;
+}
+
+// The parts of a row: the k largest numbers in order (0 where there are fewer) and the others of each.  The sum is NaN in a part that has a NaN.
 struct Parts { Number* numbers; Others* others; };
 
 template <int THREADS> struct Shared {
-    static constexpr int kCap = THREADS == 64 ? 512 : 2048;     // numbers of the list
-    static constexpr int kLong = kCap / 2;                      // from here on it is cut; what an exact choice adds has room behind it
-    static constexpr int kShort = kCap / 8;                     // and at the end from here on: sorting takes the square of the numbers
     static constexpr int kWaves = THREADS / 64;
-    static constexpr int kOwn = kCap / THREADS;
-    Number list[kCap];
+    static constexpr int kRoom = 512;               // numbers of a wavefront's part of the list
+    static constexpr int kMost = THREADS < 320 ? THREADS : 320;    // numbers that a cut may leave: at most one for each work-item
+    Number list[kWaves][kRoom];
+    Number first[THREADS];                          // those of a list that is no longer than that, one behind the other
     Others others[kWaves];
-    uint32_t bounds[kWaves];
-    int counts[2][kWaves];
-    int count, bad, nan;
-    uint32_t left_top;
-    unsigned long long left_sum;
+    uint32_t words[2][kWaves];
+    Number kth;                                     // the k-th number of a row or part
+    int again;
 };
-static_assert(Shared<256>::kShort >= kMostTop && Shared<256>::kShort <= 256 && Shared<64>::kShort <= 64, "a work-item per number at the end");
 
-// The list of a row or part, kept by all work-items of a workgroup together: they all call every member but `push` and `leave`, which come between barriers.
+// The list of a row or part, kept by all work-items of a workgroup together: they all call every member but `leave`; `push` is a wavefront's.  A wavefront has a
+// part of the list to itself, in the order in which it found the numbers, so that nothing waits for it and every call sees the same list.
 template <int THREADS> struct Keeper {
     using S = Shared<THREADS>;
     S& s;
     const Top& t;
-    float bound = -FLT_MAX;     // what reaches it is listed
-    Others others{-INFINITY, 0.0};     // this work-item's
+    float bound = -FLT_MAX;         // what reaches it is listed
+    Others others{-INFINITY, 0.0};  // this work-item's
+    int mine = 0;                   // numbers of this wavefront
+    int all = 0, longest = 0;       // of all and of the longest part, as of the last `settle`
+    bool nan = false, infinite = false;     // a NaN is there; +inf is among the others
     int lane, wave, turn = 0;
 
-    __device__ __forceinline__ Keeper(S& shared, const Top& top) : s(shared), t(top), lane(threadIdx.x & 63), wave(threadIdx.x >> 6) {
-        if (threadIdx.x == 0) { s.count = 0; s.nan = 0; s.bad = 0; s.left_top = 0u; s.left_sum = 0ull; }
-    }
-    __device__ __forceinline__ void push(Number x) {
-        const int at = atomicAdd(&s.count, 1);
-        if (at < S::kCap) s.list[at] = x;
-    }
+    __device__ __forceinline__ Keeper(S& shared, const Top& top) : s(shared), t(top), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {}
+
     __device__ __forceinline__ void leave(float v) {
-        if (v == v && v != -INFINITY) join(others, v, 1.0, t);
+        if (v == INFINITY) infinite = true;
+        else if (v > -INFINITY) join(others, v, 1.0, t);
     }
-    // The same for numbers of the list, whose places vary from call to call: their shares of the largest of them are added as whole numbers of 2^-40, in whatever
-    // order.  (The first of `take(visit)`'s two passes comes after a barrier.)
-    template <class Take> __device__ __forceinline__ void leave_listed(Take&& take) {
-        uint32_t most = 0u;
-        take([&](Number x) { const uint32_t order = (uint32_t)(x >> 32); most = order > most ? order : most; });
-        if (most != 0u) atomicMax(&s.left_top, most);
-        __syncthreads();
-        const float top = value_of(s.left_top);
-        unsigned long long share = 0;
-        take([&](Number x) { const float v = number_value(x); share += (unsigned long long)((v == top ? 1.f : exp_at(v - top, t)) * 0x1p40f); });
-        if (share != 0ull) atomicAdd(&s.left_sum, share);
-        __syncthreads();
-        if (threadIdx.x == 0 && s.left_sum != 0ull) {
-            if (top == top) join(others, top, (double)s.left_sum * 0x1p-40, t);
-            s.left_top = 0u;
-            s.left_sum = 0ull;
+    // logits that are all among the others
+    template <int V> __device__ __forceinline__ void leave_all(float (&f)[V]) {
+        float m = largest(f);
+        if (m == INFINITY) {
+            infinite = true;
+            #pragma unroll
+            for (int i = 0; i < V; i++) f[i] = f[i] == INFINITY ? -INFINITY : f[i];
+            m = largest(f);
         }
+        if (m == -INFINITY) return;
+        const double power = power_of(m, t);
+        if (fabs(power) <= (double)kNear) {
+            #pragma unroll
+            for (int i = 0; i < V; i++) f[i] = __builtin_amdgcn_exp2f(fmaf(f[i], t.by, -(float)power));
+        } else {
+            #pragma unroll
+            for (int i = 0; i < V; i++) f[i] = __builtin_amdgcn_exp2f((float)((double)f[i] * (double)t.by - power));
+        }
+        join(others, m, (double)tree(f), t);
     }
-    // how many of a work-item's numbers there are over all of them
-    __device__ __forceinline__ int total(int mine) {
-        uint32_t u = (uint32_t)mine;
-        const auto add = [](uint32_t a, uint32_t b) { return a + b; };
-        u = lanes_step<0>(u, add); u = lanes_step<1>(u, add); u = lanes_step<2>(u, add);
-        u = lanes_step<3>(u, add); u = lanes_step<4>(u, add); u = lanes_step<5>(u, add);
-        if (S::kWaves == 1) return (int)u;
-        int* counts = s.counts[turn++ & 1];     // (the other one may still be read)
-        if (lane == 0) counts[wave] = (int)u;
+    static __device__ __forceinline__ int before(uint64_t lanes) {     // of them, below this one
+        return __builtin_amdgcn_mbcnt_hi((uint32_t)(lanes >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)lanes, 0u));
+    }
+    // the numbers of those lanes of the wavefront that have one here
+    __device__ __forceinline__ void push(uint64_t lanes, bool has, Number x) {
+        if (has) s.list[wave][mine + before(lanes)] = x;
+        mine += __popcll(lanes);
+    }
+    // a word of each wavefront, of which `op` makes one
+    template <class Op> __device__ __forceinline__ uint32_t share(uint32_t word, Op&& op) {
+        if (S::kWaves == 1) { __syncthreads(); return word; }
+        uint32_t* words = s.words[turn++ & 1];      // (the other ones may still be read)
+        if (lane == 0) words[wave] = word;
         __syncthreads();
-        int sum = 0;
+        uint32_t r = words[0];
         #pragma unroll
-        for (int w = 0; w < S::kWaves; w++) sum += counts[w];
-        return sum;
+        for (int w = 1; w < S::kWaves; w++) r = op(r, words[w]);
+        return r;
     }
-    // What follows has higher classes than the k numbers listed at `order` and above: it is listed above that, or from it on if `also`.
+    template <class Op> static __device__ __forceinline__ uint32_t lanes_make(uint32_t u, Op&& op) {
+        u = lanes_step<0>(u, op); u = lanes_step<1>(u, op); u = lanes_step<2>(u, op);
+        u = lanes_step<3>(u, op); u = lanes_step<4>(u, op);
+        return __builtin_amdgcn_readfirstlane(lanes_step<5>(u, op));
+    }
+    template <class Op> __device__ __forceinline__ uint32_t share_lanes(uint32_t u, Op&& op) { return share(lanes_make(u, op), op); }
+    static __device__ __forceinline__ uint32_t least_of(uint32_t a, uint32_t b) { return a < b ? a : b; }
+    // the lists' lengths
+    __device__ __forceinline__ void settle() {
+        const uint32_t r = share((uint32_t)mine << 16 | (uint32_t)mine, [](uint32_t a, uint32_t b) {
+            return (a >> 16 > b >> 16 ? a >> 16 : b >> 16) << 16 | ((a & 0xffffu) + (b & 0xffffu));
+        });
+        all = (int)(r & 0xffffu);
+        longest = (int)(r >> 16);
+    }
+    // What follows has higher classes than the k numbers or more listed at `order` and above: it is listed above that, or from it on if `also`.
     __device__ __forceinline__ void raise(uint32_t order, bool also) {
         if (order < kLowestOrder) return;
-        const float from = order >= 0xff800000u ? INFINITY : value_of(also ? order : order + 1u);
+        const float from = order >= kInfiniteOrder ? INFINITY : value_of(also ? order : order + 1u);
         bound = fmaxf(bound, from);
     }
-    // The list of n > k numbers becomes the k largest of them.
-    __device__ __forceinline__ void cut(int n) {
-        Number own[S::kOwn];
-        #pragma unroll
-        for (int i = 0; i < S::kOwn; i++) {
-            const int at = threadIdx.x + i * THREADS;
-            own[i] = at < n ? s.list[at] : 0ull;
+    // The list of more than `most` numbers becomes at least k and at most `most` of the largest of them; `out` gets the others.  OWN: the wavefront's alone.
+    template <bool OWN, class Out> __device__ __forceinline__ void cut(int most, Out&& out) {
+        const auto shared = [&](uint32_t word, auto&& op) { return OWN ? word : share(word, op); };
+        const Number* own = s.list[wave];
+        uint32_t every = ~0u, some = 0u;
+        #pragma unroll 1
+        for (int i = lane; i < mine; i += 64) {
+            const uint32_t order = number_order(own[i]);
+            every &= order;
+            some |= order;
         }
-        Number least = 0;       // the largest prefix found that k numbers reach
-        for (int bit = 63; bit >= 0; bit--) {
+        const auto both = [](uint32_t a, uint32_t b) { return a & b; };
+        const auto either = [](uint32_t a, uint32_t b) { return a | b; };
+        every = shared(lanes_make(every, both), both);
+        some = shared(lanes_make(some, either), either);
+        // the bits in which the orders differ are all that is looked for
+        const uint32_t differ = every ^ some;
+        const int high = differ == 0u ? 0 : 32 - __clz(differ);
+        Number least = (Number)(high == 32 ? 0u : every >> high << high) << 32;     // the largest prefix found that k numbers reach
+        #pragma unroll 1
+        for (int bit = 31 + high; bit >= 0; bit--) {
             const Number next = least | 1ull << bit;
             int c = 0;
-            #pragma unroll
-            for (int i = 0; i < S::kOwn; i++) c += own[i] >= next;
-            c = total(c);
-            if (c >= t.k) least = next;
-            if (c == t.k) break;
+            #pragma unroll 1
+            for (int i = 0; i < mine; i += 64) c += __popcll(__ballot(lane + i < mine && own[lane + i] >= next));
+            c = (int)shared((uint32_t)c, [](uint32_t a, uint32_t b) { return a + b; });
+            if (c < t.k) continue;
+            least = next;
+            if (c <= most) break;
         }
-        __syncthreads();
-        if (threadIdx.x == 0) s.count = 0;
-        __syncthreads();
-        #pragma unroll
-        for (int i = 0; i < S::kOwn; i++) {
-            if (own[i] >= least && own[i] != 0ull) push(own[i]);
+        const int had = mine;
+        mine = 0;
+        #pragma unroll 1
+        for (int i = 0; i < had; i += 64) {     // (what stays is stored no later than where it stood)
+            const Number x = lane + i < had ? own[lane + i] : 0ull;
+            const bool stays = x >= least && x != 0ull;
+            push(__ballot(stays), stays, x);
+            if (!stays && x != 0ull) out(x);
         }
-        leave_listed([&](auto&& visit) {
-            #pragma unroll
-            for (int i = 0; i < S::kOwn; i++)
-                if (own[i] < least && own[i] != 0ull) visit(own[i]);
-        });
-        raise((uint32_t)(least >> 32), (uint32_t)least == 0u);
+        raise(number_order(least), (uint32_t)least == 0u);
+        if (!OWN) settle();
+    }
+    // the list, at most THREADS long, in `first`
+    __device__ __forceinline__ void gather() {
+        int at = lane;
+        if (S::kWaves > 1) {
+            uint32_t* words = s.words[turn++ & 1];
+            if (lane == 0) words[wave] = (uint32_t)mine;
+            __syncthreads();
+            for (int w = 0; w < wave; w++) at += (int)words[w];
+        }
+        for (int i = lane; i < mine; i += 64, at += 64) s.first[at] = s.list[wave][i];
         __syncthreads();
     }
-    // The end of a row or part that has n numbers listed, at most one for each work-item: what `put` gets are the k largest of them with their places.
-    template <class Put> __device__ __forceinline__ void sort(int n, Put&& put) {
-        const Number mine = (int)threadIdx.x < n ? s.list[threadIdx.x] : 0ull;
+    // The end of a row or part: what `put` gets are the k largest numbers with their places, of a list of logits that is at most THREADS long.
+    template <class Put> __device__ __forceinline__ void sort(Put&& put) {
+        gather();
+        if (64 * wave >= all) return;
+        const Number own = (int)threadIdx.x < all ? s.first[threadIdx.x] : 0ull;
         int place = 0;
-        for (int j = 0; j < n; j++) place += s.list[j] > mine;
-        if (mine != 0ull && place < t.k) put(place, mine);
-        if (n > t.k) leave_listed([&](auto&& visit) { if (mine != 0ull && place >= t.k) visit(mine); });
+        #pragma unroll 4
+        for (int j = 0; j < all; j++) place += s.first[j] > own;
+        if (own != 0ull) {
+            if (place < t.k) put(place, own);
+            else leave(value_of(number_order(own)));
+            if (place == t.k - 1) s.kth = own;
+        }
     }
-    // all work-items' others, to the first one
+    // all work-items' others, to the first one; NaN where the row or part has a NaN
     __device__ __forceinline__ Others all_others() {
         const float m = group_max(others.top, 6);
-        Others o{m, group_total(others.top == m ? others.sum : others.sum * (double)exp_at(others.top - m, t), 6)};
-        if (S::kWaves > 1) {
-            if (lane == 0) s.others[wave] = o;
-            __syncthreads();
-            if (threadIdx.x == 0)
-                for (int w = 1; w < S::kWaves; w++) join(o, s.others[w].top, s.others[w].sum, t);
-        }
-        if (s.nan) o.sum = __builtin_nan("");
+        Others o{m, group_total(others.sum == 0.0 ? 0.0 : others.sum * in_powers(others.top, m, t), 6)};
+        if (lane == 0) s.others[wave] = o;
+        const uint32_t odd = share((__ballot(nan) ? 1u : 0u) | (__ballot(infinite) ? 2u : 0u), [](uint32_t x, uint32_t y) { return x | y; });
+        if (threadIdx.x == 0)
+            for (int w = 1; w < S::kWaves; w++) join(o, s.others[w].top, s.others[w].sum, t);
+        if (odd & 2) o = Others{FLT_MAX, INFINITY};
+        if (odd & 1) o.sum = __builtin_nan("");
         return o;
     }
-    // The same for a whole row: its results.
-    template <class T> __device__ __forceinline__ void finish(int n, const T* row, int64_t r) {
+    // The same for a whole row: what it chooses.
+    template <class T> __device__ __forceinline__ void finish(const T* row, int64_t r) {
         T* values = static_cast<T*>(t.values) + r * t.k;
         int* classes = t.classes + r * t.k;
-        const auto put = [&](int place, int cls) { values[place] = row[cls]; classes[place] = cls; };
-        sort(n, [&](int place, Number x) { put(place, number_class(x)); });
-        if (n < t.k) {      // the first classes that are -inf
+        const auto put = [&](int place, float v, int cls) { values[place] = Elem<T>::put(v); classes[place] = cls; };
+        sort([&](int place, Number x) { put(place, value_of(number_order(x)), number_class(x)); });
+        if (all < t.k) {      // the first classes that are -inf
             const bool none = (int)threadIdx.x < t.k && Elem<T>::get(row[threadIdx.x]) == -INFINITY;
             const uint64_t lanes = __ballot(none);
-            if (lane == 0) s.counts[0][wave] = __popcll(lanes);
-            __syncthreads();
-            int place = n + __popcll(lanes & ((1ull << lane) - 1ull));
-            for (int w = 0; w < wave; w++) place += s.counts[0][w];
-            if (none && place < t.k) put(place, threadIdx.x);
+            int place = all + before(lanes);
+            if (S::kWaves > 1) {
+                uint32_t* words = s.words[turn++ & 1];
+                if (lane == 0) words[wave] = (uint32_t)__popcll(lanes);
+                __syncthreads();
+                for (int w = 0; w < wave; w++) place += (int)words[w];
+            }
+            if (none && place < t.k) put(place, -INFINITY, threadIdx.x);
         }
-        const Others o = all_others();
-        if (threadIdx.x == 0) t.rest[r] = o.sum == 0.0 ? -INFINITY : (float)(log(o.sum) + (double)o.top * t.inverse);
+    }
+    __device__ __forceinline__ void store_rest(const Others& o, int64_t r) const {
+        t.rest[r] = o.sum == 0.0 ? -INFINITY : (float)(log(o.sum) + power_of(o.top, t) * 0.69314718055994530942);
     }
 };
 
@@ -214,6 +277,11 @@ template <class T> __device__ __forceinline__ u32x4 without_first(u32x4 v, int c
         else v[w] = 2 * w + 1 < count ? none[w] : 2 * w < count ? (v[w] & 0xffff0000u) | (none[w] & 0xffffu) : v[w];
     }
     return v;
+}
+// the vector that was read at column `at` (a multiple of V but for the last)
+template <class T> __device__ __forceinline__ void read_again(float (&f)[Elem<T>::kVec], const T* p, int at) {
+    constexpr int V = Elem<T>::kVec;
+    Elem<T>::unpack(without_first<T>(load16(p + at), (V - (at & (V - 1))) & (V - 1)), f);
 }
 
 // NV vectors of a row for each work-item, the k-th being vector threadIdx.x + k THREADS of those from c0 on; -inf behind the end
@@ -237,110 +305,16 @@ template <class T, int THREADS, int NV> __device__ __forceinline__ void load_vec
     }
 }
 
-template <int V> __device__ __forceinline__ float largest(const float (&f)[V]) {
-    float m = f[0];
-    #pragma unroll
-    for (int i = 1; i < V; i++) m = fmaxf(m, f[i]);
-    return m;
-}
+// Shares of the others below this, relative to the bound, are formed again: of terms below 2^-126 nothing is left, 2^30 of them are 2^-36 of it.
+constexpr double kLeastShare = 0x1p-60;
 
-// one of these vectors and where it begins
-template <class T> __device__ __forceinline__ int load_one(float (&f)[Elem<T>::kVec], const T* p, int c, int n) {
-    constexpr int V = Elem<T>::kVec;
-    const int at = column_of<V>(c, n);
-    if (c >= n) {
-        #pragma unroll
-        for (int i = 0; i < V; i++) f[i] = -INFINITY;
-    } else Elem<T>::unpack(without_first<T>(load16(p + at), c - at), f);
-    return at;
-}
-
-// The exact choice of the k first numbers of THREADS * nv vectors, where more of them reach the bound than the list has room for, and where a logit is NaN:
-// the k-th largest order bit by bit.  The vectors are read again for each bit: it is rare, and held in registers they would crowd out the rest.
-template <class T, int THREADS> __device__ __forceinline__ void choose_exactly(Keeper<THREADS>& keep, const T* p, int c0, int n, int class0, int have, int nv) {
-    constexpr int V = Elem<T>::kVec;
-    const int k_most = keep.t.k;
-    uint32_t kth = 0;
-    #pragma unroll 1
-    for (int bit = 31; bit >= 0; bit--) {
-        const uint32_t next = kth | 1u << bit;
-        int count = 0;
-        #pragma unroll 1
-        for (int k = 0; k < nv; k++) {
-            float f[V];
-            load_one(f, p, c0 + ((int)threadIdx.x + k * THREADS) * V, n);
-            #pragma unroll
-            for (int i = 0; i < V; i++) count += order_of(f[i]) >= next;
-        }
-        if (keep.total(count) >= k_most) kth = next;
-    }
-    const bool enough = kth >= kLowestOrder;        // else all above -inf are chosen
-    if (!enough) kth = kLowestOrder - 1u;
-    __syncthreads();
-    if (threadIdx.x == 0) keep.s.count = have;
-    __syncthreads();
-    bool nan = false;
-    #pragma unroll 1
-    for (int k = 0; k < nv; k++) {
-        float f[V];
-        const int c = load_one(f, p, c0 + ((int)threadIdx.x + k * THREADS) * V, n);
-        #pragma unroll 1
-        for (int i = 0; i < V; i++) {
-            float v = f[0];
-            #pragma unroll
-            for (int m = 1; m < V; m++) v = i == m ? f[m] : v;
-            const uint32_t order = order_of(v);
-            nan |= v != v;
-            if (order > kth) keep.push(number_of(v, class0 + c + i));
-            else if (!enough || order != kth) keep.leave(v);
-        }
-    }
-    if (nan) keep.s.nan = 1;
-    __syncthreads();
-    if (enough) {       // equal ones in the order of their classes
-        int at = keep.s.count;
-        const int end = have + k_most;
-        __syncthreads();
-        #pragma unroll 1
-        for (int k = 0; k < nv; k++) {
-            float f[V];
-            const int c = load_one(f, p, c0 + ((int)threadIdx.x + k * THREADS) * V, n);
-            uint32_t equal = 0;
-            #pragma unroll
-            for (int i = 0; i < V; i++) equal |= order_of(f[i]) == kth ? 1u << i : 0u;
-            const int mine = __popc(equal);
-            int before = mine;      // of the lanes up to this one
-            #pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const int other = __shfl_up(before, s);
-                if (keep.lane >= s) before += other;
-            }
-            int* counts = keep.s.counts[k & 1];
-            if (keep.lane == 63) counts[keep.wave] = before;
-            __syncthreads();
-            int place = at + before - mine;
-            #pragma unroll
-            for (int w = 0; w < Shared<THREADS>::kWaves; w++) {
-                if (w < keep.wave) place += counts[w];
-                at += counts[w];
-            }
-            const float value = value_of(kth);
-            for (; equal != 0u; equal &= equal - 1u, place++) {
-                if (place < end) keep.s.list[place] = (Number)kth << 32 | (uint32_t)~(class0 + c + __ffs(equal) - 1);
-                else keep.leave(value);
-            }
-        }
-        __syncthreads();
-        if (threadIdx.x == 0) keep.s.count = end;
-        keep.raise(kth, false);
-    }
-    __syncthreads();
-}
-
-// A workgroup per row, or per one of `splits` parts of `part` classes of a row.
-template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREADS, NV > 4 ? 6 : 8) top_rows_kernel(LogitRows a, Top t, int splits, int part, Parts out) {
+// A workgroup per row, or per one of `splits` parts of `part` classes of a row.  What is not listed lies below the wavefront's bound, to which the exponentials are relative;
+// where they come out too small, or the bound too large, for fp32, the others are gone through again at the end.
+template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREADS, 8) top_rows_kernel(LogitRows a, Top t, int splits, int part, Parts out) {
     constexpr int V = Elem<T>::kVec, kSpan = THREADS * NV * V;
     using S = Shared<THREADS>;
+    static_assert(64 * NV + kMostTop <= S::kRoom, "a wavefront's part of the list has room for all vectors behind the k that a cut of its own leaves");
+    static_assert(64 * V <= S::kRoom, "and for the logits of a vector for each work-item");
     __shared__ S s;
     for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
         const int64_t r = splits == 1 ? b : b / splits;
@@ -348,7 +322,23 @@ template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREAD
         const T* row = row_start<T>(a, r);
         const T* p = row + class0;
         Keeper<THREADS> keep(s, t);
-        int have = 0;
+        // a vector that is cut: its logits are among the others
+        const auto leave_vector = [&](Number x) {
+            float f[V];
+            read_again(f, p, number_class(x));
+            keep.leave_all(f);
+        };
+        double sum = 0.0;
+        float base = -FLT_MAX, power = 0.f;     // (nothing but -inf is summed as long as this is the bound)
+        bool again = false;
+        const int most = t.k + t.k / 4 < S::kMost ? t.k + t.k / 4 : S::kMost;      // vectors that a cut leaves
+        const auto rebase = [&]() {
+            if (keep.bound == base) return;
+            if (base > -FLT_MAX) sum *= in_powers(base, keep.bound, t);
+            base = keep.bound;
+            power = base * t.by;
+            if (!(fabsf(power) <= kNear)) { power = 0.f; again = true; }
+        };
         for (int c0 = 0, step = 1; c0 < n; c0 += kSpan, step++) {
             u32x4 v[NV];
             load_vectors<T, THREADS, NV>(v, p, c0, n);
@@ -371,118 +361,158 @@ template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREAD
                         if (__popcll(__ballot(order >= next)) >= want) least = next;
                     }
                 }
-                if (S::kWaves > 1) {
-                    if (keep.lane == 0) s.bounds[keep.wave] = least;
-                    __syncthreads();
-                    #pragma unroll
-                    for (int w = 0; w < S::kWaves; w++) least = s.bounds[w] < least ? s.bounds[w] : least;
-                }
-                keep.raise(least, true);
+                keep.raise(keep.share(least, Keeper<THREADS>::least_of), true);
+                rebase();
                 // what was derived from the vectors is derived again: kept, it would be twice their registers
                 #pragma unroll
                 for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
             }
-            Others mine = keep.others;
             #pragma unroll
-            for (int k = 0; k < NV; k++) {
-                asm volatile("" : "+v"(v[k]), "+v"(mine.sum));      // (one vector after the other: all of them unpacked would not fit)
-                float f[V];
-                Elem<T>::unpack(v[k], f);
-                float m = largest(f);
-                if (m >= keep.bound) {
-                    const int c = class0 + column_of<V>(c0 + ((int)threadIdx.x + k * THREADS) * V, n);
-                    #pragma unroll
-                    for (int i = 0; i < V; i++)
-                        if (f[i] >= keep.bound) {
-                            keep.push(number_of(f[i], c + i));
-                            f[i] = -INFINITY;
-                        }
-                    m = largest(f);
-                }
-                if (m > mine.top) {
-                    mine.sum *= (double)exp_at(mine.top - m, t);
-                    mine.top = m;
-                }
-                const float base = finite(mine.top);
+            for (int k = 0; k < NV; k += 2) {
+                asm volatile("" : "+v"(v[k]), "+v"(v[k + 1]), "+v"(sum));      // (two vectors after two: all of them unpacked would not fit)
+                float f[2][V], m[2];
+                bool listed[2];
                 #pragma unroll
-                for (int i = 0; i < V; i++) f[i] = exp_at(f[i] - base, t);
-                mine.sum += (double)tree(f);
+                for (int h = 0; h < 2; h++) {
+                    Elem<T>::unpack(v[k + h], f[h]);
+                    m[h] = largest(f[h]);
+                    listed[h] = m[h] >= keep.bound;
+                }
+                const auto column = [&](int h) { return column_of<V>(c0 + ((int)threadIdx.x + (k + h) * THREADS) * V, n); };
+                const int had = keep.mine;
+                const uint64_t lanes[2] = {__ballot(listed[0]), __ballot(listed[1])};
+                if (lanes[0] | lanes[1]) {
+                    #pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        if (lanes[h]) keep.push(lanes[h], listed[h], number_of(order_of(m[h]), column(h)));
+                }
+                float part[2];
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    #pragma unroll
+                    for (int i = 0; i < V; i++) f[h][i] = __builtin_amdgcn_exp2f(fmaf(f[h][i], t.by, -power));
+                    part[h] = tree(f[h]);
+                }
+                if (__ballot(part[0] + part[1] != part[0] + part[1])) {     // a NaN is above all: the vector's number is to say so, and has to be on the list
+                    #pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const bool nan = part[h] != part[h], more = nan && !listed[h];
+                        const Number x = number_of(0xffffffffu, column(h));
+                        if (nan && listed[h]) s.list[keep.wave][had + (h ? __popcll(lanes[0]) : 0) + keep.before(lanes[h])] = x;
+                        keep.push(__ballot(more), more, x);
+                        keep.nan |= nan;
+                        part[h] = nan ? 0.f : part[h];
+                    }
+                }
+                sum += (double)((listed[0] ? 0.f : part[0]) + (listed[1] ? 0.f : part[1]));
             }
-            if (mine.sum != mine.sum) s.bad = step;
-            __syncthreads();
-            const int listed = s.count, bad = s.bad;
-            __syncthreads();
-            if (listed > S::kCap || bad == step) {
-                choose_exactly<T, THREADS>(keep, p, c0, n, class0, have, NV);
-                have = s.count;
-                __syncthreads();
-            } else {
-                keep.others = mine;
-                have = listed;
+            // The wavefronts go on by themselves; they meet, and cut the list together, behind the first, second, fourth, .. and last of their steps.
+            const bool last = c0 + kSpan >= n;
+            if (last || (step & (step - 1)) == 0) {
+                keep.settle();
+                if (keep.all > most) { keep.template cut<false>(most, leave_vector); rebase(); }
             }
-            if (have > (c0 + kSpan < n ? S::kLong : S::kShort) && have > t.k) {
-                keep.cut(have);
-                have = t.k;
-            }
+            if (!last && keep.mine > S::kRoom - 64 * NV) { keep.template cut<true>(S::kRoom - 64 * NV, leave_vector); rebase(); }
         }
-        if (splits == 1) keep.template finish<T>(have, row, r);
+        // The logits of the listed vectors.  Each of these has one that reaches the least of their largest ones.
+        keep.gather();
+        const Number x = (int)threadIdx.x < keep.all ? s.first[threadIdx.x] : 0ull;
+        const uint32_t least = keep.share_lanes(x != 0ull ? number_order(x) : ~0u, Keeper<THREADS>::least_of);
+        keep.bound = -FLT_MAX;
+        if (keep.all >= t.k) keep.raise(least, true);
+        keep.mine = 0;
+        if (__ballot(x != 0ull)) {
+            float f[V];
+            const int at = x != 0ull ? number_class(x) : 0;
+            if (x != 0ull) read_again(f, p, at);
+            #pragma unroll
+            for (int i = 0; i < V; i++) {
+                const bool listed = x != 0ull && !(f[i] < keep.bound);      // (a NaN, too)
+                const uint64_t lanes = __ballot(listed);
+                if (lanes) keep.push(lanes, listed, number_of(order_of(f[i]), class0 + at + i));
+                f[i] = listed ? -INFINITY : f[i];
+            }
+            if (x != 0ull) keep.leave_all(f);
+        }
+        keep.settle();
+        if (keep.all > THREADS) keep.template cut<false>(S::kMost, [&](Number y) { keep.leave(value_of(number_order(y))); });
+        if (splits == 1) keep.template finish<T>(row, r);
         else {
             Number* numbers = out.numbers + (r * splits + q) * t.k;
-            keep.sort(have, [&](int place, Number x) { numbers[place] = x; });
-            for (int i = have + threadIdx.x; i < t.k; i += THREADS) numbers[i] = 0ull;
-            const Others o = keep.all_others();
-            if (threadIdx.x == 0) out.others[r * splits + q] = o;
+            keep.sort([&](int place, Number y) { numbers[place] = y; });
+            for (int i = keep.all + threadIdx.x; i < t.k; i += THREADS) numbers[i] = 0ull;
+        }
+        // (where fewer than k logits are above -inf there are no others)
+        if (!again) join(keep.others, base, sum, t);
+        Others o = keep.all_others();
+        const uint32_t bases = keep.share(order_of(again ? INFINITY : base), [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+        if (threadIdx.x == 0) {
+            const float highest = value_of(bases);
+            s.again = keep.all >= t.k && o.sum == o.sum && highest > -FLT_MAX && (highest == INFINITY || !(o.sum * in_powers(o.top, highest, t) >= kLeastShare));
+        }
+        __syncthreads();
+        if (s.again) {
+            const Number kth = s.kth;
+            keep.others = Others{-INFINITY, 0.0};
+            #pragma unroll 1
+            for (int c = (int)threadIdx.x * V; c < n; c += THREADS * V) {
+                float f[V];
+                const int at = column_of<V>(c, n);
+                Elem<T>::unpack(without_first<T>(load16(p + at), c - at), f);
+                #pragma unroll
+                for (int i = 0; i < V; i++)
+                    if (number_of(order_of(f[i]), class0 + at + i) < kth) keep.leave(f[i]);
+            }
+            o = keep.all_others();
+        }
+        if (threadIdx.x == 0) {
+            if (splits == 1) keep.store_rest(o, r);
+            else out.others[r * splits + q] = o;
         }
         __syncthreads();
     }
 }
 
 // A workgroup per row joins its parts' lists: of k / splits numbers of each list at least the least is a bound.
-template <class T> __global__ void __launch_bounds__(256) top_join_kernel(LogitRows a, Top t, int splits, Parts in) {
-    using S = Shared<256>;
+constexpr int kJoin = 512;
+template <class T> __global__ void __launch_bounds__(kJoin) top_join_kernel(LogitRows a, Top t, int splits, Parts in) {
+    using S = Shared<kJoin>;
+    constexpr int kTurn = (S::kRoom - kMostTop) / 64;      // numbers of a work-item before the lists' lengths are looked at
     __shared__ S s;
-    __shared__ Number leasts[4];
     for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        Keeper<256> keep(s, t);
+        Keeper<kJoin> keep(s, t);
         const Number* numbers = in.numbers + r * splits * t.k;
-        const int total = splits * t.k, nth = (t.k + splits - 1) / splits - 1;
-        Number least = ~0ull;
-        __syncthreads();
-        for (int q = threadIdx.x; q < splits; q += 256) {
-            const Number x = numbers[q * t.k + nth];
-            least = x < least ? x : least;
+        const int total = splits * t.k, nth = (t.k + splits - 1) / splits - 1, most = t.k + t.k / 4;
+        uint32_t least = ~0u;       // (by their orders: lists with nothing there have 0)
+        for (int q = threadIdx.x; q < splits; q += kJoin) {
+            least = Keeper<kJoin>::least_of(least, number_order(numbers[q * t.k + nth]));
             const Others o = in.others[r * splits + q];
-            if (o.sum != o.sum) s.bad = 1;
-            else if (o.sum != 0.0) join(keep.others, o.top, o.sum, t);
+            if (o.sum != o.sum) keep.nan = true;
+            else if (o.sum == INFINITY) keep.infinite = true;
+            else join(keep.others, o.top, o.sum, t);
         }
-        for (int step = 32; step > 0; step >>= 1) {
-            const Number x = __shfl_xor(least, step);
-            least = x < least ? x : least;
-        }
-        if (keep.lane == 0) leasts[keep.wave] = least;
-        __syncthreads();
-        #pragma unroll
-        for (int w = 0; w < 4; w++) least = leasts[w] < least ? leasts[w] : least;
-        if (threadIdx.x == 0) s.nan = s.bad;
-        int have = 0;
-        for (int i0 = 0; i0 < total; i0 += 1024) {
+        keep.raise(keep.share_lanes(least, Keeper<kJoin>::least_of), true);
+        for (int i0 = 0; i0 < total; i0 += kTurn * kJoin) {
+            const uint32_t from = order_of(keep.bound);     // (a NaN is above every bound)
             #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const int at = i0 + i * 256 + threadIdx.x;
+            for (int i = 0; i < kTurn; i++) {
+                const int at = i0 + i * kJoin + threadIdx.x;
                 const Number x = at < total ? numbers[at] : 0ull;
-                if (x == 0ull) continue;
-                if (x >= least) keep.push(x);
-                else keep.leave(number_value(x));
+                const bool listed = x != 0ull && number_order(x) >= from;
+                const uint64_t lanes = __ballot(listed);
+                if (lanes) keep.push(lanes, listed, x);
+                if (x != 0ull && !listed) keep.leave(value_of(number_order(x)));
             }
-            __syncthreads();
-            have = s.count;
-            __syncthreads();
-            if (have > (i0 + 1024 < total ? S::kLong : S::kShort) && have > t.k) {
-                keep.cut(have);
-                have = t.k;
+            keep.settle();
+            if (keep.all > kJoin || keep.longest > kMostTop) {
+                const auto leave = [&](Number y) { keep.leave(value_of(number_order(y))); };
+                if (keep.all > most) keep.template cut<false>(most, leave);
+                if (i0 + kTurn * kJoin < total && keep.mine > kMostTop) keep.template cut<true>(kMostTop, leave);
             }
         }
-        keep.template finish<T>(have, row_start<T>(a, r), r);
+        keep.template finish<T>(row_start<T>(a, r), r);
+        const Others o = keep.all_others();
+        if (threadIdx.x == 0) keep.store_rest(o, r);
         __syncthreads();
     }
 }
@@ -507,29 +537,36 @@ template <class T> __global__ void __launch_bounds__(256) top_short_kernel(Logit
             t.classes[r * t.k + place] = lane;
         }
         const float other = chosen ? -INFINITY : v, top = group_max(other, shift);
-        const double sum = group_total(other == -INFINITY ? 0.0 : other == top ? 1.0 : (double)exp_at(other - top, t), shift);
+        const double sum = group_total(other == -INFINITY ? 0.0 : other == top ? 1.0 : top == INFINITY ? 0.0 : in_powers(other, top, t), shift);
         const float nan = group_max(v != v ? 1.f : 0.f, shift);
-        if (lane == 0) t.rest[r] = nan != 0.f ? __builtin_nanf("") : sum == 0.0 ? -INFINITY : (float)(log(sum) + (double)top * t.inverse);
+        if (lane == 0)
+            t.rest[r] = nan != 0.f ? __builtin_nanf("") : sum == 0.0 ? -INFINITY : top == INFINITY ? INFINITY : (float)(log(sum) + power_of(top, t) * 0.69314718055994530942);
     }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 namespace {
 
-// How rows are read: 0 short ones by lanes, 64 by a wavefront each, 256 by workgroups, in `splits` parts.
+// How rows are read: by `threads` work-items each (0: short ones, by lanes), `vectors` of each at a time, in `splits` parts.
+// A list is cut to 1.25 k, which is no more than the work-items, so that a prefix of the numbers does for it (k = 256 with 256 of them 4096 x 131072 bf16 660 us).
+// Above that, as many as fill the card with one row or part each: rows that end together end badly, since nothing is read meanwhile.
 struct Plan { int threads, vectors, splits; int64_t part; };
 Plan plan_of(const LogitRows& a, int64_t k, int vec) {
     if (a.classes <= 64) return {0, 1, 1, a.classes};
-    if (k <= 64 && a.classes <= 64 * 4 * vec) return {64, 4, 1, a.classes};
-    const int64_t want = (2048 + a.rows - 1) / a.rows, span = 256 * vec;
-    int vectors = 8;
-    while (vectors > 2 && a.classes < want * span * vectors) vectors /= 2;
+    const int64_t most = k + k / 4, card = 1 << 19;
+    int threads = 64;
+    while (threads < most) threads *= 2;
+    if (a.classes <= (int64_t)threads * 4 * vec) return {threads, 4, 1, a.classes};
+    if (threads < 128) threads = 128;
+    while (threads < 256 && a.rows * threads < card) threads *= 2;
+    const int64_t want = (card + a.rows * threads - 1) / (a.rows * threads), span = threads * vec;
+    const int vectors = a.classes >= want * span * 4 ? 4 : 2;
     int64_t splits = (a.classes + span * vectors - 1) / (span * vectors);
     if (splits > want) splits = want;
     if (splits > 256) splits = 256;
-    if (splits == 1) return {256, vectors, 1, a.classes};
+    if (splits == 1) return {threads, 4, 1, a.classes};
     const int64_t part = ((a.classes + splits - 1) / splits + span - 1) / span * span;
-    return {256, vectors, (int)((a.classes + part - 1) / part), part};
+    return {threads, vectors, (int)((a.classes + part - 1) / part), part};
 }
 
 int64_t part_floats(const LogitRows& a, int64_t k, const Plan& plan) {
@@ -546,7 +583,10 @@ using namespace sd;
 extern "C" int64_t sd_top_scratch(const sd_logit_rows* rows, int64_t k) {
     LogitRows a;
     if (check_logits(rows, "top_scratch", &a) != SD_OK) return -1;
-    if (k < 1 || k > kMostTop || k > a.classes || a.classes >= kMostClasses) { set_error("top_scratch: k=%lld of %lld classes: 1..%d of fewer than 2^30 are possible", (long long)k, (long long)a.classes, kMostTop); return -1; }
+    if (k < 1 || k > kMostTop || k > a.classes || a.classes >= kMostClasses) {
+        set_error("top_scratch: k=%lld of %lld classes: 1..%d of fewer than 2^30 are possible", (long long)k, (long long)a.classes, kMostTop);
+        return -1;
+    }
     return (part_floats(a, k, plan_of(a, k, vec_of(rows->dtype))) + 3) / 4 * 4;
 }
 
@@ -554,17 +594,15 @@ extern "C" int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temper
     sd::CallGuard call_guard;
     LogitRows a;
     if (int rc = check_logits(rows, "top_logits", &a)) return rc;
-    SD_REQUIRE(k >= 1 && k <= kMostTop && k <= a.classes && a.classes < kMostClasses, "top_logits: k=%lld of %lld classes: 1..%d of fewer than 2^30 are possible", (long long)k, (long long)a.classes, kMostTop);
+    SD_REQUIRE(k >= 1 && k <= kMostTop && k <= a.classes && a.classes < kMostClasses, "top_logits: k=%lld of %lld classes: 1..%d of fewer than 2^30 are possible",
+               (long long)k, (long long)a.classes, kMostTop);
     SD_REQUIRE(temperature >= 1e-4 && temperature <= 1e4, "top_logits: temperature=%g outside 1e-4..1e4", temperature);
     SD_REQUIRE(values && classes && rest, "top_logits: null argument");
     SD_REQUIRE((reinterpret_cast<uintptr_t>(values) & (rows->dtype == SD_FLOAT32 ? 3 : 1)) == 0 && ((reinterpret_cast<uintptr_t>(classes) | reinterpret_cast<uintptr_t>(rest)) & 3) == 0 &&
                (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "top_logits: results are not aligned to their types, or scratch to 16 bytes");
     const Plan plan = plan_of(a, k, vec_of(rows->dtype));
     SD_REQUIRE(scratch || plan.splits == 1, "top_logits: null scratch");
-    const double by = 1.4426950408889634074 / temperature;
-    float high = (float)by;
-    if ((double)high >= by) high = nextafterf(high, 0.f);
-    const Top t{(int)k, 1.0 / temperature, high, (float)(by - (double)high), values, classes, rest};
+    const Top t{(int)k, (float)(1.4426950408889634074 / temperature), values, classes, rest};
     const int64_t lists = a.rows * plan.splits;
     Parts parts{};
     if (plan.splits > 1) parts = Parts{reinterpret_cast<Number*>(scratch), reinterpret_cast<Others*>(scratch + 2 * lists * k)};
@@ -579,11 +617,17 @@ extern "C" int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temper
             return;
         }
         const dim3 grid(blocks_for(lists));
-        if (plan.threads == 64) hipLaunchKernelGGL((top_rows_kernel<T, 64, 4>), grid, dim3(64), 0, s, a, t, 1, (int)plan.part, parts);
-        else if (plan.vectors == 2) hipLaunchKernelGGL((top_rows_kernel<T, 256, 2>), grid, dim3(256), 0, s, a, t, plan.splits, (int)plan.part, parts);
-        else if (plan.vectors == 4) hipLaunchKernelGGL((top_rows_kernel<T, 256, 4>), grid, dim3(256), 0, s, a, t, plan.splits, (int)plan.part, parts);
-        else hipLaunchKernelGGL((top_rows_kernel<T, 256, 8>), grid, dim3(256), 0, s, a, t, plan.splits, (int)plan.part, parts);
-        if (plan.splits > 1) hipLaunchKernelGGL(top_join_kernel<T>, dim3(blocks_for(a.rows)), dim3(256), 0, s, a, t, plan.splits, parts);
+        const auto launch = [&](auto threads, auto vectors) {
+            hipLaunchKernelGGL((top_rows_kernel<T, threads.value, vectors.value>), grid, dim3(threads.value), 0, s, a, t, plan.splits, (int)plan.part, parts);
+        };
+        const auto with = [&](auto threads) { plan.vectors == 4 ? launch(threads, std::integral_constant<int, 4>()) : launch(threads, std::integral_constant<int, 2>()); };
+        switch (plan.threads) {
+            case 64: launch(std::integral_constant<int, 64>(), std::integral_constant<int, 4>()); break;
+            case 128: launch(std::integral_constant<int, 128>(), std::integral_constant<int, 4>()); break;
+            case 256: with(std::integral_constant<int, 256>()); break;
+            default: with(std::integral_constant<int, 512>());
+        }
+        if (plan.splits > 1) hipLaunchKernelGGL(top_join_kernel<T>, dim3(blocks_for(a.rows)), dim3(kJoin), 0, s, a, t, plan.splits, parts);
     });
     return check_launch("top_rows_kernel");
 }

@@ -32,8 +32,8 @@ def check(z, k, temperature=1.0):
     others = s.values[:, k:] / temperature
     want = torch.logsumexp(others, 1) if others.size(1) else torch.full((len(flat),), -math.inf, dtype=torch.float64)
     got = rest.double().cpu().view(-1)
-    finite = torch.isfinite(want)
-    assert torch.equal(torch.isfinite(got), finite) and torch.equal(got[~finite], want[~finite])
+    finite = torch.isfinite(want.float())       # (a log-sum above fp32's largest number, such as 3e38 / 0.01, is rounded to infinity)
+    assert torch.equal(torch.isfinite(got), finite) and torch.equal(got[~finite], want.float().double()[~finite])
     assert ((got - want).abs()[finite] <= 2 * (z.size(-1) / 64 + 128) * U + 2 * U * want.abs()[finite]).all()
     return values, classes, rest
 
@@ -102,6 +102,20 @@ def test_the_largest_far_above_the_others(classes):
     z[3, 4], z[3, 8] = 0.0, 1e30
     check(z, 2)
     check(z, 2, 0.01)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("classes", [9, 500, 20000, 140000])
+def test_values_of_any_size(classes, dtype):
+    """Rows around any number, and rows of two numbers of one size: what is left is a few values near the ends of their spacing."""
+    z = make(14, classes, dtype, classes).float()
+    for r, size in enumerate((1e3, 1e5, 1e7, 3e8, 1e10, 1e20, 3e38)):
+        z[2 * r] = torch.where(torch.arange(classes, device="cuda") % 3 == 0, -size, size)
+        z[2 * r + 1] = (z[2 * r + 1] * size / 1e4 if size < 1e38 else 0) - size
+    z = z.to(dtype)
+    check(z, 2)
+    check(z, 5, 0.01)
+    check(z, 2, 100.0)
 
 
 @pytest.mark.parametrize("classes", [10, 1000, 30000])
