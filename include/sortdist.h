@@ -411,15 +411,17 @@ typedef struct {
  * all others: divergences[r] = sum_j q_j (log q_j - log p_j) (terms with q_j = 0 are 0); 0 for rows that do not count: those without an
  * entry, and those whose entries and rest are all -inf.  loss = weight temperature^2 mean over the rows that count (0 where there are none).
  * A class in several entries is one class.  stats (rows, 2), entries (rows, k) and scale (1), all or none NULL, are what sd_distill_gradient
- * needs; scratch: sd_distill_scratch() floats (host only, -1 for what would be refused), 16-byte aligned, any contents. */
+ * needs.  Where sd_distill_fuses(rows) is 1, `grad` may be given (else NULL): it receives the gradient for an upstream gradient of 1, and the logits
+ * are read once less.  scratch: sd_distill_scratch() floats (host only, -1 for what would be refused), 16-byte aligned, any contents. */
 int64_t sd_distill_scratch(const sd_logit_rows* rows, int64_t k);
+int sd_distill_fuses(const sd_logit_rows* rows);
 int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, double weight, float* stats, float* entries,
-                    float* scale, float* loss, float* divergences, float* scratch, sd_stream_t stream);
+                    float* scale, void* grad, float* loss, float* divergences, float* scratch, sd_stream_t stream);
 
 /* grad = scale scale2 times the gradient of the sum of divergences by logit / temperature, rows of `classes` values one behind the other in the
- * logits' type; scale2 (one float on the device) may be NULL. */
+ * logits' type; scale2 (one float on the device) may be NULL.  With unless_one nothing is written where *scale2 is 1. */
 int sd_distill_gradient(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, const float* stats, const float* entries,
-                        const float* scale, const float* scale2, void* grad, sd_stream_t stream);
+                        const float* scale, const float* scale2, int unless_one, void* grad, sd_stream_t stream);
 
 /* What constrains the choice of a class.  Rows of the history, the bias and the allowed classes lie as those of the logits, (r / inner) *
  * outer + (r % inner) * inner entries behind their pointer; strides may be 0.

@@ -85,8 +85,8 @@ SIGNATURES = {
     "sd_policy_loss": [_R, _F, _F, _l, _l, _F, _d, _d, _d, _F, _F, _F, _F, _F, _F, _F, _S],
     "sd_label_gradient": [_R, _F, _F, _F, _F, _i, _F, _S],
     "sd_top_logits": [_Z, _l, _d, _F, _I, _F, _F, _S],
-    "sd_distill_loss": [_Z, _T, _d, _d, _F, _F, _F, _F, _F, _F, _S],
-    "sd_distill_gradient": [_Z, _T, _d, _F, _F, _F, _F, _F, _S],
+    "sd_distill_loss": [_Z, _T, _d, _d, _F, _F, _F, _F, _F, _F, _F, _S],
+    "sd_distill_gradient": [_Z, _T, _d, _F, _F, _F, _F, _i, _F, _S],
     "sd_constrain_logits": [_Z, _C, _F, _S],
     "sd_constrain_gradient": [_Z, _C, _F, _F, _S],
     "sd_dropout": [_F, _F, _F, _i, _l, _d, _u, _I, _F, _F, _F, _S],
@@ -111,6 +111,7 @@ _OTHER = {
     "sd_label_scratch": ([_R, _i], _l),
     "sd_top_scratch": ([_Z, _l], _l),
     "sd_distill_scratch": ([_Z, _l], _l),
+    "sd_distill_fuses": ([_Z], _i),
     "sd_policy_fuses": ([_R], _i),
 }
 

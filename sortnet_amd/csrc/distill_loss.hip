@@ -4,17 +4,16 @@
 // the divergence is D = sum_j q_j (log q_j - log p_j) + q_r (log q_r - log p_r), the loss weight T^2 times the mean of D, and
 //   d D / d (z[v] / T) = p_v - sum of the q_j with c_j = v   for a class of an entry,   (p_r - q_r) exp(z[v] / T) / S   for another one.
 // S is formed without the entries' classes, not as a difference, so that what the student gives the others keeps its digits however small it is.
-// There are few outcomes per row: they are in 64 bits.  Both passes are bound by the bytes of the logits, and by the launches where there are few.
+// There are few outcomes per row: they are in 64 bits, as three sums over the entries (Sums) that need no S, so that what is left when S is there is a few
+// numbers per row.  Both passes are bound by the bytes of the logits, and by the launches where there are few.
 // A class that stands in several entries is one class: it counts once in p and takes the sum of their q.
 // All sums have a fixed order: results are the same in every call.
 #include <climits>
-#include <type_traits>
 #include "label_rows.h"
 
 namespace sd {
 
 constexpr int kMostEntries = SD_MOST_TOP;   // of a row: one per work-item of a workgroup
-constexpr int kVectors = 8;                 // 16-byte vectors of a long row that a work-item holds at a time
 static_assert(kMostEntries <= 256, "a work-item per entry");
 
 // The teacher's rows
@@ -48,100 +47,146 @@ struct Outcome {
     uint32_t* ticket;           // cleared for the kernel of sums behind this one
 };
 
+struct Slopes {
+    const float2* stats;
+    const float* entries;
+    const float *scale, *scale2;    // one number each that all is multiplied by (scale2 may be null)
+    void* grad;                     // rows one behind the other
+    bool unless_one;                // nothing is done where *scale2 is 1
+    __device__ __forceinline__ float by() const { return scale2 ? *scale * *scale2 : *scale; }
+};
+
 struct Others { float top; double sum; };     // of the classes in no entry: sum of exp((z - top) / T)
 
-// What makes a row count, of one of its entries: 1 for an entry, 2 for one that is not -inf.  A row counts, and is read, that has an entry and an entry or
-// a rest above -inf.
-__device__ __forceinline__ int says(const Lists& l, int64_t at) { return l.cls(at) < 0 ? 0 : l.value(at) != -INFINITY ? 3 : 1; }
+// ---- the outcomes of a row -------------------------------------------------------------------------------------------------
+// An entry: its class (negative: none), the teacher's logit and the student's.  `said`: 1 for an entry, 2 for one that is above -inf; a row counts, and is read, that
+// has an entry and an entry or a rest above -inf.
+struct Entry { int64_t cls; float t, z; };
+__device__ __forceinline__ int said(int64_t cls, float t) { return cls < 0 ? 0 : t != -INFINITY ? 3 : 1; }
 
-// The end of row r by a group of 2^shift lanes of a wavefront, all of which call it.  repeats: a class may stand in several entries.
-// Returns what stats receives.
-template <class T> __device__ __forceinline__ float2 finish_row(const LogitRows& a, const Lists& l, const Temper& t, const Outcome& e, int64_t r, Others o, bool repeats,
-                                                              int lane, int shift) {
-    const int lanes = 1 << shift;
-    const T* z = row_start<T>(a, r);
-    float most_t = -INFINITY, most_z = -INFINITY, any = 0.f, live = 0.f, bad = 0.f;
-    for (int j = lane; j < l.k; j += lanes) {
-        const int64_t c = l.cls(r * l.k + j);
-        if (c < 0) continue;
-        const float v = l.value(r * l.k + j);
-        any = 1.f;
-        if (v != -INFINITY) live = 1.f;
-        most_t = fmaxf(most_t, v);
-        if (c >= a.classes || v != v) { bad = 1.f; continue; }
-        const float u = Elem<T>::get(z[c]);
-        most_z = fmaxf(most_z, u);
-        if (u != u) bad = 1.f;
-    }
-    most_t = group_max(most_t, shift); most_z = group_max(most_z, shift); any = group_max(any, shift); live = group_max(live, shift);
-    const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
-    if (rest != rest || o.sum != o.sum) bad = 1.f;
-    bad = group_max(bad, shift);
-    const double am = fmax((double)most_t * t.inverse, rest);
-    if (any == 0.f || (live == 0.f && rest == -INFINITY)) {     // (see says)
-        if (e.entries)
-            for (int j = lane; j < l.k; j += lanes) e.entries[r * l.k + j] = 0.f;
-        if (lane == 0) {
-            e.divergences[r] = 0.f;
-            e.kept[r] = 0.f;
-            if (e.stats) e.stats[r] = make_float2(0.f, 0.f);
-        }
-        return make_float2(0.f, 0.f);
-    }
-    // the student's logits relative to the largest of all (beside it, however large, the logarithm of a sum keeps its digits)
-    const double base = (double)fmaxf(most_z, finite(o.top));
-    const auto tempered = [&](float u) { return ((double)u - base) * t.inverse; };
-    const double log_s = o.sum > 0.0 ? log(o.sum) + tempered(finite(o.top)) : -INFINITY;
-    const double um = fmax(tempered(most_z), log_s);
-    // whether an entry before j has its class
-    const auto repeated = [&](int j, int64_t c) {
-        if (repeats)
-            for (int i = 0; i < j; i++)
-                if (l.cls(r * l.k + i) == c) return true;
-        return false;
-    };
-    double sum_t = 0.0, sum_z = 0.0;
-    for (int j = lane; j < l.k; j += lanes) {
-        const int64_t c = l.cls(r * l.k + j);
-        if (c < 0 || c >= a.classes) continue;
-        sum_t += exp((double)l.value(r * l.k + j) * t.inverse - am);
-        if (!repeated(j, c)) sum_z += exp(tempered(Elem<T>::get(z[c])) - um);
-    }
-    sum_t = group_total(sum_t, shift) + exp(rest - am);
-    sum_z = group_total(sum_z, shift) + exp(log_s - um);
-    if (bad != 0.f) sum_z = __builtin_nan("");
-    const double log_t = log(sum_t), log_z = log(sum_z);
-    double divergence = 0.0;
-    for (int j = lane; j < l.k; j += lanes) {
-        const int64_t c = l.cls(r * l.k + j);
-        float slope = 0.f;
-        if (c >= 0) {
-            const bool inside = c < a.classes;
-            const double at = (double)l.value(r * l.k + j) * t.inverse - am - log_t, az = (inside ? tempered(Elem<T>::get(z[c])) : 0.0) - um - log_z;
-            double q = exp(at);
-            if (q != 0.0) divergence += q * (at - az);
-            if (repeats) {      // every entry of a class gets the same slope
-                q = 0.0;
-                for (int i = 0; i < l.k; i++)
-                    if (l.cls(r * l.k + i) == c) q += exp((double)l.value(r * l.k + i) * t.inverse - am - log_t);
-            }
-            slope = (float)(exp(az) - q);
-        }
-        if (e.entries) e.entries[r * l.k + j] = slope;
-    }
-    divergence = group_total(divergence, shift);
-    const double at = rest - am - log_t, az = log_s - um - log_z, q = exp(at);
-    if (q != 0.0) divergence += q * (at - az);
-    const float2 stats = make_float2(finite(o.top), o.sum > 0.0 || bad != 0.f ? (float)((exp(az) - q) / o.sum) : 0.f);
-    if (lane == 0) {
-        e.divergences[r] = (float)(divergence + (sum_z != sum_z ? sum_z : 0.0));
-        e.kept[r] = 1.f;
-        if (e.stats) e.stats[r] = stats;
-    }
-    return stats;
+// over the entries: of the teacher's weights w = exp((t - most_t) / T), of the student's exp((z - base) / T), each class once, and of w times the difference of the two
+// exponents
+struct Sums { double w, p, a; };
+__device__ __forceinline__ void add_entry(Sums& s, const Entry& e, float most_t, float base, bool first, const Temper& t) {
+    const double at = ((double)e.t - (double)most_t) * t.inverse, az = ((double)e.z - (double)base) * t.inverse, w = exp(at);
+    s.w += w;
+    if (w != 0.0) s.a += w * (at - az);
+    if (first) s.p += exp(az);
 }
 
-// ---- a workgroup reads a row ---------------------------------------------------------------------------------------------------
+// What a row comes to: with all in exponents relative to most_t and base (of rows where no entry is above -inf, to 0), D = (sum_a + w_r (rest - log S)) / W - log W +
+// log P, W and P being the sums with the others.
+struct Row { double divergence, per_w, per_p; float factor; };      // per_w = 1 / W, per_p = 1 / P; factor = (p_r - q_r) / S
+__device__ __forceinline__ Row finish_row(const Sums& s, float most_t, float base, double rest, const Others& o, bool bad, const Temper& t) {
+    const double log_s = o.sum > 0.0 ? log(o.sum) + ((double)finite(o.top) - (double)base) * t.inverse : -INFINITY;
+    // the rest may lie far above the entries: relative to the larger of the two
+    const double left = rest - (double)most_t * t.inverse, up = left > 0.0 ? left : 0.0;
+    const double w_r = exp(left - up), scale = up > 0.0 ? exp(-up) : 1.0, w = s.w * scale + w_r;
+    const double p_r = exp(log_s), p = s.p + p_r;
+    double a = scale != 0.0 ? s.a * scale - up * (s.w * scale) : 0.0;
+    if (w_r != 0.0) a += w_r * (left - up - log_s);
+    Row r{a / w - log(w) + log(p), scale / w, 1.0 / p, 0.f};
+    if (bad) r.divergence = r.per_p = __builtin_nan("");
+    if (o.sum > 0.0 || bad) r.factor = (float)((p_r * r.per_p - w_r / w) / o.sum);
+    return r;
+}
+__device__ __forceinline__ double teacher_share(const Row& r, float v, float most_t, const Temper& t) { return exp(((double)v - (double)most_t) * t.inverse) * r.per_w; }
+__device__ __forceinline__ double student_share(const Row& r, float z, float base, const Temper& t) { return exp(((double)z - (double)base) * t.inverse) * r.per_p; }
+
+// d D / d (z / T) of the class of an entry; q: of its entry alone, unless `repeats`: a class may stand in several
+__device__ __forceinline__ float entry_slope(const Lists& l, int64_t r, const Entry& e, const Row& row, float most_t, float base, bool repeats, const Temper& t) {
+    double q = 0.0;
+    if (repeats) {
+        for (int i = 0; i < l.k; i++)
+            if (l.cls(r * l.k + i) == e.cls) q += teacher_share(row, l.value(r * l.k + i), most_t, t);
+    } else q = teacher_share(row, e.t, most_t, t);
+    return (float)(student_share(row, e.z, base, t) - q);
+}
+// whether no entry before j has its class
+__device__ __forceinline__ bool first_of(const Lists& l, int64_t r, int j, int64_t cls) {
+    for (int i = 0; i < j; i++)
+        if (l.cls(r * l.k + i) == cls) return false;
+    return true;
+}
+
+// The outcomes of row r by a group of 2^shift lanes of a wavefront, all of which call it, with what they give for the row.  `skip`: the row does not count.
+template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& a, const Lists& l, const Temper& t, const Outcome& e, int64_t r, const Others& o, bool skip, bool repeats,
+                                                              int lane, int shift, float2& stats, float& most_t, float& base, Row& row) {
+    const int lanes = 1 << shift;
+    const T* z = row_start<T>(a, r);
+    stats = make_float2(0.f, 0.f);
+    row = Row{0.0, 0.0, 0.0, 0.f};
+    most_t = base = 0.f;
+    if (!skip) {
+        float bad = 0.f;
+        most_t = base = -INFINITY;
+        for (int j = lane; j < l.k; j += lanes) {
+            const int64_t c = l.cls(r * l.k + j);
+            if (c < 0) continue;
+            const float v = l.value(r * l.k + j), u = c < a.classes ? Elem<T>::get(z[c]) : __builtin_nanf("");
+            most_t = fmaxf(most_t, v);
+            base = fmaxf(base, u);
+            if (v != v || u != u) bad = 1.f;
+        }
+        const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
+        if (rest != rest || o.sum != o.sum) bad = 1.f;
+        most_t = group_max(most_t, shift); base = group_max(base, shift); bad = group_max(bad, shift);
+        base = fmaxf(base, finite(o.top));
+        if (most_t == -INFINITY) most_t = 0.f;
+        Sums s{0.0, 0.0, 0.0};
+        for (int j = lane; j < l.k; j += lanes) {
+            const int64_t c = l.cls(r * l.k + j);
+            if (c < 0 || c >= a.classes) continue;
+            add_entry(s, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, most_t, base, !repeats || first_of(l, r, j, c), t);
+        }
+        s.w = group_total(s.w, shift); s.p = group_total(s.p, shift); s.a = group_total(s.a, shift);
+        row = finish_row(s, most_t, base, rest, o, bad != 0.f, t);
+        stats = make_float2(finite(o.top), row.factor);
+    }
+    if (lane == 0) {
+        e.divergences[r] = (float)row.divergence;
+        e.kept[r] = skip ? 0.f : 1.f;
+        if (e.stats) e.stats[r] = stats;
+    }
+}
+
+// The entries of row r, once its outcomes are known: f gets each one's class (inside the row) and slope; the slopes are kept for a later gradient.
+template <class T, class F> __device__ __forceinline__ void each_slope(const LogitRows& a, const Lists& l, const Temper& t, const Outcome& e, int64_t r, bool skip, bool repeats, int lane, int shift,
+                                                                     float most_t, float base, const Row& row, F&& f) {
+    const T* z = row_start<T>(a, r);
+    for (int j = lane; j < l.k; j += 1 << shift) {
+        const int64_t c = skip ? -1 : l.cls(r * l.k + j);
+        const bool inside = c >= 0 && c < a.classes;
+        const float slope = inside ? entry_slope(l, r, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, row, most_t, base, repeats, t) : 0.f;
+        if (e.entries) e.entries[r * l.k + j] = slope;
+        if (inside) f(c, slope);
+    }
+}
+
+// whether row r counts, by a group of lanes that all call it
+__device__ __forceinline__ bool counts(const Lists& l, int64_t r, int lane, int shift) {
+    float entry = 0.f, live = l.rest && l.rest[r] != -INFINITY ? 1.f : 0.f;
+    for (int j = lane; j < l.k; j += 1 << shift) {
+        const int64_t c = l.cls(r * l.k + j);
+        const int what = c < 0 ? 0 : said(c, l.value(r * l.k + j));
+        if (what) entry = 1.f;
+        if (what & 2) live = 1.f;
+    }
+    return group_max(entry, shift) != 0.f && group_max(live, shift) != 0.f;
+}
+
+// (of the lanes of a wavefront, which go through these in step)
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// N values become those of a row's gradient
+template <class T, int N> __device__ __forceinline__ void gradient_values(float (&f)[N], float top, float w, const Temper& t) {
+    #pragma unroll
+    for (int i = 0; i < N; i++) f[i] = exp_stored<T>(f[i] - top, t) * w;
+}
+
 template <int N> __device__ __forceinline__ void take(const float (&f)[N], float& top, double& sum, const Temper& t) {
     float m = top, g[N];
     #pragma unroll
@@ -153,66 +198,484 @@ template <int N> __device__ __forceinline__ void take(const float (&f)[N], float
     top = m;
 }
 
-template <class T> __global__ void __launch_bounds__(256) distill_rows_kernel(LogitRows a, Lists l, Temper t, Outcome e) {
-    constexpr int V = Elem<T>::kVec, kWords = kVectors * V / 32, kSpan = 256 * kVectors * V;
-    __shared__ uint32_t marks[256][kWords];
-    __shared__ Others waves[4];
-    __shared__ int repeats;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const T* p = row_start<T>(a, r);
-        const int64_t cls = (int)threadIdx.x < l.k ? l.cls(r * l.k + threadIdx.x) : -1;
+// -inf in the place of those values of a vector whose bit is set
+template <class T> __device__ __forceinline__ u32x4 without(u32x4 v, uint32_t bits) {
+    const u32x4 none = Elem<T>::splat(Elem<T>::put(-INFINITY));
+    #pragma unroll
+    for (int w = 0; w < 4; w++) {
+        if constexpr (sizeof(T) == 4) v[w] = bits >> w & 1 ? none[w] : v[w];
+        else {
+            v[w] = bits >> (2 * w) & 1 ? (v[w] & 0xffff0000u) | (none[w] & 0xffffu) : v[w];
+            v[w] = bits >> (2 * w + 1) & 1 ? (v[w] & 0xffffu) | (none[w] & 0xffff0000u) : v[w];
+        }
+    }
+    return v;
+}
+
+// ---- short rows ------------------------------------------------------------------------------------------------------------
+// Lanes that hold a row mark the entries' classes for each other; a value of the row that is marked becomes -inf.
+template <class T, int NV> __device__ __forceinline__ bool take_out(HeldRow<T, NV>& row, const Lists& l, int64_t r, uint32_t (&marks)[256][2]) {
+    constexpr int V = Elem<T>::kVec;
+    const int first = (int)threadIdx.x - row.lane;
+    uint32_t* own = marks[threadIdx.x];
+    own[0] = own[1] = 0u;
+    wave_fence();
+    float twice = 0.f;
+    const auto mark = [&](int i, int e) {
+        const int bit = (i >> row.shift) * V + e;
+        const uint32_t one = 1u << (bit & 31);
+        return atomicOr(&marks[first + (i & ((1 << row.shift) - 1))][bit >> 5], one) & one;
+    };
+    for (int j = row.lane; j < l.k; j += 1 << row.shift) {
+        const int64_t c64 = l.cls(r * l.k + j);
+        if (c64 < 0 || c64 >= row.n) continue;
+        const int c = (int)c64, i = c / V, start = row.n >= V ? row.column(i) : 0;
+        if (mark(i, c - start)) twice = 1.f;
+        // (the last vector has some of the values of the one before it)
+        if (row.n >= V && i != row.vecs - 1 && c >= row.n - V) mark(row.vecs - 1, c - (row.n - V));
+    }
+    wave_fence();
+    const uint32_t low = own[0], high = own[1];
+    if (low | high) {
+        #pragma unroll
+        for (int k = 0; k < NV; k++) {
+            const uint32_t bits = (k * V < 32 ? low >> (k * V & 31) : high >> (k * V & 31)) & ((1u << V) - 1u);
+            if (bits) row.v[k] = without<T>(row.v[k], bits);
+        }
+    }
+    return group_max(twice, row.shift) != 0.f;
+}
+
+template <class T, int NV> __device__ __forceinline__ Others others_of(const HeldRow<T, NV>& row, const Temper& t) {
+    constexpr int V = Elem<T>::kVec;
+    float top = -INFINITY;
+    #pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (row.index(k) < row.vecs) {
+            float f[V];
+            Elem<T>::unpack(row.v[k], f);
+            #pragma unroll
+            for (int i = 0; i < V; i++) top = fmaxf(top, f[i]);
+        }
+    top = group_max(top, row.shift);
+    const float b = finite(top);
+    double s = 0.0;
+    #pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (row.index(k) < row.vecs) {
+            const int past = row.n >= V ? row.index(k) * V - row.column(row.index(k)) : 0;      // values that the vector before has, too
+            float f[V];
+            Elem<T>::unpack(row.v[k], f);
+            #pragma unroll
+            for (int i = 0; i < V; i++) f[i] = exp_at(f[i] - b, t);
+            if (past > 0) {
+                #pragma unroll
+                for (int i = 0; i < V; i++) f[i] = i < past ? 0.f : f[i];
+            }
+            s += (double)tree(f);
+        }
+    return Others{top, group_total(s, row.shift)};
+}
+
+// the row's part of a gradient, the entries' classes left to be stored
+template <class T, int NV> __device__ __forceinline__ void store_gradient(const HeldRow<T, NV>& row, T* q, float2 stats, float by, bool far, const Temper& t) {
+    constexpr int V = Elem<T>::kVec;
+    #pragma unroll
+    for (int k = 0; k < NV; k++)
+        if (row.index(k) < row.vecs) {
+            const int c = row.n >= V ? row.column(row.index(k)) : 0;
+            float f[V];
+            if (stats.y == 0.f) {
+                #pragma unroll
+                for (int i = 0; i < V; i++) f[i] = 0.f;
+            } else {
+                Elem<T>::unpack(row.v[k], f);
+                gradient_values<T>(f, stats.x, stats.y * by, t);
+            }
+            if (row.n >= V) {
+                if (far) put_stream16(q + c, Elem<T>::pack(f));
+                else store16(q + c, Elem<T>::pack(f));
+            } else {
+                #pragma unroll
+                for (int i = 0; i < V; i++)
+                    if (i < row.n) q[i] = Elem<T>::put(f[i]);
+            }
+        }
+}
+
+// Bytes of a FUSED short row from which its gradient is stored past the caches (as in label_loss.hip).
+constexpr int kStreamRow = 512;
+
+// FUSED: the gradient leaves with the row (its scale is known before)
+template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) distill_short_kernel(LogitRows a, Lists l, Temper t, Outcome e, Slopes g, int shift, int64_t row0) {
+    __shared__ uint32_t marks[256][2];
+    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
+    HeldRow<T, NV> row;
+    row.n = (int)a.classes; row.shift = shift;
+    row.lane = threadIdx.x & ((1 << shift) - 1);
+    row.vecs = (row.n + Elem<T>::kVec - 1) / Elem<T>::kVec;
+    const int64_t r = row0 + (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
+    if (r >= a.rows) return;
+    const bool skip = FUSED ? e.kept[r] == 0.f : !counts(l, r, row.lane, shift);
+    Others o{-INFINITY, 0.0};
+    bool repeats = false;
+    if (!skip) {
+        row.load(row_start<T>(a, r));
+        repeats = take_out(row, l, r, marks);
+        o = others_of(row, t);
+    }
+    float2 stats;
+    float most_t, base;
+    Row end;
+    outcomes_of<T>(a, l, t, e, r, o, skip, repeats, row.lane, shift, stats, most_t, base, end);
+    T* q = static_cast<T*>(g.grad) + r * a.classes;
+    const float by = FUSED ? *g.scale : 0.f;
+    if (FUSED) {
+        store_gradient(row, q, stats, by, row.n * (int)sizeof(T) >= kStreamRow, t);
+        wave_fence();       // (the entries' values stand where these stood)
+    }
+    if (FUSED || e.entries)
+        each_slope<T>(a, l, t, e, r, skip, repeats, row.lane, shift, most_t, base, end, [&](int64_t c, float slope) { if (FUSED) q[c] = Elem<T>::put(slope * by); });
+}
+
+template <class T, int NV> __global__ void __launch_bounds__(256) distill_short_gradient_kernel(LogitRows a, Lists l, Temper t, Slopes g, int shift) {
+    if (g.unless_one && *g.scale2 == 1.f) return;
+    const int per = 256 >> shift;
+    HeldRow<T, NV> row;
+    row.n = (int)a.classes; row.shift = shift;
+    row.lane = threadIdx.x & ((1 << shift) - 1);
+    row.vecs = (row.n + Elem<T>::kVec - 1) / Elem<T>::kVec;
+    const float by = g.by();
+    for (int64_t r = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); r < a.rows; r += (int64_t)gridDim.x * per) {
+        const float2 stats = g.stats[r];
+        if (stats.y != 0.f) row.load(row_start<T>(a, r));
+        T* q = static_cast<T*>(g.grad) + r * a.classes;
+        store_gradient(row, q, stats, by, false, t);
+        wave_fence();
+        for (int j = row.lane; j < l.k; j += 1 << shift) {
+            const int64_t c = l.cls(r * l.k + j);
+            if (c >= 0 && c < a.classes) q[c] = Elem<T>::put(g.entries[r * l.k + j] * by);
+        }
+    }
+}
+
+// ---- long rows ---------------------------------------------------------------------------------------------------------------
+// Marks of the entries' classes among the vectors that a workgroup holds, by the work-item that holds each: NV vectors, the k-th vector item + k THREADS.
+template <class T, int NV, int THREADS> struct Marks {
+    static constexpr int V = Elem<T>::kVec, kWords = (NV * V + 31) / 32;
+    uint32_t words[THREADS][kWords];
+    int repeats;
+    __device__ __forceinline__ void clear() {
+        #pragma unroll
+        for (int w = 0; w < kWords; w++) words[threadIdx.x][w] = 0u;
         if (threadIdx.x == 0) repeats = 0;
+    }
+    __device__ __forceinline__ void mark(int at) {      // at: the class behind those before the vectors
+        const int vec = at / V, bit = vec / THREADS * V + at % V;
+        const uint32_t one = 1u << (bit & 31);
+        if (atomicOr(&words[vec % THREADS][bit >> 5], one) & one) repeats = 1;
+    }
+    __device__ __forceinline__ uint32_t bits(int k) const { return words[threadIdx.x][k * V / 32] >> (k * V & 31) & ((1u << V) - 1u); }
+};
+
+// The workgroup holds a row in its registers, at most 16 vectors per work-item, and an entry per work-item.  FUSED: the logits are read once and the gradient leaves
+// with the row.  FAR: logits that the last-level cache cannot hold are read past it.
+// A row per workgroup and no loop over them: the constants of the 64-bit functions would be kept in registers that the row needs.
+template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __launch_bounds__(THREADS, 4) distill_held_kernel(LogitRows a, Lists l, Temper t, Outcome e, Slopes g, int64_t row0) {
+    constexpr int V = Elem<T>::kVec, WAVES = THREADS / 64, kChunk = (NV == 16 ? 8 : 16) / V;
+    __shared__ Marks<T, NV + 1, THREADS> marks;       // (one more: the values behind the last whole vector)
+    __shared__ float maxima[WAVES][4];
+    __shared__ double sums[WAVES][4];
+    __shared__ Row end;
+    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
+    const int n = (int)a.classes, full = n / V, rest_at = full * V + (int)threadIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const T lowest = Elem<T>::put(-INFINITY);
+    const float by = FUSED ? *g.scale : 0.f;
+    const int64_t r = a.rows - 1 - (row0 + blockIdx.x);     // (the producer's last rows may be in the caches)
+    T* q = static_cast<T*>(g.grad) + r * a.classes;
+    const bool own = (int)threadIdx.x < l.k;
+    bool skip;
+    int64_t cls = -1;
+    float value = -INFINITY;
+    if (FUSED) skip = e.kept[r] == 0.f;
+    if (own && !(FUSED && skip)) { cls = l.cls(r * l.k + threadIdx.x); value = l.value(r * l.k + threadIdx.x); }
+    if (!FUSED) {
+        const int what = said(cls, value);
+        const bool entry = __syncthreads_or(what & 1), live = __syncthreads_or(what & 2);
+        skip = !entry || !(live || (l.rest && l.rest[r] != -INFINITY));
+    }
+    if (skip) {     // (the whole workgroup's)
+        if (own && e.entries) e.entries[r * l.k + threadIdx.x] = 0.f;
+        if (threadIdx.x == 0) {
+            e.divergences[r] = 0.f;
+            e.kept[r] = 0.f;
+            if (e.stats) e.stats[r] = make_float2(0.f, 0.f);
+        }
+        if (FUSED) clear_row(q, n, THREADS);
+        return;
+    }
+    const T* p = row_start<T>(a, r);
+    u32x4 v[NV];
+    const u32x4 none = Elem<T>::splat(lowest);
+    T last = lowest;
+    #pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const int i = (int)threadIdx.x + k * THREADS;
+        v[k] = none;
+        if (i < full) v[k] = FAR ? stream16(p + i * V) : load16(p + i * V);
+    }
+    if (rest_at < n) last = p[rest_at];
+    // the entry, while the row is on its way
+    const bool inside = cls >= 0 && cls < a.classes;
+    Entry mine{cls, value, -INFINITY};
+    if (inside) mine.z = Elem<T>::get(p[cls]);
+    const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
+    marks.clear();
+    __syncthreads();
+    if (inside) {
+        const int c = (int)cls;
+        // the values behind the last whole vector are held by the first work-items, one each, as the first value of a vector of their own
+        marks.mark(c < full * V ? c : (NV * THREADS + (c - full * V)) * V);
+    }
+    __syncthreads();
+    const bool repeats = marks.repeats != 0;
+    float top = -INFINITY;
+    double sum = 0.0;
+    #pragma unroll
+    for (int k = 0; k < NV; k++) {
+        const uint32_t listed = marks.bits(k);
+        if (listed) v[k] = without<T>(v[k], listed);
+    }
+    if (marks.bits(NV) & 1u) last = lowest;
+    #pragma unroll
+    for (int c = 0; c < NV; c += kChunk) {
+        float f[kChunk * V];
+        #pragma unroll
+        for (int k = 0; k < kChunk; k++) Elem<T>::unpack(v[c + k], reinterpret_cast<float (&)[V]>(f[k * V]));
+        take(f, top, sum, t);
+    }
+    float f1[1] = {Elem<T>::get(last)};
+    take(f1, top, sum, t);
+    // all work-items': the largest of the others, of the teacher's and of the student's entries, and whether something is wrong
+    bool odd = sum != sum || rest != rest || (cls >= 0 && (!inside || value != value || mine.z != mine.z));
+    {
+        const float m0 = group_max(top, 6), m1 = group_max(inside ? value : -INFINITY, 6), m2 = group_max(mine.z, 6);
+        if (lane == 0) { maxima[wave][0] = m0; maxima[wave][1] = m1; maxima[wave][2] = m2; }
+    }
+    odd = __syncthreads_or(odd);
+    constexpr int kShift = WAVES == 4 ? 2 : WAVES == 8 ? 3 : 4;      // (the wavefronts' in the lanes of each group of so many)
+    const float* theirs = maxima[lane & (WAVES - 1)];
+    const float all = group_max(theirs[0], kShift);
+    float most_t = group_max(theirs[1], kShift), base = fmaxf(group_max(theirs[2], kShift), finite(all));
+    if (most_t == -INFINITY) most_t = 0.f;
+    Sums s{0.0, 0.0, 0.0};
+    if (inside) add_entry(s, mine, most_t, base, !repeats || first_of(l, r, threadIdx.x, cls), t);
+    sum = wave_total(sum * (double)exp_at(finite(top) - finite(all), t));
+    if (64 * wave < l.k) { s.w = wave_total(s.w); s.p = wave_total(s.p); s.a = wave_total(s.a); }
+    if (lane == 0) { sums[wave][0] = sum; sums[wave][1] = s.w; sums[wave][2] = s.p; sums[wave][3] = s.a; }
+    __syncthreads();
+    if (wave == 0) {
+        double total[4];
+        #pragma unroll
+        for (int k = 0; k < 4; k++) total[k] = group_total(sums[lane & (WAVES - 1)][k], kShift);
+        const Row row = finish_row(Sums{total[1], total[2], total[3]}, most_t, base, rest, Others{all, total[0]}, odd, t);
+        if (lane == 0) {
+            end = row;
+            e.divergences[r] = (float)row.divergence;
+            e.kept[r] = 1.f;
+            if (e.stats) e.stats[r] = make_float2(finite(all), row.factor);
+        }
+    }
+    if (!FUSED && !e.entries) return;
+    __syncthreads();
+    const Row row = end;
+    float slope = 0.f;
+    if (inside) slope = entry_slope(l, r, mine, row, most_t, base, repeats, t);
+    if (own && e.entries) e.entries[r * l.k + threadIdx.x] = slope;
+    if (FUSED) {
+        if (row.factor == 0.f) clear_row(q, n, THREADS);
+        else {
+            // what was derived from the vectors is derived again: kept, it would be twice their registers
+            int item = threadIdx.x;
+            asm("" : "+v"(item));
+            #pragma unroll
+            for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
+            const float high = finite(all), w = row.factor * by;
+            #pragma unroll
+            for (int k = 0; k < NV; k++) {
+                const int i = item + k * THREADS;
+                float f[V];
+                Elem<T>::unpack(v[k], f);
+                gradient_values<T>(f, high, w, t);
+                if (i < full) put_stream16(q + i * V, Elem<T>::pack(f));
+            }
+            if (rest_at < n) {
+                float f[1] = {Elem<T>::get(last)};
+                gradient_values<T>(f, high, w, t);
+                q[rest_at] = Elem<T>::put(f[0]);
+            }
+        }
+        __syncthreads();        // (the entries' values stand where these stood)
+        if (inside) q[cls] = Elem<T>::put(slope * by);
+    }
+}
+
+// Rows that no workgroup can hold, and those of which there are few: parts of them, whose others distill_join_kernel joins.
+constexpr int kPartVectors = 8;
+template <class T> __global__ void __launch_bounds__(256) distill_part_kernel(LogitRows a, Lists l, Temper t, Outcome e, int splits, int64_t part, Others* parts, int* twice) {
+    constexpr int V = Elem<T>::kVec, kSpan = 256 * kPartVectors * V;
+    __shared__ Marks<T, kPartVectors, 256> marks;
+    __shared__ Others waves[4];
+    if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
+    for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
+        const int64_t r = b / splits, s = b - r * splits, from = s * part, until = a.classes - from < part ? a.classes : from + part;
+        const T* p = row_start<T>(a, r);
+        int64_t cls = -1;
+        float value = -INFINITY;
+        if ((int)threadIdx.x < l.k) { cls = l.cls(r * l.k + threadIdx.x); value = l.value(r * l.k + threadIdx.x); }
+        const int what = said(cls, value);
+        const bool entry = __syncthreads_or(what & 1), live = __syncthreads_or(what & 2);
         float top = -INFINITY;
         double sum = 0.0;
-        const int said = (int)threadIdx.x < l.k ? says(l, r * l.k + threadIdx.x) : 0;
-        const bool entry = __syncthreads_or(said & 1), live = __syncthreads_or(said & 2);
+        bool repeats = false;
         if (entry && (live || (l.rest && l.rest[r] != -INFINITY))) {
-            for (int64_t c0 = 0; c0 < a.classes; c0 += kSpan) {
+            for (int64_t c0 = from; c0 < until; c0 += kSpan) {
+                const int64_t n = until - c0;
+                u32x4 v[kPartVectors];
                 #pragma unroll
-                for (int w = 0; w < kWords; w++) marks[threadIdx.x][w] = 0u;
-                __syncthreads();
-                if (cls >= c0 && cls < c0 + kSpan && cls < a.classes) {
-                    const int at = (int)(cls - c0), vec = at / V, bit = vec / 256 * V + at % V;
-                    const uint32_t one = 1u << (bit & 31);
-                    if (atomicOr(&marks[vec % 256][bit >> 5], one) & one) repeats = 1;
-                }
-                __syncthreads();
-                #pragma unroll
-                for (int k = 0; k < kVectors; k++) {
-                    const int64_t c = c0 + (int64_t)(k * 256 + (int)threadIdx.x) * V;
-                    float f[V];
-                    if (c + V <= a.classes) Elem<T>::unpack(load16(p + c), f);
-                    else {
+                for (int k = 0; k < kPartVectors; k++) {
+                    const int c = (k * 256 + (int)threadIdx.x) * V;
+                    v[k] = Elem<T>::splat(Elem<T>::put(-INFINITY));
+                    if (c + V <= n) v[k] = load16(p + c0 + c);
+                    else if (c < n) {
+                        float f[V];
                         #pragma unroll
-                        for (int i = 0; i < V; i++) f[i] = c + i < a.classes ? Elem<T>::get(p[c + i]) : -INFINITY;
+                        for (int i = 0; i < V; i++) f[i] = c + i < n ? Elem<T>::get(p[c0 + c + i]) : -INFINITY;
+                        v[k] = Elem<T>::pack(f);
                     }
-                    const uint32_t listed = marks[threadIdx.x][k * V / 32] >> (k * V & 31);
-                    #pragma unroll
-                    for (int i = 0; i < V; i++) f[i] = listed >> i & 1 ? -INFINITY : f[i];
+                }
+                marks.clear();
+                __syncthreads();
+                if (cls >= c0 && cls < until && cls < c0 + kSpan) marks.mark((int)(cls - c0));
+                __syncthreads();
+                repeats |= marks.repeats != 0;
+                #pragma unroll
+                for (int k = 0; k < kPartVectors; k += 2) {
+                    float f[2 * V];
+                    Elem<T>::unpack(without<T>(v[k], marks.bits(k)), reinterpret_cast<float (&)[V]>(f[0]));
+                    Elem<T>::unpack(without<T>(v[k + 1], marks.bits(k + 1)), reinterpret_cast<float (&)[V]>(f[V]));
                     take(f, top, sum, t);
                 }
                 __syncthreads();
             }
         }
-        {   // all work-items' to the first wavefront
-            const float m = group_max(top, 6);
-            sum = group_total(sum * (double)exp_at(finite(top) - finite(m), t), 6);
-            if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = Others{m, sum};
-            __syncthreads();
-            if (threadIdx.x < 64) {
-                Others o{-INFINITY, 0.0};
-                for (int w = 0; w < 4; w++) o.top = fmaxf(o.top, waves[w].top);
-                for (int w = 0; w < 4; w++) o.sum += waves[w].sum * (double)exp_at(finite(waves[w].top) - finite(o.top), t);
-                finish_row<T>(a, l, t, e, r, o, repeats != 0, threadIdx.x, 6);
-            }
-            __syncthreads();
+        const float m = group_max(top, 6);
+        sum = wave_total(sum * (double)exp_at(finite(top) - finite(m), t));
+        if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = Others{m, sum};
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            Others o{-INFINITY, 0.0};
+            for (int w = 0; w < 4; w++) o.top = fmaxf(o.top, waves[w].top);
+            for (int w = 0; w < 4; w++) o.sum += waves[w].sum * (double)exp_at(finite(waves[w].top) - finite(o.top), t);
+            parts[b] = o;
+            twice[b] = repeats;
         }
+        __syncthreads();
+    }
+}
+
+// a wavefront per row
+template <class T> __global__ void __launch_bounds__(256) distill_join_kernel(LogitRows a, Lists l, Temper t, Outcome e, int splits, const Others* parts, const int* twice) {
+    const int lane = threadIdx.x & 63;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < a.rows; r += (int64_t)gridDim.x * 4) {
+        const bool skip = !counts(l, r, lane, 6);
+        float top = -INFINITY, repeats = 0.f;
+        for (int k = lane; k < splits; k += 64) {
+            top = fmaxf(top, parts[r * splits + k].top);
+            if (twice[r * splits + k]) repeats = 1.f;
+        }
+        top = group_max(top, 6);
+        double sum = 0.0;
+        for (int k = lane; k < splits; k += 64) sum += parts[r * splits + k].sum * (double)exp_at(finite(parts[r * splits + k].top) - finite(top), t);
+        const Others o{top, wave_total(sum)};
+        const bool twice_there = group_max(repeats, 6) != 0.f;
+        float2 stats;
+        float most_t, base;
+        Row end;
+        outcomes_of<T>(a, l, t, e, r, o, skip, twice_there, lane, 6, stats, most_t, base, end);
+        if (e.entries) each_slope<T>(a, l, t, e, r, skip, twice_there, lane, 6, most_t, base, end, [](int64_t, float) {});
+    }
+}
+
+// A workgroup writes `part` columns of a row's gradient, then those of its entries that lie there.
+template <class T> __global__ void __launch_bounds__(256) distill_long_gradient_kernel(LogitRows a, Lists l, Temper t, Slopes g, int splits, int64_t part) {
+    constexpr int V = Elem<T>::kVec, kUnroll = 4;
+    if (g.unless_one && *g.scale2 == 1.f) return;
+    const float by = g.by();
+    for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
+        const int64_t r = b / splits, c0 = (b - r * splits) * part, c1 = a.classes - c0 < part ? a.classes : c0 + part, full = c1 / V;
+        const float2 stats = g.stats[r];
+        const float w = stats.y * by;
+        const T* src = row_start<T>(a, r);
+        T* q = static_cast<T*>(g.grad) + r * a.classes;
+        const bool own = (int)threadIdx.x < l.k;
+        const int64_t cls = own ? l.cls(r * l.k + threadIdx.x) : -1;
+        const float slope = own ? g.entries[r * l.k + threadIdx.x] * by : 0.f;
+        for (int64_t i = c0 / V + threadIdx.x; i < full; i += kUnroll * 256) {
+            u32x4 v[kUnroll];
+            #pragma unroll
+            for (int k = 0; k < kUnroll; k++)
+                if (stats.y != 0.f && i + k * 256 < full) v[k] = load16(src + (i + k * 256) * V);
+            #pragma unroll
+            for (int k = 0; k < kUnroll; k++) {
+                if (i + k * 256 >= full) continue;
+                float f[V];
+                if (stats.y == 0.f) {
+                    #pragma unroll
+                    for (int m = 0; m < V; m++) f[m] = 0.f;
+                } else {
+                    Elem<T>::unpack(v[k], f);
+                    gradient_values<T>(f, stats.x, w, t);
+                }
+                put_stream16(q + (i + k * 256) * V, Elem<T>::pack(f));
+            }
+        }
+        for (int64_t j = full * V + threadIdx.x; j < c1; j += 256) q[j] = Elem<T>::put(stats.y == 0.f ? 0.f : exp_stored<T>(Elem<T>::get(src[j]) - stats.x, t) * w);
+        __syncthreads();        // (the entries' values stand where these stood)
+        if (cls >= c0 && cls < c1) q[cls] = Elem<T>::put(slope);
     }
 }
 
 // ---- the loss --------------------------------------------------------------------------------------------------------------------
-// loss = weight T^2 mean of the divergences over the rows that count (0 where there are none), scale = weight T / their number
+// Which rows count, before they are read: a wavefront per row; the workgroups' numbers of them to `counted`.
+__global__ void __launch_bounds__(256) distill_rows_that_count_kernel(Lists l, int64_t rows, float* kept, int* counted) {
+    __shared__ int waves[4];
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+    for (int64_t r = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)gridDim.x * 4) {
+        const bool here = counts(l, r, lane, 6);
+        if (lane == 0) kept[r] = here ? 1.f : 0.f;
+        n += here;
+    }
+    if (lane == 0) waves[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) counted[blockIdx.x] = waves[0] + waves[1] + waves[2] + waves[3];
+}
+// scale = factor / their number
+__global__ void __launch_bounds__(256) distill_scale_kernel(const int* counted, int blocks, double factor, float* scale) {
+    __shared__ int waves[4];
+    int n = 0;
+    for (int i = threadIdx.x; i < blocks; i += 256) n += counted[i];
+    for (int o = 32; o > 0; o >>= 1) n += __shfl_xor(n, o);
+    if ((threadIdx.x & 63) == 0) waves[threadIdx.x >> 6] = n;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        n = waves[0] + waves[1] + waves[2] + waves[3];
+        *scale = (float)(factor / (n > 1 ? n : 1));
+    }
+}
+
+// loss = weight T^2 mean of the divergences over the rows that count (0 where there are none), scale = weight T / their number (or null: it is there)
 struct Mean { const float *divergences, *kept; int64_t rows; double loss_factor, scale_factor; float *loss, *scale; double* parts; uint32_t* ticket; };
 __global__ void __launch_bounds__(1024) distill_mean_kernel(Mean m) {
     __shared__ double waves[16][2];
@@ -251,46 +714,12 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(Mean m) {
     }
 }
 
-// ---- the gradient ----------------------------------------------------------------------------------------------------------------
-struct Slopes { const float2* stats; const float* entries; const float *scale, *scale2; void* grad; };
-
-// A workgroup writes `part` columns of a row, then those of its entries that lie there.
-template <class T> __global__ void __launch_bounds__(256) distill_gradient_kernel(LogitRows a, Lists l, Temper t, Slopes g, int splits, int64_t part) {
-    constexpr int V = Elem<T>::kVec;
-    for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
-        const int64_t r = b / splits, c0 = (b - r * splits) * part, c1 = a.classes - c0 < part ? a.classes : c0 + part;
-        const float2 st = g.stats[r];
-        const float by = g.scale2 ? *g.scale * *g.scale2 : *g.scale, w = st.y * by;
-        const T* src = row_start<T>(a, r);
-        T* q = static_cast<T*>(g.grad) + r * a.classes;
-        const int64_t full = c1 / V;
-        for (int64_t i = c0 / V + threadIdx.x; i < full; i += 256) {
-            float f[V];
-            if (st.y == 0.f) {
-                #pragma unroll
-                for (int k = 0; k < V; k++) f[k] = 0.f;
-            } else {
-                Elem<T>::unpack(load16(src + i * V), f);
-                #pragma unroll
-                for (int k = 0; k < V; k++) f[k] = exp_stored<T>(f[k] - st.x, t) * w;
-            }
-            put_stream16(q + i * V, Elem<T>::pack(f));
-        }
-        for (int64_t j = full * V + threadIdx.x; j < c1; j += 256) q[j] = Elem<T>::put(st.y == 0.f ? 0.f : exp_stored<T>(Elem<T>::get(src[j]) - st.x, t) * w);
-        __syncthreads();        // (the entries' values stand where these stood)
-        if ((int)threadIdx.x < l.k) {
-            const int64_t c = l.cls(r * l.k + threadIdx.x);
-            if (c >= c0 && c < c1) q[c] = Elem<T>::put(g.entries[r * l.k + threadIdx.x] * by);
-        }
-    }
-}
-
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 namespace {
 
-constexpr int kMeanBlocks = 128;
+constexpr int kMeanBlocks = 128, kCountBlocks = 256;
 
-int check_lists(const sd_top_lists* in, const sd_logit_rows* rows, const char* who, Lists* l) {
+int check_lists(const sd_top_lists* in, const char* who, Lists* l) {
     SD_REQUIRE(in && in->values && in->classes, "%s: null lists", who);
     SD_REQUIRE(in->k >= 1 && in->k <= kMostEntries, "%s: k=%lld entries for each row: 1..%d are possible", who, (long long)in->k, kMostEntries);
     SD_REQUIRE(in->dtype == SD_FLOAT32 || in->dtype == SD_BFLOAT16 || in->dtype == SD_FLOAT16, "%s: values of dtype=%d", who, in->dtype);
@@ -311,66 +740,160 @@ int check_temper(double temperature, double weight, const char* who, Temper* t) 
     return SD_OK;
 }
 
+// scratch: the ticket, sums of workgroups (the counts' place before), a mark for each row that counts, parts of long rows
+constexpr int64_t kDistillSums = 4 + 4 * kMeanBlocks;
+static_assert(4 * kMeanBlocks >= kCountBlocks, "counts of workgroups stand where their sums will");
+int64_t kept_floats(int64_t rows) { return (rows + 3) / 4 * 4; }
+
+struct Cut { int splits; int64_t part; };
+Cut cut_of(const LogitRows& a, int vec) {
+    int splits = row_splits(a.rows, a.classes, vec);
+    const int64_t part = part_of(a.classes, splits, vec);
+    return {(int)((a.classes + part - 1) / part), part};
+}
+
+bool in_parts(const LogitRows& a, int vec) {
+    return group_of(a.rows, a.classes, vec).shift < 0 && !((a.classes + vec - 1) / vec <= 16 * 512 && (a.rows >= kWholeRows || one_launch(a.rows, a.classes, vec)));
+}
+
+int64_t distill_floats(const LogitRows& a, int dtype) {
+    const int vec = vec_of(dtype);
+    return kDistillSums + kept_floats(a.rows) + (in_parts(a, vec) ? ((int64_t)(sizeof(Others) + sizeof(int)) / 4 * a.rows * cut_of(a, vec).splits + 3) / 4 * 4 : 0);
+}
+
+// Launches of kernels whose workgroups do one thing each: at most 2^20 of them at a time (a grid of 2^32 work-items would be too large).
+template <class F> void in_slices(int64_t blocks, F&& f) {
+    for (int64_t from = 0; from < blocks; from += 1 << 20) f(from, (unsigned)(blocks - from < 1 << 20 ? blocks - from : 1 << 20));
+}
+
+// Whether the gradient leaves with the rows: it then costs one reading of the logits less and two launches more; a workgroup must be able to hold a
+// row, and there must be rows for all compute units.
+bool fuses(const LogitRows& a, int dtype) {
+    const int vec = vec_of(dtype);
+    if (a.rows * a.classes * (16 / vec) < (32ll << 20)) return false;
+    return group_of(a.rows, a.classes, vec).shift >= 0 || (a.rows >= 512 && a.classes <= kHeldLong * vec);
+}
+
 }  // namespace
 
 }  // namespace sd
 
 using namespace sd;
 
-// scratch: the ticket, sums of workgroups, a mark for each row that counts
-static int64_t distill_floats(int64_t rows) { return 4 + 4 * kMeanBlocks + (rows + 3) / 4 * 4; }
-
 extern "C" int64_t sd_distill_scratch(const sd_logit_rows* rows, int64_t k) {
     LogitRows a;
     if (check_logits(rows, "distill_scratch", &a) != SD_OK) return -1;
     if (k < 1 || k > kMostEntries) { set_error("distill_scratch: k=%lld entries for each row: 1..%d are possible", (long long)k, kMostEntries); return -1; }
-    return distill_floats(a.rows);
+    return distill_floats(a, rows->dtype);
 }
 
-extern "C" int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, double weight, float* stats, float* entries, float* scale,
+extern "C" int sd_distill_fuses(const sd_logit_rows* rows) {
+    LogitRows a;
+    return check_logits(rows, "distill_fuses", &a) == SD_OK && fuses(a, rows->dtype) ? 1 : 0;
+}
+
+extern "C" int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, double weight, float* stats, float* entries, float* scale, void* grad,
                                float* loss, float* divergences, float* scratch, sd_stream_t stream) {
     sd::CallGuard call_guard;
     LogitRows a;
     Lists l;
     Temper t;
     if (int rc = check_logits(rows, "distill_loss", &a)) return rc;
-    if (int rc = check_lists(lists, rows, "distill_loss", &l)) return rc;
+    if (int rc = check_lists(lists, "distill_loss", &l)) return rc;
     if (int rc = check_temper(temperature, weight, "distill_loss", &t)) return rc;
     SD_REQUIRE(loss && divergences && scratch, "distill_loss: null argument");
     SD_REQUIRE(!stats == !entries && !stats == !scale, "distill_loss: the gradient needs stats, entries and scale");
-    SD_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0 && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "distill_loss: stats must be aligned to 8 bytes, scratch to 16");
+    SD_REQUIRE(!grad || stats, "distill_loss: a gradient that leaves with the rows needs stats, entries and scale, too");
+    SD_REQUIRE(!grad || fuses(a, rows->dtype), "distill_loss: the gradient of these rows does not leave with them (sd_distill_fuses)");
+    SD_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0 && (reinterpret_cast<uintptr_t>(scratch) & 15) == 0 &&
+               (reinterpret_cast<uintptr_t>(grad) & (rows->dtype == SD_FLOAT32 ? 3 : 1)) == 0, "distill_loss: stats must be aligned to 8 bytes, scratch to 16, the gradient to its type");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const Outcome e{reinterpret_cast<float2*>(stats), entries, divergences, scratch + 4 + 4 * kMeanBlocks, reinterpret_cast<uint32_t*>(scratch)};
+    float* kept = scratch + kDistillSums;
+    const Outcome e{reinterpret_cast<float2*>(stats), entries, divergences, kept, reinterpret_cast<uint32_t*>(scratch)};
+    const Slopes g{nullptr, nullptr, scale, nullptr, grad, false};
+    const double scale_factor = weight * temperature;
+    if (grad) {
+        int* counted = reinterpret_cast<int*>(scratch + 4);
+        const int64_t want = (a.rows + 3) / 4;
+        const int blocks = (int)(want < kCountBlocks ? want : kCountBlocks);
+        hipLaunchKernelGGL(distill_rows_that_count_kernel, dim3(blocks), dim3(256), 0, s, l, a.rows, kept, counted);
+        hipLaunchKernelGGL(distill_scale_kernel, dim3(1), dim3(256), 0, s, counted, blocks, scale_factor, scale);
+    }
+    const int vec = vec_of(rows->dtype);
+    const Group group = group_of(a.rows, a.classes, vec);
     with_dtype(rows->dtype, [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        hipLaunchKernelGGL(distill_rows_kernel<T>, dim3(blocks_for(a.rows)), dim3(256), 0, s, a, l, t, e);
+        if (group.shift >= 0) {
+            const int per = 256 >> group.shift;
+            with_vectors(group.vectors, [&](auto nv) {
+                in_slices((a.rows + per - 1) / per, [&](int64_t from, unsigned blocks) {
+                    if (grad) hipLaunchKernelGGL((distill_short_kernel<T, nv.value, true>), dim3(blocks), dim3(256), 0, s, a, l, t, e, g, group.shift, from * per);
+                    else hipLaunchKernelGGL((distill_short_kernel<T, nv.value, false>), dim3(blocks), dim3(256), 0, s, a, l, t, e, g, group.shift, from * per);
+                });
+            });
+            return;
+        }
+        if (grad || !in_parts(a, vec)) {
+            const int64_t vecs = (a.classes + vec - 1) / vec;
+            const auto held = [&](auto fused, auto far) {
+                in_slices(a.rows, [&](int64_t from, unsigned blocks) {
+                    const dim3 grid(blocks);
+                    if (vecs <= 4 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 4, 256, fused.value, far.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
+                    else if (vecs <= 8 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 8, 256, fused.value, far.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
+                    else if (vecs <= 16 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 16, 256, fused.value, far.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
+                    else if (vecs <= 16 * 512) hipLaunchKernelGGL((distill_held_kernel<T, 16, 512, fused.value, far.value>), grid, dim3(512), 0, s, a, l, t, e, g, from);
+                    else if constexpr (fused.value) hipLaunchKernelGGL((distill_held_kernel<T, 16, 1024, true, far.value>), grid, dim3(1024), 0, s, a, l, t, e, g, from);
+                });
+            };
+            if (!grad) held(std::false_type(), std::false_type());
+            else if (a.rows * a.classes * (int64_t)sizeof(T) >= kCached) held(std::true_type(), std::true_type());
+            else held(std::true_type(), std::false_type());
+            return;
+        }
+        const Cut cut = cut_of(a, vec);
+        Others* parts = reinterpret_cast<Others*>(kept + kept_floats(a.rows));
+        int* twice = reinterpret_cast<int*>(parts + a.rows * cut.splits);
+        hipLaunchKernelGGL(distill_part_kernel<T>, dim3(blocks_for(a.rows * cut.splits)), dim3(256), 0, s, a, l, t, e, cut.splits, cut.part, parts, twice);
+        hipLaunchKernelGGL(distill_join_kernel<T>, dim3(blocks_for((a.rows + 3) / 4)), dim3(256), 0, s, a, l, t, e, cut.splits, parts, twice);
     });
     if (int rc = check_launch("distill_rows_kernel")) return rc;
     const int64_t want = (a.rows + 16383) / 16384;
-    const Mean m{divergences, e.kept, a.rows, weight * temperature * temperature, weight * temperature, loss, scale, reinterpret_cast<double*>(scratch + 4), e.ticket};
+    const Mean m{divergences, kept, a.rows, weight * temperature * temperature, scale_factor, loss, grad ? nullptr : scale, reinterpret_cast<double*>(scratch + 4), e.ticket};
     hipLaunchKernelGGL(distill_mean_kernel, dim3((unsigned)(want < kMeanBlocks ? want : kMeanBlocks)), dim3(1024), 0, s, m);
     return check_launch("distill_mean_kernel");
 }
 
 extern "C" int sd_distill_gradient(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, const float* stats, const float* entries, const float* scale,
-                                   const float* scale2, void* grad, sd_stream_t stream) {
+                                   const float* scale2, int unless_one, void* grad, sd_stream_t stream) {
     sd::CallGuard call_guard;
     LogitRows a;
     Lists l;
     Temper t;
     if (int rc = check_logits(rows, "distill_gradient", &a)) return rc;
-    if (int rc = check_lists(lists, rows, "distill_gradient", &l)) return rc;
+    if (int rc = check_lists(lists, "distill_gradient", &l)) return rc;
     if (int rc = check_temper(temperature, 1.0, "distill_gradient", &t)) return rc;
     SD_REQUIRE(stats && entries && scale && grad, "distill_gradient: null argument");
+    SD_REQUIRE(!unless_one || scale2, "distill_gradient: unless_one needs scale2");
     SD_REQUIRE((reinterpret_cast<uintptr_t>(stats) & 7) == 0 && (reinterpret_cast<uintptr_t>(grad) & (rows->dtype == SD_FLOAT32 ? 3 : 1)) == 0,
                "distill_gradient: stats must be aligned to 8 bytes, the gradient to its type");
-    const Slopes g{reinterpret_cast<const float2*>(stats), entries, scale, scale2, grad};
+    const Slopes g{reinterpret_cast<const float2*>(stats), entries, scale, scale2, grad, unless_one != 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const int64_t part = 256 * vec_of(rows->dtype) * 4;
-    const int splits = (int)((a.classes + part - 1) / part);
+    const int vec = vec_of(rows->dtype);
+    const Group group = group_of(a.rows, a.classes, vec);
+    // a launch that mostly finds nothing to do has no more workgroups than run at once: each takes time to come and go
+    const auto blocks = [&](int64_t n) { return dim3(unless_one && n > 8 * num_cus() ? (unsigned)(8 * num_cus()) : blocks_for(n)); };
     with_dtype(rows->dtype, [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
-        hipLaunchKernelGGL(distill_gradient_kernel<T>, dim3(blocks_for(a.rows * splits)), dim3(256), 0, s, a, l, t, g, splits, part);
+        if (group.shift >= 0) {
+            const int per = 256 >> group.shift;
+            with_vectors(group.vectors, [&](auto nv) {
+                hipLaunchKernelGGL((distill_short_gradient_kernel<T, nv.value>), blocks((a.rows + per - 1) / per), dim3(256), 0, s, a, l, t, g, group.shift);
+            });
+            return;
+        }
+        const int64_t part = 256 * vec * 4;
+        const int splits = (int)((a.classes + part - 1) / part);
+        hipLaunchKernelGGL(distill_long_gradient_kernel<T>, blocks(a.rows * splits), dim3(256), 0, s, a, l, t, g, splits, part);
     });
     return check_launch("distill_gradient_kernel");
 }

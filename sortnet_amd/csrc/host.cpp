@@ -1160,6 +1160,9 @@ struct DistillWork {
 
 struct DistillNode : Node {
     SavedVariable logits, values, classes, rest, work;
+    Tensor made;            // as LabelNode's
+    int64_t capture = 0;
+    bool last = false;
     double temperature = 1.0;
 
     variable_list apply(variable_list&& grads) override {
@@ -1177,17 +1180,25 @@ struct DistillNode : Node {
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor g = incoming(*this, grads, 0);
         const c10::DeviceGuard guard(z.device());
-        out[0] = at::empty(z.sizes(), z.options());
+        // (as in LabelNode: a gradient that is there is written again for another upstream gradient than 1)
+        const int64_t now = made.defined() && last ? capture_of(stream_of(z)) : -1;
+        const bool there = now >= 0 && now == capture;
+        out[0] = there ? std::move(made) : at::empty(z.sizes(), z.options());
         const sd_logit_rows a = logit_rows(z);
         const sd_top_lists lists = l.call();
         const DistillWork w(wk, a.rows, lists.k, true);
-        require(sd_distill_gradient(&a, &lists, temperature, w.stats, w.entries, w.scale, floats(g, "grad_output"), out[0].data_ptr(), stream_of(z)), "sd_distill_gradient");
+        require(sd_distill_gradient(&a, &lists, temperature, w.stats, w.entries, w.scale, floats(g, "grad_output"), there, out[0].data_ptr(), stream_of(z)), "sd_distill_gradient");
         if (once) set_history(out[0], once);
         return out;
+    }
+    void will_release_variables() override {
+        const Locked lock(mutex_);
+        last = true;
     }
     void release_variables() override {
         const Locked lock(mutex_);
         for (SavedVariable* v : {&logits, &values, &classes, &rest, &work}) v->reset_data();
+        made.reset();
     }
     std::string name() const override { return "DistillNode"; }
 };
@@ -1212,7 +1223,7 @@ std::pair<Tensor, Tensor> distill_loss(const Tensor& outputs, const Tensor& valu
     if (classes.scalar_type() != at::kLong && classes.scalar_type() != at::kInt) throw std::runtime_error("top_classes must have dtype torch.int64 or torch.int32");
     if (classes.sizes() != values.sizes()) throw std::runtime_error("top_classes must have the sizes of top_values");
     if (has_rest && rest->scalar_type() != at::kFloat) throw std::runtime_error("top_rest must have dtype torch.float32");
-    Tensor loss, divergences, z, work;
+    Tensor loss, divergences, z, work, made;
     Lists l;
     {
         at::AutoDispatchBelowADInplaceOrView below;
@@ -1228,8 +1239,9 @@ std::pair<Tensor, Tensor> distill_loss(const Tensor& outputs, const Tensor& valu
         const DistillWork w(work, a.rows, lists.k, grad);
         loss = new_floats(z, {});
         divergences = new_floats(z, outputs.sizes().slice(0, outputs.dim() - 1));
-        require(sd_distill_loss(&a, &lists, temperature, weight, w.stats, w.entries, w.scale, floats(loss, "loss"), floats(divergences, "divergences"), w.scratch, stream_of(z)),
-                "sd_distill_loss");
+        if (grad && sd_distill_fuses(&a)) made = at::empty(z.sizes(), z.options());
+        require(sd_distill_loss(&a, &lists, temperature, weight, w.stats, w.entries, w.scale, made.defined() ? made.data_ptr() : nullptr, floats(loss, "loss"),
+                                floats(divergences, "divergences"), w.scratch, stream_of(z)), "sd_distill_loss");
     }
     if (grad) {
         auto node = new_node<DistillNode>();
@@ -1239,6 +1251,8 @@ std::pair<Tensor, Tensor> distill_loss(const Tensor& outputs, const Tensor& valu
         node->classes = SavedVariable(l.classes, false);
         if (has_rest) node->rest = SavedVariable(l.rest, false);
         node->work = SavedVariable(work, false);
+        node->made = made;
+        if (made.defined()) node->capture = capture_of(stream_of(z));
         node->temperature = temperature;
         set_history(loss, node);
     }

@@ -1,6 +1,7 @@
 // Rows of values: element types, 16-byte loads and stores, sums over lanes.
 #pragma once
 #include <cfloat>
+#include <type_traits>
 #include "common.h"
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -150,6 +151,35 @@ template <int N> __device__ __forceinline__ float tree(const float (&f)[N]) {
     return s[0];
 }
 
+// A short row, which 2^shift lanes of a wavefront hold in registers, NV vectors each.
+// The last vector of a row of at least one ends with the row and overlaps the one before it; a shorter row is one vector, padded with -inf.
+template <class T, int NV> struct HeldRow {
+    static constexpr int V = Elem<T>::kVec;
+    u32x4 v[NV];
+    int n, vecs, lane, shift;
+
+    __device__ __forceinline__ int index(int k) const { return lane + (k << shift); }
+    __device__ __forceinline__ int column(int i) const { return i * V + V <= n ? i * V : n - V; }     // (n >= V)
+
+    __device__ __forceinline__ void load(const T* p) {
+        if (n >= V) {
+            #pragma unroll
+            for (int k = 0; k < NV; k++)
+                if (index(k) < vecs) v[k] = load16(p + column(index(k)));
+        } else if (lane == 0) {
+            float f[V];
+            #pragma unroll
+            for (int i = 0; i < V; i++) f[i] = i < n ? Elem<T>::get(p[i]) : -INFINITY;
+            v[0] = Elem<T>::pack(f);
+        }
+    }
+    // What was derived from the vectors before is derived again afterwards: kept, it would be twice their registers.
+    __device__ __forceinline__ void again() {
+        #pragma unroll
+        for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
+    }
+};
+
 // zeros in a row of a gradient, by a whole workgroup
 template <class T> __device__ __forceinline__ void clear_row(T* q, int n, int threads) {
     constexpr int V = Elem<T>::kVec;
@@ -206,5 +236,58 @@ inline int check_logits(const sd_logit_rows* in, const char* who, LogitRows* a) 
 constexpr int64_t kMostBlocks = 1 << 22;
 inline unsigned blocks_for(int64_t n) { return (unsigned)(n < kMostBlocks ? n : kMostBlocks); }
 inline int vec_of(int dtype) { return dtype == SD_FLOAT32 ? 4 : 8; }
+
+constexpr int kHeld = 8;            // 16-byte vectors of a short row that a lane holds, at most
+constexpr int kHeldLong = 16 * 1024;    // and of a long row that a workgroup holds
+constexpr int kShortBlocks = 4096;      // workgroups of short rows, at most
+
+// Lanes of a wavefront that hold a row together (as a power of two) and vectors that each holds; shift = -1: a row is read by whole workgroups.
+// Many rows want few lanes with several vectors each (fewer steps to add up lanes per row), few rows one vector per lane.
+struct Group { int shift, vectors; };
+inline Group group_of(int64_t rows, int64_t classes, int vec) {
+    const int64_t vecs = (classes + vec - 1) / vec;
+    if (vecs > 64 * kHeld) return {-1, 0};
+    int shift = 0;
+    while (shift < 6 && (1 << shift) < vecs) shift++;
+    int vectors = 1;
+    while ((int64_t)vectors << shift < vecs) vectors *= 2;
+    while (vectors < 4 && shift > 0 && (rows << shift) > (1 << 16)) { shift--; vectors *= 2; }
+    return {shift, vectors};
+}
+
+template <class F> void with_vectors(int vectors, F&& f) {
+    switch (vectors) {
+        case 1: f(std::integral_constant<int, 1>()); return;
+        case 2: f(std::integral_constant<int, 2>()); return;
+        case 4: f(std::integral_constant<int, 4>()); return;
+        default: f(std::integral_constant<int, kHeld>()); return;
+    }
+}
+
+// Parts of a long row: so many that there are kWholeRows workgroups (2.75 for each compute unit), none with less than one vector per work-item.
+// With 2048: 2000 x 50001 bf16 35.8 us whole, in two parts 38.2; 1000 x 131072 43.6 and 48.2; 1030 x 131072 fp32 90.3 and 86.8.
+constexpr int64_t kWholeRows = 704;
+inline int row_splits(int64_t rows, int64_t classes, int vec) {
+    const int64_t want = (kWholeRows + rows - 1) / rows, most = (classes + 256 * vec - 1) / (256 * vec);
+    return (int)(want < most ? want : most);
+}
+
+// Rows that would be read in parts: where a workgroup can hold a row it is read whole, which spares the launch that joins the parts:
+// 128 x 8192 bf16 6.8 -> 4.4 us, 512 x 16384 8.6 -> 5.4, 512 x 32000 11.9 -> 9.3.  Rows for a workgroup of 512, of which fewer run at once: 256 x 50001
+// 10.4 -> 9.0, but 16 rows 7.1 -> 8.4 and 1024 21.2 -> 26.0.
+inline bool one_launch(int64_t rows, int64_t classes, int vec) {
+    const int64_t vecs = (classes + vec - 1) / vec;
+    return rows < kWholeRows && (vecs <= 16 * 256 || (vecs <= 16 * 512 && rows >= 32 && rows <= 512));
+}
+
+inline int64_t part_of(int64_t classes, int splits, int vec) {
+    const int64_t step = 256 * vec, n = (classes + splits - 1) / splits;
+    return (n + step - 1) / step * step;
+}
+
+inline unsigned short_blocks(int64_t rows, int per) {
+    const int64_t n = (rows + per - 1) / per;
+    return (unsigned)(n < kShortBlocks ? n : kShortBlocks);
+}
 
 }  // namespace sd

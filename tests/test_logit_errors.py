@@ -75,8 +75,8 @@ def _lists(**kw):
     return lists
 
 
-def _distill(rows=None, lists=None, temperature=1.0, weight=1.0, stats=P, entries=P, scale=P, loss=P, divergences=P, scratch=P):
-    return _lib.call("sd_distill_loss", rows or _rows(), lists or _lists(), temperature, weight, stats, entries, scale, loss, divergences, scratch, None)
+def _distill(rows=None, lists=None, temperature=1.0, weight=1.0, stats=P, entries=P, scale=P, grad=None, loss=P, divergences=P, scratch=P):
+    return _lib.call("sd_distill_loss", rows or _rows(), lists or _lists(), temperature, weight, stats, entries, scale, grad, loss, divergences, scratch, None)
 
 
 @pytest.mark.parametrize("bad", BAD_ROWS, ids=str)
@@ -105,7 +105,7 @@ def test_rows_without_a_meaning_to_the_teacher(bad):
     with pytest.raises(RuntimeError, match=r"status 1\)"):
         _distill(_rows(**bad))
     with pytest.raises(RuntimeError, match=r"status 1\)"):
-        _lib.call("sd_distill_gradient", _rows(**bad), _lists(), 1.0, P, P, P, None, P, None)
+        _lib.call("sd_distill_gradient", _rows(**bad), _lists(), 1.0, P, P, P, None, 0, P, None)
 
 
 @pytest.mark.parametrize("bad, match", [(dict(values=0), "null"), (dict(classes=0), "null"), (dict(k=0), "k=0"), (dict(k=257), "k=257"), (dict(k=-1), "k=-1"), (dict(dtype=5), "dtype"),
@@ -114,7 +114,7 @@ def test_lists_without_a_meaning(bad, match):
     with pytest.raises(RuntimeError, match=match):
         _distill(lists=_lists(**bad))
     with pytest.raises(RuntimeError, match=match):
-        _lib.call("sd_distill_gradient", _rows(), _lists(**bad), 1.0, P, P, P, None, P, None)
+        _lib.call("sd_distill_gradient", _rows(), _lists(**bad), 1.0, P, P, P, None, 0, P, None)
 
 
 def test_distillation_without_a_meaning():
@@ -124,7 +124,7 @@ def test_distillation_without_a_meaning():
         with pytest.raises(RuntimeError, match="temperature"):
             _distill(temperature=t)
         with pytest.raises(RuntimeError, match="temperature"):
-            _lib.call("sd_distill_gradient", _rows(), _lists(), t, P, P, P, None, P, None)
+            _lib.call("sd_distill_gradient", _rows(), _lists(), t, P, P, P, None, 0, P, None)
     for w in (math.nan, math.inf, -math.inf, 1e39):
         with pytest.raises(RuntimeError, match="weight"):
             _distill(weight=w)
@@ -134,6 +134,13 @@ def test_distillation_without_a_meaning():
     for missing in ("stats", "entries", "scale"):
         with pytest.raises(RuntimeError, match="needs stats"):
             _distill(**{missing: None})
+    assert _lib.load().sd_distill_fuses(_rows()) == 0
+    with pytest.raises(RuntimeError, match="does not leave"):       # too few rows for a gradient that leaves with them
+        _distill(grad=P)
+    with pytest.raises(RuntimeError, match="needs stats"):
+        _distill(grad=P, stats=None, entries=None, scale=None)
+    with pytest.raises(RuntimeError, match="unless_one"):
+        _lib.call("sd_distill_gradient", _rows(), _lists(), 1.0, P, P, P, None, 1, P, None)
     with pytest.raises(RuntimeError, match="aligned"):
         _distill(stats=P + 4)
     with pytest.raises(RuntimeError, match="aligned"):
