@@ -29,6 +29,20 @@ struct Lists {
         if (dtype == SD_BFLOAT16) return Elem<bf16>::get(static_cast<const bf16*>(values)[at]);
         return Elem<fp16>::get(static_cast<const fp16*>(values)[at]);
     }
+    // An entry as it is stored, for kernels that have other loads under way behind these: a conversion beside the load would wait for it.
+    struct Raw { int low, high; uint32_t value; };
+    __device__ __forceinline__ Raw raw(int64_t at) const {
+        const int* c = static_cast<const int*>(classes);
+        Raw e{c[wide ? 2 * at : at], c[wide ? 2 * at + 1 : at], 0};
+        if (dtype == SD_FLOAT32) e.value = static_cast<const uint32_t*>(values)[at];
+        else e.value = static_cast<const uint16_t*>(values)[at];
+        return e;
+    }
+    __device__ __forceinline__ int64_t cls(const Raw& e) const { return wide ? (int64_t)((uint64_t)(uint32_t)e.high << 32 | (uint32_t)e.low) : (int64_t)e.low; }
+    __device__ __forceinline__ float value(const Raw& e) const {
+        if (dtype == SD_FLOAT32) return __uint_as_float(e.value);
+        return dtype == SD_BFLOAT16 ? Elem<bf16>::get(bf16{(uint16_t)e.value}) : Elem<fp16>::get(fp16{(uint16_t)e.value});
+    }
 };
 
 // z / T as an exponent of 2: log2(e) / T is the sum of two positive numbers, the first rounded down (see exp_of)
@@ -67,28 +81,34 @@ __device__ __forceinline__ int said(int64_t cls, float t) { return cls < 0 ? 0 :
 // over the entries: of the teacher's weights w = exp((t - most_t) / T), of the student's exp((z - base) / T), each class once, and of w times the difference of the two
 // exponents
 struct Sums { double w, p, a; };
-__device__ __forceinline__ void add_entry(Sums& s, const Entry& e, float most_t, float base, bool first, const Temper& t) {
-    const double at = ((double)e.t - (double)most_t) * t.inverse, az = ((double)e.z - (double)base) * t.inverse, w = exp(at);
+__device__ __forceinline__ double add_entry(Sums& s, const Entry& e, float most_t, float base, bool first, const Temper& t) {
+    const double at = ((double)e.t - (double)most_t) * t.inverse, az = ((double)e.z - (double)base) * t.inverse, w = exp(at), p = exp(az);
     s.w += w;
     if (w != 0.0) s.a += w * (at - az);
-    if (first) s.p += exp(az);
+    if (first) s.p += p;
+    return p;
 }
 
-// What a row comes to: with all in exponents relative to most_t and base (of rows where no entry is above -inf, to 0), D = (sum_a + w_r (rest - log S)) / W - log W +
-// log P, W and P being the sums with the others.
-struct Row { double divergence, per_w, per_p; float factor; };      // per_w = 1 / W, per_p = 1 / P; factor = (p_r - q_r) / S
-__device__ __forceinline__ Row finish_row(const Sums& s, float most_t, float base, double rest, const Others& o, bool bad, const Temper& t) {
-    const double log_s = o.sum > 0.0 ? log(o.sum) + ((double)finite(o.top) - (double)base) * t.inverse : -INFINITY;
-    // the rest may lie far above the entries: relative to the larger of the two
+// What a row comes to.  All is relative to most_t and base (of rows where no entry is above -inf, to 0), the rest, which may lie far above the entries, to the
+// larger of the two: W = sum_w exp(-up) + w_r, P = sum_p + S o, o = exp((top - base) / T),
+//   D = (sum_a exp(-up) - up sum_w exp(-up) + w_r (left - up - log(S o))) / W - log W + log P.
+struct Rest { double left, up, scale, w, o; };      // of the teacher's others, with exp(-up) and w_r, and o
+__device__ __forceinline__ Rest rest_of(double rest, float most_t, float base, float top, const Temper& t) {
     const double left = rest - (double)most_t * t.inverse, up = left > 0.0 ? left : 0.0;
-    const double w_r = exp(left - up), scale = up > 0.0 ? exp(-up) : 1.0, w = s.w * scale + w_r;
-    const double p_r = exp(log_s), p = s.p + p_r;
-    double a = scale != 0.0 ? s.a * scale - up * (s.w * scale) : 0.0;
-    if (w_r != 0.0) a += w_r * (left - up - log_s);
-    Row r{a / w - log(w) + log(p), scale / w, 1.0 / p, 0.f};
-    if (bad) r.divergence = r.per_p = __builtin_nan("");
-    if (o.sum > 0.0 || bad) r.factor = (float)((p_r * r.per_p - w_r / w) / o.sum);
-    return r;
+    return Rest{left, up, up > 0.0 ? exp(-up) : 1.0, exp(left - up), exp(((double)finite(top) - (double)base) * t.inverse)};
+}
+struct Row { double per_w, per_p; float factor; };      // 1 / W (for sum_w), 1 / P; factor = (p_r - q_r) / S
+__device__ __forceinline__ Row ratios_of(const Sums& s, const Rest& rest, const Others& o, bool bad) {
+    const double w = 1.0 / (s.w * rest.scale + rest.w), p = bad ? __builtin_nan("") : 1.0 / (s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0));
+    return Row{rest.scale * w, p, o.sum > 0.0 || bad ? (float)(rest.o * p - rest.w * w / o.sum) : 0.f};
+}
+__device__ __forceinline__ double divergence_of(const Sums& s, const Rest& rest, const Others& o, bool bad, float base, const Temper& t) {
+    if (bad) return __builtin_nan("");
+    const double log_s = o.sum > 0.0 ? log(o.sum) + ((double)finite(o.top) - (double)base) * t.inverse : -INFINITY;
+    const double w = s.w * rest.scale + rest.w, p = s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0);
+    double a = rest.scale != 0.0 ? s.a * rest.scale - rest.up * (s.w * rest.scale) : 0.0;
+    if (rest.w != 0.0) a += rest.w * (rest.left - rest.up - log_s);
+    return a / w - log(w) + log(p);
 }
 __device__ __forceinline__ double teacher_share(const Row& r, float v, float most_t, const Temper& t) { return exp(((double)v - (double)most_t) * t.inverse) * r.per_w; }
 __device__ __forceinline__ double student_share(const Row& r, float z, float base, const Temper& t) { return exp(((double)z - (double)base) * t.inverse) * r.per_p; }
@@ -115,7 +135,8 @@ template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& 
     const int lanes = 1 << shift;
     const T* z = row_start<T>(a, r);
     stats = make_float2(0.f, 0.f);
-    row = Row{0.0, 0.0, 0.0, 0.f};
+    row = Row{0.0, 0.0, 0.f};
+    double divergence = 0.0;
     most_t = base = 0.f;
     if (!skip) {
         float bad = 0.f;
@@ -140,11 +161,13 @@ template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& 
             add_entry(s, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, most_t, base, !repeats || first_of(l, r, j, c), t);
         }
         s.w = group_total(s.w, shift); s.p = group_total(s.p, shift); s.a = group_total(s.a, shift);
-        row = finish_row(s, most_t, base, rest, o, bad != 0.f, t);
+        const Rest left = rest_of(rest, most_t, base, o.top, t);
+        row = ratios_of(s, left, o, bad != 0.f);
+        divergence = divergence_of(s, left, o, bad != 0.f, base, t);
         stats = make_float2(finite(o.top), row.factor);
     }
     if (lane == 0) {
-        e.divergences[r] = (float)row.divergence;
+        e.divergences[r] = (float)divergence;
         e.kept[r] = skip ? 0.f : 1.f;
         if (e.stats) e.stats[r] = stats;
     }
@@ -382,11 +405,13 @@ template <class T, int NV, int THREADS> struct Marks {
 // with the row.  FAR: logits that the last-level cache cannot hold are read past it.
 // A row per workgroup and no loop over them: the constants of the 64-bit functions would be kept in registers that the row needs.
 template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __launch_bounds__(THREADS, 4) distill_held_kernel(LogitRows a, Lists l, Temper t, Outcome e, Slopes g, int64_t row0) {
-    constexpr int V = Elem<T>::kVec, WAVES = THREADS / 64, kChunk = (NV == 16 ? 8 : 16) / V;
+    constexpr int V = Elem<T>::kVec, WAVES = THREADS / 64, kChunk = NV < 32 / V ? NV : 32 / V;
+    constexpr int kShift = WAVES == 4 ? 2 : WAVES == 8 ? 3 : 4;      // (the wavefronts' results in the lanes of each group of so many)
     __shared__ Marks<T, NV + 1, THREADS> marks;       // (one more: the values behind the last whole vector)
     __shared__ float maxima[WAVES][4];
     __shared__ double sums[WAVES][4];
-    __shared__ Row end;
+    __shared__ double weights[kMostEntries];        // the teacher's, relative to the largest, and what
+    __shared__ int theirs_of[kMostEntries];         // class each is for
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
     const int n = (int)a.classes, full = n / V, rest_at = full * V + (int)threadIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const T lowest = Elem<T>::put(-INFINITY);
@@ -395,14 +420,23 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
     T* q = static_cast<T*>(g.grad) + r * a.classes;
     const bool own = (int)threadIdx.x < l.k;
     bool skip;
-    int64_t cls = -1;
-    float value = -INFINITY;
+    // a work-item's entry: its class (-1: none, n: one that is not in the row) and the two logits
+    int cls = -1;
+    float value = -INFINITY, z = -INFINITY;
+    const auto decode = [&](const Lists::Raw& mine) {
+        if (own) {
+            const int64_t c = l.cls(mine);
+            cls = c < 0 ? -1 : c < n ? (int)c : n;
+            value = l.value(mine);
+        }
+    };
     if (FUSED) skip = e.kept[r] == 0.f;
-    if (own && !(FUSED && skip)) { cls = l.cls(r * l.k + threadIdx.x); value = l.value(r * l.k + threadIdx.x); }
+    const Lists::Raw entry = l.raw(r * l.k + (own ? (int)threadIdx.x : 0));
     if (!FUSED) {
+        decode(entry);
         const int what = said(cls, value);
-        const bool entry = __syncthreads_or(what & 1), live = __syncthreads_or(what & 2);
-        skip = !entry || !(live || (l.rest && l.rest[r] != -INFINITY));
+        const bool any = __syncthreads_or(what & 1), live = __syncthreads_or(what & 2);
+        skip = !any || !(live || (l.rest && l.rest[r] != -INFINITY));
     }
     if (skip) {     // (the whole workgroup's)
         if (own && e.entries) e.entries[r * l.k + threadIdx.x] = 0.f;
@@ -416,82 +450,78 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
     }
     const T* p = row_start<T>(a, r);
     u32x4 v[NV];
-    const u32x4 none = Elem<T>::splat(lowest);
-    T last = lowest;
     #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int i = (int)threadIdx.x + k * THREADS;
-        v[k] = none;
-        if (i < full) v[k] = FAR ? stream16(p + i * V) : load16(p + i * V);
+        const uint32_t at = (uint32_t)(i < full ? i : full - 1) * V;        // (under no condition: behind one no load can be waited for by itself)
+        v[k] = FAR ? stream16(p + at) : load16(p + at);
     }
-    if (rest_at < n) last = p[rest_at];
+    T last = p[rest_at < n ? rest_at : n - 1];
     // the entry, while the row is on its way
-    const bool inside = cls >= 0 && cls < a.classes;
-    Entry mine{cls, value, -INFINITY};
-    if (inside) mine.z = Elem<T>::get(p[cls]);
+    if (FUSED) decode(entry);
+    const bool inside = cls >= 0 && cls < n;
+    const T theirs_z = p[inside ? cls : 0];
     const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
     marks.clear();
     __syncthreads();
-    if (inside) {
-        const int c = (int)cls;
-        // the values behind the last whole vector are held by the first work-items, one each, as the first value of a vector of their own
-        marks.mark(c < full * V ? c : (NV * THREADS + (c - full * V)) * V);
-    }
+    // (the values behind the last whole vector are held by the first work-items, one each, as the first value of a vector of their own)
+    if (inside) marks.mark(cls < full * V ? cls : (NV * THREADS + (cls - full * V)) * V);
+    if (own) theirs_of[threadIdx.x] = inside ? cls : -1;
     __syncthreads();
     const bool repeats = marks.repeats != 0;
     float top = -INFINITY;
     double sum = 0.0;
     #pragma unroll
-    for (int k = 0; k < NV; k++) {
-        const uint32_t listed = marks.bits(k);
-        if (listed) v[k] = without<T>(v[k], listed);
-    }
-    if (marks.bits(NV) & 1u) last = lowest;
-    #pragma unroll
     for (int c = 0; c < NV; c += kChunk) {
         float f[kChunk * V];
         #pragma unroll
-        for (int k = 0; k < kChunk; k++) Elem<T>::unpack(v[c + k], reinterpret_cast<float (&)[V]>(f[k * V]));
+        for (int k = c; k < c + kChunk; k++) {
+            const uint32_t listed = marks.bits(k);
+            if ((k + 1) * THREADS > full) {
+                asm volatile("");       // (a branch of the whole workgroup's)
+                if ((int)threadIdx.x + k * THREADS >= full) v[k] = Elem<T>::splat(lowest);
+            }
+            if (listed) v[k] = without<T>(v[k], listed);
+            Elem<T>::unpack(v[k], reinterpret_cast<float (&)[V]>(f[(k - c) * V]));
+        }
         take(f, top, sum, t);
+        asm volatile("" : "+v"(top), "+v"(sum));     // (here, while the next vectors are on their way, and not behind them all)
     }
+    if (rest_at >= n || (marks.bits(NV) & 1u)) last = lowest;
+    if (inside) z = Elem<T>::get(theirs_z);
     float f1[1] = {Elem<T>::get(last)};
     take(f1, top, sum, t);
     // all work-items': the largest of the others, of the teacher's and of the student's entries, and whether something is wrong
-    bool odd = sum != sum || rest != rest || (cls >= 0 && (!inside || value != value || mine.z != mine.z));
+    bool odd = sum != sum || rest != rest || (cls >= 0 && (!inside || value != value || z != z));
     {
-        const float m0 = group_max(top, 6), m1 = group_max(inside ? value : -INFINITY, 6), m2 = group_max(mine.z, 6);
+        const float m0 = group_max(top, 6), m1 = group_max(inside ? value : -INFINITY, 6), m2 = group_max(z, 6);
         if (lane == 0) { maxima[wave][0] = m0; maxima[wave][1] = m1; maxima[wave][2] = m2; }
     }
     odd = __syncthreads_or(odd);
-    constexpr int kShift = WAVES == 4 ? 2 : WAVES == 8 ? 3 : 4;      // (the wavefronts' in the lanes of each group of so many)
     const float* theirs = maxima[lane & (WAVES - 1)];
     const float all = group_max(theirs[0], kShift);
     float most_t = group_max(theirs[1], kShift), base = fmaxf(group_max(theirs[2], kShift), finite(all));
     if (most_t == -INFINITY) most_t = 0.f;
     Sums s{0.0, 0.0, 0.0};
-    if (inside) add_entry(s, mine, most_t, base, !repeats || first_of(l, r, threadIdx.x, cls), t);
-    sum = wave_total(sum * (double)exp_at(finite(top) - finite(all), t));
-    if (64 * wave < l.k) { s.w = wave_total(s.w); s.p = wave_total(s.p); s.a = wave_total(s.a); }
-    if (lane == 0) { sums[wave][0] = sum; sums[wave][1] = s.w; sums[wave][2] = s.p; sums[wave][3] = s.a; }
-    __syncthreads();
-    if (wave == 0) {
-        double total[4];
-        #pragma unroll
-        for (int k = 0; k < 4; k++) total[k] = group_total(sums[lane & (WAVES - 1)][k], kShift);
-        const Row row = finish_row(Sums{total[1], total[2], total[3]}, most_t, base, rest, Others{all, total[0]}, odd, t);
-        if (lane == 0) {
-            end = row;
-            e.divergences[r] = (float)row.divergence;
-            e.kept[r] = 1.f;
-            if (e.stats) e.stats[r] = make_float2(finite(all), row.factor);
+    double share = 0.0;
+    if (64 * wave < l.k) {
+        if (inside) {
+            bool first = true;
+            if (repeats)
+                for (int i = 0; i < (int)threadIdx.x; i++) first = first && theirs_of[i] != cls;
+            share = add_entry(s, Entry{cls, value, z}, most_t, base, first, t);
+            weights[threadIdx.x] = s.w;
         }
+        s.w = wave_total(s.w); s.p = wave_total(s.p); s.a = wave_total(s.a);
     }
-    if (!FUSED && !e.entries) return;
+    sum = wave_total(sum * (double)exp_at(finite(top) - finite(all), t));
+    if (lane == 0) { sums[wave][0] = sum; sums[wave][1] = s.w; sums[wave][2] = s.p; sums[wave][3] = s.a; }
+    const Rest left = rest_of(rest, most_t, base, all, t);
     __syncthreads();
-    const Row row = end;
-    float slope = 0.f;
-    if (inside) slope = entry_slope(l, r, mine, row, most_t, base, repeats, t);
-    if (own && e.entries) e.entries[r * l.k + threadIdx.x] = slope;
+    const double* totals = sums[lane & (WAVES - 1)];
+    const Others o{all, group_total(totals[0], kShift)};
+    s = Sums{group_total(totals[1], kShift), group_total(totals[2], kShift), group_total(totals[3], kShift)};
+    const Row row = ratios_of(s, left, o, odd);
     if (FUSED) {
         if (row.factor == 0.f) clear_row(q, n, THREADS);
         else {
@@ -515,7 +545,27 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
                 q[rest_at] = Elem<T>::put(f[0]);
             }
         }
-        __syncthreads();        // (the entries' values stand where these stood)
+    }
+    float slope = 0.f;
+    if (inside) {
+        double weight = weights[threadIdx.x];
+        if (repeats) {
+            weight = 0.0;
+            for (int i = 0; i < l.k; i++) weight += theirs_of[i] == cls ? weights[i] : 0.0;
+        }
+        slope = (float)(share * row.per_p - weight * row.per_w);
+    }
+    if (own && e.entries) e.entries[r * l.k + threadIdx.x] = slope;
+    if (wave == WAVES - 1) {
+        const double divergence = divergence_of(s, left, o, odd, base, t);
+        if (lane == 0) {
+            e.divergences[r] = (float)divergence;
+            e.kept[r] = 1.f;
+            if (e.stats) e.stats[r] = make_float2(finite(all), row.factor);
+        }
+    }
+    if (FUSED) {
+        __syncthreads();        // (the entries' values stand where the others' stood)
         if (inside) q[cls] = Elem<T>::put(slope * by);
     }
 }

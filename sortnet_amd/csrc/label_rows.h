@@ -48,9 +48,13 @@ template <> struct Elem<bf16> {
     static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
         u32x4 v;
         #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = (uint32_t)bits(f[2 * i]) | (uint32_t)bits(f[2 * i + 1]) << 16;
+        for (int i = 0; i < 4; i++) v[i] = both(f[2 * i], f[2 * i + 1]);
         return v;
     }
+    // (two at once: one conversion instead of two, a shift and an or)
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t both(float low, float high) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{low, high}), bf16x2)); }
     static __device__ __forceinline__ u32x4 splat(bf16 v) { const uint32_t w = v.bits | (uint32_t)v.bits << 16; return u32x4{w, w, w, w}; }
 };
 struct fp16 { uint16_t bits; };
@@ -68,9 +72,12 @@ template <> struct Elem<fp16> {
     static __device__ __forceinline__ u32x4 pack(const float (&f)[8]) {
         u32x4 v;
         #pragma unroll
-        for (int i = 0; i < 4; i++) v[i] = (uint32_t)bits(f[2 * i]) | (uint32_t)bits(f[2 * i + 1]) << 16;
+        for (int i = 0; i < 4; i++) v[i] = both(f[2 * i], f[2 * i + 1]);
         return v;
     }
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 fp16x2 __attribute__((ext_vector_type(2)));
+    static __device__ __forceinline__ uint32_t both(float low, float high) { return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{low, high}), fp16x2)); }
     static __device__ __forceinline__ u32x4 splat(fp16 v) { const uint32_t w = v.bits | (uint32_t)v.bits << 16; return u32x4{w, w, w, w}; }
 };
 
