@@ -92,23 +92,40 @@ __device__ __forceinline__ double add_entry(Sums& s, const Entry& e, float most_
 // What a row comes to.  All is relative to most_t and base (of rows where no entry is above -inf, to 0), the rest, which may lie far above the entries, to the
 // larger of the two: W = sum_w exp(-up) + w_r, P = sum_p + S o, o = exp((top - base) / T),
 //   D = (sum_a exp(-up) - up sum_w exp(-up) + w_r (left - up - log(S o))) / W - log W + log P.
+// The four lanes of a quad hold the same row: one call of a 64-bit function, some 50 instructions, is for three numbers of it.
+template <int LANE> __device__ __forceinline__ double of_quad(double v) {
+    const uint64_t bits = __builtin_bit_cast(uint64_t, v);
+    const uint32_t low = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)bits, LANE * 0x55, 0xf, 0xf, false);
+    const uint32_t high = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(bits >> 32), LANE * 0x55, 0xf, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)high << 32 | low);
+}
+template <class F> __device__ __forceinline__ void three_of(double& x, double& y, double& z, F&& f) {
+    const int lane = threadIdx.x & 3;
+    const double v = f(lane == 0 ? x : lane == 1 ? y : z);
+    x = of_quad<0>(v); y = of_quad<1>(v); z = of_quad<2>(v);
+}
+
 struct Rest { double left, up, scale, w, o; };      // of the teacher's others, with exp(-up) and w_r, and o
 __device__ __forceinline__ Rest rest_of(double rest, float most_t, float base, float top, const Temper& t) {
     const double left = rest - (double)most_t * t.inverse, up = left > 0.0 ? left : 0.0;
-    return Rest{left, up, up > 0.0 ? exp(-up) : 1.0, exp(left - up), exp(((double)finite(top) - (double)base) * t.inverse)};
+    Rest e{left, up, -up, left - up, ((double)finite(top) - (double)base) * t.inverse};
+    three_of(e.scale, e.w, e.o, [](double v) { return exp(v); });
+    return e;
 }
-struct Row { double per_w, per_p; float factor; };      // 1 / W (for sum_w), 1 / P; factor = (p_r - q_r) / S
+struct Row { double over_w, per_w, per_p; float factor; };      // 1 / W, the same for sum_w, 1 / P; factor = (p_r - q_r) / S
 __device__ __forceinline__ Row ratios_of(const Sums& s, const Rest& rest, const Others& o, bool bad) {
-    const double w = 1.0 / (s.w * rest.scale + rest.w), p = bad ? __builtin_nan("") : 1.0 / (s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0));
-    return Row{rest.scale * w, p, o.sum > 0.0 || bad ? (float)(rest.o * p - rest.w * w / o.sum) : 0.f};
+    double w = s.w * rest.scale + rest.w, p = s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0), others = o.sum;
+    three_of(w, p, others, [](double v) { return 1.0 / v; });
+    if (bad) p = __builtin_nan("");
+    return Row{w, rest.scale * w, p, o.sum > 0.0 || bad ? (float)(rest.o * p - rest.w * w * others) : 0.f};
 }
-__device__ __forceinline__ double divergence_of(const Sums& s, const Rest& rest, const Others& o, bool bad, float base, const Temper& t) {
-    if (bad) return __builtin_nan("");
-    const double log_s = o.sum > 0.0 ? log(o.sum) + ((double)finite(o.top) - (double)base) * t.inverse : -INFINITY;
-    const double w = s.w * rest.scale + rest.w, p = s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0);
+__device__ __forceinline__ double divergence_of(const Sums& s, const Rest& rest, const Others& o, const Row& row, bool bad, float base, const Temper& t) {
+    double log_s = o.sum, w = s.w * rest.scale + rest.w, p = s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0);
+    three_of(log_s, w, p, [](double v) { return log(v); });
+    log_s = o.sum > 0.0 ? log_s + ((double)finite(o.top) - (double)base) * t.inverse : -INFINITY;
     double a = rest.scale != 0.0 ? s.a * rest.scale - rest.up * (s.w * rest.scale) : 0.0;
     if (rest.w != 0.0) a += rest.w * (rest.left - rest.up - log_s);
-    return a / w - log(w) + log(p);
+    return bad ? __builtin_nan("") : a * row.over_w - w + p;
 }
 __device__ __forceinline__ double teacher_share(const Row& r, float v, float most_t, const Temper& t) { return exp(((double)v - (double)most_t) * t.inverse) * r.per_w; }
 __device__ __forceinline__ double student_share(const Row& r, float z, float base, const Temper& t) { return exp(((double)z - (double)base) * t.inverse) * r.per_p; }
@@ -129,13 +146,16 @@ __device__ __forceinline__ bool first_of(const Lists& l, int64_t r, int j, int64
     return true;
 }
 
+struct First { double share, weight; };     // of a lane's first entry, the student's and the teacher's, where no class repeats: there seldom is a second one
+
 // The outcomes of row r by a group of 2^shift lanes of a wavefront, all of which call it, with what they give for the row.  `skip`: the row does not count.
 template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& a, const Lists& l, const Temper& t, const Outcome& e, int64_t r, const Others& o, bool skip, bool repeats,
-                                                              int lane, int shift, float2& stats, float& most_t, float& base, Row& row) {
+                                                              int lane, int shift, float2& stats, float& most_t, float& base, Row& row, First& first) {
     const int lanes = 1 << shift;
     const T* z = row_start<T>(a, r);
     stats = make_float2(0.f, 0.f);
-    row = Row{0.0, 0.0, 0.f};
+    row = Row{0.0, 0.0, 0.0, 0.f};
+    first = First{0.0, 0.0};
     double divergence = 0.0;
     most_t = base = 0.f;
     if (!skip) {
@@ -158,12 +178,13 @@ template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& 
         for (int j = lane; j < l.k; j += lanes) {
             const int64_t c = l.cls(r * l.k + j);
             if (c < 0 || c >= a.classes) continue;
-            add_entry(s, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, most_t, base, !repeats || first_of(l, r, j, c), t);
+            const double share = add_entry(s, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, most_t, base, !repeats || first_of(l, r, j, c), t);
+            if (j == lane) first = First{share, s.w};
         }
         s.w = group_total(s.w, shift); s.p = group_total(s.p, shift); s.a = group_total(s.a, shift);
         const Rest left = rest_of(rest, most_t, base, o.top, t);
         row = ratios_of(s, left, o, bad != 0.f);
-        divergence = divergence_of(s, left, o, bad != 0.f, base, t);
+        divergence = divergence_of(s, left, o, row, bad != 0.f, base, t);
         stats = make_float2(finite(o.top), row.factor);
     }
     if (lane == 0) {
@@ -175,12 +196,14 @@ template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& 
 
 // The entries of row r, once its outcomes are known: f gets each one's class (inside the row) and slope; the slopes are kept for a later gradient.
 template <class T, class F> __device__ __forceinline__ void each_slope(const LogitRows& a, const Lists& l, const Temper& t, const Outcome& e, int64_t r, bool skip, bool repeats, int lane, int shift,
-                                                                     float most_t, float base, const Row& row, F&& f) {
+                                                                     float most_t, float base, const Row& row, const First& first, F&& f) {
     const T* z = row_start<T>(a, r);
     for (int j = lane; j < l.k; j += 1 << shift) {
         const int64_t c = skip ? -1 : l.cls(r * l.k + j);
         const bool inside = c >= 0 && c < a.classes;
-        const float slope = inside ? entry_slope(l, r, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, row, most_t, base, repeats, t) : 0.f;
+        float slope = 0.f;
+        if (inside) slope = j == lane && !repeats ? (float)(first.share * row.per_p - first.weight * row.per_w)
+                                                  : entry_slope(l, r, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, row, most_t, base, repeats, t);
         if (e.entries) e.entries[r * l.k + j] = slope;
         if (inside) f(c, slope);
     }
@@ -350,7 +373,8 @@ template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) di
     float2 stats;
     float most_t, base;
     Row end;
-    outcomes_of<T>(a, l, t, e, r, o, skip, repeats, row.lane, shift, stats, most_t, base, end);
+    First first;
+    outcomes_of<T>(a, l, t, e, r, o, skip, repeats, row.lane, shift, stats, most_t, base, end, first);
     T* q = static_cast<T*>(g.grad) + r * a.classes;
     const float by = FUSED ? *g.scale : 0.f;
     if (FUSED) {
@@ -358,7 +382,7 @@ template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) di
         wave_fence();       // (the entries' values stand where these stood)
     }
     if (FUSED || e.entries)
-        each_slope<T>(a, l, t, e, r, skip, repeats, row.lane, shift, most_t, base, end, [&](int64_t c, float slope) { if (FUSED) q[c] = Elem<T>::put(slope * by); });
+        each_slope<T>(a, l, t, e, r, skip, repeats, row.lane, shift, most_t, base, end, first, [&](int64_t c, float slope) { if (FUSED) q[c] = Elem<T>::put(slope * by); });
 }
 
 template <class T, int NV> __global__ void __launch_bounds__(256) distill_short_gradient_kernel(LogitRows a, Lists l, Temper t, Slopes g, int shift) {
@@ -557,7 +581,7 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
     }
     if (own && e.entries) e.entries[r * l.k + threadIdx.x] = slope;
     if (wave == WAVES - 1) {
-        const double divergence = divergence_of(s, left, o, odd, base, t);
+        const double divergence = divergence_of(s, left, o, row, odd, base, t);
         if (lane == 0) {
             e.divergences[r] = (float)divergence;
             e.kept[r] = 1.f;
@@ -652,8 +676,9 @@ template <class T> __global__ void __launch_bounds__(256) distill_join_kernel(Lo
         float2 stats;
         float most_t, base;
         Row end;
-        outcomes_of<T>(a, l, t, e, r, o, skip, twice_there, lane, 6, stats, most_t, base, end);
-        if (e.entries) each_slope<T>(a, l, t, e, r, skip, twice_there, lane, 6, most_t, base, end, [](int64_t, float) {});
+        First first;
+        outcomes_of<T>(a, l, t, e, r, o, skip, twice_there, lane, 6, stats, most_t, base, end, first);
+        if (e.entries) each_slope<T>(a, l, t, e, r, skip, twice_there, lane, 6, most_t, base, end, first, [](int64_t, float) {});
     }
 }
 
@@ -802,8 +827,19 @@ Cut cut_of(const LogitRows& a, int vec) {
     return {(int)((a.classes + part - 1) / part), part};
 }
 
+// Lanes for a short row: whole quads (see three_of), and of many rows more of them in a wavefront, for each of which a row's 64-bit functions cost
+// as much: 8192 x 1000 fp32 22.0 us with 64 lanes for a row, 17.4 with 32.
+constexpr int64_t kFewLanes = 1 << 18;
+Group short_group(const LogitRows& a, int vec) {
+    Group g = group_of(a.rows, a.classes, vec);
+    if (g.shift < 0) return g;
+    while (g.shift < 2) { g.shift++; g.vectors = g.vectors > 1 ? g.vectors / 2 : 1; }
+    while (g.vectors < kHeld && g.shift > 2 && a.rows << g.shift > kFewLanes) { g.shift--; g.vectors *= 2; }
+    return g;
+}
+
 bool in_parts(const LogitRows& a, int vec) {
-    return group_of(a.rows, a.classes, vec).shift < 0 && !((a.classes + vec - 1) / vec <= 16 * 512 && (a.rows >= kWholeRows || one_launch(a.rows, a.classes, vec)));
+    return short_group(a, vec).shift < 0 && !((a.classes + vec - 1) / vec <= 16 * 512 && (a.rows >= kWholeRows || one_launch(a.rows, a.classes, vec)));
 }
 
 int64_t distill_floats(const LogitRows& a, int dtype) {
@@ -821,7 +857,7 @@ template <class F> void in_slices(int64_t blocks, F&& f) {
 bool fuses(const LogitRows& a, int dtype) {
     const int vec = vec_of(dtype);
     if (a.rows * a.classes * (16 / vec) < (32ll << 20)) return false;
-    return group_of(a.rows, a.classes, vec).shift >= 0 || (a.rows >= 512 && a.classes <= kHeldLong * vec);
+    return short_group(a, vec).shift >= 0 || (a.rows >= 512 && a.classes <= kHeldLong * vec);
 }
 
 }  // namespace
@@ -870,7 +906,7 @@ extern "C" int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* li
         hipLaunchKernelGGL(distill_scale_kernel, dim3(1), dim3(256), 0, s, counted, blocks, scale_factor, scale);
     }
     const int vec = vec_of(rows->dtype);
-    const Group group = group_of(a.rows, a.classes, vec);
+    const Group group = short_group(a, vec);
     with_dtype(rows->dtype, [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
         if (group.shift >= 0) {
@@ -929,7 +965,7 @@ extern "C" int sd_distill_gradient(const sd_logit_rows* rows, const sd_top_lists
     const Slopes g{reinterpret_cast<const float2*>(stats), entries, scale, scale2, grad, unless_one != 0};
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int vec = vec_of(rows->dtype);
-    const Group group = group_of(a.rows, a.classes, vec);
+    const Group group = short_group(a, vec);
     // a launch that mostly finds nothing to do has no more workgroups than run at once: each takes time to come and go
     const auto blocks = [&](int64_t n) { return dim3(unless_one && n > 8 * num_cus() ? (unsigned)(8 * num_cus()) : blocks_for(n)); };
     with_dtype(rows->dtype, [&](auto* p) {
