@@ -847,11 +847,6 @@ int64_t distill_floats(const LogitRows& a, int dtype) {
     return kDistillSums + kept_floats(a.rows) + (in_parts(a, vec) ? ((int64_t)(sizeof(Others) + sizeof(int)) / 4 * a.rows * cut_of(a, vec).splits + 3) / 4 * 4 : 0);
 }
 
-// Launches of kernels whose workgroups do one thing each: at most 2^20 of them at a time (a grid of 2^32 work-items would be too large).
-template <class F> void in_slices(int64_t blocks, F&& f) {
-    for (int64_t from = 0; from < blocks; from += 1 << 20) f(from, (unsigned)(blocks - from < 1 << 20 ? blocks - from : 1 << 20));
-}
-
 // Whether the gradient leaves with the rows: it then costs one reading of the logits less and two launches more; a workgroup must be able to hold a
 // row, and there must be rows for all compute units.
 bool fuses(const LogitRows& a, int dtype) {

@@ -297,4 +297,9 @@ inline unsigned short_blocks(int64_t rows, int per) {
     return (unsigned)(n < kShortBlocks ? n : kShortBlocks);
 }
 
+// Launches of kernels whose workgroups do one thing each: at most 2^20 of them at a time (a grid of 2^32 work-items would be too large).
+template <class F> inline void in_slices(int64_t blocks, F&& f) {
+    for (int64_t from = 0; from < blocks; from += 1 << 20) f(from, (unsigned)(blocks - from < 1 << 20 ? blocks - from : 1 << 20));
+}
+
 }  // namespace sd

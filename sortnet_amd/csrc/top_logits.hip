@@ -310,13 +310,14 @@ constexpr double kLeastShare = 0x1p-60;
 
 // A workgroup per row, or per one of `splits` parts of `part` classes of a row.  What is not listed lies below the wavefront's bound, to which the exponentials are relative;
 // where they come out too small, or the bound too large, for fp32, the others are gone through again at the end.
-template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREADS, 8) top_rows_kernel(LogitRows a, Top t, int splits, int part, Parts out) {
+template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREADS, 8) top_rows_kernel(LogitRows a, Top t, int splits, int part, Parts out, int64_t first) {
     constexpr int V = Elem<T>::kVec, kSpan = THREADS * NV * V;
     using S = Shared<THREADS>;
     static_assert(64 * NV + kMostTop <= S::kRoom, "a wavefront's part of the list has room for all vectors behind the k that a cut of its own leaves");
     static_assert(64 * V <= S::kRoom, "and for the logits of a vector for each work-item");
     __shared__ S s;
-    for (int64_t b = blockIdx.x; b < a.rows * splits; b += gridDim.x) {
+    {
+        const int64_t b = first + blockIdx.x;
         const int64_t r = splits == 1 ? b : b / splits;
         const int q = (int)(b - r * splits), class0 = q * part, n = a.classes - class0 < part ? (int)a.classes - class0 : part;
         const T* row = row_start<T>(a, r);
@@ -616,9 +617,10 @@ extern "C" int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temper
             hipLaunchKernelGGL(top_short_kernel<T>, dim3(blocks_for(blocks)), dim3(256), 0, s, a, t, shift);
             return;
         }
-        const dim3 grid(blocks_for(lists));
         const auto launch = [&](auto threads, auto vectors) {
-            hipLaunchKernelGGL((top_rows_kernel<T, threads.value, vectors.value>), grid, dim3(threads.value), 0, s, a, t, plan.splits, (int)plan.part, parts);
+            in_slices(lists, [&](int64_t from, unsigned blocks) {
+                hipLaunchKernelGGL((top_rows_kernel<T, threads.value, vectors.value>), dim3(blocks), dim3(threads.value), 0, s, a, t, plan.splits, (int)plan.part, parts, from);
+            });
         };
         const auto with = [&](auto threads) { plan.vectors == 4 ? launch(threads, std::integral_constant<int, 4>()) : launch(threads, std::integral_constant<int, 2>()); };
         switch (plan.threads) {
