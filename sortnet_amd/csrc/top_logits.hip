@@ -236,8 +236,12 @@ template <int THREADS> struct Keeper {
         Others o{m, group_total(others.sum == 0.0 ? 0.0 : others.sum * in_powers(others.top, m, t), 6)};
         if (lane == 0) s.others[wave] = o;
         const uint32_t odd = share((__ballot(nan) ? 1u : 0u) | (__ballot(infinite) ? 2u : 0u), [](uint32_t x, uint32_t y) { return x | y; });
-        if (threadIdx.x == 0)
-            for (int w = 1; w < S::kWaves; w++) join(o, s.others[w].top, s.others[w].sum, t);
+        if (S::kWaves > 1) {
+            constexpr int kShift = S::kWaves == 2 ? 1 : S::kWaves == 4 ? 2 : 3;
+            const Others theirs = s.others[lane & (S::kWaves - 1)];
+            o.top = group_max(theirs.top, kShift);
+            o.sum = group_total(theirs.sum == 0.0 ? 0.0 : theirs.sum * in_powers(theirs.top, o.top, t), kShift);
+        }
         if (odd & 2) o = Others{FLT_MAX, INFINITY};
         if (odd & 1) o.sum = __builtin_nan("");
         return o;
@@ -316,206 +320,201 @@ template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREAD
     static_assert(64 * NV + kMostTop <= S::kRoom, "a wavefront's part of the list has room for all vectors behind the k that a cut of its own leaves");
     static_assert(64 * V <= S::kRoom, "and for the logits of a vector for each work-item");
     __shared__ S s;
-    {
-        const int64_t b = first + blockIdx.x;
-        const int64_t r = splits == 1 ? b : b / splits;
-        const int q = (int)(b - r * splits), class0 = q * part, n = a.classes - class0 < part ? (int)a.classes - class0 : part;
-        const T* row = row_start<T>(a, r);
-        const T* p = row + class0;
-        Keeper<THREADS> keep(s, t);
-        // a vector that is cut: its logits are among the others
-        const auto leave_vector = [&](Number x) {
-            float f[V];
-            read_again(f, p, number_class(x));
-            keep.leave_all(f);
-        };
-        double sum = 0.0;
-        float base = -FLT_MAX, power = 0.f;     // (nothing but -inf is summed as long as this is the bound)
-        bool again = false;
-        const int most = t.k + t.k / 4 < S::kMost ? t.k + t.k / 4 : S::kMost;      // vectors that a cut leaves
-        const auto rebase = [&]() {
-            if (keep.bound == base) return;
-            if (base > -FLT_MAX) sum *= in_powers(base, keep.bound, t);
-            base = keep.bound;
-            power = base * t.by;
-            if (!(fabsf(power) <= kNear)) { power = 0.f; again = true; }
-        };
-        for (int c0 = 0, step = 1; c0 < n; c0 += kSpan, step++) {
-            u32x4 v[NV];
-            load_vectors<T, THREADS, NV>(v, p, c0, n);
-            if (c0 == 0) {
-                float m = -INFINITY;
-                #pragma unroll
-                for (int k = 0; k < NV; k++) {
-                    float f[V];
-                    Elem<T>::unpack(v[k], f);
-                    m = fmaxf(m, largest(f));
-                }
-                // the largest number of 16 bits that at least k / wavefronts of the lanes' maxima reach
-                const int want = (t.k + S::kWaves - 1) / S::kWaves;
-                const uint32_t order = order_of(m);
-                uint32_t least = 0;
-                if (want <= 64) {
-                    #pragma unroll
-                    for (int bit = 31; bit >= 16; bit--) {
-                        const uint32_t next = least | 1u << bit;
-                        if (__popcll(__ballot(order >= next)) >= want) least = next;
-                    }
-                }
-                keep.raise(keep.share(least, Keeper<THREADS>::least_of), true);
-                rebase();
-                // what was derived from the vectors is derived again: kept, it would be twice their registers
-                #pragma unroll
-                for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
-            }
+    const int64_t b = first + blockIdx.x;
+    const int64_t r = splits == 1 ? b : b / splits;
+    const int q = (int)(b - r * splits), class0 = q * part, n = a.classes - class0 < part ? (int)a.classes - class0 : part;
+    const T* row = row_start<T>(a, r);
+    const T* p = row + class0;
+    Keeper<THREADS> keep(s, t);
+    // a vector that is cut: its logits are among the others
+    const auto leave_vector = [&](Number x) {
+        float f[V];
+        read_again(f, p, number_class(x));
+        keep.leave_all(f);
+    };
+    double sum = 0.0;
+    float base = -FLT_MAX, power = 0.f;     // (nothing but -inf is summed as long as this is the bound)
+    bool again = false;
+    const int most = t.k + t.k / 4 < S::kMost ? t.k + t.k / 4 : S::kMost;      // vectors that a cut leaves
+    const auto rebase = [&]() {
+        if (keep.bound == base) return;
+        if (base > -FLT_MAX) sum *= in_powers(base, keep.bound, t);
+        base = keep.bound;
+        power = base * t.by;
+        if (!(fabsf(power) <= kNear)) { power = 0.f; again = true; }
+    };
+    for (int c0 = 0, step = 1; c0 < n; c0 += kSpan, step++) {
+        u32x4 v[NV];
+        load_vectors<T, THREADS, NV>(v, p, c0, n);
+        if (c0 == 0) {
+            float m = -INFINITY;
             #pragma unroll
-            for (int k = 0; k < NV; k += 2) {
-                asm volatile("" : "+v"(v[k]), "+v"(v[k + 1]), "+v"(sum));      // (two vectors after two: all of them unpacked would not fit)
-                float f[2][V], m[2];
-                bool listed[2];
-                #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    Elem<T>::unpack(v[k + h], f[h]);
-                    m[h] = largest(f[h]);
-                    listed[h] = m[h] >= keep.bound;
-                }
-                const auto column = [&](int h) { return column_of<V>(c0 + ((int)threadIdx.x + (k + h) * THREADS) * V, n); };
-                const int had = keep.mine;
-                const uint64_t lanes[2] = {__ballot(listed[0]), __ballot(listed[1])};
-                if (lanes[0] | lanes[1]) {
-                    #pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        if (lanes[h]) keep.push(lanes[h], listed[h], number_of(order_of(m[h]), column(h)));
-                }
-                float part[2];
-                #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    #pragma unroll
-                    for (int i = 0; i < V; i++) f[h][i] = __builtin_amdgcn_exp2f(fmaf(f[h][i], t.by, -power));
-                    part[h] = tree(f[h]);
-                }
-                if (__ballot(part[0] + part[1] != part[0] + part[1])) {     // a NaN is above all: the vector's number is to say so, and has to be on the list
-                    #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        const bool nan = part[h] != part[h], more = nan && !listed[h];
-                        const Number x = number_of(0xffffffffu, column(h));
-                        if (nan && listed[h]) s.list[keep.wave][had + (h ? __popcll(lanes[0]) : 0) + keep.before(lanes[h])] = x;
-                        keep.push(__ballot(more), more, x);
-                        keep.nan |= nan;
-                        part[h] = nan ? 0.f : part[h];
-                    }
-                }
-                sum += (double)((listed[0] ? 0.f : part[0]) + (listed[1] ? 0.f : part[1]));
-            }
-            // The wavefronts go on by themselves; they meet, and cut the list together, behind the first, second, fourth, .. and last of their steps.
-            const bool last = c0 + kSpan >= n;
-            if (last || (step & (step - 1)) == 0) {
-                keep.settle();
-                if (keep.all > most) { keep.template cut<false>(most, leave_vector); rebase(); }
-            }
-            if (!last && keep.mine > S::kRoom - 64 * NV) { keep.template cut<true>(S::kRoom - 64 * NV, leave_vector); rebase(); }
-        }
-        // The logits of the listed vectors.  Each of these has one that reaches the least of their largest ones.
-        keep.gather();
-        const Number x = (int)threadIdx.x < keep.all ? s.first[threadIdx.x] : 0ull;
-        const uint32_t least = keep.share_lanes(x != 0ull ? number_order(x) : ~0u, Keeper<THREADS>::least_of);
-        keep.bound = -FLT_MAX;
-        if (keep.all >= t.k) keep.raise(least, true);
-        keep.mine = 0;
-        if (__ballot(x != 0ull)) {
-            float f[V];
-            const int at = x != 0ull ? number_class(x) : 0;
-            if (x != 0ull) read_again(f, p, at);
-            #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const bool listed = x != 0ull && !(f[i] < keep.bound);      // (a NaN, too)
-                const uint64_t lanes = __ballot(listed);
-                if (lanes) keep.push(lanes, listed, number_of(order_of(f[i]), class0 + at + i));
-                f[i] = listed ? -INFINITY : f[i];
-            }
-            if (x != 0ull) keep.leave_all(f);
-        }
-        keep.settle();
-        if (keep.all > THREADS) keep.template cut<false>(S::kMost, [&](Number y) { keep.leave(value_of(number_order(y))); });
-        if (splits == 1) keep.template finish<T>(row, r);
-        else {
-            Number* numbers = out.numbers + (r * splits + q) * t.k;
-            keep.sort([&](int place, Number y) { numbers[place] = y; });
-            for (int i = keep.all + threadIdx.x; i < t.k; i += THREADS) numbers[i] = 0ull;
-        }
-        // (where fewer than k logits are above -inf there are no others)
-        if (!again) join(keep.others, base, sum, t);
-        Others o = keep.all_others();
-        const uint32_t bases = keep.share(order_of(again ? INFINITY : base), [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-        if (threadIdx.x == 0) {
-            const float highest = value_of(bases);
-            s.again = keep.all >= t.k && o.sum == o.sum && highest > -FLT_MAX && (highest == INFINITY || !(o.sum * in_powers(o.top, highest, t) >= kLeastShare));
-        }
-        __syncthreads();
-        if (s.again) {
-            const Number kth = s.kth;
-            keep.others = Others{-INFINITY, 0.0};
-            #pragma unroll 1
-            for (int c = (int)threadIdx.x * V; c < n; c += THREADS * V) {
+            for (int k = 0; k < NV; k++) {
                 float f[V];
-                const int at = column_of<V>(c, n);
-                Elem<T>::unpack(without_first<T>(load16(p + at), c - at), f);
-                #pragma unroll
-                for (int i = 0; i < V; i++)
-                    if (number_of(order_of(f[i]), class0 + at + i) < kth) keep.leave(f[i]);
+                Elem<T>::unpack(v[k], f);
+                m = fmaxf(m, largest(f));
             }
-            o = keep.all_others();
+            // the largest number of 16 bits that at least k / wavefronts of the lanes' maxima reach
+            const int want = (t.k + S::kWaves - 1) / S::kWaves;
+            const uint32_t order = order_of(m);
+            uint32_t least = 0;
+            if (want <= 64) {
+                #pragma unroll
+                for (int bit = 31; bit >= 16; bit--) {
+                    const uint32_t next = least | 1u << bit;
+                    if (__popcll(__ballot(order >= next)) >= want) least = next;
+                }
+            }
+            keep.raise(keep.share(least, Keeper<THREADS>::least_of), true);
+            rebase();
+            // what was derived from the vectors is derived again: kept, it would be twice their registers
+            #pragma unroll
+            for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
         }
-        if (threadIdx.x == 0) {
-            if (splits == 1) keep.store_rest(o, r);
-            else out.others[r * splits + q] = o;
+        #pragma unroll
+        for (int k = 0; k < NV; k += 2) {
+            asm volatile("" : "+v"(v[k]), "+v"(v[k + 1]), "+v"(sum));      // (two vectors after two: all of them unpacked would not fit)
+            float f[2][V], m[2];
+            bool listed[2];
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                Elem<T>::unpack(v[k + h], f[h]);
+                m[h] = largest(f[h]);
+                listed[h] = m[h] >= keep.bound;
+            }
+            const auto column = [&](int h) { return column_of<V>(c0 + ((int)threadIdx.x + (k + h) * THREADS) * V, n); };
+            const int had = keep.mine;
+            const uint64_t lanes[2] = {__ballot(listed[0]), __ballot(listed[1])};
+            if (lanes[0] | lanes[1]) {
+                #pragma unroll
+                for (int h = 0; h < 2; h++)
+                    if (lanes[h]) keep.push(lanes[h], listed[h], number_of(order_of(m[h]), column(h)));
+            }
+            float part[2];
+            #pragma unroll
+            for (int h = 0; h < 2; h++) {
+                #pragma unroll
+                for (int i = 0; i < V; i++) f[h][i] = __builtin_amdgcn_exp2f(fmaf(f[h][i], t.by, -power));
+                part[h] = tree(f[h]);
+            }
+            if (__ballot(part[0] + part[1] != part[0] + part[1])) {     // a NaN is above all: the vector's number is to say so, and has to be on the list
+                #pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const bool nan = part[h] != part[h], more = nan && !listed[h];
+                    const Number x = number_of(0xffffffffu, column(h));
+                    if (nan && listed[h]) s.list[keep.wave][had + (h ? __popcll(lanes[0]) : 0) + keep.before(lanes[h])] = x;
+                    keep.push(__ballot(more), more, x);
+                    keep.nan |= nan;
+                    part[h] = nan ? 0.f : part[h];
+                }
+            }
+            sum += (double)((listed[0] ? 0.f : part[0]) + (listed[1] ? 0.f : part[1]));
         }
-        __syncthreads();
+        // The wavefronts go on by themselves; they meet, and cut the list together, behind the first, second, fourth, .. and last of their steps.
+        const bool last = c0 + kSpan >= n;
+        if (last || (step & (step - 1)) == 0) {
+            keep.settle();
+            if (keep.all > most) { keep.template cut<false>(most, leave_vector); rebase(); }
+        }
+        if (!last && keep.mine > S::kRoom - 64 * NV) { keep.template cut<true>(S::kRoom - 64 * NV, leave_vector); rebase(); }
+    }
+    // The logits of the listed vectors.  Each of these has one that reaches the least of their largest ones.
+    keep.gather();
+    const Number x = (int)threadIdx.x < keep.all ? s.first[threadIdx.x] : 0ull;
+    const uint32_t least = keep.share_lanes(x != 0ull ? number_order(x) : ~0u, Keeper<THREADS>::least_of);
+    keep.bound = -FLT_MAX;
+    if (keep.all >= t.k) keep.raise(least, true);
+    keep.mine = 0;
+    if (__ballot(x != 0ull)) {
+        float f[V];
+        const int at = x != 0ull ? number_class(x) : 0;
+        if (x != 0ull) read_again(f, p, at);
+        #pragma unroll
+        for (int i = 0; i < V; i++) {
+            const bool listed = x != 0ull && !(f[i] < keep.bound);      // (a NaN, too)
+            const uint64_t lanes = __ballot(listed);
+            if (lanes) keep.push(lanes, listed, number_of(order_of(f[i]), class0 + at + i));
+            f[i] = listed ? -INFINITY : f[i];
+        }
+        if (x != 0ull) keep.leave_all(f);
+    }
+    keep.settle();
+    if (keep.all > THREADS) keep.template cut<false>(S::kMost, [&](Number y) { keep.leave(value_of(number_order(y))); });
+    if (splits == 1) keep.template finish<T>(row, r);
+    else {
+        Number* numbers = out.numbers + (r * splits + q) * t.k;
+        keep.sort([&](int place, Number y) { numbers[place] = y; });
+        for (int i = keep.all + threadIdx.x; i < t.k; i += THREADS) numbers[i] = 0ull;
+    }
+    // (where fewer than k logits are above -inf there are no others)
+    if (!again) join(keep.others, base, sum, t);
+    Others o = keep.all_others();
+    const uint32_t bases = keep.share(order_of(again ? INFINITY : base), [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+    if (threadIdx.x == 0) {
+        const float highest = value_of(bases);
+        s.again = keep.all >= t.k && o.sum == o.sum && highest > -FLT_MAX && (highest == INFINITY || !(o.sum * in_powers(o.top, highest, t) >= kLeastShare));
+    }
+    __syncthreads();
+    if (s.again) {
+        const Number kth = s.kth;
+        keep.others = Others{-INFINITY, 0.0};
+        #pragma unroll 1
+        for (int c = (int)threadIdx.x * V; c < n; c += THREADS * V) {
+            float f[V];
+            const int at = column_of<V>(c, n);
+            Elem<T>::unpack(without_first<T>(load16(p + at), c - at), f);
+            #pragma unroll
+            for (int i = 0; i < V; i++)
+                if (number_of(order_of(f[i]), class0 + at + i) < kth) keep.leave(f[i]);
+        }
+        o = keep.all_others();
+    }
+    if (threadIdx.x == 0) {
+        if (splits == 1) keep.store_rest(o, r);
+        else out.others[r * splits + q] = o;
     }
 }
 
 // A workgroup per row joins its parts' lists: of k / splits numbers of each list at least the least is a bound.
 constexpr int kJoin = 512;
-template <class T> __global__ void __launch_bounds__(kJoin) top_join_kernel(LogitRows a, Top t, int splits, Parts in) {
+template <class T> __global__ void __launch_bounds__(kJoin) top_join_kernel(LogitRows a, Top t, int splits, Parts in, int64_t first) {
     using S = Shared<kJoin>;
     constexpr int kTurn = (S::kRoom - kMostTop) / 64;      // numbers of a work-item before the lists' lengths are looked at
     __shared__ S s;
-    for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        Keeper<kJoin> keep(s, t);
-        const Number* numbers = in.numbers + r * splits * t.k;
-        const int total = splits * t.k, nth = (t.k + splits - 1) / splits - 1, most = t.k + t.k / 4;
-        uint32_t least = ~0u;       // (by their orders: lists with nothing there have 0)
-        for (int q = threadIdx.x; q < splits; q += kJoin) {
-            least = Keeper<kJoin>::least_of(least, number_order(numbers[q * t.k + nth]));
-            const Others o = in.others[r * splits + q];
-            if (o.sum != o.sum) keep.nan = true;
-            else if (o.sum == INFINITY) keep.infinite = true;
-            else join(keep.others, o.top, o.sum, t);
-        }
-        keep.raise(keep.share_lanes(least, Keeper<kJoin>::least_of), true);
-        for (int i0 = 0; i0 < total; i0 += kTurn * kJoin) {
-            const uint32_t from = order_of(keep.bound);     // (a NaN is above every bound)
-            #pragma unroll
-            for (int i = 0; i < kTurn; i++) {
-                const int at = i0 + i * kJoin + threadIdx.x;
-                const Number x = at < total ? numbers[at] : 0ull;
-                const bool listed = x != 0ull && number_order(x) >= from;
-                const uint64_t lanes = __ballot(listed);
-                if (lanes) keep.push(lanes, listed, x);
-                if (x != 0ull && !listed) keep.leave(value_of(number_order(x)));
-            }
-            keep.settle();
-            if (keep.all > kJoin || keep.longest > kMostTop) {
-                const auto leave = [&](Number y) { keep.leave(value_of(number_order(y))); };
-                if (keep.all > most) keep.template cut<false>(most, leave);
-                if (i0 + kTurn * kJoin < total && keep.mine > kMostTop) keep.template cut<true>(kMostTop, leave);
-            }
-        }
-        keep.template finish<T>(row_start<T>(a, r), r);
-        const Others o = keep.all_others();
-        if (threadIdx.x == 0) keep.store_rest(o, r);
-        __syncthreads();
+    const int64_t r = first + blockIdx.x;
+    Keeper<kJoin> keep(s, t);
+    const Number* numbers = in.numbers + r * splits * t.k;
+    const int total = splits * t.k, nth = (t.k + splits - 1) / splits - 1, most = t.k + t.k / 4;
+    uint32_t least = ~0u;       // (by their orders: lists with nothing there have 0)
+    for (int q = threadIdx.x; q < splits; q += kJoin) {
+        least = Keeper<kJoin>::least_of(least, number_order(numbers[q * t.k + nth]));
+        const Others o = in.others[r * splits + q];
+        if (o.sum != o.sum) keep.nan = true;
+        else if (o.sum == INFINITY) keep.infinite = true;
+        else join(keep.others, o.top, o.sum, t);
     }
+    keep.raise(keep.share_lanes(least, Keeper<kJoin>::least_of), true);
+    for (int i0 = 0; i0 < total; i0 += kTurn * kJoin) {
+        const uint32_t from = order_of(keep.bound);     // (a NaN is above every bound)
+        #pragma unroll
+        for (int i = 0; i < kTurn; i++) {
+            const int at = i0 + i * kJoin + threadIdx.x;
+            const Number x = at < total ? numbers[at] : 0ull;
+            const bool listed = x != 0ull && number_order(x) >= from;
+            const uint64_t lanes = __ballot(listed);
+            if (lanes) keep.push(lanes, listed, x);
+            if (x != 0ull && !listed) keep.leave(value_of(number_order(x)));
+        }
+        keep.settle();
+        if (keep.all > kJoin || keep.longest > kMostTop) {
+            const auto leave = [&](Number y) { keep.leave(value_of(number_order(y))); };
+            if (keep.all > most) keep.template cut<false>(most, leave);
+            if (i0 + kTurn * kJoin < total && keep.mine > kMostTop) keep.template cut<true>(kMostTop, leave);
+        }
+    }
+    keep.template finish<T>(row_start<T>(a, r), r);
+    const Others o = keep.all_others();
+    if (threadIdx.x == 0) keep.store_rest(o, r);
 }
 
 // Rows of at most 64 classes: 2^shift lanes of a wavefront per row, one class each, whose place is the number of classes before it.
@@ -629,7 +628,9 @@ extern "C" int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temper
             case 256: with(std::integral_constant<int, 256>()); break;
             default: with(std::integral_constant<int, 512>());
         }
-        if (plan.splits > 1) hipLaunchKernelGGL(top_join_kernel<T>, dim3(blocks_for(a.rows)), dim3(kJoin), 0, s, a, t, plan.splits, parts);
+        if (plan.splits > 1) {
+            in_slices(a.rows, [&](int64_t from, unsigned blocks) { hipLaunchKernelGGL(top_join_kernel<T>, dim3(blocks), dim3(kJoin), 0, s, a, t, plan.splits, parts, from); });
+        }
     });
     return check_launch("top_rows_kernel");
 }
