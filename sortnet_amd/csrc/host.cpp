@@ -972,7 +972,7 @@ struct Constraints {
         if (out.numel() == 0) return;
         const sd_logit_rows a = logit_rows(z);
         sd_constraints c{};
-        if (history.t.defined()) {
+        if (history.t.defined() && history.t.size(-1) > 0) {     // (a history of no places, which has no address, penalises nothing)
             c.history = history.t.data_ptr();
             c.history_bytes = (int)history.t.element_size();
             c.history_length = history.t.size(-1);
@@ -1003,8 +1003,8 @@ struct ConstrainNode : Node {
         given = c;
         given.z = given.history.t = given.bias.t = given.allowed.t = given.lengths = Tensor();
         for (Tensor& t : given.rows) t = Tensor();
-        logits = SavedVariable(c.z, false);
         const auto keep = [](SavedVariable& v, const Tensor& t) { if (t.defined()) v = SavedVariable(t, false); };
+        if (c.history.t.defined()) keep(logits, c.z);      // (else the gradient does not depend on them)
         keep(history, c.history.t); keep(allowed, c.allowed.t); keep(lengths, c.lengths);
         for (int k = 0; k < 3; k++) keep(rows[k], c.rows[k]);
     }
@@ -1024,6 +1024,7 @@ struct ConstrainNode : Node {
         }
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor g = incoming(*this, grads, 0);
+        if (!c.z.defined()) c.z = g;
         const c10::DeviceGuard guard(c.z.device());
         out[0] = at::empty(c.z.sizes(), c.z.options());
         c.call(&g, out[0]);

@@ -31,6 +31,7 @@ struct Shape {
     int64_t part;                               // columns of a workgroup, a multiple of 8
     bool far;                                   // results that the last-level cache cannot hold are stored past it
     int parts, group;                           // parts of a row, or (with one part) rows of a workgroup
+    uint32_t first;                             // of the launch's workgroups (see in_slices)
 };
 
 struct __attribute__((packed, aligned(1))) Bytes8 { uint32_t lo, hi; };
@@ -139,7 +140,8 @@ template <class T, int ALLOWED, int HISTORY, int KIND> __global__ void __launch_
     constexpr bool GRAD = KIND == kGradient, BIAS = KIND == kBiased;
     constexpr int V = Elem<T>::kVec, kAny = ALLOWED == kAll ? kBits : ALLOWED, kPer = HISTORY == kLong ? 1 : 2;     // (kPer: columns of a word of counts)
     __shared__ __align__(16) uint32_t counts[HISTORY ? kCountWords : 4];
-    const int64_t r0 = (int64_t)(blockIdx.x / s.parts) * s.group, c0 = (int64_t)(blockIdx.x % s.parts) * s.part;
+    const uint32_t block = s.first + blockIdx.x;
+    const int64_t r0 = (int64_t)(block / s.parts) * s.group, c0 = (int64_t)(block % s.parts) * s.part;
     const int rows = (int)(a.rows - r0 < s.group ? a.rows - r0 : s.group);
     const int columns = (int)(a.classes - c0 < s.part ? a.classes - c0 : s.part), width = (columns + 7) & ~7, vecs = columns / V, items = rows * vecs;
     const auto place = [&](int64_t r, int64_t outer, int64_t inner) {
@@ -315,9 +317,12 @@ static int shape_logits(const char* who, const sd_logit_rows* in, const sd_const
     with_dtype(in->dtype, [&](auto* t) {
         using T = std::remove_pointer_t<decltype(t)>;
         const auto launch = [&](auto allowed, auto with_history) {
-            if (grad) hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kGradient>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
-            else if (s.bias) hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kBiased>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
-            else hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kPlain>), dim3((unsigned)blocks), dim3(256), 0, stream, a, s);
+            in_slices(blocks, [&](int64_t from, unsigned n) {
+                s.first = (uint32_t)from;
+                if (grad) hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kGradient>), dim3(n), dim3(256), 0, stream, a, s);
+                else if (s.bias) hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kBiased>), dim3(n), dim3(256), 0, stream, a, s);
+                else hipLaunchKernelGGL((shape_kernel<T, allowed.value, with_history.value, kPlain>), dim3(n), dim3(256), 0, stream, a, s);
+            });
         };
         const auto with = [&](auto allowed) {
             if (!history) launch(allowed, std::integral_constant<int, kNone>());

@@ -229,10 +229,52 @@ def test_changed_inputs_before_the_backward():
         out.sum().backward()
 
 
+def test_logits_changed_after_a_mask():
+    """Under a mask alone the gradient does not depend on the logits: they are not kept, and may be changed."""
+    z = torch.randn(2, 3, 40, device="cuda")
+    flags = torch.rand(2, 3, 40, device="cuda") < 0.5
+    leaf = z.clone().requires_grad_()
+    logits = leaf * 1.0
+    out = F.constrain_logits(logits, allowed=flags)
+    with torch.no_grad():
+        logits.zero_()
+    up = torch.randn_like(z)
+    assert torch.equal(torch.autograd.grad(out, leaf, up)[0], up * flags)
+    out = F.constrain_logits(logits, torch.zeros(2, 3, 1, device="cuda", dtype=torch.int64), repetition=2.0)
+    with torch.no_grad():
+        logits.zero_()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(out, leaf, up)
+
+
 def test_empty_batches():
     z = torch.empty(0, 7, device="cuda", requires_grad=True)
     out = F.constrain_logits(z, torch.empty(0, 3, device="cuda", dtype=torch.int64), repetition=2.0, allowed=torch.ones(7, device="cuda", dtype=torch.bool))
     assert out.shape == (0, 7) and torch.autograd.grad(out.sum(), z)[0].shape == (0, 7)
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32], ids=str)
+def test_histories_of_no_places(kind):
+    """The first step of an answer: nothing was chosen yet, with and without lengths."""
+    z, _, g = make(3, 700, torch.bfloat16, 3, 5)
+    flags = (torch.rand(3, 700, generator=g) < 0.5).cuda()
+    none, lengths = torch.empty(3, 0, device="cuda", dtype=kind), torch.zeros(3, device="cuda", dtype=kind)
+    leaf, up = z.clone().requires_grad_(), torch.ones_like(z)
+    for given in (None, lengths):
+        out = F.constrain_logits(leaf, none, given, repetition=2.0, presence=1.0, frequency=torch.ones(3, device="cuda"), allowed=flags)
+        assert torch.equal(out.detach(), z.masked_fill(~flags, -math.inf))
+        assert torch.equal(torch.autograd.grad(out, leaf, up)[0], flags.to(z.dtype))
+
+
+def test_more_workgroups_than_a_launch_has():
+    rows, classes = (1 << 20) + 5, 4104
+    z = torch.randn(64, classes, device="cuda").half().repeat(rows // 64 + 1, 1)[:rows]
+    history = torch.randint(0, classes, (rows, 2), device="cuda", dtype=torch.int32)
+    out = F.constrain_logits(z, history, presence=8.0)
+    for r in range(0, rows, 1 << 16):
+        part, past = z[r:r + (1 << 16)], history[r:r + (1 << 16)].long()
+        want = part.scatter(1, past, part.gather(1, past) - 8.0)        # (exact: the difference is rounded to the type once on either side)
+        assert torch.equal(out[r:r + (1 << 16)], want), r
 
 
 def test_captured_and_on_other_streams():

@@ -114,6 +114,42 @@ def test_loss_and_gradient(rows, classes, k, dtype):
     check(z, values, chosen.int(), None, 1.0, weight=-3.0, up=16.0)
 
 
+@pytest.mark.parametrize("rows, classes, k, dtype", [(17001, 1003, 3, torch.bfloat16), (4200, 4100, 3, torch.float16), (1100, 8003, 40, torch.float32), (600, 30001, 256, torch.bfloat16),
+                                                     (512, 131072, 5, torch.bfloat16), (2100, 33001, 20, torch.float32), (70003, 2005, 2, torch.bfloat16)])
+def test_gradient_with_the_loss(rows, classes, k, dtype):
+    """Batches of 32 MiB and more, for which the gradient is made with the loss: some rows against the definition, all of them against the loss."""
+    z, values, chosen, rest, g = make(rows, classes, k, dtype, classes)
+    leaf = z.requires_grad_()
+    loss, divergences = losses.distill_loss(leaf, values, chosen, rest, temperature=0.8, weight=64.0)
+    grad, = torch.autograd.grad(loss, leaf, retain_graph=True)
+    counted = (chosen >= 0).any(1)
+    some = torch.cat((torch.tensor([0, 1, rows - 1]), torch.randint(0, rows, (30,), generator=g))).cuda()
+    share = int(counted[some].sum()) / int(counted.sum())
+    _, want_d, want_grad, _ = exact(z[some], values[some], chosen[some], rest[some], 0.8, 64.0 * share)
+    close(divergences[some], want_d, "divergences")
+    close(grad[some], want_grad, "gradient")
+    assert (grad[~counted] == 0).all() and (divergences[~counted] == 0).all()
+    # (a mean of numbers of fp32 in 64 bits and two products: rounded once at the end)
+    want = 64.0 * 0.8 ** 2 * divergences.double().sum() / counted.sum()
+    assert abs(loss.double() - want) <= 2 * U * want.abs()
+    twice, = torch.autograd.grad(loss, leaf, torch.tensor(-2.0, device="cuda"))
+    _, _, want_grad, _ = exact(z[some], values[some], chosen[some], rest[some], 0.8, -128.0 * share)
+    close(twice[some], want_grad, "gradient")
+
+
+def test_more_workgroups_than_a_launch_has():
+    rows = (1 << 26) + 70
+    z = torch.randn(1 << 12, 12, device="cuda").half().repeat((1 << 14) + 1, 1)[:rows].requires_grad_()
+    chosen = torch.full((rows, 1), 3, device="cuda", dtype=torch.int32)
+    values = torch.zeros(rows, 1, device="cuda")
+    loss, divergences = losses.distill_loss(z, values, chosen, weight=float(rows))
+    grad, = torch.autograd.grad(loss, z)
+    assert torch.equal(divergences[:1 << 12], divergences[1 << 25:(1 << 25) + (1 << 12)]) and torch.equal(grad[:1 << 12], grad[1 << 25:(1 << 25) + (1 << 12)])
+    assert torch.equal(divergences[-70:], divergences[:70]) and torch.equal(grad[-70:], grad[:70])
+    want = -torch.log_softmax(z[:1 << 12].detach().double(), 1)[:, 3]       # (q is 1 for the only entry)
+    assert ((divergences[:1 << 12] - want).abs() <= 2 * sum_error(12) + U * want.abs()).all()
+
+
 @pytest.mark.parametrize("temperature", [0.1, 0.5, 1.0, 3.0, 100.0])
 @pytest.mark.parametrize("teacher", TYPES, ids=str)
 def test_temperatures_and_types_of_the_teacher(teacher, temperature):

@@ -129,6 +129,16 @@ def test_strides(classes):
     assert torch.equal(F.top_logits(turned, 3)[1], F.top_logits(turned.contiguous(), 3)[1])
 
 
+def test_more_rows_than_a_launch_has():
+    rows = (1 << 20) + 5
+    z = torch.randn(rows, 70, device="cuda").half()
+    values, classes, rest = F.top_logits(z, 2)
+    assert torch.equal(values, z.topk(2, dim=1).values) and torch.equal(z.gather(1, classes.long()), values)
+    check(z[-40:], 2)
+    for got, want in zip(F.top_logits(z[-40:], 2), (values, classes, rest)):
+        assert torch.equal(got, want[-40:])
+
+
 def test_no_rows_and_no_gradient():
     z = torch.empty(0, 3, 7, device="cuda")
     values, classes, rest = F.top_logits(z, 2)
