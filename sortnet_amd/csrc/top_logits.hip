@@ -558,7 +558,7 @@ Plan plan_of(const LogitRows& a, int64_t k, int vec) {
     while (threads < most) threads *= 2;
     if (a.classes <= (int64_t)threads * 4 * vec) return {threads, 4, 1, a.classes};
     if (threads < 128) threads = 128;
-    while (threads < 256 && a.rows * threads < card) threads *= 2;
+    while (threads < 256 && a.rows * threads * 2 <= card) threads *= 2;
     const int64_t fit = card / (a.rows * threads), want = fit > 1 ? fit : 1, span = threads * vec;
     const int vectors = a.classes >= want * span * 4 ? 4 : 2;
     int64_t splits = (a.classes + span * vectors - 1) / (span * vectors);
