@@ -78,7 +78,7 @@ template <int THREADS> struct Shared {
     Number list[kWaves][kRoom];
     Number first[THREADS];                          // those of a list that is no longer than that, one behind the other
     Others others[kWaves];
-    uint32_t words[2][kWaves];
+    uint64_t words[2][kWaves];                      // (or as many of 32 bits)
     Number kth;                                     // the k-th number of a row or part
     int again;
 };
@@ -131,12 +131,12 @@ template <int THREADS> struct Keeper {
         mine += __popcll(lanes);
     }
     // a word of each wavefront, of which `op` makes one
-    template <class Op> __device__ __forceinline__ uint32_t share(uint32_t word, Op&& op) {
+    template <class Word, class Op> __device__ __forceinline__ Word share(Word word, Op&& op) {
         if (S::kWaves == 1) { __syncthreads(); return word; }
-        uint32_t* words = s.words[turn++ & 1];      // (the other ones may still be read)
+        Word* words = reinterpret_cast<Word*>(s.words[turn++ & 1]);      // (the other ones may still be read)
         if (lane == 0) words[wave] = word;
         __syncthreads();
-        uint32_t r = words[0];
+        Word r = words[0];
         #pragma unroll
         for (int w = 1; w < S::kWaves; w++) r = op(r, words[w]);
         return r;
@@ -164,33 +164,50 @@ template <int THREADS> struct Keeper {
     }
     // The list of more than `most` numbers becomes at least k and at most `most` of the largest of them; `out` gets the others.  OWN: the wavefront's alone.
     template <bool OWN, class Out> __device__ __forceinline__ void cut(int most, Out&& out) {
-        const auto shared = [&](uint32_t word, auto&& op) { return OWN ? word : share(word, op); };
+        constexpr int kOwn = 4;         // numbers that a lane has in registers meanwhile
+        const auto shared = [&](auto word, auto&& op) { return OWN ? word : share(word, op); };
         const Number* own = s.list[wave];
+        Number held[kOwn];
         uint32_t every = ~0u, some = 0u;
-        #pragma unroll 1
-        for (int i = lane; i < mine; i += 64) {
-            const uint32_t order = number_order(own[i]);
-            every &= order;
-            some |= order;
+        const auto look = [&](Number x) {
+            every &= number_order(x);
+            some |= number_order(x);
+        };
+        #pragma unroll
+        for (int h = 0; h < kOwn; h++) {
+            held[h] = lane + 64 * h < mine ? own[lane + 64 * h] : 0ull;
+            if (lane + 64 * h < mine) look(held[h]);
         }
+        #pragma unroll 1
+        for (int i = lane + 64 * kOwn; i < mine; i += 64) look(own[i]);
         const auto both = [](uint32_t a, uint32_t b) { return a & b; };
         const auto either = [](uint32_t a, uint32_t b) { return a | b; };
         every = shared(lanes_make(every, both), both);
         some = shared(lanes_make(some, either), either);
-        // the bits in which the orders differ are all that is looked for
+        // The bits in which the orders differ are all that is looked for, two at a time: three counts, of at most kRoom numbers in each wavefront, and one barrier.
         const uint32_t differ = every ^ some;
         const int high = differ == 0u ? 0 : 32 - __clz(differ);
         Number least = (Number)(high == 32 ? 0u : every >> high << high) << 32;     // the largest prefix found that k numbers reach
+        static_assert(S::kWaves * S::kRoom < 1 << 16, "a count of all wavefronts' numbers has 16 bits");
         #pragma unroll 1
-        for (int bit = 31 + high; bit >= 0; bit--) {
-            const Number next = least | 1ull << bit;
-            int c = 0;
+        for (int bit = 30 + high + (high & 1); bit >= 0; bit -= 2) {     // (of an odd number of bits the first one is one that all share, or none has)
+            const Number low = least | 1ull << bit, next = least | 2ull << bit, top = next | low;
+            uint64_t c = 0;
+            const auto count = [&](Number x) {
+                c += (uint64_t)__popcll(__ballot(x >= low)) | (uint64_t)__popcll(__ballot(x >= next)) << 16 | (uint64_t)__popcll(__ballot(x >= top)) << 32;
+            };
+            #pragma unroll
+            for (int h = 0; h < kOwn; h++) count(held[h]);
             #pragma unroll 1
-            for (int i = 0; i < mine; i += 64) c += __popcll(__ballot(lane + i < mine && own[lane + i] >= next));
-            c = (int)shared((uint32_t)c, [](uint32_t a, uint32_t b) { return a + b; });
-            if (c < t.k) continue;
-            least = next;
-            if (c <= most) break;
+            for (int i = 64 * kOwn; i < mine; i += 64) count(lane + i < mine ? own[lane + i] : 0ull);
+            c = shared(c, [](uint64_t a, uint64_t b) { return a + b; });
+            const int low_and_next = __builtin_amdgcn_readfirstlane((int)(uint32_t)c), reach[3] = {low_and_next & 0xffff, low_and_next >> 16 & 0xffff, __builtin_amdgcn_readfirstlane((int)(c >> 32))};
+            int reached;
+            if (reach[2] >= t.k) { least = top; reached = reach[2]; }
+            else if (reach[1] >= t.k) { least = next; reached = reach[1]; }
+            else if (reach[0] >= t.k) { least = low; reached = reach[0]; }
+            else continue;
+            if (reached <= most) break;
         }
         const int had = mine;
         mine = 0;
@@ -208,7 +225,7 @@ template <int THREADS> struct Keeper {
     __device__ __forceinline__ void gather() {
         int at = lane;
         if (S::kWaves > 1) {
-            uint32_t* words = s.words[turn++ & 1];
+            uint32_t* words = reinterpret_cast<uint32_t*>(s.words[turn++ & 1]);
             if (lane == 0) words[wave] = (uint32_t)mine;
             __syncthreads();
             for (int w = 0; w < wave; w++) at += (int)words[w];
@@ -257,7 +274,7 @@ template <int THREADS> struct Keeper {
             const uint64_t lanes = __ballot(none);
             int place = all + before(lanes);
             if (S::kWaves > 1) {
-                uint32_t* words = s.words[turn++ & 1];
+                uint32_t* words = reinterpret_cast<uint32_t*>(s.words[turn++ & 1]);
                 if (lane == 0) words[wave] = (uint32_t)__popcll(lanes);
                 __syncthreads();
                 for (int w = 0; w < wave; w++) place += (int)words[w];
