@@ -436,6 +436,7 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
     __shared__ double sums[WAVES][4];
     __shared__ double weights[kMostEntries];        // the teacher's, relative to the largest, and what
     __shared__ int theirs_of[kMostEntries];         // class each is for
+    __shared__ Row end;
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
     const int n = (int)a.classes, full = n / V, rest_at = full * V + (int)threadIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const T lowest = Elem<T>::put(-INFINITY);
@@ -540,12 +541,19 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
     }
     sum = wave_total(sum * (double)exp_at(finite(top) - finite(all), t));
     if (lane == 0) { sums[wave][0] = sum; sums[wave][1] = s.w; sums[wave][2] = s.p; sums[wave][3] = s.a; }
-    const Rest left = rest_of(rest, most_t, base, all, t);
     __syncthreads();
-    const double* totals = sums[lane & (WAVES - 1)];
-    const Others o{all, group_total(totals[0], kShift)};
-    s = Sums{group_total(totals[1], kShift), group_total(totals[2], kShift), group_total(totals[3], kShift)};
-    const Row row = ratios_of(s, left, o, odd);
+    Rest left;
+    Others o{all, 0.0};
+    if (wave == 0) {        // (the others wait: with four wavefronts to a unit that each did this it would take four times as long)
+        left = rest_of(rest, most_t, base, all, t);
+        const double* totals = sums[lane & (WAVES - 1)];
+        o.sum = group_total(totals[0], kShift);
+        s = Sums{group_total(totals[1], kShift), group_total(totals[2], kShift), group_total(totals[3], kShift)};
+        const Row row = ratios_of(s, left, o, odd);
+        if (lane == 0) end = row;
+    }
+    __syncthreads();
+    const Row row = end;
     if (FUSED) {
         if (row.factor == 0.f) clear_row(q, n, THREADS);
         else {
@@ -580,7 +588,7 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
         slope = (float)(share * row.per_p - weight * row.per_w);
     }
     if (own && e.entries) e.entries[r * l.k + threadIdx.x] = slope;
-    if (wave == WAVES - 1) {
+    if (wave == 0) {
         const double divergence = divergence_of(s, left, o, row, odd, base, t);
         if (lane == 0) {
             e.divergences[r] = (float)divergence;
