@@ -89,41 +89,43 @@ __device__ __forceinline__ double add_entry(Sums& s, const Entry& e, float most_
     return p;
 }
 
-// What a row comes to.  All is relative to most_t and base (of rows where no entry is above -inf, to 0), the rest, which may lie far above the entries, to the
-// larger of the two: W = sum_w exp(-up) + w_r, P = sum_p + S o, o = exp((top - base) / T),
-//   D = (sum_a exp(-up) - up sum_w exp(-up) + w_r (left - up - log(S o))) / W - log W + log P.
-// The four lanes of a quad hold the same row: one call of a 64-bit function, some 50 instructions, is for three numbers of it.
+// What a row comes to.  The entries' sums are relative to most_t and to their own largest logit (where none is above -inf, to 0); the rest, which may lie far above the
+// entries, to the larger of the two, and the student's outcomes to base, the largest of its logits: with p = exp((entries - base) / T), o = exp((top - base) / T),
+//   W = sum_w exp(-up) + w_r,  P = sum_p p + S o,  D = (exp(-up) (sum_a - (up + log p) sum_w) + w_r (left - up - log(S o))) / W - log W + log P.
+// The four lanes of a quad hold the same row: one call of a 64-bit function, some 50 instructions, is for up to four numbers of it.
 template <int LANE> __device__ __forceinline__ double of_quad(double v) {
     const uint64_t bits = __builtin_bit_cast(uint64_t, v);
     const uint32_t low = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)bits, LANE * 0x55, 0xf, 0xf, false);
     const uint32_t high = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(bits >> 32), LANE * 0x55, 0xf, 0xf, false);
     return __builtin_bit_cast(double, (uint64_t)high << 32 | low);
 }
-template <class F> __device__ __forceinline__ void three_of(double& x, double& y, double& z, F&& f) {
+template <class F> __device__ __forceinline__ void four_of(double& x, double& y, double& z, double& w, F&& f) {
     const int lane = threadIdx.x & 3;
-    const double v = f(lane == 0 ? x : lane == 1 ? y : z);
-    x = of_quad<0>(v); y = of_quad<1>(v); z = of_quad<2>(v);
+    const double v = f(lane == 0 ? x : lane == 1 ? y : lane == 2 ? z : w);
+    x = of_quad<0>(v); y = of_quad<1>(v); z = of_quad<2>(v); w = of_quad<3>(v);
 }
 
-struct Rest { double left, up, scale, w, o; };      // of the teacher's others, with exp(-up) and w_r, and o
-__device__ __forceinline__ Rest rest_of(double rest, float most_t, float base, float top, const Temper& t) {
-    const double left = rest - (double)most_t * t.inverse, up = left > 0.0 ? left : 0.0;
-    Rest e{left, up, -up, left - up, ((double)finite(top) - (double)base) * t.inverse};
-    three_of(e.scale, e.w, e.o, [](double v) { return exp(v); });
+struct Rest { double left, up, log_p, top, scale, w, p, o; };      // of the teacher's others; (top - base) / T; exp(-up), w_r, p and o
+__device__ __forceinline__ Rest rest_of(double rest, float most_t, float entries, float top, const Temper& t) {
+    const double left = rest - (double)most_t * t.inverse, up = left > 0.0 ? left : 0.0, high = (double)finite(top);
+    const double base = entries == -INFINITY ? high : fmax((double)entries, high);
+    const double log_p = entries == -INFINITY ? 0.0 : ((double)entries - base) * t.inverse, log_o = (high - base) * t.inverse;
+    Rest e{left, up, log_p, log_o, -up, left - up, log_p, log_o};
+    four_of(e.scale, e.w, e.p, e.o, [](double v) { return exp(v); });
     return e;
 }
-struct Row { double over_w, per_w, per_p; float factor; };      // 1 / W, the same for sum_w, 1 / P; factor = (p_r - q_r) / S
+struct Row { double over_w, per_w, per_p; float factor; };      // 1 / W, the same for sum_w, p / P; factor = (p_r - q_r) / S
 __device__ __forceinline__ Row ratios_of(const Sums& s, const Rest& rest, const Others& o, bool bad) {
-    double w = s.w * rest.scale + rest.w, p = s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0), others = o.sum;
-    three_of(w, p, others, [](double v) { return 1.0 / v; });
+    double w = s.w * rest.scale + rest.w, p = s.p * rest.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0), others = o.sum, one = 1.0;
+    four_of(w, p, others, one, [](double v) { return 1.0 / v; });
     if (bad) p = __builtin_nan("");
-    return Row{w, rest.scale * w, p, o.sum > 0.0 || bad ? (float)(rest.o * p - rest.w * w * others) : 0.f};
+    return Row{w, rest.scale * w, rest.p * p, o.sum > 0.0 || bad ? (float)(rest.o * p - rest.w * w * others) : 0.f};
 }
-__device__ __forceinline__ double divergence_of(const Sums& s, const Rest& rest, const Others& o, const Row& row, bool bad, float base, const Temper& t) {
-    double log_s = o.sum, w = s.w * rest.scale + rest.w, p = s.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0);
-    three_of(log_s, w, p, [](double v) { return log(v); });
-    log_s = o.sum > 0.0 ? log_s + ((double)finite(o.top) - (double)base) * t.inverse : -INFINITY;
-    double a = rest.scale != 0.0 ? s.a * rest.scale - rest.up * (s.w * rest.scale) : 0.0;
+__device__ __forceinline__ double divergence_of(const Sums& s, const Rest& rest, const Others& o, const Row& row, bool bad) {
+    double log_s = o.sum, w = s.w * rest.scale + rest.w, p = s.p * rest.p + (o.sum > 0.0 ? o.sum * rest.o : 0.0), one = 1.0;
+    four_of(log_s, w, p, one, [](double v) { return log(v); });
+    log_s = o.sum > 0.0 ? log_s + rest.top : -INFINITY;
+    double a = rest.scale != 0.0 ? rest.scale * (s.a - (rest.up + rest.log_p) * s.w) : 0.0;
     if (rest.w != 0.0) a += rest.w * (rest.left - rest.up - log_s);
     return bad ? __builtin_nan("") : a * row.over_w - w + p;
 }
@@ -172,8 +174,9 @@ template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& 
         const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
         if (rest != rest || o.sum != o.sum) bad = 1.f;
         most_t = group_max(most_t, shift); base = group_max(base, shift); bad = group_max(bad, shift);
-        base = fmaxf(base, finite(o.top));
+        const float entries = base;
         if (most_t == -INFINITY) most_t = 0.f;
+        if (base == -INFINITY) base = 0.f;
         Sums s{0.0, 0.0, 0.0};
         for (int j = lane; j < l.k; j += lanes) {
             const int64_t c = l.cls(r * l.k + j);
@@ -182,9 +185,9 @@ template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& 
             if (j == lane) first = First{share, s.w};
         }
         s.w = group_total(s.w, shift); s.p = group_total(s.p, shift); s.a = group_total(s.a, shift);
-        const Rest left = rest_of(rest, most_t, base, o.top, t);
+        const Rest left = rest_of(rest, most_t, entries, o.top, t);
         row = ratios_of(s, left, o, bad != 0.f);
-        divergence = divergence_of(s, left, o, row, bad != 0.f, base, t);
+        divergence = divergence_of(s, left, o, row, bad != 0.f);
         stats = make_float2(finite(o.top), row.factor);
     }
     if (lane == 0) {
@@ -427,18 +430,22 @@ template <class T, int NV, int THREADS> struct Marks {
 
 // The workgroup holds a row in its registers, at most 16 vectors per work-item, and an entry per work-item.  FUSED: the logits are read once and the gradient leaves
 // with the row.  FAR: logits that the last-level cache cannot hold are read past it.
-// A row per workgroup and no loop over them: the constants of the 64-bit functions would be kept in registers that the row needs.
+// A row per workgroup and no loop over them: the constants of the 64-bit functions would be kept in registers that the row needs.  What the entries give is summed
+// while the row is on its way; when it is there a wavefront's part, one barrier and a few 64-bit functions of one wavefront stand between its sums and its gradient.
 template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __launch_bounds__(THREADS, 4) distill_held_kernel(LogitRows a, Lists l, Temper t, Outcome e, Slopes g, int64_t row0) {
     constexpr int V = Elem<T>::kVec, WAVES = THREADS / 64, kChunk = NV < 32 / V ? NV : 32 / V;
     constexpr int kShift = WAVES == 4 ? 2 : WAVES == 8 ? 3 : 4;      // (the wavefronts' results in the lanes of each group of so many)
+    static_assert(kMostEntries <= 256 && WAVES >= 4, "the first four wavefronts have the entries");
     __shared__ Marks<T, NV + 1, THREADS> marks;       // (one more: the values behind the last whole vector)
-    __shared__ float maxima[WAVES][4];
-    __shared__ double sums[WAVES][4];
+    __shared__ float most[4][2];
+    __shared__ double sums[4][3];
+    __shared__ Others others[WAVES];
     __shared__ double weights[kMostEntries];        // the teacher's, relative to the largest, and what
     __shared__ int theirs_of[kMostEntries];         // class each is for
     __shared__ Row end;
+    __shared__ float end_top;
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
-    const int n = (int)a.classes, full = n / V, rest_at = full * V + (int)threadIdx.x, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int n = (int)a.classes, full = n / V, rest_at = full * V + (int)threadIdx.x, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const T lowest = Elem<T>::put(-INFINITY);
     const float by = FUSED ? *g.scale : 0.f;
     const int64_t r = a.rows - 1 - (row0 + blockIdx.x);     // (the producer's last rows may be in the caches)
@@ -474,6 +481,12 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
         return;
     }
     const T* p = row_start<T>(a, r);
+    // the entries' logits are asked for before the row: loads arrive in their order
+    T theirs_z = lowest;
+    if (64 * wave < l.k) {
+        if (FUSED) decode(entry);
+        theirs_z = p[cls >= 0 && cls < n ? cls : 0];
+    }
     u32x4 v[NV];
     #pragma unroll
     for (int k = 0; k < NV; k++) {
@@ -482,18 +495,40 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
         v[k] = FAR ? stream16(p + at) : load16(p + at);
     }
     T last = p[rest_at < n ? rest_at : n - 1];
-    // the entry, while the row is on its way
-    if (FUSED) decode(entry);
-    const bool inside = cls >= 0 && cls < n;
-    const T theirs_z = p[inside ? cls : 0];
     const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
+    const bool inside = cls >= 0 && cls < n;
     marks.clear();
     __syncthreads();
     // (the values behind the last whole vector are held by the first work-items, one each, as the first value of a vector of their own)
     if (inside) marks.mark(cls < full * V ? cls : (NV * THREADS + (cls - full * V)) * V);
     if (own) theirs_of[threadIdx.x] = inside ? cls : -1;
+    if (wave < 4) {
+        if (inside) z = Elem<T>::get(theirs_z);
+        const float m0 = group_max(inside ? value : -INFINITY, 6), m1 = group_max(z, 6);
+        if (lane == 0) { most[wave][0] = m0; most[wave][1] = m1; }
+    }
     __syncthreads();
     const bool repeats = marks.repeats != 0;
+    float most_t = 0.f, entries = 0.f;
+    double share = 0.0;
+    if (wave < 4) {
+        most_t = fmaxf(fmaxf(most[0][0], most[1][0]), fmaxf(most[2][0], most[3][0]));
+        entries = fmaxf(fmaxf(most[0][1], most[1][1]), fmaxf(most[2][1], most[3][1]));
+        if (most_t == -INFINITY) most_t = 0.f;
+        Sums s{0.0, 0.0, 0.0};
+        if (64 * wave < l.k) {
+            if (inside) {
+                bool first = true;
+                if (repeats)
+                    for (int i = 0; i < (int)threadIdx.x; i++) first = first && theirs_of[i] != cls;
+                share = add_entry(s, Entry{cls, value, z}, most_t, entries == -INFINITY ? 0.f : entries, first, t);
+                weights[threadIdx.x] = s.w;
+            }
+            if (rest != rest || (cls >= 0 && (!inside || value != value || z != z))) s.p = __builtin_nan("");      // (something is wrong with the row)
+            s.w = wave_total(s.w); s.p = wave_total(s.p); s.a = wave_total(s.a);
+        }
+        if (lane == 0) { sums[wave][0] = s.w; sums[wave][1] = s.p; sums[wave][2] = s.a; }
+    }
     float top = -INFINITY;
     double sum = 0.0;
     #pragma unroll
@@ -513,47 +548,31 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
         asm volatile("" : "+v"(top), "+v"(sum));     // (here, while the next vectors are on their way, and not behind them all)
     }
     if (rest_at >= n || (marks.bits(NV) & 1u)) last = lowest;
-    if (inside) z = Elem<T>::get(theirs_z);
     float f1[1] = {Elem<T>::get(last)};
     take(f1, top, sum, t);
-    // all work-items': the largest of the others, of the teacher's and of the student's entries, and whether something is wrong
-    bool odd = sum != sum || rest != rest || (cls >= 0 && (!inside || value != value || z != z));
     {
-        const float m0 = group_max(top, 6), m1 = group_max(inside ? value : -INFINITY, 6), m2 = group_max(z, 6);
-        if (lane == 0) { maxima[wave][0] = m0; maxima[wave][1] = m1; maxima[wave][2] = m2; }
+        const float m = group_max(top, 6);
+        sum = wave_total(sum * (double)exp_at(finite(top) - finite(m), t));
+        if (lane == 0) others[wave] = Others{m, sum};
     }
-    odd = __syncthreads_or(odd);
-    const float* theirs = maxima[lane & (WAVES - 1)];
-    const float all = group_max(theirs[0], kShift);
-    float most_t = group_max(theirs[1], kShift), base = fmaxf(group_max(theirs[2], kShift), finite(all));
-    if (most_t == -INFINITY) most_t = 0.f;
-    Sums s{0.0, 0.0, 0.0};
-    double share = 0.0;
-    if (64 * wave < l.k) {
-        if (inside) {
-            bool first = true;
-            if (repeats)
-                for (int i = 0; i < (int)threadIdx.x; i++) first = first && theirs_of[i] != cls;
-            share = add_entry(s, Entry{cls, value, z}, most_t, base, first, t);
-            weights[threadIdx.x] = s.w;
-        }
-        s.w = wave_total(s.w); s.p = wave_total(s.p); s.a = wave_total(s.a);
-    }
-    sum = wave_total(sum * (double)exp_at(finite(top) - finite(all), t));
-    if (lane == 0) { sums[wave][0] = sum; sums[wave][1] = s.w; sums[wave][2] = s.p; sums[wave][3] = s.a; }
     __syncthreads();
+    Others o{-INFINITY, 0.0};
+    Sums s{0.0, 0.0, 0.0};
     Rest left;
-    Others o{all, 0.0};
+    bool odd = false;
     if (wave == 0) {        // (the others wait: with four wavefronts to a unit that each did this it would take four times as long)
-        left = rest_of(rest, most_t, base, all, t);
-        const double* totals = sums[lane & (WAVES - 1)];
-        o.sum = group_total(totals[0], kShift);
-        s = Sums{group_total(totals[1], kShift), group_total(totals[2], kShift), group_total(totals[3], kShift)};
+        const Others part = others[lane & (WAVES - 1)];
+        o.top = group_max(part.top, kShift);
+        o.sum = group_total(part.sum * (double)exp_at(finite(part.top) - finite(o.top), t), kShift);
+        s = Sums{group_total(sums[lane & 3][0], 2), group_total(sums[lane & 3][1], 2), group_total(sums[lane & 3][2], 2)};
+        odd = o.sum != o.sum || s.p != s.p;
+        left = rest_of(rest, most_t, entries, o.top, t);
         const Row row = ratios_of(s, left, o, odd);
-        if (lane == 0) end = row;
+        if (lane == 0) { end = row; end_top = finite(o.top); }
     }
     __syncthreads();
     const Row row = end;
+    const float high = end_top;
     if (FUSED) {
         if (row.factor == 0.f) clear_row(q, n, THREADS);
         else {
@@ -562,7 +581,7 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
             asm("" : "+v"(item));
             #pragma unroll
             for (int k = 0; k < NV; k++) asm("" : "+v"(v[k]));
-            const float high = finite(all), w = row.factor * by;
+            const float w = row.factor * by;
             #pragma unroll
             for (int k = 0; k < NV; k++) {
                 const int i = item + k * THREADS;
@@ -589,11 +608,11 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
     }
     if (own && e.entries) e.entries[r * l.k + threadIdx.x] = slope;
     if (wave == 0) {
-        const double divergence = divergence_of(s, left, o, row, odd, base, t);
+        const double divergence = divergence_of(s, left, o, row, odd);
         if (lane == 0) {
             e.divergences[r] = (float)divergence;
             e.kept[r] = 1.f;
-            if (e.stats) e.stats[r] = make_float2(finite(all), row.factor);
+            if (e.stats) e.stats[r] = make_float2(high, row.factor);
         }
     }
     if (FUSED) {
