@@ -198,8 +198,8 @@ template <class T> __device__ __forceinline__ void outcomes_of(const LogitRows& 
 }
 
 // The entries of row r, once its outcomes are known: f gets each one's class (inside the row) and slope; the slopes are kept for a later gradient.
-template <class T, class F> __device__ __forceinline__ void each_slope(const LogitRows& a, const Lists& l, const Temper& t, const Outcome& e, int64_t r, bool skip, bool repeats, int lane, int shift,
-                                                                     float most_t, float base, const Row& row, const First& first, F&& f) {
+template <class T> __device__ __forceinline__ void each_slope(const LogitRows& a, const Lists& l, const Temper& t, const Outcome& e, int64_t r, bool skip, bool repeats, int lane, int shift,
+                                                                     float most_t, float base, const Row& row, const First& first) {
     const T* z = row_start<T>(a, r);
     for (int j = lane; j < l.k; j += 1 << shift) {
         const int64_t c = skip ? -1 : l.cls(r * l.k + j);
@@ -207,8 +207,7 @@ template <class T, class F> __device__ __forceinline__ void each_slope(const Log
         float slope = 0.f;
         if (inside) slope = j == lane && !repeats ? (float)(first.share * row.per_p - first.weight * row.per_w)
                                                   : entry_slope(l, r, Entry{c, l.value(r * l.k + j), Elem<T>::get(z[c])}, row, most_t, base, repeats, t);
-        if (e.entries) e.entries[r * l.k + j] = slope;
-        if (inside) f(c, slope);
+        e.entries[r * l.k + j] = slope;
     }
 }
 
@@ -327,7 +326,7 @@ template <class T, int NV> __device__ __forceinline__ Others others_of(const Hel
 }
 
 // the row's part of a gradient, the entries' classes left to be stored
-template <class T, int NV> __device__ __forceinline__ void store_gradient(const HeldRow<T, NV>& row, T* q, float2 stats, float by, bool far, const Temper& t) {
+template <class T, int NV> __device__ __forceinline__ void store_gradient(const HeldRow<T, NV>& row, T* q, float2 stats, float by, const Temper& t) {
     constexpr int V = Elem<T>::kVec;
     #pragma unroll
     for (int k = 0; k < NV; k++)
@@ -342,8 +341,7 @@ template <class T, int NV> __device__ __forceinline__ void store_gradient(const 
                 gradient_values<T>(f, stats.x, stats.y * by, t);
             }
             if (row.n >= V) {
-                if (far) put_stream16(q + c, Elem<T>::pack(f));
-                else store16(q + c, Elem<T>::pack(f));
+                store16(q + c, Elem<T>::pack(f));
             } else {
                 #pragma unroll
                 for (int i = 0; i < V; i++)
@@ -352,11 +350,7 @@ template <class T, int NV> __device__ __forceinline__ void store_gradient(const 
         }
 }
 
-// Bytes of a FUSED short row from which its gradient is stored past the caches (as in label_loss.hip).
-constexpr int kStreamRow = 512;
-
-// FUSED: the gradient leaves with the row (its scale is known before)
-template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) distill_short_kernel(LogitRows a, Lists l, Temper t, Outcome e, Slopes g, int shift, int64_t row0) {
+template <class T, int NV> __global__ void __launch_bounds__(256) distill_short_kernel(LogitRows a, Lists l, Temper t, Outcome e, int shift, int64_t row0) {
     __shared__ uint32_t marks[256][2];
     if (e.ticket && blockIdx.x == 0 && threadIdx.x == 0) *e.ticket = 0u;
     HeldRow<T, NV> row;
@@ -365,7 +359,7 @@ template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) di
     row.vecs = (row.n + Elem<T>::kVec - 1) / Elem<T>::kVec;
     const int64_t r = row0 + (int64_t)blockIdx.x * (256 >> shift) + (threadIdx.x >> shift);
     if (r >= a.rows) return;
-    const bool skip = FUSED ? e.kept[r] == 0.f : !counts(l, r, row.lane, shift);
+    const bool skip = !counts(l, r, row.lane, shift);
     Others o{-INFINITY, 0.0};
     bool repeats = false;
     if (!skip) {
@@ -378,14 +372,7 @@ template <class T, int NV, bool FUSED> __global__ void __launch_bounds__(256) di
     Row end;
     First first;
     outcomes_of<T>(a, l, t, e, r, o, skip, repeats, row.lane, shift, stats, most_t, base, end, first);
-    T* q = static_cast<T*>(g.grad) + r * a.classes;
-    const float by = FUSED ? *g.scale : 0.f;
-    if (FUSED) {
-        store_gradient(row, q, stats, by, row.n * (int)sizeof(T) >= kStreamRow, t);
-        wave_fence();       // (the entries' values stand where these stood)
-    }
-    if (FUSED || e.entries)
-        each_slope<T>(a, l, t, e, r, skip, repeats, row.lane, shift, most_t, base, end, first, [&](int64_t c, float slope) { if (FUSED) q[c] = Elem<T>::put(slope * by); });
+    if (e.entries) each_slope<T>(a, l, t, e, r, skip, repeats, row.lane, shift, most_t, base, end, first);
 }
 
 template <class T, int NV> __global__ void __launch_bounds__(256) distill_short_gradient_kernel(LogitRows a, Lists l, Temper t, Slopes g, int shift) {
@@ -400,7 +387,7 @@ template <class T, int NV> __global__ void __launch_bounds__(256) distill_short_
         const float2 stats = g.stats[r];
         if (stats.y != 0.f) row.load(row_start<T>(a, r));
         T* q = static_cast<T*>(g.grad) + r * a.classes;
-        store_gradient(row, q, stats, by, false, t);
+        store_gradient(row, q, stats, by, t);
         wave_fence();
         for (int j = row.lane; j < l.k; j += 1 << shift) {
             const int64_t c = l.cls(r * l.k + j);
@@ -429,10 +416,10 @@ template <class T, int NV, int THREADS> struct Marks {
 };
 
 // The workgroup holds a row in its registers, at most 16 vectors per work-item, and an entry per work-item.  FUSED: the logits are read once and the gradient leaves
-// with the row.  FAR: logits that the last-level cache cannot hold are read past it.
+// with the row, and these are read past the caches.
 // A row per workgroup and no loop over them: the constants of the 64-bit functions would be kept in registers that the row needs.  What the entries give is summed
 // while the row is on its way; when it is there a wavefront's part, one barrier and a few 64-bit functions of one wavefront stand between its sums and its gradient.
-template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __launch_bounds__(THREADS, 4) distill_held_kernel(LogitRows a, Lists l, Temper t, Outcome e, Slopes g, int64_t row0) {
+template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bounds__(THREADS, 4) distill_held_kernel(LogitRows a, Lists l, Temper t, Outcome e, Slopes g, int64_t row0) {
     constexpr int V = Elem<T>::kVec, WAVES = THREADS / 64, kChunk = NV < 32 / V ? NV : 32 / V;
     constexpr int kShift = WAVES == 4 ? 2 : WAVES == 8 ? 3 : 4;      // (the wavefronts' results in the lanes of each group of so many)
     static_assert(kMostEntries <= 256 && WAVES >= 4, "the first four wavefronts have the entries");
@@ -492,7 +479,7 @@ template <class T, int NV, int THREADS, bool FUSED, bool FAR> __global__ void __
     for (int k = 0; k < NV; k++) {
         const int i = (int)threadIdx.x + k * THREADS;
         const uint32_t at = (uint32_t)(i < full ? i : full - 1) * V;        // (under no condition: behind one no load can be waited for by itself)
-        v[k] = FAR ? stream16(p + at) : load16(p + at);
+        v[k] = FUSED ? stream16(p + at) : load16(p + at);
     }
     T last = p[rest_at < n ? rest_at : n - 1];
     const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
@@ -705,7 +692,7 @@ template <class T> __global__ void __launch_bounds__(256) distill_join_kernel(Lo
         Row end;
         First first;
         outcomes_of<T>(a, l, t, e, r, o, skip, twice_there, lane, 6, stats, most_t, base, end, first);
-        if (e.entries) each_slope<T>(a, l, t, e, r, skip, twice_there, lane, 6, most_t, base, end, first, [](int64_t, float) {});
+        if (e.entries) each_slope<T>(a, l, t, e, r, skip, twice_there, lane, 6, most_t, base, end, first);
     }
 }
 
@@ -865,21 +852,20 @@ Group short_group(const LogitRows& a, int vec) {
     return g;
 }
 
-bool in_parts(const LogitRows& a, int vec) {
-    return short_group(a, vec).shift < 0 && !((a.classes + vec - 1) / vec <= 16 * 512 && (a.rows >= kWholeRows || one_launch(a.rows, a.classes, vec)));
-}
+// Whether a row is read in parts, being more than a workgroup can hold.  Where it can, few rows are no reason: 16 x 65536 bf16 21.5 us with the gradient, held 18.7.
+bool in_parts(const LogitRows& a, int vec) { return (a.classes + vec - 1) / vec > 16 * 512; }
 
 int64_t distill_floats(const LogitRows& a, int dtype) {
     const int vec = vec_of(dtype);
     return kDistillSums + kept_floats(a.rows) + (in_parts(a, vec) ? ((int64_t)(sizeof(Others) + sizeof(int)) / 4 * a.rows * cut_of(a, vec).splits + 3) / 4 * 4 : 0);
 }
 
-// Whether the gradient leaves with the rows: it then costs one reading of the logits less and two launches more; a workgroup must be able to hold a
-// row, and there must be rows for all compute units.
+// Whether the gradient leaves with the rows: it then costs one reading of the logits less and two launches more.  A workgroup must be able to hold a row, and there
+// must be rows for all compute units.  Loss and gradient of 4500 x 4096 bf16 (35 MiB) 43.7 us with it and 39.9 without, 800 x 30001 (46 MiB) 42.0 and 44.4, 8192 x 4096
+// 63.7 and 68.7, 4096 x 131072 479 and 665; of short rows, whose 64-bit functions the gradient would wait for, 65536 x 1000 fp32 232 and 207.
 bool fuses(const LogitRows& a, int dtype) {
     const int vec = vec_of(dtype);
-    if (a.rows * a.classes * (16 / vec) < (32ll << 20)) return false;
-    return short_group(a, vec).shift >= 0 || (a.rows >= 512 && a.classes <= kHeldLong * vec);
+    return a.rows * a.classes * (16 / vec) >= (40ll << 20) && short_group(a, vec).shift < 0 && a.rows >= 512 && a.classes <= kHeldLong * vec;
 }
 
 }  // namespace
@@ -935,27 +921,25 @@ extern "C" int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* li
             const int per = 256 >> group.shift;
             with_vectors(group.vectors, [&](auto nv) {
                 in_slices((a.rows + per - 1) / per, [&](int64_t from, unsigned blocks) {
-                    if (grad) hipLaunchKernelGGL((distill_short_kernel<T, nv.value, true>), dim3(blocks), dim3(256), 0, s, a, l, t, e, g, group.shift, from * per);
-                    else hipLaunchKernelGGL((distill_short_kernel<T, nv.value, false>), dim3(blocks), dim3(256), 0, s, a, l, t, e, g, group.shift, from * per);
+                    hipLaunchKernelGGL((distill_short_kernel<T, nv.value>), dim3(blocks), dim3(256), 0, s, a, l, t, e, group.shift, from * per);
                 });
             });
             return;
         }
         if (grad || !in_parts(a, vec)) {
             const int64_t vecs = (a.classes + vec - 1) / vec;
-            const auto held = [&](auto fused, auto far) {
+            const auto held = [&](auto fused) {
                 in_slices(a.rows, [&](int64_t from, unsigned blocks) {
                     const dim3 grid(blocks);
-                    if (vecs <= 4 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 4, 256, fused.value, far.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
-                    else if (vecs <= 8 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 8, 256, fused.value, far.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
-                    else if (vecs <= 16 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 16, 256, fused.value, far.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
-                    else if (vecs <= 16 * 512) hipLaunchKernelGGL((distill_held_kernel<T, 16, 512, fused.value, far.value>), grid, dim3(512), 0, s, a, l, t, e, g, from);
-                    else if constexpr (fused.value) hipLaunchKernelGGL((distill_held_kernel<T, 16, 1024, true, far.value>), grid, dim3(1024), 0, s, a, l, t, e, g, from);
+                    if (vecs <= 4 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 4, 256, fused.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
+                    else if (vecs <= 8 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 8, 256, fused.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
+                    else if (vecs <= 16 * 256) hipLaunchKernelGGL((distill_held_kernel<T, 16, 256, fused.value>), grid, dim3(256), 0, s, a, l, t, e, g, from);
+                    else if (vecs <= 16 * 512) hipLaunchKernelGGL((distill_held_kernel<T, 16, 512, fused.value>), grid, dim3(512), 0, s, a, l, t, e, g, from);
+                    else if constexpr (fused.value) hipLaunchKernelGGL((distill_held_kernel<T, 16, 1024, true>), grid, dim3(1024), 0, s, a, l, t, e, g, from);
                 });
             };
-            if (!grad) held(std::false_type(), std::false_type());
-            else if (a.rows * a.classes * (int64_t)sizeof(T) >= kCached) held(std::true_type(), std::true_type());
-            else held(std::true_type(), std::false_type());
+            if (grad) held(std::true_type());
+            else held(std::false_type());
             return;
         }
         const Cut cut = cut_of(a, vec);

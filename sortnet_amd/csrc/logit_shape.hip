@@ -29,7 +29,6 @@ struct Shape {
     const void* grad;                           // backward: what flows into the result, rows one behind the other
     void* out;
     int64_t part;                               // columns of a workgroup, a multiple of 8
-    bool far;                                   // results that the last-level cache cannot hold are stored past it
     int parts, group;                           // parts of a row, or (with one part) rows of a workgroup
     uint32_t first;                             // of the launch's workgroups (see in_slices)
 };
@@ -99,6 +98,8 @@ template <bool WIDE, int HISTORY> __device__ __forceinline__ void count_places(u
         if (first + i < n && at < columns && (!WIDE || p.v[2 * i + 1] == 0u)) count_one<HISTORY>(counts, at);
     }
 }
+constexpr int64_t kGroupPlaces = 1 << 12;       // of the histories of rows that a workgroup shapes together
+
 // the first places of a history, which are on their way before it is known how many of them count
 constexpr int kAhead = 2;
 template <bool WIDE> __device__ __forceinline__ void load_ahead(Places (&p)[kAhead], const void* past, int64_t length) {
@@ -109,24 +110,21 @@ template <bool WIDE> __device__ __forceinline__ void load_ahead(Places (&p)[kAhe
         if ((pack + 1) * kPer <= length) p[k] = load_places<WIDE>(past, pack);
     }
 }
-template <bool WIDE, int HISTORY> __device__ __forceinline__ void count_history(uint32_t* counts, const Places (&ahead)[kAhead], bool with_ahead, const void* past, int64_t length, int64_t n,
+template <bool WIDE, int HISTORY> __device__ __forceinline__ void count_history(uint32_t* counts, const Places (&ahead)[kAhead], const void* past, int64_t length, int64_t n,
                                                                   uint32_t c0, uint32_t columns) {
     constexpr int kPer = WIDE ? 2 : 4;
-    int64_t from = 0;
-    if (with_ahead) {
-        #pragma unroll
-        for (int k = 0; k < kAhead; k++) {
-            const int64_t pack = (int)threadIdx.x + k * 256;
-            if ((pack + 1) * kPer <= length) count_places<WIDE, HISTORY>(counts, ahead[k], pack * kPer, n, c0, columns);
-        }
-        from = kAhead * 256;
+    constexpr int64_t from = kAhead * 256;
+    #pragma unroll
+    for (int k = 0; k < kAhead; k++) {
+        const int64_t pack = (int)threadIdx.x + k * 256;
+        if ((pack + 1) * kPer <= length) count_places<WIDE, HISTORY>(counts, ahead[k], pack * kPer, n, c0, columns);
     }
     const int64_t packs = n / kPer;
     #pragma unroll 2
     for (int64_t pack = from + threadIdx.x; pack < packs; pack += 256) count_places<WIDE, HISTORY>(counts, load_places<WIDE>(past, pack), pack * kPer, n, c0, columns);
     // the places behind the last whole 16 bytes, unless they were among those
     int64_t j = packs * kPer + threadIdx.x;
-    if (with_ahead && packs < from && (packs + 1) * kPer <= length) return;
+    if (packs < from && (packs + 1) * kPer <= length) return;
     if (j < n) {
         const uint32_t* word = static_cast<const uint32_t*>(past) + (WIDE ? 2 * j : j);
         const uint32_t at = word[0] - c0;
@@ -171,9 +169,8 @@ template <class T, int ALLOWED, int HISTORY, int KIND> __global__ void __launch_
     };
     // (loads arrive in their order: the history's first)
     Places ahead[kAhead];
-    const bool with_ahead = HISTORY != kNone && rows == 1;
     const void* past = nullptr;
-    if (with_ahead) {
+    if (HISTORY != kNone && rows == 1) {
         past = static_cast<const uint8_t*>(s.history) + place(r0, s.history_outer, s.history_inner) * (s.wide_history ? 8 : 4);
         if (s.wide_history) load_ahead<true>(ahead, past, s.length);
         else load_ahead<false>(ahead, past, s.length);
@@ -182,16 +179,36 @@ template <class T, int ALLOWED, int HISTORY, int KIND> __global__ void __launch_
     if (HISTORY) {
         for (int i = threadIdx.x; i < rows * width / (4 * kPer); i += 256) reinterpret_cast<u32x4*>(counts)[i] = u32x4{0u, 0u, 0u, 0u};
         __syncthreads();
-        for (int i = 0; i < rows; i++) {
-            const int64_t r = r0 + i;
-            int64_t n = s.length;
-            if (s.lengths) {
-                const int64_t given = s.wide_lengths ? static_cast<const int64_t*>(s.lengths)[r] : static_cast<const int*>(s.lengths)[r];
-                n = given < 0 ? 0 : given < n ? given : n;
-            }
-            if (!with_ahead) past = static_cast<const uint8_t*>(s.history) + place(r, s.history_outer, s.history_inner) * (s.wide_history ? 8 : 4);
-            if (s.wide_history) count_history<true, HISTORY>(counts + i * width / kPer, ahead, with_ahead, past, s.length, n, (uint32_t)c0, (uint32_t)columns);
-            else count_history<false, HISTORY>(counts + i * width / kPer, ahead, with_ahead, past, s.length, n, (uint32_t)c0, (uint32_t)columns);
+        const auto counted = [&](int64_t r) {       // places of a row's history that count
+            if (!s.lengths) return s.length;
+            const int64_t given = s.wide_lengths ? static_cast<const int64_t*>(s.lengths)[r] : static_cast<const int*>(s.lengths)[r];
+            return given < 0 ? 0 : given < s.length ? given : s.length;
+        };
+        if (rows == 1) {
+            const int64_t n = counted(r0);
+            if (s.wide_history) count_history<true, HISTORY>(counts, ahead, past, s.length, n, (uint32_t)c0, (uint32_t)columns);
+            else count_history<false, HISTORY>(counts, ahead, past, s.length, n, (uint32_t)c0, (uint32_t)columns);
+        } else {        // all rows' places one behind the other: in a turn for each row there would be little to do
+            const auto count_rows = [&](auto wide) {
+                constexpr bool WIDE = decltype(wide)::value;
+                constexpr uint32_t kPlaces = WIDE ? 2 : 4;
+                const uint32_t length = (uint32_t)s.length, packs = (length + kPlaces - 1) / kPlaces;
+                #pragma unroll 2
+                for (uint32_t j = threadIdx.x; j < rows * packs; j += 256) {
+                    const uint32_t i = j / packs, pack = j - i * packs;
+                    const int64_t r = r0 + i, n = counted(r);
+                    const uint32_t* words = static_cast<const uint32_t*>(s.history) + place(r, s.history_outer, s.history_inner) * (WIDE ? 2 : 1);
+                    Places p;
+                    if ((pack + 1) * kPlaces <= length) p = load_places<WIDE>(words, pack);
+                    else {
+                        #pragma unroll
+                        for (int m = 0; m < 4; m++) p.v[m] = (pack * 4 + m) < length * (WIDE ? 2 : 1) ? words[pack * 4 + m] : ~0u;
+                    }
+                    count_places<WIDE, HISTORY>(counts + i * width / kPer, p, pack * kPlaces, n, 0, (uint32_t)columns);
+                }
+            };
+            if (s.wide_history) count_rows(std::true_type());
+            else count_rows(std::false_type());
         }
         __syncthreads();
     }
@@ -245,8 +262,7 @@ template <class T, int ALLOWED, int HISTORY, int KIND> __global__ void __launch_
                 for (int m = 0; m < V; m++) f[m] = bits[k] >> m & 1 ? f[m] : GRAD ? 0.f : -INFINITY;
             }
             T* to = static_cast<T*>(s.out) + r * a.classes + c0 + c;
-            if (s.far) put_stream16(to, Elem<T>::pack(f));
-            else store16(to, Elem<T>::pack(f));
+            store16(to, Elem<T>::pack(f));
         }
     }
     // the values behind the last whole vector of each row
@@ -299,11 +315,13 @@ static int shape_logits(const char* who, const sd_logit_rows* in, const sd_const
     s.bias = c->bias; s.bias_outer = c->bias_outer; s.bias_inner = c->bias_inner;
     s.allowed = c->allowed; s.allowed_outer = c->allowed_outer; s.allowed_inner = c->allowed_inner;
     s.grad = grad; s.out = out;
-    s.far = a.rows * a.classes * (16 / vec_of(in->dtype)) > kCached;
     const int64_t width = (a.classes + 7) / 8 * 8, most = s.length >= 1 << 16 ? kCountWords : 2 * kCountWords;
     if (width <= most) {
-        const int64_t fit = most / width, want = (a.rows + 1023) / 1024;
-        s.group = (int)(want < fit ? want : fit);
+        // Short rows are shaped together, as many as leave 1024 workgroups: 100000 x 10 fp32 with 4 places each 6.9 us, in a workgroup each 136.  But a long history is
+        // read faster where a workgroup has one row: 8192 x 2000 bf16 with 2000 places 43 us, in groups of 2 47, of 4 52.5.
+        const int64_t places = s.length > 0 ? kGroupPlaces / s.length : most, fit = most / width, want = (a.rows + 1023) / 1024;
+        const int64_t group = want < fit ? want : fit;
+        s.group = (int)(group < places ? group : places > 1 ? places : 1);
         s.parts = 1;
         s.part = width;
     } else {

@@ -19,6 +19,7 @@ namespace sd {
 
 constexpr int kMostTop = SD_MOST_TOP;
 constexpr int64_t kMostClasses = 1ll << 30;
+constexpr int kTopVectors = 4;          // 16-byte vectors of a row for each work-item at a time
 
 __device__ __forceinline__ uint32_t order_of(float v) {
     const uint32_t b = __float_as_uint(v + 0.f);
@@ -331,8 +332,8 @@ constexpr double kLeastShare = 0x1p-60;
 
 // A workgroup per row, or per one of `splits` parts of `part` classes of a row.  What is not listed lies below the wavefront's bound, to which the exponentials are relative;
 // where they come out too small, or the bound too large, for fp32, the others are gone through again at the end.
-template <class T, int THREADS, int NV> __global__ void __launch_bounds__(THREADS, 8) top_rows_kernel(LogitRows a, Top t, int splits, int part, Parts out, int64_t first) {
-    constexpr int V = Elem<T>::kVec, kSpan = THREADS * NV * V;
+template <class T, int THREADS> __global__ void __launch_bounds__(THREADS, 8) top_rows_kernel(LogitRows a, Top t, int splits, int part, Parts out, int64_t first) {
+    constexpr int V = Elem<T>::kVec, NV = kTopVectors, kSpan = THREADS * NV * V;
     using S = Shared<THREADS>;
     static_assert(64 * NV + kMostTop <= S::kRoom, "a wavefront's part of the list has room for all vectors behind the k that a cut of its own leaves");
     static_assert(64 * V <= S::kRoom, "and for the logits of a vector for each work-item");
@@ -564,26 +565,26 @@ template <class T> __global__ void __launch_bounds__(256) top_short_kernel(Logit
 // ---- host ------------------------------------------------------------------------------------------------------------------------
 namespace {
 
-// How rows are read: by `threads` work-items each (0: short ones, by lanes), `vectors` of each at a time, in `splits` parts.
-// A list is cut to 1.25 k, which is no more than the work-items, so that a prefix of the numbers does for it (k = 256 with 256 of them 4096 x 131072 bf16 660 us).
-// Above that, as many as fill the card with one row or part each: rows that end together end badly, since nothing is read meanwhile.
-struct Plan { int threads, vectors, splits; int64_t part; };
+// How rows are read: by `threads` work-items each (0: short ones, by lanes; 30000 x 10 fp32 8.6 us, by a wavefront each 35), in `splits` parts.
+// A list is cut to 1.25 k, which is no more than the work-items, so that a prefix of the numbers does for it (k = 256 with 256 of them 4096 x 131072 bf16 660 us, with
+// 512 316).  Above that as many as the card runs at once, since what is left over costs as much time as all the others: 300 x 50001 fp16, k = 200, in 7 parts 70 us, in
+// 5 53; 20000 x 9001 fp32, k = 20, by 256 work-items 232 us, by 128 168 (but 4096 x 131072 bf16, which is twice the card by 256, 206 and 218).
+struct Plan { int threads, splits; int64_t part; };
 Plan plan_of(const LogitRows& a, int64_t k, int vec) {
-    if (a.classes <= 64) return {0, 1, 1, a.classes};
+    if (a.classes <= 64) return {0, 1, a.classes};
     const int64_t most = k + k / 4, card = 1 << 19;
     int threads = 64;
     while (threads < most) threads *= 2;
-    if (a.classes <= (int64_t)threads * 4 * vec) return {threads, 4, 1, a.classes};
+    if (a.classes <= (int64_t)threads * kTopVectors * vec) return {threads, 1, a.classes};
     if (threads < 128) threads = 128;
     while (threads < 256 && a.rows * threads * 2 <= card) threads *= 2;
     const int64_t fit = card / (a.rows * threads), want = fit > 1 ? fit : 1, span = threads * vec;
-    const int vectors = a.classes >= want * span * 4 ? 4 : 2;
-    int64_t splits = (a.classes + span * vectors - 1) / (span * vectors);
+    int64_t splits = (a.classes + span * kTopVectors - 1) / (span * kTopVectors);
     if (splits > want) splits = want;
     if (splits > 256) splits = 256;
-    if (splits == 1) return {threads, 4, 1, a.classes};
+    if (splits == 1) return {threads, 1, a.classes};
     const int64_t part = ((a.classes + splits - 1) / splits + span - 1) / span * span;
-    return {threads, vectors, (int)((a.classes + part - 1) / part), part};
+    return {threads, (int)((a.classes + part - 1) / part), part};
 }
 
 int64_t part_floats(const LogitRows& a, int64_t k, const Plan& plan) {
@@ -633,17 +634,16 @@ extern "C" int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temper
             hipLaunchKernelGGL(top_short_kernel<T>, dim3(blocks_for(blocks)), dim3(256), 0, s, a, t, shift);
             return;
         }
-        const auto launch = [&](auto threads, auto vectors) {
+        const auto launch = [&](auto threads) {
             in_slices(lists, [&](int64_t from, unsigned blocks) {
-                hipLaunchKernelGGL((top_rows_kernel<T, threads.value, vectors.value>), dim3(blocks), dim3(threads.value), 0, s, a, t, plan.splits, (int)plan.part, parts, from);
+                hipLaunchKernelGGL((top_rows_kernel<T, threads.value>), dim3(blocks), dim3(threads.value), 0, s, a, t, plan.splits, (int)plan.part, parts, from);
             });
         };
-        const auto with = [&](auto threads) { plan.vectors == 4 ? launch(threads, std::integral_constant<int, 4>()) : launch(threads, std::integral_constant<int, 2>()); };
         switch (plan.threads) {
-            case 64: launch(std::integral_constant<int, 64>(), std::integral_constant<int, 4>()); break;
-            case 128: launch(std::integral_constant<int, 128>(), std::integral_constant<int, 4>()); break;
-            case 256: with(std::integral_constant<int, 256>()); break;
-            default: with(std::integral_constant<int, 512>());
+            case 64: launch(std::integral_constant<int, 64>()); break;
+            case 128: launch(std::integral_constant<int, 128>()); break;
+            case 256: launch(std::integral_constant<int, 256>()); break;
+            default: launch(std::integral_constant<int, 512>());
         }
         if (plan.splits > 1) {
             in_slices(a.rows, [&](int64_t from, unsigned blocks) { hipLaunchKernelGGL(top_join_kernel<T>, dim3(blocks), dim3(kJoin), 0, s, a, t, plan.splits, parts, from); });
