@@ -152,7 +152,7 @@ def main():
     if "shift" in on:
         t("mean_shift_forward", lambda: ext.mean_shift_forward(y, mean, None, 0.1, y2), None, 4 * (3 * B * M))
     if "head" in on:
-        # training of a head: B x M logits, one label each; dropout of the B x N features
+        # training of a head and answers with it: B x M logits, one label each; dropout of the B x N features
         from sortnet_amd import functional as F, losses
         z = torch.randn(B, M, generator=g).to(dev).requires_grad_()
         labels = torch.randint(0, M, (B,), generator=g).to(dev)
@@ -166,6 +166,14 @@ def main():
         t("policy_loss, fwd + bwd",
           lambda: backward(losses.policy_loss(z, labels, ref, adv, ref_log_probs=ref, kl_coef=0.05)[0], z), None, 8 * B * M)
         t("dropout q=0.9, fwd + bwd", lambda: backward(F.dropout(feats, 0.9, 1), feats, x[..., 0]), None, 16 * B * N)
+        k = min(16, M)
+        lists = F.top_logits(z.detach() + 1.0, k, 2.0)
+        flags = torch.rand(B, M, generator=g).to(dev) < 0.5
+        history = torch.randint(0, M, (B, 100), generator=g).to(dev)
+        t("distill_loss k=%d, fwd + bwd" % k, lambda: backward(losses.distill_loss(z, *lists, temperature=2.0)[0], z), None, 8 * B * M)
+        t("top_logits k=%d" % k, lambda: F.top_logits(z, k), None, 4 * B * M)
+        t("constrain_logits, history and mask", lambda: F.constrain_logits(z.detach(), history, repetition=1.2, allowed=flags),
+          None, 9 * B * M)
     if args.json:
         print(json.dumps({"shape": {"B": B, "N": N, "M": M}, "rows": rows}))
 
