@@ -535,30 +535,53 @@ template <class T> __global__ void __launch_bounds__(kJoin) top_join_kernel(Logi
     if (threadIdx.x == 0) keep.store_rest(o, r);
 }
 
-// Rows of at most 64 classes: 2^shift lanes of a wavefront per row, one class each, whose place is the number of classes before it.
+__device__ __forceinline__ uint32_t group_most(uint32_t u, int shift) {
+    const auto larger = [](uint32_t a, uint32_t b) { return a > b ? a : b; };
+    if (shift > 0) u = lanes_step<0>(u, larger);
+    if (shift > 1) u = lanes_step<1>(u, larger);
+    if (shift > 2) u = lanes_step<2>(u, larger);
+    if (shift > 3) u = lanes_step<3>(u, larger);
+    if (shift > 4) u = lanes_step<4>(u, larger);
+    if (shift > 5) u = lanes_step<5>(u, larger);
+    return u;
+}
+
+// Rows of at most 64 classes: 2^shift lanes of a wavefront per row, one class each.  Its place is the number of classes before it, or the turn in which it is the first of
+// the largest ones that are left, where the turns, each of which takes as long as four comparisons with a class, are few: 65536 x 50 bf16, k = 5, 58 and 35 us.
 template <class T> __global__ void __launch_bounds__(256) top_short_kernel(LogitRows a, Top t, int shift) {
     const int lane = threadIdx.x & ((1 << shift) - 1), lead = (threadIdx.x & 63) - lane, n = (int)a.classes;
+    const uint64_t whole = shift == 6 ? ~0ull : (1ull << (1 << shift)) - 1ull;
     const int64_t per = 256 >> shift;
     for (int64_t r = (int64_t)blockIdx.x * per + (threadIdx.x >> shift); r < a.rows; r += gridDim.x * per) {
         const T* p = row_start<T>(a, r);
         const T raw = p[lane < n ? lane : 0];
         const float v = lane < n ? Elem<T>::get(raw) : -INFINITY;
         const uint32_t mine = lane < n ? order_of(v) : 0u;
-        int place = 0;
-        for (int j = 0; j < n; j++) {
-            const uint32_t other = (uint32_t)__shfl((int)mine, lead + j);
-            place += other > mine || (other == mine && j < lane);
+        int place = t.k;
+        if (4 * t.k <= n) {
+            uint32_t left = mine;
+            for (int turn = 0; turn < t.k; turn++) {
+                const uint32_t most = group_most(left, shift);
+                if (lane == __ffsll((long long)(__ballot(left == most) >> lead & whole)) - 1) { place = turn; left = 0u; }
+            }
+        } else {
+            place = 0;
+            for (int j = 0; j < n; j++) {
+                const uint32_t other = (uint32_t)__shfl((int)mine, lead + j);
+                place += other > mine || (other == mine && j < lane);
+            }
         }
         const bool chosen = lane < n && place < t.k;
         if (chosen) {
             static_cast<T*>(t.values)[r * t.k + place] = raw;
             t.classes[r * t.k + place] = lane;
         }
+        // (exponentials and the logarithm in 32 bits: there are 63 numbers at most, 1 among them, and in 64 they took longer than all the rest)
         const float other = chosen ? -INFINITY : v, top = group_max(other, shift);
-        const double sum = group_total(other == -INFINITY ? 0.0 : other == top ? 1.0 : top == INFINITY ? 0.0 : in_powers(other, top, t), shift);
+        const float sum = (float)group_total(other == -INFINITY ? 0.0 : other == top ? 1.0 : top == INFINITY ? 0.0 : (double)__builtin_amdgcn_exp2f((other - top) * t.by), shift);
         const float nan = group_max(v != v ? 1.f : 0.f, shift);
         if (lane == 0)
-            t.rest[r] = nan != 0.f ? __builtin_nanf("") : sum == 0.0 ? -INFINITY : top == INFINITY ? INFINITY : (float)(log(sum) + power_of(top, t) * 0.69314718055994530942);
+            t.rest[r] = nan != 0.f ? __builtin_nanf("") : sum == 0.f ? -INFINITY : top == INFINITY ? INFINITY : (float)((double)logf(sum) + power_of(top, t) * 0.69314718055994530942);
     }
 }
 
