@@ -1,6 +1,7 @@
 """The operators on logits as they are used together: a teacher's lists and the student that learns from them, answers under a grammar, a policy that learns under a
 mask of its actions.  Tolerances: those of the single operators' tests, rounded up to a few units of the types."""
 import math
+import threading
 
 import pytest
 import torch
@@ -91,3 +92,36 @@ def test_model_learns_from_a_model():
     loss, divergences = losses.distill_loss(out, *lists, temperature=2.0, weight=0.5)
     grads = torch.autograd.grad(loss, [p for p in student.fc_final.parameters()])
     assert torch.isfinite(loss) and divergences.shape == (16,) and all(torch.isfinite(g).all() and g.abs().max() > 0 for g in grads)
+
+
+def test_two_threads_at_once():
+    """Two host threads, each on a stream of its own, get what one alone gets."""
+    g = torch.Generator().manual_seed(9)
+    sets = []
+    for rows, classes, k, dtype in [(700, 40001, 20, torch.bfloat16), (3, 90001, 64, torch.float32), (900, 30, 4, torch.float16)]:
+        z, t = ((2 * torch.randn(rows, classes, generator=g)).to(dtype).cuda() for _ in range(2))
+        sets.append((z.requires_grad_(), t, k, torch.randint(0, classes, (rows, 40), generator=g).cuda(), (torch.rand(rows, classes, generator=g) < 0.7).cuda()))
+
+    def chain(z, t, k, history, flags):
+        lists = F.top_logits(F.constrain_logits(t, history, repetition=1.2, allowed=flags), k)
+        loss, divergences = losses.distill_loss(F.constrain_logits(z, history, presence=0.5), *lists, temperature=1.5)
+        return [t.clone() for t in (*lists, loss.detach(), divergences, torch.autograd.grad(loss, z)[0])]
+
+    want = [chain(*s) for s in sets]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(first):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for n in range(12):
+                i = (first + n) % len(sets)
+                got = chain(*sets[i])
+                torch.cuda.current_stream().synchronize()
+                wrong.extend((first, n, j) for j, (a, b) in enumerate(zip(got, want[i])) if not torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
