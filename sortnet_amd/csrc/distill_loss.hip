@@ -415,6 +415,9 @@ template <class T, int NV, int THREADS> struct Marks {
     __device__ __forceinline__ uint32_t bits(int k) const { return words[threadIdx.x][k * V / 32] >> (k * V & 31) & ((1u << V) - 1u); }
 };
 
+// the vector `item` behind a pointer that is the same for all lanes: an offset of 32 bits is added by the load or store itself
+template <class T> __device__ __forceinline__ T* behind(T* p, int item) { return (T*)((const char*)p + (uint32_t)item * 16u); }
+
 // The workgroup holds a row in its registers, at most 16 vectors per work-item, and an entry per work-item.  FUSED: the logits are read once and the gradient leaves
 // with the row, and these are read past the caches.
 // A row per workgroup and no loop over them: the constants of the 64-bit functions would be kept in registers that the row needs.  What the entries give is summed
@@ -478,8 +481,8 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
     #pragma unroll
     for (int k = 0; k < NV; k++) {
         const int i = (int)threadIdx.x + k * THREADS;
-        const uint32_t at = (uint32_t)(i < full ? i : full - 1) * V;        // (under no condition: behind one no load can be waited for by itself)
-        v[k] = FUSED ? stream16(p + at) : load16(p + at);
+        const T* from = behind(p, i < full ? i : full - 1);     // (under no condition: behind one no load can be waited for by itself)
+        v[k] = FUSED ? stream16(from) : load16(from);
     }
     T last = p[rest_at < n ? rest_at : n - 1];
     const double rest = l.rest ? (double)l.rest[r] : -INFINITY;
@@ -575,7 +578,7 @@ template <class T, int NV, int THREADS, bool FUSED> __global__ void __launch_bou
                 float f[V];
                 Elem<T>::unpack(v[k], f);
                 gradient_values<T>(f, high, w, t);
-                if (i < full) put_stream16(q + i * V, Elem<T>::pack(f));
+                if (i < full) put_stream16(behind(q, i), Elem<T>::pack(f));
             }
             if (rest_at < n) {
                 float f[1] = {Elem<T>::get(last)};
