@@ -49,7 +49,7 @@ struct Gradient {
 };
 
 // The same for what is stored in T: one product will do where that has 16 bits, whose half step is 2^-11 of a value at least.  (4096 x 131072 bf16,
-// policy with its gradient: 437 us with two everywhere, 425 so, 413 with one in the sums, too.)
+// policy with its gradient: 437 us with two everywhere, 425 so, 413 with one in the sums, too; since then 409 so.)
 template <class T> __device__ __forceinline__ float exp_to(float v) {
     if constexpr (sizeof(T) == 2) return __builtin_amdgcn_exp2f(v * 1.44269504f);
     else return exp_of(v);

@@ -131,6 +131,7 @@ template <bool WIDE, int HISTORY> __device__ __forceinline__ void count_history(
     }
 }
 
+// 4096 x 65536 bf16 with 1024 places and a bit mask 211 us (5.1 TB/s), its gradient 254 (4.2: a cache line for each counted logit).
 // A workgroup shapes `part` columns of a row, or `group` whole rows.  A work-item's vectors are on their way together, the first of them while the
 // history is counted.
 template <class T, int ALLOWED, int HISTORY, int KIND> __global__ void __launch_bounds__(256, HISTORY == kNone ? 8 : 6) shape_kernel(LogitRows a, Shape s) {

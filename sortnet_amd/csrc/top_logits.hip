@@ -332,6 +332,7 @@ constexpr double kLeastShare = 0x1p-60;
 
 // A workgroup per row, or per one of `splits` parts of `part` classes of a row.  What is not listed lies below the wavefront's bound, to which the exponentials are relative;
 // where they come out too small, or the bound too large, for fp32, the others are gone through again at the end.
+// 4096 x 131072 bf16, k = 64, 217 us (4.9 TB/s; reading alone 163 to 185); 1 x 131072, k = 50, in 16 parts 12 us and the join 7, of which each waits for its own steps.
 template <class T, int THREADS> __global__ void __launch_bounds__(THREADS, 8) top_rows_kernel(LogitRows a, Top t, int splits, int part, Parts out, int64_t first) {
     constexpr int V = Elem<T>::kVec, NV = kTopVectors, kSpan = THREADS * NV * V;
     using S = Shared<THREADS>;
