@@ -592,7 +592,7 @@ namespace {
 // How rows are read: by `threads` work-items each (0: short ones, by lanes; 30000 x 10 fp32 8.6 us, by a wavefront each 35), in `splits` parts.
 // A list is cut to 1.25 k, which is no more than the work-items, so that a prefix of the numbers does for it (k = 256 with 256 of them 4096 x 131072 bf16 660 us, with
 // 512 316).  Above that as many as the card runs at once, since what is left over costs as much time as all the others: 300 x 50001 fp16, k = 200, in 7 parts 70 us, in
-// 5 53; 20000 x 9001 fp32, k = 20, by 256 work-items 232 us, by 128 168 (but 4096 x 131072 bf16, which is twice the card by 256, 206 and 218).
+// 5 53 (whole 38, see below); 20000 x 9001 fp32, k = 20, by 256 work-items 232 us, by 128 168 (but 4096 x 131072 bf16, which is twice the card by 256, 206 and 218).
 struct Plan { int threads, splits; int64_t part; };
 Plan plan_of(const LogitRows& a, int64_t k, int vec) {
     if (a.classes <= 64) return {0, 1, a.classes};
