@@ -578,6 +578,13 @@ Tensor readable_logits(const Tensor& z) {
     return rows ? z : z.contiguous();
 }
 
+// A saved tensor of a few entries for each row: the caller's hooks may hand it back with other strides than it had, and so may they the logits.
+Tensor handed_back(const Tensor& t, const Tensor& grad) {
+    if (!t.defined()) return t;
+    same_device(t, "what a saved tensor's hook gives", grad);
+    return t.contiguous();
+}
+
 sd_label_rows label_rows(const Tensor& z, const Tensor& labels, int64_t ignore) {
     sd_label_rows a{};
     a.dtype = element_type(z, "outputs");
@@ -662,14 +669,14 @@ struct LabelNode : Node {
         const Locked lock(mutex_);
         variable_list out(1);
         if (!task_should_compute_output(0)) return out;
-        const Tensor z = logits.unpack(), l = labels.unpack(), wk = work.unpack();
+        const Tensor saved = logits.unpack(), saved_labels = labels.unpack(), wk = work.unpack();
         std::shared_ptr<OnceNode> once;
         if (at::GradMode::is_enabled()) {
             once = new_node<OnceNode>();
             once->set_next_edges({next_edge(0), grads[0].defined() ? torch::autograd::impl::gradient_edge(grads[0]) : torch::autograd::Edge()});
         }
         at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor g = incoming(*this, grads, 0);
+        const Tensor g = incoming(*this, grads, 0), z = readable_logits(saved), l = handed_back(saved_labels, g);
         const c10::DeviceGuard guard(z.device());
         // A gradient that is there already is only written again for another upstream gradient than 1, which the device knows; one that a
         // later backward may want, too, stays as it is, and so does one of another capture: that graph may run again without the forward that
@@ -944,18 +951,23 @@ struct Beside {
     Tensor t;
     int64_t outer = 0, inner = 0;
     Beside() = default;
-    Beside(const Tensor& given, const char* name, const Tensor& z, bool may_be_shared, int64_t entries) : t(given) {
-        same_device(t, name, z);
-        const bool shared = may_be_shared && t.dim() == 1;
-        if (!shared && (t.dim() != z.dim() || t.sizes().slice(0, t.dim() - 1) != z.sizes().slice(0, z.dim() - 1)))
-            throw std::runtime_error(std::string(name) + " must have the sizes of outputs before the classes");
-        if (entries >= 0 && t.size(-1) != entries) throw std::runtime_error(std::string(name) + " must have " + std::to_string(entries) + " entries for each row, not " + std::to_string(t.size(-1)));
+    explicit Beside(const Tensor& given) : t(given) {
+        if (!t.defined()) return;
         if ((t.size(-1) > 1 && t.stride(-1) != 1) || t.dim() > 3) t = t.contiguous();
-        if (shared) return;
+        if (t.dim() == 1) return;
         if (t.dim() == 3) outer = t.stride(0);
         inner = t.dim() <= 3 ? t.stride(-2) : t.size(-1);
     }
 };
+
+Beside beside(const Tensor& t, const char* name, const Tensor& z, bool may_be_shared, int64_t entries) {
+    same_device(t, name, z);
+    const bool shared = may_be_shared && t.dim() == 1;
+    if (!shared && (t.dim() != z.dim() || t.sizes().slice(0, t.dim() - 1) != z.sizes().slice(0, z.dim() - 1)))
+        throw std::runtime_error(std::string(name) + " must have the sizes of outputs before the classes");
+    if (entries >= 0 && t.size(-1) != entries) throw std::runtime_error(std::string(name) + " must have " + std::to_string(entries) + " entries for each row, not " + std::to_string(t.size(-1)));
+    return Beside(t);
+}
 
 void no_gradient(const Tensor& t, const char* name) {
     if (at::GradMode::is_enabled() && t.requires_grad()) throw std::runtime_error(std::string(name) + " must not require a gradient: the result is differentiated with respect to outputs alone");
@@ -1024,8 +1036,15 @@ struct ConstrainNode : Node {
         }
         at::AutoDispatchBelowADInplaceOrView below;
         const Tensor g = incoming(*this, grads, 0);
-        if (!c.z.defined()) c.z = g;
-        const c10::DeviceGuard guard(c.z.device());
+        const c10::DeviceGuard guard(g.device());
+        c.z = c.z.defined() ? readable_logits(c.z) : g;
+        for (Beside* b : {&c.history, &c.allowed}) {        // (see handed_back; strides of their own are read as they are)
+            if (!b->t.defined()) continue;
+            same_device(b->t, "what a saved tensor's hook gives", g);
+            *b = Beside(b->t);
+        }
+        c.lengths = handed_back(c.lengths, g);
+        for (Tensor& t : c.rows) t = handed_back(t, g);
         out[0] = at::empty(c.z.sizes(), c.z.options());
         c.call(&g, out[0]);
         if (again) set_history(out[0], next);
@@ -1071,7 +1090,7 @@ Tensor constrain_logits(const Tensor& outputs, const OptTensor& history, const O
         }
         if (there(history)) {
             if (!whole(*history)) throw std::runtime_error("history must have dtype torch.int64 or torch.int32");
-            c.history = Beside(*history, "history", outputs, false, -1);
+            c.history = beside(*history, "history", outputs, false, -1);
         }
         if (there(lengths)) {
             if (!there(history)) throw std::runtime_error("lengths are those of a history: none was given");
@@ -1082,11 +1101,11 @@ Tensor constrain_logits(const Tensor& outputs, const OptTensor& history, const O
         }
         if (there(bias)) {
             if (bias->scalar_type() != at::kFloat) throw std::runtime_error("bias must have dtype torch.float32");
-            c.bias = Beside(*bias, "bias", outputs, true, outputs.size(-1));
+            c.bias = beside(*bias, "bias", outputs, true, outputs.size(-1));
         }
         if (there(allowed)) {
             if (allowed->scalar_type() != at::kBool && allowed->scalar_type() != at::kInt) throw std::runtime_error("allowed must have dtype torch.bool, or torch.int32 with a bit for each class");
-            c.allowed = Beside(*allowed, "allowed", outputs, true, allowed->scalar_type() == at::kBool ? outputs.size(-1) : (outputs.size(-1) + 31) / 32);
+            c.allowed = beside(*allowed, "allowed", outputs, true, allowed->scalar_type() == at::kBool ? outputs.size(-1) : (outputs.size(-1) + 31) / 32);
         }
         c.z = readable_logits(outputs);
         out = at::empty(c.z.sizes(), c.z.options());
@@ -1170,7 +1189,7 @@ struct DistillNode : Node {
         const Locked lock(mutex_);
         variable_list out(1);
         if (!task_should_compute_output(0)) return out;
-        const Tensor z = logits.unpack(), wk = work.unpack();
+        const Tensor saved = logits.unpack(), wk = work.unpack();
         Lists l;
         l.values = values.unpack(); l.classes = classes.unpack(); l.rest = rest.unpack();
         std::shared_ptr<OnceNode> once;
@@ -1179,7 +1198,8 @@ struct DistillNode : Node {
             once->set_next_edges({next_edge(0), grads[0].defined() ? torch::autograd::impl::gradient_edge(grads[0]) : torch::autograd::Edge()});
         }
         at::AutoDispatchBelowADInplaceOrView below;
-        const Tensor g = incoming(*this, grads, 0);
+        const Tensor g = incoming(*this, grads, 0), z = readable_logits(saved);
+        for (Tensor* t : {&l.values, &l.classes, &l.rest}) *t = handed_back(*t, g);
         const c10::DeviceGuard guard(z.device());
         // (as in LabelNode: a gradient that is there is written again for another upstream gradient than 1)
         const int64_t now = made.defined() && last ? capture_of(stream_of(z)) : -1;

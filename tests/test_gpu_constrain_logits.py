@@ -329,3 +329,42 @@ def test_refusals():
     with fwd.dual_level():
         with pytest.raises(NotImplementedError, match="forward mode"):
             F.constrain_logits(fwd.make_dual(z, z))
+
+
+def _save_on_cpu_and_back(t):
+    """A saved tensor as a hook that keeps it on the host hands it back: as large, contiguous."""
+    return torch.empty(t.shape, dtype=t.dtype, device="cuda").copy_(t)
+
+
+def _turned(t):
+    """The same with another order of its last two dimensions in memory."""
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() > 1 else t
+
+
+@pytest.mark.parametrize("unpack", [_save_on_cpu_and_back, _turned])
+@pytest.mark.parametrize("given", ["permuted", "padded", "contiguous"])
+def test_saved_tensors_that_come_back_laid_out_otherwise(given, unpack):
+    """Hooks may hand back what a call saved with other strides than it had (torch.autograd.graph.save_on_cpu does): the gradient reads it as it lies then."""
+    z, history, g = make(30, 700, torch.bfloat16, 11, 40)
+    z, history = z.view(6, 5, 700), history.view(6, 5, 40)
+    flags = (torch.rand(6, 5, 700, generator=g) < 0.5).cuda()
+    words = words_of(flags)
+    lengths, numbers = torch.randint(0, 41, (6, 5), generator=g).cuda(), (1.0 + torch.rand(6, 5, generator=g)).cuda()
+    up = torch.randn(6, 5, 700, generator=g).to(torch.bfloat16).cuda()
+
+    def laid_out(t):
+        if given == "permuted":
+            return t.transpose(0, 1).contiguous().transpose(0, 1)
+        return torch.cat((t, t), -1)[..., :t.size(-1)] if given == "padded" else t
+
+    for allowed in (flags, words, None):
+        leaf = laid_out(z).detach().requires_grad_()
+        call = lambda: F.constrain_logits(leaf, laid_out(history), lengths, repetition=numbers, allowed=None if allowed is None else laid_out(allowed))
+        want, = torch.autograd.grad(call(), leaf, up)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            out = call()
+        source = up.clone().requires_grad_()
+        got, = torch.autograd.grad(out, leaf, source, create_graph=True)
+        assert torch.equal(got, want)
+        again, = torch.autograd.grad(got, source, up)       # (the same factors once more)
+        assert torch.equal(again, want)

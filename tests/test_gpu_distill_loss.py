@@ -334,3 +334,31 @@ def test_captured_and_on_other_streams(rows, classes):
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), n
+
+
+def _save_on_cpu_and_back(t):
+    """A saved tensor as a hook that keeps it on the host hands it back: as large, contiguous."""
+    return torch.empty(t.shape, dtype=t.dtype, device="cuda").copy_(t)
+
+
+def _turned(t):
+    """The same with another order of its last two dimensions in memory."""
+    return t.transpose(-1, -2).contiguous().transpose(-1, -2) if t.dim() > 1 else t
+
+
+@pytest.mark.parametrize("unpack", [_save_on_cpu_and_back, _turned])
+@pytest.mark.parametrize("rows, classes", [(40, 10), (7, 9001), (3, 140001)])
+def test_saved_tensors_that_come_back_laid_out_otherwise(rows, classes, unpack):
+    """Hooks may hand back what a call saved with other strides than it had: the gradients of all losses on logits read it as it lies then."""
+    z, values, chosen, rest, g = make(rows, classes, 3, torch.bfloat16, 8, ignored=0.0)
+    leaf = z.requires_grad_()
+    labels = torch.randint(0, classes, (rows,), generator=g).cuda()
+    runs = [lambda: losses.distill_loss(leaf, values, chosen, rest, temperature=2.0)[0],
+            lambda: losses.label_log_probs(leaf, labels).sum(),
+            lambda: losses.policy_loss(leaf, labels, torch.full((rows,), -3.0, device="cuda"), torch.ones(rows, device="cuda"))[0]]
+    for run in runs:
+        want, = torch.autograd.grad(run(), leaf)
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+            out = run()
+        got, = torch.autograd.grad(out, leaf)
+        assert torch.equal(got, want)
