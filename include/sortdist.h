@@ -427,7 +427,8 @@ int sd_distill_gradient(const sd_logit_rows* rows, const sd_top_lists* lists, do
  * outer + (r % inner) * inner entries behind their pointer; strides may be 0.
  *   history (NULL: none): history_length classes of history_bytes = 4 or 8 each, of which row r's first lengths[r] count (NULL: all; of
  *     length_bytes; taken as 0..history_length); entries outside 0..classes-1 are no class.
- *   repetition_rows, presence_rows, frequency_rows: one number for each row, or NULL: the number that follows.
+ *   repetition_rows, presence_rows, frequency_rows: one number for each row, or NULL: the number that follows.  A repetition lies in 2^-126..2^126 (a
+ *     number outside is refused, a row's makes its penalised logits and their gradients NaN); presence and frequency are finite.
  *   bias (NULL: none): fp32, one for each class.
  *   allowed (NULL: all): SD_ALLOWED_FLAGS one byte for each class, or SD_ALLOWED_BITS, bit v % 32 of the 32-bit word v / 32; strides in bytes
  *     and in words. */
@@ -447,8 +448,8 @@ typedef struct {
 } sd_constraints;
 
 /* out[r, v], rows of `classes` values one behind the other in the logits' type: with n = how often v stands in row r's history, z where n = 0, else
- * (z > 0 ? z / repetition : z * repetition) - frequency n - presence; plus bias; -inf where v is not allowed.  The gradient reads the
- * logits only where n > 0. */
+ * (z > 0 ? z / repetition : z * repetition) - frequency n - presence; plus bias; -inf where v is not allowed.  In fp32, z / repetition as the product with
+ * the rounded reciprocal (up to 1.5 units of fp32 off), then rounded to the logits' type.  The gradient reads the logits only where n > 0. */
 int sd_constrain_logits(const sd_logit_rows* rows, const sd_constraints* constraints, void* out, sd_stream_t stream);
 int sd_constrain_gradient(const sd_logit_rows* rows, const sd_constraints* constraints, const void* grad_output, void* grad, sd_stream_t stream);
 

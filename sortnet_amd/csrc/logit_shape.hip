@@ -57,11 +57,18 @@ template <int ALLOWED> __device__ __forceinline__ bool allowed_one(const void* r
     else return static_cast<const uint8_t*>(row)[c] != 0;
 }
 
-// What classes of the history pay: a positive logit times `inverse`, another one times `repetition`.
+// What classes of the history pay: a positive logit times `inverse`, another one times `repetition`.  A quotient is a product with the reciprocal in fp32, off by up to 1.5 units
+// of fp32 instead of half of one: a division is about ten instructions for each logit of a vector in which one counts.  Both numbers have to be normal ones;
+// a row's repetition that is none makes what it applies to NaN.
+constexpr float kLeastRepetition = 0x1p-126f, kMostRepetition = 0x1p126f;
 struct Penalties { float repetition, inverse, presence, frequency; };
 __device__ __forceinline__ Penalties penalties_of(const Shape& s, int64_t r) {
     Penalties p{s.repetition, s.inverse, s.presence, s.frequency};
-    if (s.repetition_rows) { p.repetition = s.repetition_rows[r]; p.inverse = 1.f / p.repetition; }
+    if (s.repetition_rows) {
+        const float given = s.repetition_rows[r];
+        p.repetition = given >= kLeastRepetition && given <= kMostRepetition ? given : __builtin_nanf("");
+        p.inverse = 1.f / p.repetition;
+    }
     if (s.presence_rows) p.presence = s.presence_rows[r];
     if (s.frequency_rows) p.frequency = s.frequency_rows[r];
     return p;
@@ -299,7 +306,7 @@ static int shape_logits(const char* who, const sd_logit_rows* in, const sd_const
     SD_REQUIRE(!c->history || (reinterpret_cast<uintptr_t>(c->history) & (c->history_bytes - 1)) == 0, "%s: the history is not aligned to its type", who);
     SD_REQUIRE(!c->lengths || (reinterpret_cast<uintptr_t>(c->lengths) & (c->length_bytes - 1)) == 0, "%s: lengths are not aligned to their type", who);
     SD_REQUIRE(!c->lengths || c->history, "%s: lengths without a history", who);
-    SD_REQUIRE(c->repetition_rows || (c->repetition > 0.0 && c->repetition <= FLT_MAX && (float)c->repetition > 0.f), "%s: repetition=%g must be positive and finite", who, c->repetition);
+    SD_REQUIRE(c->repetition_rows || (c->repetition >= kLeastRepetition && c->repetition <= kMostRepetition), "%s: repetition=%g outside 2^-126..2^126", who, c->repetition);
     SD_REQUIRE(c->presence_rows || (c->presence >= -FLT_MAX && c->presence <= FLT_MAX), "%s: presence=%g must be finite", who, c->presence);
     SD_REQUIRE(c->frequency_rows || (c->frequency >= -FLT_MAX && c->frequency <= FLT_MAX), "%s: frequency=%g must be finite", who, c->frequency);
     SD_REQUIRE(((reinterpret_cast<uintptr_t>(c->repetition_rows) | reinterpret_cast<uintptr_t>(c->presence_rows) | reinterpret_cast<uintptr_t>(c->frequency_rows) |

@@ -349,7 +349,8 @@ def constrain_logits(outputs, history=None, lengths=None, repetition=1.0, presen
 
     history  (..., places) int32 or int64: the classes chosen before; of row r the first lengths[r] places (all without `lengths`) that hold a
              class, others (a padding of -1) are none.
-    repetition, presence, frequency: numbers, or fp32 with one for each row.
+    repetition, presence, frequency: numbers, or fp32 with one for each row.  A repetition lies in 2^-126..2^126: a number outside is refused, a row's makes the
+             penalised logits of that row, and their gradients, NaN.  z / repetition is the product with the reciprocal in fp32, up to 1.5 units of fp32 off.
     bias     (classes) or the sizes of `outputs`, fp32.
     allowed  bool (classes) or the sizes of `outputs`; or int32 (words) or (..., words) with words = ceil(classes / 32), class v being bit
              v % 32 of word v // 32.  A row with nothing allowed is -inf all over.

@@ -368,3 +368,25 @@ def test_saved_tensors_that_come_back_laid_out_otherwise(given, unpack):
         assert torch.equal(got, want)
         again, = torch.autograd.grad(got, source, up)       # (the same factors once more)
         assert torch.equal(again, want)
+
+
+def test_repetitions_of_rows_without_a_meaning():
+    """A row's repetition that no number may be (0 or less, NaN, outside 2^-126..2^126) makes what it applies to NaN, gradients too, and nothing else."""
+    odd = [0.0, -0.0, -1.5, math.nan, math.inf, -math.inf, 1e-39, 2.0 ** -149, 2.0 ** 127, 3e38, 2.0 ** -126, 2.0 ** 126, 1.5]
+    rows, good = len(odd), 3
+    for classes, group in ((12, "together"), (9001, "in parts")):
+        z = torch.randn(rows, classes, device="cuda").clamp(-3.0, 3.0)
+        history = torch.tensor([[1, 4, 1, -1]] * rows, device="cuda")
+        numbers = torch.tensor(odd, dtype=torch.float32, device="cuda")
+        leaf = z.clone().requires_grad_()
+        out = F.constrain_logits(leaf, history, repetition=numbers)
+        grad, = torch.autograd.grad(out, leaf, torch.zeros_like(out))
+        for t in (out.detach(), grad):
+            assert torch.isnan(t[:-good][:, [1, 4]]).all() and not torch.isnan(t[-good:]).any()
+            t = t.clone()
+            t[:, [1, 4]] = 0.0
+            assert torch.equal(t, torch.zeros_like(t) if t[0, 0] == 0 else z.index_fill(1, torch.tensor([1, 4], device="cuda"), 0.0))
+        ends = numbers[-good:].double().view(-1, 1)
+        counted = z[-good:, [1, 4]].double()
+        want = torch.where(counted > 0, counted / ends, counted * ends)
+        assert ((out[-good:, [1, 4]].double() - want).abs() <= 3 * U * want.abs() + 2.0 ** -149).all()      # (a reciprocal and a product; the smallest numbers have fewer digits)

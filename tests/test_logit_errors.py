@@ -145,3 +145,11 @@ def test_distillation_without_a_meaning():
         _distill(stats=P + 4)
     with pytest.raises(RuntimeError, match="aligned"):
         _distill(scratch=P + 8)
+
+
+@pytest.mark.parametrize("value", [1e-39, 2.0 ** -127, 2.0 ** 127, 3e38], ids=str)
+def test_repetitions_whose_reciprocal_loses_digits(value):
+    """Penalised logits are products with a repetition or its reciprocal in fp32: both have to be normal numbers."""
+    for name, args in (("sd_constrain_logits", (P,)), ("sd_constrain_gradient", (P, P))):
+        with pytest.raises(RuntimeError, match="repetition="):
+            _lib.call(name, _rows(), _constraints(repetition=value), *args, None)
