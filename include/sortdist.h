@@ -388,8 +388,8 @@ typedef struct {
     int dtype;
 } sd_logit_rows;
 
-/* The k largest logits of each row (1..SD_MOST_TOP, at most `classes`), of equal ones the lower class first, NaN above all: values (rows, k) in
- * the logits' type, classes (rows, k), and rest (rows), the log of the sum of exp(logit / temperature) over the row's other classes (-inf where
+/* The k largest logits of each row (1..SD_MOST_TOP, at most `classes`), of equal ones the lower class first, NaN above all, zeros alike: values (rows, k), bit by
+ * bit those of the logits, classes (rows, k), and rest (rows), the log of the sum of exp(logit / temperature) over the row's other classes (-inf where
  * there are none; NaN in a row that has one).  temperature: 1e-4..1e4.  scratch: sd_top_scratch() floats (host only, -1 for what would be
  * refused), 16-byte aligned, any contents; may be NULL where that is 0. */
 int64_t sd_top_scratch(const sd_logit_rows* rows, int64_t k);

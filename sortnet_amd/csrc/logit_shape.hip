@@ -58,8 +58,8 @@ template <int ALLOWED> __device__ __forceinline__ bool allowed_one(const void* r
 }
 
 // What classes of the history pay: a positive logit times `inverse`, another one times `repetition`.  A quotient is a product with the reciprocal in fp32, off by up to 1.5 units
-// of fp32 instead of half of one: a division is about ten instructions for each logit of a vector in which one counts.  Both numbers have to be normal ones;
-// a row's repetition that is none makes what it applies to NaN.
+// of fp32 instead of half of one: with a division, whose instructions each logit of a vector pays in which one counts, 4096 x 65536 bf16 with 1024 places and a bit mask
+// takes 220 us instead of 209.  Both numbers have to be normal ones; a row's repetition that is none makes what it applies to NaN.
 constexpr float kLeastRepetition = 0x1p-126f, kMostRepetition = 0x1p126f;
 struct Penalties { float repetition, inverse, presence, frequency; };
 __device__ __forceinline__ Penalties penalties_of(const Shape& s, int64_t r) {

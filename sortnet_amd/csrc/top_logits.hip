@@ -30,6 +30,9 @@ __device__ __forceinline__ float value_of(uint32_t order) {
 }
 constexpr uint32_t kLowestOrder = 0x00800000u;      // of -FLT_MAX; that of -inf is one less
 constexpr uint32_t kInfiniteOrder = 0xff800000u;
+constexpr uint32_t kZeroOrder = 0x80000000u, kNanOrder = 0xffffffffu;
+// of several values (two zeros, all NaN): which of them it was stands in the row
+__device__ __forceinline__ bool shared_order(uint32_t order) { return order == kZeroOrder || order == kNanOrder; }
 
 typedef unsigned long long Number;      // order << 32 | ~class; 0: none
 __device__ __forceinline__ Number number_of(uint32_t order, int cls) { return (Number)order << 32 | (uint32_t)~cls; }
@@ -268,8 +271,12 @@ template <int THREADS> struct Keeper {
     template <class T> __device__ __forceinline__ void finish(const T* row, int64_t r) {
         T* values = static_cast<T*>(t.values) + r * t.k;
         int* classes = t.classes + r * t.k;
-        const auto put = [&](int place, float v, int cls) { values[place] = Elem<T>::put(v); classes[place] = cls; };
-        sort([&](int place, Number x) { put(place, value_of(number_order(x)), number_class(x)); });
+        const auto put = [&](int place, T v, int cls) { values[place] = v; classes[place] = cls; };
+        sort([&](int place, Number x) {
+            const uint32_t order = number_order(x);
+            const int cls = number_class(x);
+            put(place, shared_order(order) ? row[cls] : Elem<T>::put(value_of(order)), cls);
+        });
         if (all < t.k) {      // the first classes that are -inf
             const bool none = (int)threadIdx.x < t.k && Elem<T>::get(row[threadIdx.x]) == -INFINITY;
             const uint64_t lanes = __ballot(none);
@@ -280,7 +287,7 @@ template <int THREADS> struct Keeper {
                 __syncthreads();
                 for (int w = 0; w < wave; w++) place += (int)words[w];
             }
-            if (none && place < t.k) put(place, -INFINITY, threadIdx.x);
+            if (none && place < t.k) put(place, Elem<T>::put(-INFINITY), threadIdx.x);
         }
     }
     __device__ __forceinline__ void store_rest(const Others& o, int64_t r) const {

@@ -335,7 +335,7 @@ def bound_dropout(x, lower, upper, q, seed):
 def top_logits(outputs, k, temperature=1.0):
     """The k (up to 256) largest logits of each row of `outputs` (..., classes; fp32, bf16 or fp16) and what is left: (values, classes, rest).
 
-    values (..., k) in the type of `outputs`, from the largest on, of equal ones the lower class first (NaN above all, -0 as 0; classes masked by -inf come
+    values (..., k), the logits bit by bit, from the largest on, of equal ones the lower class first (NaN above all, -0 and 0 alike; classes masked by -inf come
     last, and are given where there are not k others); classes (..., k) int32; rest (...) fp32, the log of the sum of exp(logit / temperature) over the other
     classes: -inf where there are none, NaN in a row that has one.  What `losses.distill_loss` learns from; with it the log
     probabilities at the temperature are values / temperature - logaddexp(logsumexp(values / temperature), rest).  No gradient flows through it."""

@@ -173,3 +173,28 @@ def test_captured_and_on_other_streams(rows, classes, k):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), n
         check(z[:5], k)
+
+
+BITS = {torch.float32: torch.int32, torch.bfloat16: torch.int16, torch.float16: torch.int16}
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=str)
+@pytest.mark.parametrize("classes", [9, 64, 65, 500, 20000, 140000])
+def test_values_are_the_logits_bit_by_bit(classes, dtype):
+    """Zeros of both signs and NaN of any payload are given as they stand, whatever form reads the row."""
+    z = make(5, classes, dtype, classes)
+    z[0] = -z[0].abs() - 1.0
+    z[0, 2], z[0, 3], z[0, 5] = -0.0, 0.0, -0.0
+    z[1] = -0.0
+    z[2, 1:8:3] = math.nan
+    bits = z.view(BITS[dtype])
+    bits[2, 4] += 5                     # another payload
+    bits[2, 7] |= -1 << (31 if dtype == torch.float32 else 15)      # and a sign
+    z[3] = math.nan
+    for t in (z, z[:1]):
+        values, chosen, _ = F.top_logits(t, 6)
+        assert torch.equal(values.view(BITS[dtype]), t.contiguous().view(BITS[dtype]).gather(1, chosen.long()))
+    values, chosen, _ = F.top_logits(z, 6)
+    assert chosen[0, :3].tolist() == [2, 3, 5] and torch.signbit(values[0, :3]).tolist() == [True, False, True] and torch.signbit(values[1]).all()
+    assert torch.isnan(values[2, :3]).all() and chosen[2, :3].tolist() == [1, 4, 7] and torch.isnan(values[3]).all() and chosen[3].tolist() == list(range(6))
+    assert not torch.isnan(values[4]).any()
