@@ -42,20 +42,18 @@ __device__ __forceinline__ int number_class(Number x) { return (int)~(uint32_t)x
 struct Top {
     int k;
     float by;               // log2(e) / temperature
+    double inverse;         // 1 / temperature
     void* values;
     int* classes;
     float* rest;
 };
 
-// Sums of exp(v / T) are kept as multiples of 2 to the power of what this gives for the largest v in them: a number of fp32, so that v `by` minus it is
-// rounded once, and 2^4 at most where v is the largest; beyond 2^28, where the rounding of the power itself would be more, in 64 bits.
+// Sums of exp(v / T) are kept as multiples of exp(top / T), top being the largest v in them: differences to it, by log2(e) / T rounded to fp32, are all that an exponential
+// sees, and top / T, in 64 bits, comes to the logarithm of the sum at the end.  Where many values are taken relative to one number m, m log2(e) / T is the sum of two fp32
+// numbers, of which a fused multiply-add takes the first; beyond 2^28, where the second would be more than 2^4, differences are formed in 64 bits.
 constexpr float kNear = 0x1p28f;
-__device__ __forceinline__ double power_of(float top, const Top& t) {
-    const float p = top * t.by;
-    return fabsf(p) <= kNear ? (double)p : (double)top * (double)t.by;
-}
 struct Others { float top; double sum; };       // (top: -inf where there are none, never +inf)
-__device__ __forceinline__ double in_powers(float top, float of, const Top& t) { return top == of ? 1.0 : (double)__builtin_amdgcn_exp2f((float)(power_of(top, t) - power_of(of, t))); }
+__device__ __forceinline__ double in_powers(float top, float of, const Top& t) { return top == of ? 1.0 : (double)__builtin_amdgcn_exp2f((float)(((double)top - (double)of) * (double)t.by)); }
 __device__ __forceinline__ void join(Others& o, float top, double sum, const Top& t) {
     if (sum == 0.0) return;
     if (top > o.top) {
@@ -116,13 +114,14 @@ template <int THREADS> struct Keeper {
             m = largest(f);
         }
         if (m == -INFINITY) return;
-        const double power = power_of(m, t);
-        if (fabs(power) <= (double)kNear) {
+        const float power = m * t.by;
+        if (fabsf(power) <= kNear) {
+            const float low = fmaf(m, t.by, -power);
             #pragma unroll
-            for (int i = 0; i < V; i++) f[i] = __builtin_amdgcn_exp2f(fmaf(f[i], t.by, -(float)power));
+            for (int i = 0; i < V; i++) f[i] = __builtin_amdgcn_exp2f(fmaf(f[i], t.by, -power) - low);
         } else {
             #pragma unroll
-            for (int i = 0; i < V; i++) f[i] = __builtin_amdgcn_exp2f((float)((double)f[i] * (double)t.by - power));
+            for (int i = 0; i < V; i++) f[i] = __builtin_amdgcn_exp2f((float)(((double)f[i] - (double)m) * (double)t.by));
         }
         join(others, m, (double)tree(f), t);
     }
@@ -291,7 +290,7 @@ template <int THREADS> struct Keeper {
         }
     }
     __device__ __forceinline__ void store_rest(const Others& o, int64_t r) const {
-        t.rest[r] = o.sum == 0.0 ? -INFINITY : (float)(log(o.sum) + power_of(o.top, t) * 0.69314718055994530942);
+        t.rest[r] = o.sum == 0.0 ? -INFINITY : (float)(log(o.sum) + (double)o.top * t.inverse);
     }
 };
 
@@ -358,16 +357,17 @@ template <class T, int THREADS> __global__ void __launch_bounds__(THREADS, 8) to
         read_again(f, p, number_class(x));
         keep.leave_all(f);
     };
-    double sum = 0.0;
+    double sum = 0.0;                       // of 2^(v by - power)
     float base = -FLT_MAX, power = 0.f;     // (nothing but -inf is summed as long as this is the bound)
     bool again = false;
     const int most = t.k + t.k / 4 < S::kMost ? t.k + t.k / 4 : S::kMost;      // vectors that a cut leaves
     const auto rebase = [&]() {
         if (keep.bound == base) return;
-        if (base > -FLT_MAX) sum *= in_powers(base, keep.bound, t);
+        const float before = power;
         base = keep.bound;
         power = base * t.by;
         if (!(fabsf(power) <= kNear)) { power = 0.f; again = true; }
+        if (sum != 0.0) sum *= (double)__builtin_amdgcn_exp2f((float)((double)before - (double)power));
     };
     for (int c0 = 0, step = 1; c0 < n; c0 += kSpan, step++) {
         u32x4 v[NV];
@@ -473,7 +473,7 @@ template <class T, int THREADS> __global__ void __launch_bounds__(THREADS, 8) to
         for (int i = keep.all + threadIdx.x; i < t.k; i += THREADS) numbers[i] = 0ull;
     }
     // (where fewer than k logits are above -inf there are no others)
-    if (!again) join(keep.others, base, sum, t);
+    if (!again && sum != 0.0) join(keep.others, base, sum * (double)__builtin_amdgcn_exp2f(-fmaf(base, t.by, -power)), t);
     Others o = keep.all_others();
     const uint32_t bases = keep.share(order_of(again ? INFINITY : base), [](uint32_t x, uint32_t y) { return x > y ? x : y; });
     if (threadIdx.x == 0) {
@@ -589,7 +589,7 @@ template <class T> __global__ void __launch_bounds__(256) top_short_kernel(Logit
         const float sum = (float)group_total(other == -INFINITY ? 0.0 : other == top ? 1.0 : top == INFINITY ? 0.0 : (double)__builtin_amdgcn_exp2f((other - top) * t.by), shift);
         const float nan = group_max(v != v ? 1.f : 0.f, shift);
         if (lane == 0)
-            t.rest[r] = nan != 0.f ? __builtin_nanf("") : sum == 0.f ? -INFINITY : top == INFINITY ? INFINITY : (float)((double)logf(sum) + power_of(top, t) * 0.69314718055994530942);
+            t.rest[r] = nan != 0.f ? __builtin_nanf("") : sum == 0.f ? -INFINITY : top == INFINITY ? INFINITY : (float)((double)logf(sum) + (double)top * t.inverse);
     }
 }
 
@@ -654,7 +654,7 @@ extern "C" int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temper
                (reinterpret_cast<uintptr_t>(scratch) & 15) == 0, "top_logits: results are not aligned to their types, or scratch to 16 bytes");
     const Plan plan = plan_of(a, k, vec_of(rows->dtype));
     SD_REQUIRE(scratch || plan.splits == 1, "top_logits: null scratch");
-    const Top t{(int)k, (float)(1.4426950408889634074 / temperature), values, classes, rest};
+    const Top t{(int)k, (float)(1.4426950408889634074 / temperature), 1.0 / temperature, values, classes, rest};
     const int64_t lists = a.rows * plan.splits;
     Parts parts{};
     if (plan.splits > 1) parts = Parts{reinterpret_cast<Number*>(scratch), reinterpret_cast<Others*>(scratch + 2 * lists * k)};

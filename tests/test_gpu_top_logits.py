@@ -198,3 +198,12 @@ def test_values_are_the_logits_bit_by_bit(classes, dtype):
     assert chosen[0, :3].tolist() == [2, 3, 5] and torch.signbit(values[0, :3]).tolist() == [True, False, True] and torch.signbit(values[1]).all()
     assert torch.isnan(values[2, :3]).all() and chosen[2, :3].tolist() == [1, 4, 7] and torch.isnan(values[3]).all() and chosen[3].tolist() == list(range(6))
     assert not torch.isnan(values[4]).any()
+
+
+@pytest.mark.parametrize("classes", [3, 9, 64, 65, 500, 20000, 140000])
+def test_others_of_large_logits(classes):
+    """Log-sums of some 1e5, in temperatures whose log2(e) / T is rounded by as much as a number of fp32 can be: the factor and the result are, and nothing else of their size."""
+    for temperature in (1.429, 1.426, 0.713):
+        z = make(40, classes, torch.float32, classes) * 3e4
+        z[20:] = z[20:].abs()
+        check(z, 2, temperature)
