@@ -449,7 +449,8 @@ typedef struct {
 
 /* out[r, v], rows of `classes` values one behind the other in the logits' type: with n = how often v stands in row r's history, z where n = 0, else
  * (z > 0 ? z / repetition : z * repetition) - frequency n - presence; plus bias; -inf where v is not allowed.  In fp32, z / repetition as the product with
- * the rounded reciprocal (up to 1.5 units of fp32 off), then rounded to the logits' type.  The gradient reads the logits only where n > 0. */
+ * the rounded reciprocal (up to 1.5 units of fp32 off), then rounded to the logits' type.  The gradient reads
+ * the logits only where n > 0, and those in the same 16 bytes from the row's start on. */
 int sd_constrain_logits(const sd_logit_rows* rows, const sd_constraints* constraints, void* out, sd_stream_t stream);
 int sd_constrain_gradient(const sd_logit_rows* rows, const sd_constraints* constraints, const void* grad_output, void* grad, sd_stream_t stream);
 

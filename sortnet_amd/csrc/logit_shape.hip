@@ -281,12 +281,13 @@ template <class T, int ALLOWED, int HISTORY, int KIND> __global__ void __launch_
         int i;
         const int c = vecs * V + split(item, rest, i);
         const int64_t r = r0 + i;
-        const T z = row_start<T>(a, r)[c0 + c];
-        float f = Elem<T>::get(GRAD ? static_cast<const T*>(s.grad)[r * a.classes + c0 + c] : z);
+        const T* z = row_start<T>(a, r) + c0 + c;
+        float f = Elem<T>::get(GRAD ? static_cast<const T*>(s.grad)[r * a.classes + c0 + c] : *z);
         if (HISTORY) {
             const uint32_t n = count_of<HISTORY>(counts, i * width + c);
             if (rows > 1) paid = penalties_of(s, r);
-            f = GRAD ? penalised_slope(f, Elem<T>::get(z), n, paid) : penalised(f, n, paid);
+            if (!GRAD) f = penalised(f, n, paid);
+            else if (n) f = penalised_slope(f, Elem<T>::get(*z), n, paid);
         }
         if (BIAS) f += s.bias[place(r, s.bias_outer, s.bias_inner) + c0 + c];
         if (ALLOWED != kAll && !allowed_one<kAny>(allowed_row(r), (int)c0 + c)) f = GRAD ? 0.f : -INFINITY;

@@ -390,3 +390,23 @@ def test_repetitions_of_rows_without_a_meaning():
         counted = z[-good:, [1, 4]].double()
         want = torch.where(counted > 0, counted / ends, counted * ends)
         assert ((out[-good:, [1, 4]].double() - want).abs() <= 3 * U * want.abs() + 2.0 ** -149).all()      # (a reciprocal and a product; the smallest numbers have fewer digits)
+
+
+def test_gradient_reads_logits_where_something_counts():
+    """The C entry's promise: of logits that nothing of the history names, nothing is read - the rows here are 64 classes long in memory, and named below that."""
+    from sortnet_amd import _lib
+    classes, rows = 1003, 1
+    g = torch.Generator().manual_seed(2)
+    for dtype, kind in ((torch.float32, 0), (torch.bfloat16, 1), (torch.float16, 2)):
+        short = torch.randn(64, generator=g).to(dtype).cuda()
+        up = torch.randn(rows, classes, generator=g).to(dtype).cuda()
+        history = torch.randint(0, 64, (rows, 9), generator=g).cuda()
+        got = torch.empty_like(up)
+        a, c = _lib.LogitRows(), _lib.Constraints()
+        a.logits, a.rows, a.inner, a.classes, a.inner_stride, a.dtype = short.data_ptr(), rows, rows, classes, classes, kind
+        c.history, c.history_bytes, c.history_length, c.history_inner, c.repetition = history.data_ptr(), 8, 9, 9, 2.0
+        _lib.call("sd_constrain_gradient", a, c, up.data_ptr(), got.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        want = up.clone()
+        seen = torch.zeros(64, dtype=torch.bool, device="cuda").index_fill(0, history[0], True)
+        want[0, :64] = torch.where(seen, torch.where(short > 0, up[0, :64] / 2, up[0, :64] * 2), up[0, :64])
+        assert torch.equal(got, want)
