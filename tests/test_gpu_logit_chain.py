@@ -125,3 +125,45 @@ def test_two_threads_at_once():
     for t in threads:
         t.join()
     assert not wrong
+
+
+def test_two_threads_finish_what_they_began():
+    """The same from two threads whose errors are seen: every pass of both has come to its end."""
+    g = torch.Generator().manual_seed(10)
+    z, t = ((2 * torch.randn(600, 30001, generator=g)).to(torch.bfloat16).cuda() for _ in range(2))
+    short, teacher = (torch.randn(500, 40, generator=g).cuda() for _ in range(2))
+    history, flags = torch.randint(0, 40, (500, 12), generator=g).cuda(), (torch.rand(500, 40, generator=g) < 0.7).cuda()
+    z.requires_grad_()
+    short.requires_grad_()
+
+    def large():
+        loss, divergences = losses.distill_loss(z, *F.top_logits(t, 40), temperature=1.5)
+        return loss.detach(), divergences, torch.autograd.grad(loss, z)[0]
+
+    def small():
+        shaped = F.constrain_logits(short, history, presence=0.5, allowed=flags)
+        loss, divergences = losses.distill_loss(shaped, *F.top_logits(F.constrain_logits(teacher, allowed=flags), 4))
+        return shaped.detach(), divergences, torch.autograd.grad(loss, short)[0]
+
+    want = {f: [r.clone() for r in f()] for f in (large, small)}
+    torch.cuda.synchronize()
+    wrong, ended = [], []
+
+    def work(first, second):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for n in range(12):
+                    f = first if n % 2 == 0 else second
+                    got = f()
+                    torch.cuda.current_stream().synchronize()
+                    wrong.extend((n, j) for j, (a, b) in enumerate(zip(got, want[f])) if not torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)))
+                    ended.append(n)
+        except BaseException as e:
+            wrong.append(repr(e))
+
+    threads = [threading.Thread(target=work, args=fs) for fs in ((large, small), (small, large))]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong and len(ended) == 24
