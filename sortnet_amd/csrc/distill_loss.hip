@@ -6,7 +6,8 @@
 // S is formed without the entries' classes, not as a difference, so that what the student gives the others keeps its digits however small it is.
 // There are few outcomes per row: they are in 64 bits, as three sums over the entries (Sums) that need no S, so that what is left when S is there is a few
 // numbers per row.  Both passes are bound by the bytes of the logits, and by the launches where there are few.
-// A class that stands in several entries is one class: it counts once in p and takes the sum of their q.
+// A class that stands in several entries counts once in p and takes the sum of their q in the gradient.  D keeps a term for each entry, q_j log q_j, which is below that of
+// the merged class by q_j log(q / q_j): merging them would cost each row a search among its entries for what the logits do not change.
 // All sums have a fixed order: results are the same in every call.
 #include <climits>
 #include "label_rows.h"

@@ -362,3 +362,20 @@ def test_saved_tensors_that_come_back_laid_out_otherwise(rows, classes, unpack):
             out = run()
         got, = torch.autograd.grad(out, leaf)
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("classes", [6, 900, 20000, 140001])
+def test_entries_of_one_class(classes):
+    """A class of several entries is one class of the student's and takes the sum of their q in the gradient; the divergence is a sum over the entries, each with its own
+    q log q.  It lies below that of a list in which they are one entry by the sum of q_j log(q / q_j), which the logits do not change."""
+    g = torch.Generator().manual_seed(classes)
+    z = torch.randn(1, classes, generator=g).cuda().requires_grad_()
+    twice = losses.distill_loss(z, torch.zeros(1, 2, device="cuda"), torch.full((1, 2), 3, device="cuda"))
+    once = losses.distill_loss(z, torch.zeros(1, 1, device="cuda"), torch.full((1, 1), 3, device="cuda"))
+    off = 4 * sum_error(classes) + 2 * U * once[1].item()
+    assert abs((once[1] - twice[1]).item() - math.log(2.0)) <= off      # (q = 1/2 twice)
+    a, b = (torch.autograd.grad(loss, z)[0] for loss, _ in (twice, once))
+    assert ((a - b).abs() <= 2 * U * a.abs() + 2.0 ** -126).all()       # (1/2 + 1/2 is 1 in 64 bits; one rounding each)
+    sure = torch.full((1, classes), -200.0, device="cuda")
+    sure[0, 3] = 200.0
+    assert abs(losses.distill_loss(sure, torch.zeros(1, 2, device="cuda"), torch.full((1, 2), 3, device="cuda"))[1].item() + math.log(2.0)) <= 2 * U
