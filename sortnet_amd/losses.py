@@ -106,7 +106,7 @@ def distill_loss(outputs, top_values, top_classes, top_rest=None, temperature=1.
     A row without an entry, or whose entries and rest are all -inf, is not read, whatever it holds, does not count in the mean, and gets zeros.
     A class in several entries counts once in p and takes all their q in the gradient; in the divergence each entry is an outcome with its own q log q, so that it
     lies below that of the list without repeats, perhaps below 0, by an amount that `outputs` do not change.  A class past the end gives NaN.  Only
-    `outputs` gets a gradient; `divergences` has none.  From 40 MiB of logits on (512 rows at least, of more than 8 KiB) the gradient is made
+    `outputs` gets a gradient; `divergences` has none.  From 40 MiB of logits on (512 rows at least, of more than 8 KiB and at most 256 KiB) the gradient is made
     with the loss, for an upstream gradient of 1: a known factor is cheaper as `weight`."""
     return ext.host().distill_loss(outputs, top_values, top_classes, top_rest, float(temperature), float(weight))
 

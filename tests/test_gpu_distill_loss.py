@@ -379,3 +379,9 @@ def test_entries_of_one_class(classes):
     sure = torch.full((1, classes), -200.0, device="cuda")
     sure[0, 3] = 200.0
     assert abs(losses.distill_loss(sure, torch.zeros(1, 2, device="cuda"), torch.full((1, 2), 3, device="cuda"))[1].item() + math.log(2.0)) <= 2 * U
+
+
+@pytest.mark.parametrize("rows, classes, k, dtype", [(540, 65537, 7, torch.float32), (600, 65536, 7, torch.float32), (520, 131073, 256, torch.bfloat16), (515, 140007, 20, torch.float16)])
+def test_batches_of_rows_that_no_workgroup_holds(rows, classes, k, dtype):
+    """Large batches on both sides of the longest row that a workgroup holds, 16384 vectors of 16 bytes: beyond it rows are read in parts and the gradient is made by itself."""
+    test_gradient_with_the_loss(rows, classes, k, dtype)
