@@ -9,7 +9,6 @@
 // A class that stands in several entries counts once in p and takes the sum of their q in the gradient.  D keeps a term for each entry, q_j log q_j, which is below that of
 // the merged class by q_j log(q / q_j): merging them would cost each row a search among its entries for what the logits do not change.
 // All sums have a fixed order: results are the same in every call.
-#include <climits>
 #include "label_rows.h"
 
 namespace sd {
@@ -920,9 +919,11 @@ extern "C" int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* li
         const int blocks = (int)(want < kCountBlocks ? want : kCountBlocks);
         hipLaunchKernelGGL(distill_rows_that_count_kernel, dim3(blocks), dim3(256), 0, s, l, a.rows, kept, counted);
         hipLaunchKernelGGL(distill_scale_kernel, dim3(1), dim3(256), 0, s, counted, blocks, scale_factor, scale);
+        if (int rc = check_launch("distill_rows_that_count_kernel or distill_scale_kernel")) return rc;
     }
     const int vec = vec_of(rows->dtype);
     const Group group = short_group(a, vec);
+    const char* kernel = group.shift >= 0 ? "distill_short_kernel" : grad || !in_parts(a, vec) ? "distill_held_kernel" : "distill_part_kernel or distill_join_kernel";
     with_dtype(rows->dtype, [&](auto* p) {
         using T = std::remove_pointer_t<decltype(p)>;
         if (group.shift >= 0) {
@@ -956,7 +957,7 @@ extern "C" int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* li
         hipLaunchKernelGGL(distill_part_kernel<T>, dim3(blocks_for(a.rows * cut.splits)), dim3(256), 0, s, a, l, t, e, cut.splits, cut.part, parts, twice);
         hipLaunchKernelGGL(distill_join_kernel<T>, dim3(blocks_for((a.rows + 3) / 4)), dim3(256), 0, s, a, l, t, e, cut.splits, parts, twice);
     });
-    if (int rc = check_launch("distill_rows_kernel")) return rc;
+    if (int rc = check_launch(kernel)) return rc;
     const int64_t want = (a.rows + 16383) / 16384;
     const Mean m{divergences, kept, a.rows, weight * temperature * temperature, scale_factor, loss, grad ? nullptr : scale, reinterpret_cast<double*>(scratch + 4), e.ticket};
     hipLaunchKernelGGL(distill_mean_kernel, dim3((unsigned)(want < kMeanBlocks ? want : kMeanBlocks)), dim3(1024), 0, s, m);
@@ -995,5 +996,5 @@ extern "C" int sd_distill_gradient(const sd_logit_rows* rows, const sd_top_lists
         const int splits = (int)((a.classes + part - 1) / part);
         hipLaunchKernelGGL(distill_long_gradient_kernel<T>, blocks(a.rows * splits), dim3(256), 0, s, a, l, t, g, splits, part);
     });
-    return check_launch("distill_gradient_kernel");
+    return check_launch(group.shift >= 0 ? "distill_short_gradient_kernel" : "distill_long_gradient_kernel");
 }

@@ -1008,7 +1008,7 @@ struct Constraints {
 
 // The results are linear in the gradients, with one factor each: the derivative of this node's is the node again.
 struct ConstrainNode : Node {
-    SavedVariable logits, history, bias, allowed, lengths, rows[3];
+    SavedVariable logits, history, allowed, lengths, rows[3];
     Constraints given;      // all but the tensors
 
     void save(const Constraints& c) {
@@ -1052,7 +1052,7 @@ struct ConstrainNode : Node {
     }
     void release_variables() override {
         const Locked lock(mutex_);
-        for (SavedVariable* v : {&logits, &history, &bias, &allowed, &lengths, &rows[0], &rows[1], &rows[2]}) v->reset_data();
+        for (SavedVariable* v : {&logits, &history, &allowed, &lengths, &rows[0], &rows[1], &rows[2]}) v->reset_data();
     }
     std::string name() const override { return "ConstrainNode"; }
 };
@@ -1152,7 +1152,6 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor& outputs, int64_t k, 
 // k entries for each row, one behind the other
 struct Lists {
     Tensor values, classes, rest;
-    double temperature = 1.0;
     sd_top_lists call() const {
         sd_top_lists l{};
         l.values = values.data_ptr();

@@ -11,7 +11,6 @@
 // parts, whose results a second kernel joins.  Logits of -inf are never listed: where there are not k others the first classes that are -inf follow,
 // which are among the row's first k.
 // Bound by the instructions of a logit, of which the exponential is half (it takes the time of four), and by the bytes of the logits.
-#include <climits>
 #include <type_traits>
 #include "label_rows.h"
 
@@ -683,5 +682,5 @@ extern "C" int sd_top_logits(const sd_logit_rows* rows, int64_t k, double temper
             in_slices(a.rows, [&](int64_t from, unsigned blocks) { hipLaunchKernelGGL(top_join_kernel<T>, dim3(blocks), dim3(kJoin), 0, s, a, t, plan.splits, parts, from); });
         }
     });
-    return check_launch("top_rows_kernel");
+    return check_launch(plan.threads == 0 ? "top_short_kernel" : plan.splits == 1 ? "top_rows_kernel" : "top_rows_kernel or top_join_kernel");
 }

@@ -153,3 +153,18 @@ def test_repetitions_whose_reciprocal_loses_digits(value):
     for name, args in (("sd_constrain_logits", (P,)), ("sd_constrain_gradient", (P, P))):
         with pytest.raises(RuntimeError, match="repetition="):
             _lib.call(name, _rows(), _constraints(repetition=value), *args, None)
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="where there is a GPU the kernels would be launched")
+def test_launches_that_fail_name_their_kernels():
+    for classes, kernel in ((60, "top_short_kernel"), (200, "top_rows_kernel"), (1 << 20, "top_join_kernel")):
+        with pytest.raises(RuntimeError, match=kernel):
+            _lib.call("sd_top_logits", _rows(classes=classes), 2, 1.0, P, P, P, P, None)
+    for rows, kernel, slopes in ((dict(classes=60), "distill_short_kernel", "distill_short_gradient_kernel"), (dict(classes=9000), "distill_held_kernel", "distill_long_gradient_kernel"),
+                                 (dict(classes=1 << 20), "distill_join_kernel", "distill_long_gradient_kernel")):
+        with pytest.raises(RuntimeError, match=kernel):
+            _distill(_rows(**rows))
+        with pytest.raises(RuntimeError, match=slopes):
+            _lib.call("sd_distill_gradient", _rows(**rows), _lists(), 1.0, P, P, P, None, 0, P, None)
+    with pytest.raises(RuntimeError, match="distill_rows_that_count_kernel"):
+        _distill(_rows(rows=4096, inner=4096, classes=9000), grad=P)
