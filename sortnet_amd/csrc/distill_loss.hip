@@ -849,7 +849,9 @@ Cut cut_of(const LogitRows& a, int vec) {
 }
 
 // Lanes for a short row: whole quads (see four_of), and of many rows more of them in a wavefront, for each of which a row's 64-bit functions cost
-// as much: 8192 x 1000 fp32 22.0 us with 64 lanes for a row, 17.4 with 32.
+// as much: 8192 x 1000 fp32, k = 16, 22.0 us with 64 lanes for a row, 17.4 with 32.  The border at half and at four times as many, k = 3 and 16:
+// 4000 x 2000 bf16 14.6 and 16.3 us (2^17 and 2^18), 16384 x 200 fp32 13.4 and 14.7, 65536 x 200 bf16 30 and 29 (2^18 and 2^20); of lists longer than a row's lanes each lane
+// has several entries, one behind the other: k = 64, 65536 x 200 fp32 110 and 58.
 constexpr int64_t kFewLanes = 1 << 18;
 Group short_group(const LogitRows& a, int vec) {
     Group g = group_of(a.rows, a.classes, vec);

@@ -606,8 +606,9 @@ Plan plan_of(const LogitRows& a, int64_t k, int vec) {
     int threads = 64;
     while (threads < most) threads *= 2;
     if (a.classes <= (int64_t)threads * kTopVectors * vec) return {threads, 1, a.classes};
-    // A workgroup that is done with a row in two turns needs no parts and no join, nor in four where every compute unit has one: 1 x 16000 bf16, k = 50, 13.5 us, in parts
-    // 18.1; 300 x 50001 fp16, k = 200, 38.4 and 51.4; but 100 x 65536 bf16, k = 20, 33.4 and 25.2.
+    // A workgroup that is done with a row in two turns needs no parts and no join, nor in four where every compute unit has one: bf16, k = 5 / 50 / 200, 64 x 12000 24 / 15.5 / 19 us,
+    // in parts 24 / 19.5 / 28.5; 64 x 30000 28 / 21 / 23 and 24 / 20 / 31; 300 x 50001 43 / 35 / 39 and 39 / 37 / 52; 512 x 65536 47 / 36 / 40 and 49 / 42 / 59; where it would take
+    // four turns and there are fewer rows 16 x 50001 32 / 28 / 31 and 24 / 25 / 33; 200 x 50001 35 / 29 / 32 and 32 / 32 / 46.
     if (a.rows * 512 <= card && a.classes <= 512 * kTopVectors * vec * (a.rows >= 256 ? 4 : 2)) return {512, 1, a.classes};
     if (threads < 128) threads = 128;
     while (threads < 256 && a.rows * threads * 2 <= card) threads *= 2;
