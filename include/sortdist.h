@@ -410,9 +410,9 @@ typedef struct {
 /* Divergence of the student's softmax at `temperature` (1e-4..1e4) from the teacher's, over the classes of the entries and, as one more outcome,
  * all others: divergences[r] = sum_j q_j (log q_j - log p_j) (terms with q_j = 0 are 0); 0 for rows that do not count: those without an
  * entry, and those whose entries and rest are all -inf.  loss = weight temperature^2 mean over the rows that count (0 where there are none).
- * A class in several entries counts once in p, in one term for each entry, and takes the sum of their q in the gradient.  stats (rows, 2), entries (rows, k) and scale (1), all or none NULL, are what sd_distill_gradient
- * needs.  Where sd_distill_fuses(rows) is 1, `grad` may be given (else NULL): it receives the gradient for an upstream gradient of 1, and the logits
- * are read once less.  scratch: sd_distill_scratch() floats (host only, -1 for what would be refused), 16-byte aligned, any contents. */
+ * A class in several entries counts once in p; the divergence has a term for each of its entries, the gradient the sum of their q.
+ * stats (rows, 2), entries (rows, k) and scale (1), all or none NULL, are what sd_distill_gradient needs.  Where sd_distill_fuses(rows) is 1,
+ * `grad` may be given (else NULL): it receives the gradient for an upstream gradient of 1, and the logits are read once less.  scratch: sd_distill_scratch() floats (host only, -1 for what would be refused), 16-byte aligned, any contents. */
 int64_t sd_distill_scratch(const sd_logit_rows* rows, int64_t k);
 int sd_distill_fuses(const sd_logit_rows* rows);
 int sd_distill_loss(const sd_logit_rows* rows, const sd_top_lists* lists, double temperature, double weight, float* stats, float* entries,
